@@ -29,11 +29,11 @@ def listed():
         # a large layer, zero points, half a percent of the entries kept apart as outliers
         case("quantize large", "quantize", 0, 8192, 8192, "bf16", 128, True, 2.8),
         # decoding one token through a small layer: latency is everything
-        case("product one token, small", "product", 1, 1024, 1024, "fp16", 32, False, 0.0),
+        case("product 1 token small", "product", 1, 1024, 1024, "fp16", 32, False, 0.0),
         # decoding one token through a large layer with outliers: the weights' bytes are everything
-        case("product one token, large", "product", 1, 16384, 8192, "bf16", 128, True, 2.8),
+        case("product 1 token large", "product", 1, 16384, 8192, "bf16", 128, True, 2.8),
         # a ragged batch of decoded tokens; odd rows, a short last group
-        case("product 13 tokens, ragged", "product", 13, 4099, 4104, "fp16", 64, True, 2.8),
+        case("product 13 tokens ragged", "product", 13, 4099, 4104, "fp16", 64, True, 2.8),
         # a prompt
         case("product 2048 tokens", "product", 2048, 8192, 8192, "bf16", 128, False, 2.8),
         # gradient of the inputs of a handful of tokens through a frozen layer
@@ -41,13 +41,13 @@ def listed():
         # the same for a training batch
         case("transposed 2048 tokens", "transposed", 2048, 8192, 8192, "bf16", 128, True, 2.8),
         # odd everything
-        case("transposed 333 tokens, ragged", "transposed", 333, 2050, 2088, "bf16", 32, True, 2.8),
+        case("transposed 333 tokens ragged", "transposed", 333, 2050, 2088, "bf16", 32, True, 2.8),
         # training scales on few tokens
         case("gradient 16 tokens", "gradient", 16, 4096, 4096, "bf16", 128, False, 0.0),
         # training scales and outliers on a batch
         case("gradient 2048 tokens", "gradient", 2048, 8192, 8192, "bf16", 64, True, 2.8),
         # odd everything
-        case("gradient 517 tokens, ragged", "gradient", 517, 1000, 4100, "fp16", 32, False, 2.8),
+        case("gradient 517 tokens ragged", "gradient", 517, 1000, 4100, "fp16", 32, False, 2.8),
     ]
 
 
