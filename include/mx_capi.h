@@ -346,6 +346,71 @@ int mx_se_tcspmv(int dtype, const void *csrVal, const int *csrRowPtr, const int 
 int mx_csr_spmv_static(int dtype, int n_rows, int n_cols, int nnz, const int *row_ptr_dev, const int *col_ind_dev,
                        const void *val_dev, const void *x_dev, void *y_dev, void *stream);
 
+/* ---- 4-bit matrices with group scales and a CSR residual (no counterpart in the reference) ------------------- */
+/* The split of this library for a matrix that has no zeros to leave out but values that need few bits: a compressed core
+ * (4-bit codes, one scale per `group` consecutive columns of a row) and a CSR residual of the entries that are too
+ * large for the codes:
+ *     W[i][k] = scales[i][k / group] * (codes[i][k] - zeros[i][k / group]) + R[i][k]
+ * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls allocate nothing, keep nothing
+ * between calls, are asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured
+ * into a graph (mx_q4_check excepted) and leave the calling thread's current device as it was.  Calls on different
+ * streams are independent of each other as far as their buffers are.  Results do not depend on anything but the
+ * inputs: no sum is taken in an order that varies.  n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do
+ * not overlap inputs.
+ *
+ * codes: row i starts at codes + i * code_ld; two codes a byte, even column in the low half.  The base is 16-byte
+ *   aligned, code_ld a multiple of 16 and at least (n_cols + 1) / 2; the buffer has n_rows * code_ld bytes.  What the
+ *   bytes behind a row's last code hold is never used.
+ * scales: [n_rows][n_groups], n_groups = ceil(n_cols / group); the last group of a row may be short.
+ * zeros: [n_rows][n_groups], one byte each of which the low four bits count; NULL = 8 everywhere.
+ * group: a positive multiple of 32, at most 2^30.
+ * dtype: MX_FP16 or MX_BF16, the type of scales, residual values, vectors and results.
+ * residual: CSR with res_row_ptr[n_rows + 1], ascending columns inside a row (repeated columns add up) and buffers with
+ *   room for res_cap entries; res_row_ptr = NULL: none.  Entries are used only as far as they lie inside [0, res_cap)
+ *   and [0, n_cols): a bad residual gives wrong values, never a bad address (mx_q4_check tells). */
+enum { MX_BF16 = 2, MX_FP32 = 3 }; /* types of the mx_q4_* entry points only */
+typedef struct {
+    int n_rows, n_cols;
+    int group;
+    int dtype;
+    int device;
+    int res_cap;
+    long long code_ld; /* bytes from one row of codes to the next */
+    void *codes;
+    void *scales;
+    void *zeros;
+    int *res_row_ptr;
+    int *res_col_ind;
+    void *res_val;
+} mx_q4_matrix;
+/* Fills codes, scales, zeros (if given) and the residual (if given) of *m from the dense row-major matrix w (w_dtype:
+ * MX_FP16, MX_BF16 or MX_FP32; ld_w elements from row to row).  With a residual, entries with |w| > threshold go there
+ * (rounded to dtype) and count as 0 for the codes; without one, threshold is ignored.  Per group, over the entries that
+ * stay:  without zeros  s = max|w| / 7, code = 8 + w / s;  with zeros  s = (max(w, 0) - min(w, 0)) / 15,
+ * zero = -min(w, 0) / s, code = zero + w / s.  s is taken in 32 bits and rounded to dtype first, the quotients by the rounded s to the
+ * nearest whole number, ties to even; codes are clamped to 1..15 (0..15 with zeros).  A group whose s is 0 gets
+ * codes = zero; one that holds a NaN gets s = NaN, one that holds an infinity s = infinity.
+ * res_row_ptr always receives the true counts: where res_row_ptr[n_rows] > res_cap the residual did not fit, and the
+ * entries behind res_cap are lost (quantise again with more room).  Buffer parts behind the last entry stay untouched. */
+int mx_q4_quantize(const mx_q4_matrix *m, int w_dtype, const void *w, long long ld_w, float threshold, void *stream);
+/* w[i][k] = W[i][k], dense row-major in the matrix's dtype, rounded once. */
+int mx_q4_expand(const mx_q4_matrix *m, void *w, long long ld_w, void *stream);
+/* y[t][i] = sum_k W[i][k] x[t][k] for n_vec vectors (rows of x and y, ld_x and ld_y elements apart): what mx_spmv is
+ * for a sparse matrix.  Sums in 32 bits, rounded once at the end. */
+int mx_q4_product(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, void *y, long long ld_y, void *stream);
+/* dx[t][k] = sum_i W[i][k] dy[t][i]: the product with the transposed matrix, which is also the gradient of x. */
+int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long ld_dy, void *dx, long long ld_dx,
+                    void *stream);
+/* Gradients of the matrix's own numbers, G[i][k] = sum_t dy[t][i] x[t][k] (never stored):
+ *     d_scales[i][g] = sum of (codes - zeros)[i][k] G[i][k] over the group's columns,   [n_rows][n_groups]
+ *     d_res_val[e]   = G[row of e][column of e] for every residual entry e < res_row_ptr[n_rows],   [res_cap]
+ * both in the matrix's dtype; either may be NULL.  The matrix's scales and res_val are not read. */
+int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, const void *dy, long long ld_dy,
+               void *d_scales, void *d_res_val, void *stream);
+/* Checks the residual once, on the device: res_row_ptr starts at 0, never decreases and ends inside res_cap, columns lie
+ * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  Synchronises the stream. */
+int mx_q4_check(const mx_q4_matrix *m, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ The package is a thin Python view of ``libmatxtract_b200.so`` (hand-written CUDA
 inspected), but creating a handle without a CUDA device raises.
 """
 from .capi import (  # noqa: F401
+    BF16,
     COLSPACE_AUTO,
     COLSPACE_ORIGINAL,
     COLSPACE_PERMUTED,
@@ -13,6 +14,7 @@ from .capi import (  # noqa: F401
     DD_SE,
     DD_TILE,
     FP16,
+    FP32,
     HOT_AUTO,
     HOT_OFF,
     HOT_ON,
@@ -22,6 +24,7 @@ from .capi import (  # noqa: F401
     mg_partition_rows,
     MxError,
     PartitionStats,
+    Q4Matrix,
     cdspmv,
     du_tcspmv,
     lib,
@@ -30,4 +33,4 @@ from .capi import (  # noqa: F401
 )
 from . import synth  # noqa: F401
 
-__all__ = ["FP16", "FP64", "MatXtract", "MxError", "PartitionStats", "cdspmv", "du_tcspmv", "se_tcspmv", "lib", "read_matrix_market", "synth"]
+__all__ = ["FP16", "FP64", "MatXtract", "MxError", "PartitionStats", "Q4Matrix", "BF16", "FP32", "cdspmv", "du_tcspmv", "se_tcspmv", "lib", "read_matrix_market", "synth"]

@@ -7,6 +7,7 @@ from pathlib import Path
 import numpy as np
 
 FP64, FP16 = 0, 1
+BF16, FP32 = 2, 3  # 4-bit matrices only
 DD_AUTO, DD_TILE, DD_CSR, DD_SE = 0, 1, 2, 3
 COLSPACE_AUTO, COLSPACE_PERMUTED, COLSPACE_ORIGINAL = 0, 1, 2
 HOT_AUTO, HOT_OFF, HOT_ON = 0, 1, 2
@@ -57,6 +58,13 @@ class _PartitionArrays(C.Structure):
 # every symbol include/mx_capi.h declares: name -> (restype, argtypes)
 _vp, _i, _d = C.c_void_p, C.c_int, C.c_double
 _ip = C.POINTER(C.c_int)
+class _Q4Matrix(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("n_cols", C.c_int), ("group", C.c_int), ("dtype", C.c_int), ("device", C.c_int),
+                ("res_cap", C.c_int), ("code_ld", C.c_longlong), ("codes", C.c_void_p), ("scales", C.c_void_p),
+                ("zeros", C.c_void_p), ("res_row_ptr", C.c_void_p), ("res_col_ind", C.c_void_p),
+                ("res_val", C.c_void_p)]
+
+
 SYMBOLS = {
     "mx_version": (_i, []),
     "mx_status_string": (C.c_char_p, [_i]),
@@ -125,6 +133,12 @@ SYMBOLS = {
     "mx_se_tcspmv": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _d, _i, _i, _i, C.POINTER(_d)]),
     "mx_dd_executor_times": (_i, [_vp, C.POINTER(C.c_float), C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "mx_csr_spmv_static": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mx_q4_quantize": (_i, [_vp, _i, _vp, C.c_longlong, C.c_float, _vp]),
+    "mx_q4_expand": (_i, [_vp, _vp, C.c_longlong, _vp]),
+    "mx_q4_product": (_i, [_vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp]),
+    "mx_q4_product_t": (_i, [_vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp]),
+    "mx_q4_grad": (_i, [_vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp, _vp, _vp]),
+    "mx_q4_check": (_i, [_vp, _vp]),
 }
 
 _lib = None
@@ -584,3 +598,116 @@ def csr_spmv_static(dtype, n_rows, n_cols, nnz, row_ptr_dev, col_ind_dev, val_de
     st = lib().mx_csr_spmv_static(dtype, n_rows, n_cols, nnz, _ptr(row_ptr_dev), _ptr(col_ind_dev), _ptr(val_dev),
                                   _ptr(x_dev), _ptr(y_dev), C.c_void_p(stream))
     _raise(st)
+
+
+class Q4Matrix:
+    """A 4-bit matrix with group scales and an optional CSR residual (mx_q4_* of the C ABI): a view of CUDA tensors
+    that the caller owns, kept alive by this object.
+
+    ``codes`` uint8 [n_rows, >= ceil(n_cols / 2)] (rows a multiple of 16 bytes apart), ``scales`` float16 or bfloat16
+    [n_rows, ceil(n_cols / group)], ``zeros`` uint8 of the same shape or None (= 8 everywhere); the residual is
+    ``res_row_ptr`` int32 [n_rows + 1], ``res_col_ind`` int32 and ``res_val`` in the scales' type, or None.
+    Calls run asynchronously on ``stream`` (a cudaStream_t as int; 0 = the default stream) of the tensors' GPU."""
+
+    _TYPES = {"torch.float16": FP16, "torch.bfloat16": BF16, "torch.float32": FP32}
+
+    def __init__(self, n_rows: int, n_cols: int, group: int, codes, scales, zeros=None, res_row_ptr=None,
+                 res_col_ind=None, res_val=None):
+        n_rows, n_cols, group = int(n_rows), int(n_cols), int(group)
+        _need(n_rows >= 0 and n_cols >= 0 and group > 0 and group % 32 == 0, "sizes are not negative, the group a "
+              "positive multiple of 32")
+        n_groups = -(-n_cols // group)
+        self.vdt, self.device = scales.dtype, scales.device
+        _need(str(self.vdt) in ("torch.float16", "torch.bfloat16"), "scales are float16 or bfloat16")
+        self.dtype = self._TYPES[str(self.vdt)]
+        self.n_rows, self.n_cols, self.group = n_rows, n_cols, group
+        self._tensor(scales, "scales", self.vdt, (n_rows, n_groups))
+        _need(codes.dim() == 2 and codes.shape[0] == n_rows and codes.shape[1] >= (n_cols + 1) // 2,
+              "codes: [n_rows, >= ceil(n_cols / 2)] bytes")
+        self._tensor(codes, "codes", "torch.uint8", None)
+        _need(codes.shape[1] <= 1 or codes.stride(1) == 1, "codes of a row are adjacent")
+        code_ld = codes.stride(0) if n_rows > 1 else max(16, -(-codes.shape[1] // 16) * 16)
+        if zeros is not None:
+            self._tensor(zeros, "zeros", "torch.uint8", (n_rows, n_groups))
+        cap = 0
+        if res_row_ptr is not None:
+            _need(res_col_ind is not None and res_val is not None, "a residual has row pointers, columns and values")
+            cap = res_col_ind.numel()
+            self._tensor(res_row_ptr, "res_row_ptr", "torch.int32", (n_rows + 1,))
+            self._tensor(res_col_ind, "res_col_ind", "torch.int32", (cap,))
+            self._tensor(res_val, "res_val", self.vdt, (cap,))
+        # the buffer ends with the last row's codes: a last row that is shorter than code_ld must not be read past it
+        end = codes.storage_offset() + max(0, n_rows - 1) * code_ld + code_ld
+        _need(n_rows == 0 or n_cols == 0 or end <= codes.untyped_storage().nbytes(), "every row of codes, the last one too, has "
+              "code_ld bytes (a multiple of 16)")
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.res_row_ptr, self.res_col_ind, self.res_val = res_row_ptr, res_col_ind, res_val
+        a = _address
+        self._m = _Q4Matrix(n_rows, n_cols, group, self.dtype, self.device.index or 0, cap, code_ld, a(codes),
+                            a(scales), a(zeros), a(res_row_ptr), a(res_col_ind), a(res_val))
+        self._r = C.byref(self._m)
+
+    def _tensor(self, a, name, dtype, shape):
+        _need(str(a.dtype) == str(dtype), f"{name} has type {a.dtype}, not {dtype}")
+        _need(a.device == self.device and a.is_cuda, f"{name} is on {a.device}, the scales on {self.device}")
+        if shape is not None:
+            _need(tuple(a.shape) == shape and a.is_contiguous(), f"{name}: a contiguous {shape} tensor is wanted")
+
+    def _rows(self, a, name, cols, dtype=None):
+        """Leading dimension of a row-major [n, cols] tensor of the matrix's type."""
+        _need(a.dim() == 2 and a.shape[1] == cols, f"{name}: [n, {cols}] is wanted, not {tuple(a.shape)}")
+        _need(a.dtype == (dtype or self.vdt) and a.device == self.device, f"{name}: another type or GPU than the matrix")
+        ld = a.stride(0) if a.shape[0] > 1 else max(cols, 1)
+        _need((cols <= 1 or a.stride(1) == 1) and ld >= cols, f"{name}: the entries of a row are adjacent, rows apart")
+        return ld
+
+    def quantize(self, w, threshold=None, stream=0):
+        """Fills codes, scales, zeros and residual from the dense w [n_rows, n_cols] (float16, bfloat16 or float32);
+        with a residual, entries above ``threshold`` in magnitude go there."""
+        _need(self.res_row_ptr is None or threshold is not None, "a matrix with a residual wants a threshold")
+        _need(str(w.dtype) in self._TYPES and w.shape[0] == self.n_rows, "w: [n_rows, n_cols] of a floating type")
+        ld = self._rows(w, "w", self.n_cols, w.dtype)
+        _raise(lib().mx_q4_quantize(self._r, self._TYPES[str(w.dtype)], w.data_ptr(), ld, threshold or 0.0, stream))
+
+    def expand(self, w, stream=0):
+        """w [n_rows, n_cols] = the dense matrix."""
+        ld = self._rows(w, "w", self.n_cols)
+        _need(w.shape[0] == self.n_rows, "w: [n_rows, n_cols]")
+        _raise(lib().mx_q4_expand(self._r, w.data_ptr(), ld, stream))
+
+    def product(self, x, y, stream=0):
+        """y [n, n_rows] = x [n, n_cols] times the transposed matrix: one product per row of x."""
+        ld_x, ld_y = self._rows(x, "x", self.n_cols), self._rows(y, "y", self.n_rows)
+        _need(x.shape[0] == y.shape[0], "x and y: as many rows")
+        _raise(lib().mx_q4_product(self._r, x.shape[0], x.data_ptr(), ld_x, y.data_ptr(), ld_y, stream))
+
+    def product_t(self, dy, dx, stream=0):
+        """dx [n, n_cols] = dy [n, n_rows] times the matrix: the gradient of ``product``'s x."""
+        ld_dy, ld_dx = self._rows(dy, "dy", self.n_rows), self._rows(dx, "dx", self.n_cols)
+        _need(dx.shape[0] == dy.shape[0], "dy and dx: as many rows")
+        _raise(lib().mx_q4_product_t(self._r, dy.shape[0], dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, stream))
+
+    def grad(self, x, dy, d_scales=None, d_res_val=None, stream=0):
+        """Gradients of the scales and of the residual's values for ``product``'s x and the gradient dy of its y."""
+        ld_x, ld_dy = self._rows(x, "x", self.n_cols), self._rows(dy, "dy", self.n_rows)
+        _need(x.shape[0] == dy.shape[0], "x and dy: as many rows")
+        if d_scales is not None:
+            self._tensor(d_scales, "d_scales", self.vdt, tuple(self.scales.shape))
+        if d_res_val is not None:
+            _need(self.res_val is not None, "d_res_val: the matrix has no residual")
+            self._tensor(d_res_val, "d_res_val", self.vdt, tuple(self.res_val.shape))
+        _raise(lib().mx_q4_grad(self._r, x.shape[0], x.data_ptr(), ld_x, dy.data_ptr(), ld_dy, _address(d_scales),
+                                _address(d_res_val), stream))
+
+    def check(self, stream=0):
+        """Raises when the residual's row pointers or columns are not what the products rely on; waits for the GPU."""
+        _raise(lib().mx_q4_check(self._r, stream))
+
+
+def _need(ok, what):
+    if not ok:
+        raise MxError(1, what)
+
+
+def _address(a):
+    return None if a is None else a.data_ptr()
