@@ -408,7 +408,9 @@ int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long 
 int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, const void *dy, long long ld_dy,
                void *d_scales, void *d_res_val, void *stream);
 /* Checks the residual once, on the device: res_row_ptr starts at 0, never decreases and ends inside res_cap, columns lie
- * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  Synchronises the stream. */
+ * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  MX_ERR_TIMEOUT when a bounded
+ * wait inside an earlier mx_q4_* kernel on this GPU ran out (its results are then not complete).  Synchronises the
+ * stream. */
 int mx_q4_check(const mx_q4_matrix *m, void *stream);
 
 #ifdef __cplusplus

@@ -3,6 +3,7 @@
 
 #include "mx_internal.h"
 #include "q4.h"
+#include "q4_gemm.h"
 
 namespace mx {
 namespace q4 {
@@ -183,23 +184,23 @@ int mx_q4_check(const mx_q4_matrix *m, void *stream) {
     if (!valid(m)) return MX_ERR_INVALID;
     OnDevice on(m->device);
     if (on.status != MX_OK) return on.status;
-    if (!m->res_row_ptr) return MX_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int *flag = nullptr, bad = 0;
+    int *flag = nullptr, bad = 0, late = 0;
     cudaError_t e = cudaMallocAsync((void **)&flag, sizeof(int), s);
     if (e != cudaSuccess) return done(e);
     e = cudaMemsetAsync(flag, 0, sizeof(int), s);
-    if (e == cudaSuccess) {
+    if (e == cudaSuccess && m->res_row_ptr) {
         const int blocks = (int)std::min<long long>(((long long)m->n_rows + 256) / 256, 148 * 8);
         check_kernel<<<blocks, 256, 0, s>>>(m->n_rows, m->n_cols, m->res_cap, m->res_row_ptr, m->res_col_ind, flag);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof(int), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = waits_ran_out(&late, s);
     cudaError_t f = cudaFreeAsync(flag, s);
     if (e == cudaSuccess) e = f;
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return done(e);
-    return bad ? MX_ERR_INVALID : MX_OK;
+    return late ? MX_ERR_TIMEOUT : bad ? MX_ERR_INVALID : MX_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,665 @@
+// Products of a 4-bit matrix with many vectors, and the gradients of its numbers, on the fifth-generation tensor cores.
+//
+// One block computes D[128 x BN] in tensor memory, contraction 64 deep a stage:
+//   product    D[i][t] = sum_k W[i][k] x[t][k]     A = W's rows, depth-major         B = x's rows, depth-major
+//   transposed D[k][t] = sum_i W[i][k] dy[t][i]    A = W's columns, line-major       B = dy's rows, depth-major
+//   gradient   D[i][k] = sum_t dy[t][i] x[t][k]    A = dy's columns, line-major      B = x's columns, line-major
+// x and dy come through tiled bulk copies.  W is made on the way: its codes come through a ring of their own (128 rows x
+// 128 columns = 8 KB each) and two groups of four warps turn them into 16-bit values s * (c - z), rounded once, add the
+// residual's entries that fall into the tile, and store them in the operand's swizzled layout; in this form a tile of W
+// has the same bytes for the product and its transpose, only the operand descriptor differs.  The gradient keeps D and
+// reduces it against the codes in the epilogue: G is never stored.
+// Where there are fewer tiles than SMs, up to eight blocks of a cluster share a tile's contraction and add their parts
+// through distributed shared memory, in the order of their ranks.
+#include <limits.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "q4.h"
+#include "q4_gemm.h"
+#include "q4_ptx.cuh"
+
+namespace mx {
+namespace q4 {
+namespace {
+
+enum { PRODUCT, TRANSPOSED, GRADIENT };
+
+constexpr int THREADS = 384;          // copies of B, tensor core issue, copies of codes, spare; two groups of four warps
+constexpr int CODE_TILE = 128 * 64;   // bytes of 128 x 128 codes
+constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
+constexpr int LOADERS = 64;           // threads that fetch x and dy where bulk copies cannot
+
+template <int MODE, int BN>
+struct Shape {
+    static constexpr int STAGE = A_BYTES + BN * 128;
+    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 3 : BN == 128 ? 6 : 12;
+    static constexpr int STAGES = BN == 128 ? 5 : 4;
+    static constexpr int SUMS = MODE == GRADIENT ? 2 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
+    static constexpr int BARS = 3 * STAGES + 2 * CODES + 2;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SUMS + BARS * 8;
+    static_assert(SMEM <= 227 * 1024, "shared memory of one block");
+    static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
+};
+
+template <typename V>
+struct Args {
+    Matrix<V> m;
+    int n_vec, tiles_m, splits;
+    const V *a, *b;  // dy and x as operands A and B, for the loads that bulk copies cannot do
+    long long ld_a, ld_b;
+    V *out;
+    long long ld_out;
+    V *d_res;
+    int groups_per_unit;  // gradient: groups that one block owns
+};
+
+__device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
+
+template <typename V>
+struct Pair;
+template <>
+struct Pair<__half> {
+    using T = __half2;
+    // 1024 + c is exact in the type; so is (1024 + 16 c) / 16
+    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) {
+        const uint32_t base = 0x6400u | z, low = 0xD400u | z << 4;  // 1024 + z, -(64 + z)
+        const T zz = bits(base | base << 16), zl = bits(low | low << 16), sixteenth = bits(0x2C002C00u);
+        p[0] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
+        p[1] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+        w >>= 8;
+        p[2] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
+        p[3] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+    }
+    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
+    static __device__ __forceinline__ T both(__half v) { return __half2half2(v); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    using T = __nv_bfloat162;
+    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) {  // 128 + c is exact in the type
+        const uint32_t base = 0x4300u | z;
+        const T zz = bits(base | base << 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __hsub2(bits((w >> 4 * j & 0x000F000Fu) | 0x43004300u), zz);
+    }
+    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
+    static __device__ __forceinline__ T both(__nv_bfloat16 v) { return __bfloat162bfloat162(v); }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t raw(T v) { return *reinterpret_cast<uint32_t *>(&v); }
+
+// eight codes -> eight values in order; codes j and j + 4 sit in one register until the end
+template <typename V>
+__device__ __forceinline__ uint4 values(uint32_t w, typename Pair<V>::T s, int z) {
+    typename Pair<V>::T p[4];
+    Pair<V>::steps(w, z, p);
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = raw(__hmul2(p[j], s));
+    return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410),
+                      __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
+}
+
+// scale and zero point of the two halves of 64 columns
+template <typename V>
+struct Scales {
+    V s[2];
+    int z[2];
+    __device__ __forceinline__ void load(const Matrix<V> &m, int i, int k) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            s[j] = from_float<V>(0.f);
+            z[j] = 8;
+        }
+        if (i >= m.n_rows || k >= m.n_cols) return;
+        const int g0 = k / m.group, g1 = min(k + 32, m.n_cols - 1) / m.group;
+        const long long at = (long long)i * m.n_groups;
+        s[0] = m.scales[at + g0];
+        s[1] = g1 == g0 ? s[0] : m.scales[at + g1];
+        if (m.zeros) {
+            z[0] = m.zeros[at + g0] & 15;
+            z[1] = g1 == g0 ? z[0] : m.zeros[at + g1] & 15;
+        }
+    }
+};
+
+// entries of one row, columns ascending, the next two already loaded
+template <typename V>
+struct Cursor {
+    int at = 0, end = 0, col[2];
+    V val[2];
+    __device__ __forceinline__ void fetch(const Matrix<V> &m, int j) {
+        const int p = at + j;
+        col[j] = p < end ? m.res_col[p] : 0x7fffffff;
+        val[j] = p < end ? m.res_val[p] : from_float<V>(0.f);
+    }
+    __device__ __forceinline__ void start(const Matrix<V> &m, int i, int k) {
+        at = end = 0;
+        if (m.res_ptr && i < m.n_rows) {
+            res_range(m, i, at, end);
+            at = first_at_least(m.res_col, at, end, k);
+        }
+        fetch(m, 0);
+        fetch(m, 1);
+    }
+    __device__ __forceinline__ void next(const Matrix<V> &m) {
+        ++at;
+        col[0] = col[1];
+        val[0] = val[1];
+        fetch(m, 1);
+    }
+};
+
+// `rows` rows of 64 columns from (row, col) on into a swizzled tile, zero outside; `threads` threads
+template <typename V>
+__device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n_rows, long long n_cols, long long row,
+                           long long col, int rows, int thread, int threads) {
+    for (int c = thread; c < rows * 8; c += threads) {
+        const int r = c / 8, j = c % 8;
+        V v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const long long k = col + j * 8 + e;
+            v[e] = row + r < n_rows && k < n_cols ? src[(row + r) * ld + k] : from_float<V>(0.f);
+        }
+        *reinterpret_cast<uint4 *>(dst + r * 128 + ((j ^ r & 7) << 4)) = *reinterpret_cast<uint4 *>(v);
+    }
+}
+
+template <typename V, int MODE, int BN, bool TMA>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
+                const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
+    using S = Shape<MODE, BN>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_shared;
+    __shared__ volatile int failed;
+    uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t base = smem_addr(smem);
+    uint8_t *codes_at = smem + S::STAGES * S::STAGE;
+    float *sums = reinterpret_cast<float *>(codes_at + S::CODES * CODE_TILE);
+    const uint32_t bars = smem_addr(sums) + S::SUMS;
+    auto b_full = [&](int s) { return bars + 8 * s; };
+    auto a_full = [&](int s) { return bars + 8 * (S::STAGES + s); };
+    auto empty = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
+    auto c_full = [&](int s) { return bars + 8 * (3 * S::STAGES + s); };
+    auto c_empty = [&](int s) { return bars + 8 * (3 * S::STAGES + S::CODES + s); };
+    const uint32_t done = bars + 8 * (3 * S::STAGES + 2 * S::CODES), drained = done + 8;
+    constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
+
+    const Matrix<V> &m = g.m;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = g.splits > 1 ? (int)cluster_rank() : 0;
+    const int tile = blockIdx.x / g.splits;
+    const int line0 = tile % g.tiles_m * 128;  // first row of D: a row of W, or a column for the transposed product
+    const int unit = tile / g.tiles_m;
+
+    // what is contracted, in steps of 64: columns, rows or vectors
+    const int depth = MODE == PRODUCT ? m.n_cols : MODE == TRANSPOSED ? m.n_rows : g.n_vec;
+    const int blocks128 = (int)(((long long)depth + 127) / 128);
+    const int block0 = (int)((long long)blocks128 * rank / g.splits);
+    const int blocks = (int)((long long)blocks128 * (rank + 1) / g.splits) - block0;
+    const int steps = MODE == GRADIENT ? (depth + 63) / 64 : 2 * blocks;
+    // columns of D: vectors, or for the gradient the columns of a whole number of groups, in turns of BN
+    const int col0 = MODE == GRADIENT ? unit * g.groups_per_unit * m.group : unit * BN;
+    const int col_end = MODE == GRADIENT
+                            ? (int)min((long long)m.n_cols, col0 + (long long)g.groups_per_unit * m.group)
+                            : min(g.n_vec, col0 + BN);
+    const int turns = MODE == GRADIENT ? (col_end - col0 + BN - 1) / BN : 1;
+    const long long polls = (1ll << 22) + 64ll * steps;
+
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(b_full(s), TMA ? 1 : LOADERS / 32);
+            mbar_init(a_full(s), 4);
+            mbar_init(empty(s), 1);
+        }
+        for (int s = 0; s < S::CODES; ++s) {
+            mbar_init(c_full(s), 1);
+            mbar_init(c_empty(s), 8);
+        }
+        mbar_init(done, 1);
+        mbar_init(drained, 8);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_addr(&tmem_shared), COLUMNS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_shared;
+
+    if (TMA && warp == 0 && lane == 0) {  // ---- x and dy through bulk copies
+        int n = 0;
+        bool ok = true;
+        for (int turn = 0; turn < turns && ok; ++turn) {
+            for (int step = 0; step < steps; ++step, ++n) {
+                const int s = n % S::STAGES;
+                if (!(ok = mbar_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
+                const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
+                if (MODE == GRADIENT) {
+                    mbar_expect(b_full(s), S::STAGE);
+                    for (int j = 0; j < 2; ++j)
+                        tma_load(a + j * 8192, &map_a, line0 + 64 * j, step * 64, b_full(s));
+                    for (int j = 0; j < BN / 64; ++j)
+                        tma_load(b + j * 8192, &map_b, col0 + turn * BN + 64 * j, step * 64, b_full(s));
+                } else {
+                    mbar_expect(b_full(s), BN * 128);
+                    tma_load(b, &map_b, block0 * 128 + step * 64, col0, b_full(s));
+                }
+            }
+        }
+        if (!ok) {  // nothing of this block may still be on its way when it ends
+            failed = 1;
+            for (int k = max(0, n - S::STAGES); k < n; ++k)
+                mbar_wait(b_full(k % S::STAGES), k / S::STAGES & 1, polls);
+        }
+    } else if (!TMA && (warp == 0 || warp == 3)) {  // ---- the same with ordinary loads, where rows lie on any border
+        const int t = (warp == 3) * 32 + lane;
+        int n = 0;
+        bool ok = true;
+        for (int turn = 0; turn < turns && ok; ++turn) {
+            for (int step = 0; step < steps; ++step, ++n) {
+                const int s = n % S::STAGES;
+                if (!(ok = mbar_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
+                uint8_t *a = smem + s * S::STAGE, *b = a + A_BYTES;
+                if (MODE == GRADIENT) {
+                    for (int j = 0; j < 2; ++j)
+                        plain_tile(a + j * 8192, g.a, g.ld_a, g.n_vec, m.n_rows, step * 64ll, line0 + 64ll * j, 64, t,
+                                   LOADERS);
+                    for (int j = 0; j < BN / 64; ++j)
+                        plain_tile(b + j * 8192, g.b, g.ld_b, g.n_vec, m.n_cols, step * 64ll,
+                                   col0 + (long long)turn * BN + 64 * j, 64, t, LOADERS);
+                } else {
+                    plain_tile(b, g.b, g.ld_b, g.n_vec, depth, col0, block0 * 128ll + step * 64, BN, t, LOADERS);
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_full(s));
+            }
+        }
+        if (!ok) failed = 1;
+    } else if (warp == 1 && lane == 0) {  // ---- tensor cores
+        constexpr bool BF16 = sizeof(V) == 2 && !std::is_same<V, __half>::value;
+        constexpr uint32_t idesc = mma_shape(BF16, BN, MODE != PRODUCT, MODE == GRADIENT);
+        int n = 0;
+        bool ok = true;
+        for (int turn = 0; turn < turns && ok; ++turn) {
+            if (turn > 0) {
+                if (!(ok = mbar_wait(drained, (turn - 1) & 1, polls))) break;
+                tc_fence_after();
+            }
+            for (int step = 0; step < steps; ++step, ++n) {
+                const int s = n % S::STAGES;
+                const uint32_t parity = n / S::STAGES & 1;
+                ok = mbar_wait(b_full(s), parity, polls) &&
+                     (MODE == GRADIENT || mbar_wait(a_full(s), parity, polls));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // 16 of the depth: 32 bytes of each row, or 16 rows of 128 bytes
+                    const uint64_t da = MODE == PRODUCT ? operand(a + 32 * j, 16, 1024) : operand(a + 2048 * j, 8192, 1024);
+                    const uint64_t db = MODE == GRADIENT ? operand(b + 2048 * j, 8192, 1024) : operand(b + 32 * j, 16, 1024);
+                    tc_mma(tmem, da, db, idesc, step > 0 || j > 0);
+                }
+                tc_commit(empty(s));
+            }
+            tc_commit(done);
+        }
+        if (!ok) {
+            failed = 1;
+            tc_commit(done);
+        }
+    } else if (MODE != GRADIENT && warp == 2 && lane == 0) {  // ---- codes
+        int n = 0;
+        bool ok = true;
+        for (; n < blocks; ++n) {
+            const int s = n % max(S::CODES, 1);
+            if (!(ok = mbar_wait(c_empty(s), (n / max(S::CODES, 1) & 1) ^ 1, polls))) break;
+            mbar_expect(c_full(s), CODE_TILE);
+            const int at = (block0 + n) * 128;
+            tma_load(smem_addr(codes_at) + s * CODE_TILE, &map_codes, (MODE == PRODUCT ? at : line0) / 2,
+                     MODE == PRODUCT ? line0 : at, c_full(s));
+        }
+        if (!ok) {
+            failed = 1;
+            for (int k = max(0, n - S::CODES); k < n; ++k)
+                mbar_wait(c_full(k % max(S::CODES, 1)), k / max(S::CODES, 1) & 1, polls);
+        }
+    } else if (MODE != GRADIENT && warp >= 4) {  // ---- codes -> 16-bit values
+        const int half = (warp - 4) / 4, t = threadIdx.x - 128 - 128 * half;
+        // this thread's 64 values: a row of the tile (product), or half of one of its own group's 64 rows (transposed)
+        const int tile_row = MODE == PRODUCT ? t : 64 * half + t % 64;
+        const int part = MODE == PRODUCT ? half : t / 64;
+        const int out_row = MODE == PRODUCT ? t : t % 64;
+        const int out_block = MODE == PRODUCT ? 0 : t / 64 * 8192;
+        auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + tile_row : (block0 + n) * 128 + tile_row; };
+        auto col_at = [&](int n) { return (MODE == PRODUCT ? (block0 + n) * 128 : line0) + 64 * part; };
+        Scales<V> next;
+        Cursor<V> cursor;
+        if (blocks > 0) {
+            next.load(m, row_at(0), col_at(0));
+            if (MODE == PRODUCT) cursor.start(m, row_at(0), col_at(0));
+        }
+        bool ok = true;
+        for (int n = 0; n < blocks; ++n) {
+            const Scales<V> now = next;
+            if (n + 1 < blocks) next.load(m, row_at(n + 1), col_at(n + 1));
+            const int cs = n % max(S::CODES, 1), step = 2 * n + half, s = step % S::STAGES;
+            if (!(ok = mbar_wait(c_full(cs), n / max(S::CODES, 1) & 1, polls))) break;
+            uint4 c[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                c[j] = *reinterpret_cast<const uint4 *>(codes_at + cs * CODE_TILE + tile_row * 64 +
+                                                        ((2 * part + j ^ tile_row >> 1 & 3) << 4));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c_empty(cs));
+            if (!(ok = mbar_wait(empty(s), (step / S::STAGES & 1) ^ 1, polls))) break;
+            uint8_t *a = smem + s * S::STAGE + out_block + out_row * 128;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const typename Pair<V>::T sc = Pair<V>::both(now.s[j]);
+                const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], sc, now.z[j]);
+            }
+            if (m.res_ptr) {
+                const int k0 = col_at(n);
+                if (MODE == TRANSPOSED) cursor.start(m, row_at(n), k0);
+                while (cursor.col[0] < min(k0 + 64, m.n_cols)) {
+                    const int k = cursor.col[0] - k0;
+                    if (k >= 0) {
+                        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
+                        *e = from_float<V>(to_float(*e) + to_float(cursor.val[0]));
+                    }
+                    cursor.next(m);
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_full(s));
+        }
+        if (!ok) failed = 1;
+    }
+    __syncwarp();
+
+    // ---- D leaves tensor memory: warps 4-7 and 8-11 hold the four quarters of its rows, each a half of its columns
+    const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;
+    const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+    if (MODE != GRADIENT) {
+        const int line = line0 + row, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
+        bool ok = false;
+        if (warp >= 4) {
+            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, polls) && !failed);
+            if (!ok) failed = 1;
+            tc_fence_after();
+        }
+        float v[32];
+        if (ok) {
+            for (int c = 32 * half; c < BN; c += 64) {
+                if (steps > 0) {
+                    tmem_load32(quarter + c, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                }
+                if (g.splits == 1) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (line < lines && col0 + c + j < col_end)
+                            g.out[(col0 + c + j) * g.ld_out + line] = from_float<V>(v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) reinterpret_cast<float *>(smem)[(c + j) * 128 + row] = v[j];
+                }
+            }
+        }
+        if (g.splits > 1) {
+            __syncwarp();
+            cluster_barrier();
+            if (ok) {
+                const int width = BN / g.splits;
+                for (int j = half; j < width; j += 2) {
+                    const int c = rank * width + j;
+                    const uint32_t at = base + (c * 128 + row) * 4;
+                    float sum = 0.f;
+                    for (int p = 0; p < g.splits; ++p) sum += cluster_load(at, p);
+                    if (line < lines && col0 + c < col_end) g.out[(col0 + c) * g.ld_out + line] = from_float<V>(sum);
+                }
+            }
+            __syncwarp();
+            cluster_barrier();
+        }
+    } else if (warp >= 4) {
+        const int i = line0 + row;
+        const bool real = i < m.n_rows;
+        float *mine = sums + half * 8 * 128 + row;  // [group of the unit][row], one per half
+        for (int j = 0; j < 8; ++j) mine[j * 128] = 0.f;
+        Cursor<V> cursor;
+        bool ok = true;
+        for (int turn = 0; turn < turns; ++turn) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(done, turn & 1, polls) && !failed))) break;
+            tc_fence_after();
+            const int from = col0 + turn * BN + half * (BN / 2), to = min(from + BN / 2, col_end);
+            if (g.d_res) cursor.start(m, i, from);
+            for (int k = from; k < to; k += 32) {
+                float v[32];
+                if (steps > 0) {
+                    tmem_load32(quarter + (k - col0 - turn * BN), v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                }
+                if (real && g.out) {
+                    // codes behind the last column take part with G = 0
+                    const uint4 c = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
+                    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+                    const float z = 8388608.f + zero_of(m, i, k / m.group);
+                    float part = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)  // c - z through 2^23 + c, exact
+                        part = fmaf(__uint_as_float(0x4B000000u | (w[j / 8] >> 4 * (j % 8) & 15)) - z, v[j], part);
+                    mine[(k - col0) / m.group * 128] += part;
+                }
+                if (real && g.d_res) {
+                    while (cursor.col[0] < min(k + 32, to)) {
+                        const int d = cursor.col[0] - k;
+                        float e = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) e = j == d ? v[j] : e;
+                        if (d >= 0) g.d_res[cursor.at] = from_float<V>(e);
+                        cursor.next(m);
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained);
+        }
+        if (!ok) failed = 1;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight warps of the epilogue
+        if (ok && real && g.out && half == 0) {
+            const int g0 = col0 / m.group, n = min(g.groups_per_unit, m.n_groups - g0);
+            for (int j = 0; j < n; ++j)
+                g.out[(long long)i * m.n_groups + g0 + j] = from_float<V>(mine[j * 128] + mine[(8 + j) * 128]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (threadIdx.x == 0 && failed) wait_ran_out = 1;
+    if (warp == 1) tmem_free(tmem, COLUMNS);
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                            const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static const Encode f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<Encode>(p);
+    }();
+    return f;
+}
+
+bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t cols, uint64_t rows, uint64_t ld_bytes,
+            uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld_bytes};
+    const cuuint32_t box[2] = {box_cols, box_rows}, ones[2] = {1, 1};
+    return encoder() && encoder()(map, type, 2, const_cast<void *>(p), dims, strides, box, ones,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename V>
+bool encode_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows) {
+    return encode(map, std::is_same<V, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  p, cols, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// rows that bulk copies can fetch: base and distance on 16-byte borders
+template <typename V>
+bool bulk_rows(const V *p, long long ld, int rows) { return (uintptr_t)p % 16 == 0 && (ld % 8 == 0 || rows == 1); }
+
+template <typename V, int MODE, int BN, bool TMA>
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtensorMap &b, const Args<V> &g,
+                   long long tiles, cudaStream_t s) {
+    if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
+    auto kernel = gemm_kernel<V, MODE, BN, TMA>;
+    constexpr int bytes = Shape<MODE, BN>::SMEM;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * g.splits));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = g.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, codes, a, b, g);
+}
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// Width of a tile and number of blocks that share its contraction.
+void plan(int lines, int depth, int n_vec, int &bn, int &splits) {
+    const long long m_tiles = ceil_div(lines, 128), blocks = std::max<long long>(ceil_div(depth, 128), 1);
+    double best = 0;
+    for (int w : {32, 64, 128, 256}) {
+        for (int s = 1; s <= 8; s *= 2) {
+            if (s > blocks) break;
+            const long long tiles = m_tiles * ceil_div(n_vec, w);
+            const double waves = (double)ceil_div(tiles * s, 148);
+            const double cost = waves * (ceil_div(blocks, s) * (double)std::max(2 * 2 * w, 400) + 3000 + 8 * w + (s > 1 ? 1500 : 0));
+            if (best == 0 || cost < best) {
+                best = cost;
+                bn = w;
+                splits = s;
+            }
+        }
+    }
+}
+
+template <typename V, int MODE>
+cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, V *out, long long ld_out, cudaStream_t s) {
+    const int lines = MODE == PRODUCT ? m.n_rows : m.n_cols, depth = MODE == PRODUCT ? m.n_cols : m.n_rows;
+    const bool tma = bulk_rows(b, ld_b, n_vec) && depth > 0;
+    Args<V> g = {};
+    g.m = m;
+    g.n_vec = n_vec;
+    g.b = b;
+    g.ld_b = ld_b;
+    g.out = out;
+    g.ld_out = ld_out;
+    g.tiles_m = (int)ceil_div(lines, 128);
+    int bn = 128;
+    g.splits = 1;
+    if (tma) plan(lines, depth, n_vec, bn, g.splits);
+    CUtensorMap codes = {}, vectors = {};
+    if (depth > 0) {
+        if (!encode(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, m.codes, ceil_div(m.n_cols, 32) * 16, m.n_rows, m.code_ld, 64,
+                    128, CU_TENSOR_MAP_SWIZZLE_64B))
+            return cudaErrorInvalidValue;
+        if (tma && !encode_vectors(&vectors, b, depth, n_vec, n_vec == 1 ? ceil_div(depth, 8) * 8 : ld_b, bn))
+            return cudaErrorInvalidValue;
+    }
+    const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
+    if (!tma) return launch<V, MODE, 128, false>(codes, codes, vectors, g, tiles, s);
+    switch (bn) {
+        case 32: return launch<V, MODE, 32, true>(codes, codes, vectors, g, tiles, s);
+        case 64: return launch<V, MODE, 64, true>(codes, codes, vectors, g, tiles, s);
+        case 128: return launch<V, MODE, 128, true>(codes, codes, vectors, g, tiles, s);
+        default: return launch<V, MODE, 256, true>(codes, codes, vectors, g, tiles, s);
+    }
+}
+
+}  // namespace
+
+template <typename V>
+cudaError_t product_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
+    return tiles_of<V, PRODUCT>(m, n_vec, x, ld_x, y, ld_y, s);
+}
+
+template <typename V>
+cudaError_t product_t_many(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
+                           cudaStream_t s) {
+    return tiles_of<V, TRANSPOSED>(m, n_vec, dy, ld_dy, dx, ld_dx, s);
+}
+
+template <typename V>
+cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy,
+                      V *d_scales, V *d_res, cudaStream_t s) {
+    const bool tma = n_vec > 0 && bulk_rows(x, ld_x, n_vec) && bulk_rows(dy, ld_dy, n_vec);
+    Args<V> g = {};
+    g.m = m;
+    g.n_vec = n_vec;
+    g.a = dy;
+    g.ld_a = ld_dy;
+    g.b = x;
+    g.ld_b = ld_x;
+    g.out = d_scales;
+    g.d_res = m.res_ptr ? d_res : nullptr;
+    g.tiles_m = (int)ceil_div(m.n_rows, 128);
+    g.splits = 1;
+    g.groups_per_unit = std::max(1, 256 / m.group);
+    CUtensorMap a = {}, b = {};
+    if (tma && (!encode_vectors(&a, dy, m.n_rows, n_vec, n_vec == 1 ? ceil_div(m.n_rows, 8) * 8 : ld_dy, 64) ||
+                !encode_vectors(&b, x, m.n_cols, n_vec, n_vec == 1 ? ceil_div(m.n_cols, 8) * 8 : ld_x, 64)))
+        return cudaErrorInvalidValue;
+    const long long tiles = g.tiles_m * ceil_div(m.n_groups, g.groups_per_unit);
+    return tma ? launch<V, GRADIENT, 256, true>(a, a, b, g, tiles, s) : launch<V, GRADIENT, 256, false>(a, a, b, g, tiles, s);
+}
+
+cudaError_t waits_ran_out(int *flag, cudaStream_t s) {
+    void *p = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out);
+    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
+}
+
+#define INSTANTIATE(V)                                                                                             \
+    template cudaError_t product_many<V>(const Matrix<V> &, int, const V *, long long, V *, long long, cudaStream_t); \
+    template cudaError_t product_t_many<V>(const Matrix<V> &, int, const V *, long long, V *, long long,           \
+                                           cudaStream_t);                                                         \
+    template cudaError_t grad_many<V>(const Matrix<V> &, int, const V *, long long, const V *, long long, V *, V *, \
+                                      cudaStream_t);
+INSTANTIATE(__half)
+INSTANTIATE(__nv_bfloat16)
+
+}  // namespace q4
+}  // namespace mx

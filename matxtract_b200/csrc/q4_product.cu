@@ -1,11 +1,13 @@
 // Products with a 4-bit matrix and the gradients of its numbers, straight from the definitions.
 #include "q4.h"
+#include "q4_gemm.h"
 
 namespace mx {
 namespace q4 {
 namespace {
 
 constexpr int WARPS = 8;
+constexpr int FEW = 8;  // vectors up to which these kernels run; the tensor core kernels' tiles are wider
 
 template <typename V>
 __device__ __forceinline__ int step_at(const Matrix<V> &m, int i, int k) {
@@ -105,6 +107,7 @@ unsigned blocks_for(long long units, int per_block) { return (unsigned)((units +
 
 template <typename V>
 cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
+    if (n_vec > FEW) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
     product_kernel<<<blocks_for((long long)m.n_rows * n_vec, WARPS), 32 * WARPS, 0, s>>>(m, n_vec, x, ld_x, y, ld_y);
     return cudaGetLastError();
 }
@@ -112,6 +115,7 @@ cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V
 template <typename V>
 cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
                       cudaStream_t s) {
+    if (n_vec > FEW) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
     product_t_kernel<<<blocks_for((long long)m.n_cols * n_vec, 256), 256, 0, s>>>(m, n_vec, dy, ld_dy, dx, ld_dx);
     return cudaGetLastError();
 }
@@ -119,6 +123,7 @@ cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_d
 template <typename V>
 cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy, V *d_scales,
                  V *d_res, cudaStream_t s) {
+    if (n_vec > FEW) return grad_many(m, n_vec, x, ld_x, dy, ld_dy, d_scales, d_res, s);
     if (d_scales)
         grad_scales_kernel<<<blocks_for((long long)m.n_rows * m.n_groups, WARPS), 32 * WARPS, 0, s>>>(
             m, n_vec, x, ld_x, dy, ld_dy, d_scales);
