@@ -26,19 +26,27 @@ namespace {
 
 enum { PRODUCT, TRANSPOSED, GRADIENT };
 
-constexpr int THREADS = 384;          // copies of B, tensor core issue, copies of codes, spare; two groups of four warps
+// Warps: 0 copies of x and dy, 1 tensor core issue, 2 copies of codes, 3 spare; then four groups of four warps that turn
+// codes into values and empty the tensor memory; then four warps that look for the residual's entries.
+constexpr int THREADS = 32 * 24;
+constexpr int CONVERT = 4, FIND = 20; // first warps of the latter
 constexpr int CODE_TILE = 128 * 64;   // bytes of 128 x 128 codes
 constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
 constexpr int LOADERS = 64;           // threads that fetch x and dy where bulk copies cannot
+// Lists of a code tile's residual entries, one for each half of it (a stage's A): position in A << 16 | value.
+constexpr int LIST = 128;
+constexpr int LIST_BYTES = 2 * (4 + 4 * LIST);
+constexpr int AHEAD = 4;  // code tiles whose entries are looked for at the same time (transposed)
 
 template <int MODE, int BN>
 struct Shape {
     static constexpr int STAGE = A_BYTES + BN * 128;
-    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 3 : BN == 128 ? 6 : 12;
+    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 6 : 12;
     static constexpr int STAGES = BN == 128 ? 5 : 4;
-    static constexpr int SUMS = MODE == GRADIENT ? 2 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
-    static constexpr int BARS = 3 * STAGES + 2 * CODES + 2;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SUMS + BARS * 8;
+    static constexpr int LISTS = MODE == GRADIENT ? 0 : 8;
+    static constexpr int SUMS = MODE == GRADIENT ? 4 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
+    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2 * LISTS + 2 + 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + LISTS * LIST_BYTES + SUMS + BARS * 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of one block");
     static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
 };
@@ -168,29 +176,41 @@ __device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n
     }
 }
 
+// Entries of the 64 x 64 or 128 x 64 values of one A go into its list as they are found; the order does not matter, since
+// no two have the same place.
+template <typename V>
+__device__ __forceinline__ void list_entry(uint32_t *list, int place, V v) {
+    const uint32_t at = atomicAdd(list, 1u);
+    if (at < LIST) list[1 + at] = (uint32_t)place << 16 | *reinterpret_cast<uint16_t *>(&v);
+}
+__device__ __forceinline__ int place_in_tile(int row, int k) { return row * 64 + ((k / 8 ^ row & 7) << 3) + k % 8; }
+
 template <typename V, int MODE, int BN, bool TMA>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
                 const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
     using S = Shape<MODE, BN>;
+    constexpr int CODES = S::CODES ? S::CODES : 1, LISTS = S::LISTS ? S::LISTS : 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_shared;
     __shared__ volatile int failed;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
-    float *sums = reinterpret_cast<float *>(codes_at + S::CODES * CODE_TILE);
+    uint32_t *lists = reinterpret_cast<uint32_t *>(codes_at + S::CODES * CODE_TILE);
+    float *sums = reinterpret_cast<float *>(lists + S::LISTS * LIST_BYTES / 4);
     const uint32_t bars = smem_addr(sums) + S::SUMS;
-    auto b_full = [&](int s) { return bars + 8 * s; };
-    auto a_full = [&](int s) { return bars + 8 * (S::STAGES + s); };
-    auto empty = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
-    auto c_full = [&](int s) { return bars + 8 * (3 * S::STAGES + s); };
-    auto c_empty = [&](int s) { return bars + 8 * (3 * S::STAGES + S::CODES + s); };
-    const uint32_t done = bars + 8 * (3 * S::STAGES + 2 * S::CODES), drained = done + 8;
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (S::STAGES + s); };
+    auto c_full = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
+    auto c_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + S::CODES + s); };
+    auto l_full = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + s); };
+    auto l_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + S::LISTS + s); };
+    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES + 2 * S::LISTS), drained = done + 8, groups = done + 16;
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
 
     const Matrix<V> &m = g.m;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const int rank = g.splits > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / g.splits;
     const int line0 = tile % g.tiles_m * 128;  // first row of D: a row of W, or a column for the transposed product
@@ -208,21 +228,26 @@ __global__ void __launch_bounds__(THREADS, 1)
                             ? (int)min((long long)m.n_cols, col0 + (long long)g.groups_per_unit * m.group)
                             : min(g.n_vec, col0 + BN);
     const int turns = MODE == GRADIENT ? (col_end - col0 + BN - 1) / BN : 1;
-    const long long polls = (1ll << 22) + 64ll * steps;
+    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
 
     if (threadIdx.x == 0) {
         failed = 0;
         for (int s = 0; s < S::STAGES; ++s) {
-            mbar_init(b_full(s), TMA ? 1 : LOADERS / 32);
-            mbar_init(a_full(s), 4);
+            mbar_init(full(s), (TMA ? 1 : LOADERS / 32) + (MODE == GRADIENT ? 0 : 4));
             mbar_init(empty(s), 1);
         }
         for (int s = 0; s < S::CODES; ++s) {
             mbar_init(c_full(s), 1);
             mbar_init(c_empty(s), 8);
         }
+        for (int s = 0; s < S::LISTS; ++s) {
+            mbar_init(l_full(s), 4);
+            mbar_init(l_empty(s), 8);
+            lists[s * LIST_BYTES / 4] = lists[s * LIST_BYTES / 4 + 1 + LIST] = 0;
+        }
         mbar_init(done, 1);
-        mbar_init(drained, 8);
+        mbar_init(drained, 16);
+        for (int j = 0; j < 4; ++j) mbar_init(groups + 8 * j, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_addr(&tmem_shared), COLUMNS);
@@ -240,21 +265,21 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!(ok = mbar_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
                 const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
                 if (MODE == GRADIENT) {
-                    mbar_expect(b_full(s), S::STAGE);
+                    mbar_expect(full(s), S::STAGE);
                     for (int j = 0; j < 2; ++j)
-                        tma_load(a + j * 8192, &map_a, line0 + 64 * j, step * 64, b_full(s));
+                        tma_load(a + j * 8192, &map_a, line0 + 64 * j, step * 64, full(s));
                     for (int j = 0; j < BN / 64; ++j)
-                        tma_load(b + j * 8192, &map_b, col0 + turn * BN + 64 * j, step * 64, b_full(s));
+                        tma_load(b + j * 8192, &map_b, col0 + turn * BN + 64 * j, step * 64, full(s));
                 } else {
-                    mbar_expect(b_full(s), BN * 128);
-                    tma_load(b, &map_b, block0 * 128 + step * 64, col0, b_full(s));
+                    mbar_expect(full(s), BN * 128);
+                    tma_load(b, &map_b, block0 * 128 + step * 64, col0, full(s));
                 }
             }
         }
         if (!ok) {  // nothing of this block may still be on its way when it ends
             failed = 1;
             for (int k = max(0, n - S::STAGES); k < n; ++k)
-                mbar_wait(b_full(k % S::STAGES), k / S::STAGES & 1, polls);
+                mbar_wait(full(k % S::STAGES), k / S::STAGES & 1, polls);
         }
     } else if (!TMA && (warp == 0 || warp == 3)) {  // ---- the same with ordinary loads, where rows lie on any border
         const int t = (warp == 3) * 32 + lane;
@@ -263,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int turn = 0; turn < turns && ok; ++turn) {
             for (int step = 0; step < steps; ++step, ++n) {
                 const int s = n % S::STAGES;
-                if (!(ok = mbar_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
+                if (!(ok = warp_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
                 uint8_t *a = smem + s * S::STAGE, *b = a + A_BYTES;
                 if (MODE == GRADIENT) {
                     for (int j = 0; j < 2; ++j)
@@ -277,48 +302,53 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 fence_async_shared();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b_full(s));
+                if (lane == 0) mbar_arrive(full(s));
             }
         }
         if (!ok) failed = 1;
-    } else if (warp == 1 && lane == 0) {  // ---- tensor cores
-        constexpr bool BF16 = sizeof(V) == 2 && !std::is_same<V, __half>::value;
+    } else if (warp == 1) {  // ---- tensor cores; the whole warp waits, one lane issues
+        constexpr bool BF16 = !std::is_same<V, __half>::value;
         constexpr uint32_t idesc = mma_shape(BF16, BN, MODE != PRODUCT, MODE == GRADIENT);
-        int n = 0;
+        const uint64_t da0 = MODE == PRODUCT ? operand(base, 16, 1024) : operand(base, 8192, 1024);
+        const uint64_t db0 = MODE == GRADIENT ? operand(base + A_BYTES, 8192, 1024) : operand(base + A_BYTES, 16, 1024);
+        // 16 of the depth, in 16 bytes: 32 bytes of each row, or 16 rows of 128 bytes
+        constexpr uint32_t NEXT_A = (MODE == PRODUCT ? 32 : 2048) / 16, NEXT_B = (MODE == GRADIENT ? 2048 : 32) / 16;
+        int s = 0;
+        uint32_t parity = 0;
         bool ok = true;
         for (int turn = 0; turn < turns && ok; ++turn) {
             if (turn > 0) {
-                if (!(ok = mbar_wait(drained, (turn - 1) & 1, polls))) break;
+                if (!(ok = warp_wait(drained, (turn - 1) & 1, polls))) break;
                 tc_fence_after();
             }
-            for (int step = 0; step < steps; ++step, ++n) {
-                const int s = n % S::STAGES;
-                const uint32_t parity = n / S::STAGES & 1;
-                ok = mbar_wait(b_full(s), parity, polls) &&
-                     (MODE == GRADIENT || mbar_wait(a_full(s), parity, polls));
-                if (!ok) break;
+            for (int step = 0; step < steps; ++step) {
+                if (!(ok = warp_wait(full(s), parity, polls))) break;
                 tc_fence_after();
-                const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
+                const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
+                if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {  // 16 of the depth: 32 bytes of each row, or 16 rows of 128 bytes
-                    const uint64_t da = MODE == PRODUCT ? operand(a + 32 * j, 16, 1024) : operand(a + 2048 * j, 8192, 1024);
-                    const uint64_t db = MODE == GRADIENT ? operand(b + 2048 * j, 8192, 1024) : operand(b + 32 * j, 16, 1024);
-                    tc_mma(tmem, da, db, idesc, step > 0 || j > 0);
+                    for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
+                    tc_commit(empty(s));
                 }
-                tc_commit(empty(s));
+                __syncwarp();
+                if (++s == S::STAGES) {
+                    s = 0;
+                    parity ^= 1;
+                }
             }
-            tc_commit(done);
+            if (ok && elect_one()) tc_commit(done);
+            __syncwarp();
         }
         if (!ok) {
             failed = 1;
-            tc_commit(done);
+            if (elect_one()) tc_commit(done);
         }
     } else if (MODE != GRADIENT && warp == 2 && lane == 0) {  // ---- codes
         int n = 0;
         bool ok = true;
         for (; n < blocks; ++n) {
-            const int s = n % max(S::CODES, 1);
-            if (!(ok = mbar_wait(c_empty(s), (n / max(S::CODES, 1) & 1) ^ 1, polls))) break;
+            const int s = n % CODES;
+            if (!(ok = mbar_wait(c_empty(s), (n / CODES & 1) ^ 1, polls))) break;
             mbar_expect(c_full(s), CODE_TILE);
             const int at = (block0 + n) * 128;
             tma_load(smem_addr(codes_at) + s * CODE_TILE, &map_codes, (MODE == PRODUCT ? at : line0) / 2,
@@ -326,12 +356,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (!ok) {
             failed = 1;
-            for (int k = max(0, n - S::CODES); k < n; ++k)
-                mbar_wait(c_full(k % max(S::CODES, 1)), k / max(S::CODES, 1) & 1, polls);
+            for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k % CODES), k / CODES & 1, polls);
         }
-    } else if (MODE != GRADIENT && warp >= 4) {  // ---- codes -> 16-bit values
-        const int half = (warp - 4) / 4, t = threadIdx.x - 128 - 128 * half;
-        // this thread's 64 values: a row of the tile (product), or half of one of its own group's 64 rows (transposed)
+    } else if (MODE != GRADIENT && warp >= CONVERT && warp < FIND) {  // ---- codes -> 16-bit values
+        // group 0 and 1 take the two halves of the even code tiles, group 2 and 3 those of the odd ones
+        const int group = (warp - CONVERT) / 4, half = group & 1, t = threadIdx.x - 32 * CONVERT - 128 * group;
+        // this thread's 64 values: a row of the tile (product), or half of one of its half's 64 rows (transposed)
         const int tile_row = MODE == PRODUCT ? t : 64 * half + t % 64;
         const int part = MODE == PRODUCT ? half : t / 64;
         const int out_row = MODE == PRODUCT ? t : t % 64;
@@ -339,17 +369,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + tile_row : (block0 + n) * 128 + tile_row; };
         auto col_at = [&](int n) { return (MODE == PRODUCT ? (block0 + n) * 128 : line0) + 64 * part; };
         Scales<V> next;
-        Cursor<V> cursor;
-        if (blocks > 0) {
-            next.load(m, row_at(0), col_at(0));
-            if (MODE == PRODUCT) cursor.start(m, row_at(0), col_at(0));
-        }
+        if (group / 2 < blocks) next.load(m, row_at(group / 2), col_at(group / 2));
         bool ok = true;
-        for (int n = 0; n < blocks; ++n) {
+        for (int n = group / 2; n < blocks; n += 2) {
             const Scales<V> now = next;
-            if (n + 1 < blocks) next.load(m, row_at(n + 1), col_at(n + 1));
-            const int cs = n % max(S::CODES, 1), step = 2 * n + half, s = step % S::STAGES;
-            if (!(ok = mbar_wait(c_full(cs), n / max(S::CODES, 1) & 1, polls))) break;
+            if (n + 2 < blocks) next.load(m, row_at(n + 2), col_at(n + 2));
+            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES, ls = n % LISTS;
+            if (!(ok = warp_wait(c_full(cs), n / CODES & 1, polls))) break;
             uint4 c[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -357,8 +383,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                                                         ((2 * part + j ^ tile_row >> 1 & 3) << 4));
             __syncwarp();
             if (lane == 0) mbar_arrive(c_empty(cs));
-            if (!(ok = mbar_wait(empty(s), (step / S::STAGES & 1) ^ 1, polls))) break;
-            uint8_t *a = smem + s * S::STAGE + out_block + out_row * 128;
+            if (!(ok = warp_wait(empty(s), (step / S::STAGES & 1) ^ 1, polls))) break;
+            uint8_t *tile_a = smem + s * S::STAGE, *a = tile_a + out_block + out_row * 128;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const typename Pair<V>::T sc = Pair<V>::both(now.s[j]);
@@ -368,39 +394,183 @@ __global__ void __launch_bounds__(THREADS, 1)
                     *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], sc, now.z[j]);
             }
             if (m.res_ptr) {
-                const int k0 = col_at(n);
-                if (MODE == TRANSPOSED) cursor.start(m, row_at(n), k0);
-                while (cursor.col[0] < min(k0 + 64, m.n_cols)) {
-                    const int k = cursor.col[0] - k0;
-                    if (k >= 0) {
-                        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
-                        *e = from_float<V>(to_float(*e) + to_float(cursor.val[0]));
+                if (!(ok = warp_wait(l_full(ls), n / LISTS & 1, polls))) break;
+                uint32_t *list = lists + ls * LIST_BYTES / 4 + half * (1 + LIST);
+                const uint32_t count = *reinterpret_cast<volatile uint32_t *>(list);
+                auto add = [&](V *e, V v) { *e = from_float<V>(to_float(*e) + to_float(v)); };
+                __syncwarp();
+                if (lane == 0) mbar_arrive(groups + 8 * group);
+                if (!(ok = warp_wait(groups + 8 * group, n / 2 & 1, polls))) break;  // the group's values are all there
+                if (count <= LIST) {
+                    for (int e = t; e < (int)count; e += 128) {
+                        const uint16_t v = (uint16_t)list[1 + e];
+                        add(reinterpret_cast<V *>(tile_a) + (list[1 + e] >> 16), *reinterpret_cast<const V *>(&v));
                     }
-                    cursor.next(m);
+                } else {  // more than the list holds: every thread looks for its own row's
+                    const int i = row_at(n), k0 = col_at(n);
+                    if (i < m.n_rows) {
+                        int b, e;
+                        res_range(m, i, b, e);
+                        for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
+                            const int k = m.res_col[b] - k0;
+                            if (k < 0 || k >= 64 || k0 + k >= m.n_cols) break;
+                            add(reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2), m.res_val[b]);
+                        }
+                    }
                 }
+                if (t == 0) *list = 0;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(l_empty(ls));
             }
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive(a_full(s));
+            if (lane == 0) mbar_arrive(full(s));
+        }
+        if (!ok) failed = 1;
+    } else if (MODE == PRODUCT && warp >= FIND && m.res_ptr) {  // ---- residual: each thread walks along one row
+        const int t = threadIdx.x - 32 * FIND, i = line0 + t;
+        int at = 0, end = 0;
+        if (i < m.n_rows && blocks > 0) {
+            res_range(m, i, at, end);
+            at = first_at_least(m.res_col, at, end, block0 * 128);
+        }
+        constexpr int WINDOW = 4;  // entries loaded ahead
+        int col[WINDOW];
+        V val[WINDOW];
+#pragma unroll
+        for (int j = 0; j < WINDOW; ++j) {
+            col[j] = at + j < end ? m.res_col[at + j] : INT_MAX;
+            val[j] = at + j < end ? m.res_val[at + j] : from_float<V>(0.f);
+        }
+        bool ok = true;
+        for (int n = 0; n < blocks; ++n) {
+            const int ls = n % LISTS, k0 = (block0 + n) * 128, k1 = min(k0 + 128, m.n_cols);
+            if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) break;
+            uint32_t *list = lists + ls * LIST_BYTES / 4;
+            while (col[0] < k1) {
+                const int k = col[0] - k0;
+                float v = to_float(val[0]);
+                bool again;
+                do {  // a repeated column adds to the same place
+                    ++at;
+#pragma unroll
+                    for (int j = 0; j + 1 < WINDOW; ++j) {
+                        col[j] = col[j + 1];
+                        val[j] = val[j + 1];
+                    }
+                    const int p = at + WINDOW - 1;
+                    col[WINDOW - 1] = p < end ? m.res_col[p] : INT_MAX;
+                    val[WINDOW - 1] = p < end ? m.res_val[p] : from_float<V>(0.f);
+                    again = col[0] == k + k0;
+                    if (again) v += to_float(val[0]);
+                } while (again);
+                if (k >= 0) list_entry(list + k / 64 * (1 + LIST), place_in_tile(t, k % 64), from_float<V>(v));
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l_full(ls));
+        }
+        if (!ok) failed = 1;
+    } else if (MODE == TRANSPOSED && warp >= FIND && m.res_ptr) {
+        // ---- residual: a thread looks up one row of each of AHEAD code tiles, all at the same time
+        const int t = threadIdx.x - 32 * FIND, k0 = line0, k1 = min(line0 + 128, m.n_cols);
+        bool ok = true;
+        for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
+            int lo[AHEAD], end[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = (block0 + n0 + u) * 128 + t;
+                lo[u] = end[u] = 0;
+                if (n0 + u < blocks && i < m.n_rows) res_range(m, i, lo[u], end[u]);
+            }
+            int hi[AHEAD], width = 0;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                hi[u] = end[u];
+                width = max(width, hi[u] - lo[u]);
+            }
+            // the first entry not left of k0 lies in [lo, hi]; three probes a round leave a quarter of it
+            while (__any_sync(0xffffffffu, width > 0)) {
+                int c[AHEAD][3];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        const int p = lo[u] + (int)((long long)(hi[u] - lo[u]) * (q + 1) / 4);
+                        c[u][q] = p < hi[u] ? m.res_col[p] : INT_MAX;
+                    }
+                width = 0;
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const long long w = hi[u] - lo[u];
+                    const int l = lo[u];
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) {
+                        const int p = l + (int)(w * (q + 1) / 4);
+                        if (p < hi[u] && c[u][q] < k0) lo[u] = max(lo[u], p + 1);
+                    }
+#pragma unroll
+                    for (int q = 2; q >= 0; --q) {
+                        const int p = l + (int)(w * (q + 1) / 4);
+                        if (p >= lo[u] && p < hi[u] && c[u][q] >= k0) hi[u] = p;
+                    }
+                    width = max(width, hi[u] - lo[u]);
+                }
+            }
+            int col[AHEAD][2];
+            V val[AHEAD][2];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int p = lo[u] + j;
+                    col[u][j] = p < end[u] ? m.res_col[p] : INT_MAX;
+                    val[u][j] = p < end[u] ? m.res_val[p] : from_float<V>(0.f);
+                }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int n = n0 + u, ls = n % LISTS;
+                if (n >= blocks || !ok) continue;
+                if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) continue;
+                uint32_t *list = lists + ls * LIST_BYTES / 4 + t / 64 * (1 + LIST);
+                while (col[u][0] < k1) {
+                    const int k = col[u][0] - k0;
+                    float v = to_float(val[u][0]);
+                    bool again;
+                    do {
+                        ++lo[u];
+                        col[u][0] = col[u][1];
+                        val[u][0] = val[u][1];
+                        const int p = lo[u] + 1;
+                        col[u][1] = p < end[u] ? m.res_col[p] : INT_MAX;
+                        val[u][1] = p < end[u] ? m.res_val[p] : from_float<V>(0.f);
+                        again = col[u][0] == k + k0;
+                        if (again) v += to_float(val[u][0]);
+                    } while (again);
+                    if (k >= 0) list_entry(list, k / 64 * 4096 + place_in_tile(t % 64, k % 64), from_float<V>(v));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(l_full(ls));
+            }
         }
         if (!ok) failed = 1;
     }
     __syncwarp();
 
-    // ---- D leaves tensor memory: warps 4-7 and 8-11 hold the four quarters of its rows, each a half of its columns
-    const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;
+    // ---- D leaves tensor memory: each group of four warps holds the four quarters of its rows, and every fourth 32 columns
+    const int group = (warp - CONVERT) / 4, row = warp % 4 * 32 + lane;
+    const bool drains = warp >= CONVERT && warp < FIND;
     const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
     if (MODE != GRADIENT) {
         const int line = line0 + row, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
         bool ok = false;
-        if (warp >= 4) {
-            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, polls) && !failed);
+        if (drains) {
+            ok = __all_sync(0xffffffffu, warp_wait(done, 0, polls) && !failed);
             if (!ok) failed = 1;
             tc_fence_after();
         }
         float v[32];
         if (ok) {
-            for (int c = 32 * half; c < BN; c += 64) {
+            for (int c = 32 * group; c < BN; c += 128) {
                 if (steps > 0) {
                     tmem_load32(quarter + c, v);
                 } else {
@@ -423,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             cluster_barrier();
             if (ok) {
                 const int width = BN / g.splits;
-                for (int j = half; j < width; j += 2) {
+                for (int j = group; j < width; j += 4) {
                     const int c = rank * width + j;
                     const uint32_t at = base + (c * 128 + row) * 4;
                     float sum = 0.f;
@@ -434,17 +604,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
             cluster_barrier();
         }
-    } else if (warp >= 4) {
+    } else if (drains) {
         const int i = line0 + row;
         const bool real = i < m.n_rows;
-        float *mine = sums + half * 8 * 128 + row;  // [group of the unit][row], one per half
+        float *mine = sums + group * 8 * 128 + row;  // [group of the unit][row], one for each four warps
         for (int j = 0; j < 8; ++j) mine[j * 128] = 0.f;
         Cursor<V> cursor;
         bool ok = true;
         for (int turn = 0; turn < turns; ++turn) {
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(done, turn & 1, polls) && !failed))) break;
+            if (!(ok = __all_sync(0xffffffffu, warp_wait(done, turn & 1, polls) && !failed))) break;
             tc_fence_after();
-            const int from = col0 + turn * BN + half * (BN / 2), to = min(from + BN / 2, col_end);
+            const int from = col0 + turn * BN + group * (BN / 4), to = min(from + BN / 4, col_end);
             if (g.d_res) cursor.start(m, i, from);
             for (int k = from; k < to; k += 32) {
                 float v[32];
@@ -482,11 +652,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) mbar_arrive(drained);
         }
         if (!ok) failed = 1;
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight warps of the epilogue
-        if (ok && real && g.out && half == 0) {
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sixteen warps of the epilogue
+        if (ok && real && g.out && group == 0) {
             const int g0 = col0 / m.group, n = min(g.groups_per_unit, m.n_groups - g0);
             for (int j = 0; j < n; ++j)
-                g.out[(long long)i * m.n_groups + g0 + j] = from_float<V>(mine[j * 128] + mine[(8 + j) * 128]);
+                g.out[(long long)i * m.n_groups + g0 + j] =
+                    from_float<V>(mine[j * 128] + mine[(8 + j) * 128] + mine[(16 + j) * 128] + mine[(24 + j) * 128]);
         }
     }
     tc_fence_before();

@@ -19,18 +19,32 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
 // Waits until the phase of the given parity is over; false after `polls` polls.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, long long polls) {
-    for (long long n = 0; n < polls; ++n) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
+    if (mbar_try(bar, parity)) return true;
+#pragma unroll 1
+    for (uint32_t n = 0; n < polls; ++n)
+        if (mbar_try(bar, parity)) return true;
     return false;
+}
+// The same for a whole warp, whose lanes get one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, polls));
+}
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p;
 }
 
 // One tile of a two-dimensional tensor map, (x, y) = (column, row); x * element size is a multiple of 16 bytes.
