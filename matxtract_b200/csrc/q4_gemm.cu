@@ -9,7 +9,7 @@
 // residual's entries that fall into the tile, and store them in the operand's swizzled layout; in this form a tile of W
 // has the same bytes for the product and its transpose, only the operand descriptor differs.  The gradient keeps D and
 // reduces it against the codes in the epilogue: G is never stored.
-// Where there are fewer tiles than SMs, up to eight blocks of a cluster share a tile's contraction and add their parts
+// Where there are fewer tiles than SMs, up to four blocks of a cluster share a tile's contraction and add their parts
 // through distributed shared memory, in the order of their ranks.
 #include <limits.h>
 
@@ -160,6 +160,50 @@ struct Cursor {
     }
 };
 
+// N neighbouring entries of a row in registers, loaded together, with the column behind them.  (Entries that
+// move up one by one as they are used would wait for the newest load at every move.)
+template <typename V, int N>
+struct Window {
+    int at, col[N + 1];
+    V val[N];
+    __device__ __forceinline__ void load(const Matrix<V> &m, int from, int end) {
+        at = from;
+#pragma unroll
+        for (int j = 0; j < N + 1; ++j) col[j] = from + j < end ? m.res_col[from + j] : INT_MAX;
+#pragma unroll
+        for (int j = 0; j < N; ++j) val[j] = from + j < end ? m.res_val[from + j] : from_float<V>(0.f);
+    }
+    // calls f(column - k0, value) for the columns in [k0, k1), repeated ones added up; moves on while there may be more
+    template <typename F>
+    __device__ __forceinline__ void each(const Matrix<V> &m, int end, int k0, int k1, F f) {
+        while (true) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int k = col[j];
+                if (k < k0 || k >= k1) continue;
+                if (j > 0 && col[j - 1] == k) continue;  // not the first of its column
+                V v = val[j];
+                if (col[j + 1] == k) {
+                    float sum = to_float(v);
+                    for (int p = at + j + 1; p < end && m.res_col[p] == k; ++p) sum += to_float(m.res_val[p]);
+                    v = from_float<V>(sum);
+                }
+                f(k - k0, v);
+            }
+            if (col[N - 1] >= k1) return;
+            int next = at + N;
+            while (next < end && m.res_col[next] == col[N - 1]) ++next;  // a column's entries stay together
+            load(m, next, end);
+        }
+    }
+    __device__ __forceinline__ int first_not_below(long long k) const {
+        int p = at;
+#pragma unroll
+        for (int j = 0; j < N; ++j) p += col[j] < k;
+        return p;
+    }
+};
+
 // `rows` rows of 64 columns from (row, col) on into a swizzled tile, zero outside; `threads` threads
 template <typename V>
 __device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n_rows, long long n_cols, long long row,
@@ -306,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
         if (!ok) failed = 1;
-    } else if (warp == 1) {  // ---- tensor cores; the whole warp waits, one lane issues
+    } else if (warp == 1 && elect_one()) {  // ---- tensor cores
         constexpr bool BF16 = !std::is_same<V, __half>::value;
         constexpr uint32_t idesc = mma_shape(BF16, BN, MODE != PRODUCT, MODE == GRADIENT);
         const uint64_t da0 = MODE == PRODUCT ? operand(base, 16, 1024) : operand(base, 8192, 1024);
@@ -318,30 +362,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true;
         for (int turn = 0; turn < turns && ok; ++turn) {
             if (turn > 0) {
-                if (!(ok = warp_wait(drained, (turn - 1) & 1, polls))) break;
+                if (!(ok = mbar_wait(drained, (turn - 1) & 1, polls))) break;
                 tc_fence_after();
             }
             for (int step = 0; step < steps; ++step) {
-                if (!(ok = warp_wait(full(s), parity, polls))) break;
+                if (!(ok = mbar_wait(full(s), parity, polls))) break;
                 tc_fence_after();
                 const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
-                if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
-                    tc_commit(empty(s));
-                }
-                __syncwarp();
+                for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
+                tc_commit(empty(s));
                 if (++s == S::STAGES) {
                     s = 0;
                     parity ^= 1;
                 }
             }
-            if (ok && elect_one()) tc_commit(done);
-            __syncwarp();
+            if (ok) tc_commit(done);
         }
         if (!ok) {
             failed = 1;
-            if (elect_one()) tc_commit(done);
+            tc_commit(done);
         }
     } else if (MODE != GRADIENT && warp == 2 && lane == 0) {  // ---- codes
         int n = 0;
@@ -427,64 +467,52 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) mbar_arrive(full(s));
         }
         if (!ok) failed = 1;
-    } else if (MODE == PRODUCT && warp >= FIND && m.res_ptr) {  // ---- residual: each thread walks along one row
+    } else if (MODE == PRODUCT && warp >= FIND && m.res_ptr) {
+        // ---- residual: each thread walks along one row, AHEAD code tiles at a time
         const int t = threadIdx.x - 32 * FIND, i = line0 + t;
         int at = 0, end = 0;
         if (i < m.n_rows && blocks > 0) {
             res_range(m, i, at, end);
             at = first_at_least(m.res_col, at, end, block0 * 128);
         }
-        constexpr int WINDOW = 4;  // entries loaded ahead
-        int col[WINDOW];
-        V val[WINDOW];
-#pragma unroll
-        for (int j = 0; j < WINDOW; ++j) {
-            col[j] = at + j < end ? m.res_col[at + j] : INT_MAX;
-            val[j] = at + j < end ? m.res_val[at + j] : from_float<V>(0.f);
-        }
+        Window<V, 8> w;
         bool ok = true;
-        for (int n = 0; n < blocks; ++n) {
-            const int ls = n % LISTS, k0 = (block0 + n) * 128, k1 = min(k0 + 128, m.n_cols);
-            if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) break;
-            uint32_t *list = lists + ls * LIST_BYTES / 4;
-            while (col[0] < k1) {
-                const int k = col[0] - k0;
-                float v = to_float(val[0]);
-                bool again;
-                do {  // a repeated column adds to the same place
-                    ++at;
+        for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
+            w.load(m, at, end);
 #pragma unroll
-                    for (int j = 0; j + 1 < WINDOW; ++j) {
-                        col[j] = col[j + 1];
-                        val[j] = val[j + 1];
-                    }
-                    const int p = at + WINDOW - 1;
-                    col[WINDOW - 1] = p < end ? m.res_col[p] : INT_MAX;
-                    val[WINDOW - 1] = p < end ? m.res_val[p] : from_float<V>(0.f);
-                    again = col[0] == k + k0;
-                    if (again) v += to_float(val[0]);
-                } while (again);
-                if (k >= 0) list_entry(list + k / 64 * (1 + LIST), place_in_tile(t, k % 64), from_float<V>(v));
+            for (int u = 0; u < AHEAD; ++u) {
+                const int n = n0 + u, ls = n % LISTS, k0 = (block0 + n) * 128;
+                if (n >= blocks || !ok) continue;
+                if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) continue;
+                uint32_t *list = lists + ls * LIST_BYTES / 4;
+                w.each(m, end, k0, min(k0 + 128, m.n_cols), [&](int k, V v) {
+                    list_entry(list + k / 64 * (1 + LIST), place_in_tile(t, k % 64), v);
+                });
+                __syncwarp();
+                if (lane == 0) mbar_arrive(l_full(ls));
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(l_full(ls));
+            at = w.first_not_below(min((long long)(block0 + n0 + AHEAD) * 128, (long long)INT_MAX));
         }
         if (!ok) failed = 1;
     } else if (MODE == TRANSPOSED && warp >= FIND && m.res_ptr) {
         // ---- residual: a thread looks up one row of each of AHEAD code tiles, all at the same time
         const int t = threadIdx.x - 32 * FIND, k0 = line0, k1 = min(line0 + 128, m.n_cols);
+        int begin[AHEAD], end[AHEAD];
+        auto rows = [&](int n0) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const long long i = (block0 + n0 + u) * 128ll + t;
+                begin[u] = end[u] = 0;
+                if (n0 + u < blocks && i < m.n_rows) res_range(m, (int)i, begin[u], end[u]);
+            }
+        };
+        rows(0);
         bool ok = true;
         for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
-            int lo[AHEAD], end[AHEAD];
+            int lo[AHEAD], hi[AHEAD], width = 0;
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int i = (block0 + n0 + u) * 128 + t;
-                lo[u] = end[u] = 0;
-                if (n0 + u < blocks && i < m.n_rows) res_range(m, i, lo[u], end[u]);
-            }
-            int hi[AHEAD], width = 0;
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
+                lo[u] = begin[u];
                 hi[u] = end[u];
                 width = max(width, hi[u] - lo[u]);
             }
@@ -495,59 +523,43 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
                     for (int q = 0; q < 3; ++q) {
-                        const int p = lo[u] + (int)((long long)(hi[u] - lo[u]) * (q + 1) / 4);
+                        const int p = lo[u] + (int)((unsigned)(hi[u] - lo[u]) / 4 * (q + 1));
                         c[u][q] = p < hi[u] ? m.res_col[p] : INT_MAX;
                     }
                 width = 0;
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
-                    const long long w = hi[u] - lo[u];
-                    const int l = lo[u];
+                    const int quarter = (unsigned)(hi[u] - lo[u]) / 4, l = lo[u], h = hi[u];
 #pragma unroll
                     for (int q = 0; q < 3; ++q) {
-                        const int p = l + (int)(w * (q + 1) / 4);
-                        if (p < hi[u] && c[u][q] < k0) lo[u] = max(lo[u], p + 1);
+                        const int p = l + quarter * (q + 1);
+                        if (p < h && c[u][q] < k0) lo[u] = max(lo[u], p + 1);
                     }
 #pragma unroll
                     for (int q = 2; q >= 0; --q) {
-                        const int p = l + (int)(w * (q + 1) / 4);
-                        if (p >= lo[u] && p < hi[u] && c[u][q] >= k0) hi[u] = p;
+                        const int p = l + quarter * (q + 1);
+                        if (p >= lo[u] && p < h && c[u][q] >= k0) hi[u] = p;
                     }
                     width = max(width, hi[u] - lo[u]);
                 }
             }
-            int col[AHEAD][2];
-            V val[AHEAD][2];
+            Window<V, 4> w[AHEAD];
+            int ends[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int p = lo[u] + j;
-                    col[u][j] = p < end[u] ? m.res_col[p] : INT_MAX;
-                    val[u][j] = p < end[u] ? m.res_val[p] : from_float<V>(0.f);
-                }
+            for (int u = 0; u < AHEAD; ++u) {
+                ends[u] = end[u];
+                w[u].load(m, lo[u], end[u]);
+            }
+            rows(n0 + AHEAD);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int n = n0 + u, ls = n % LISTS;
                 if (n >= blocks || !ok) continue;
                 if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) continue;
                 uint32_t *list = lists + ls * LIST_BYTES / 4 + t / 64 * (1 + LIST);
-                while (col[u][0] < k1) {
-                    const int k = col[u][0] - k0;
-                    float v = to_float(val[u][0]);
-                    bool again;
-                    do {
-                        ++lo[u];
-                        col[u][0] = col[u][1];
-                        val[u][0] = val[u][1];
-                        const int p = lo[u] + 1;
-                        col[u][1] = p < end[u] ? m.res_col[p] : INT_MAX;
-                        val[u][1] = p < end[u] ? m.res_val[p] : from_float<V>(0.f);
-                        again = col[u][0] == k + k0;
-                        if (again) v += to_float(val[u][0]);
-                    } while (again);
-                    if (k >= 0) list_entry(list, k / 64 * 4096 + place_in_tile(t % 64, k % 64), from_float<V>(v));
-                }
+                w[u].each(m, ends[u], k0, k1, [&](int k, V v) {
+                    list_entry(list, k / 64 * 4096 + place_in_tile(t % 64, k % 64), v);
+                });
                 __syncwarp();
                 if (lane == 0) mbar_arrive(l_full(ls));
             }
@@ -728,16 +740,19 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Width of a tile and number of blocks that share its contraction.
+// Width of a tile and number of blocks that share its contraction: the choice with the least time by a model in clocks.
+// Measured on 2048 to 8192 rows and columns, 16 to 2048 vectors: a code tile takes 1020 to 1520 clocks (nearly the same
+// for 32 to 128 vectors: the conversion bounds it), a block 11,000 to 14,000 to begin and to end, adding up parts through
+// the cluster 30 a vector.
 void plan(int lines, int depth, int n_vec, int &bn, int &splits) {
     const long long m_tiles = ceil_div(lines, 128), blocks = std::max<long long>(ceil_div(depth, 128), 1);
     double best = 0;
     for (int w : {32, 64, 128, 256}) {
-        for (int s = 1; s <= 8; s *= 2) {
+        for (int s = 1; s <= 4; s *= 2) {
             if (s > blocks) break;
-            const long long tiles = m_tiles * ceil_div(n_vec, w);
-            const double waves = (double)ceil_div(tiles * s, 148);
-            const double cost = waves * (ceil_div(blocks, s) * (double)std::max(2 * 2 * w, 400) + 3000 + 8 * w + (s > 1 ? 1500 : 0));
+            const double per_block = w == 32 ? 1020 : w == 64 ? 1080 : w == 128 ? 1140 : 1520;
+            const double waves = (double)ceil_div(m_tiles * ceil_div(n_vec, w) * s, 148);
+            const double cost = waves * (ceil_div(blocks, s) * per_block + 12000 + (s > 1 ? 30 * w : 0));
             if (best == 0 || cost < best) {
                 best = cost;
                 bn = w;
