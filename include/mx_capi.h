@@ -351,8 +351,8 @@ int mx_csr_spmv_static(int dtype, int n_rows, int n_cols, int nnz, const int *ro
  * (4-bit codes, one scale per `group` consecutive columns of a row) and a CSR residual of the entries that are too
  * large for the codes:
  *     W[i][k] = scales[i][k / group] * (codes[i][k] - zeros[i][k / group]) + R[i][k]
- * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls allocate nothing, keep nothing
- * between calls, are asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured
+ * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls keep nothing between calls (a
+ * workspace comes from the device's stream-ordered pool and goes back to it within the call), are asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured
  * into a graph (mx_q4_check excepted) and leave the calling thread's current device as it was.  Calls on different
  * streams are independent of each other as far as their buffers are.  Results do not depend on anything but the
  * inputs: no sum is taken in an order that varies.  n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do

@@ -14,6 +14,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "q4.h"
@@ -33,20 +34,21 @@ constexpr int CONVERT = 4, FIND = 20; // first warps of the latter
 constexpr int CODE_TILE = 128 * 64;   // bytes of 128 x 128 codes
 constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
 constexpr int LOADERS = 64;           // threads that fetch x and dy where bulk copies cannot
-// Lists of a code tile's residual entries, one for each half of it (a stage's A): position in A << 16 | value.
-constexpr int LIST = 128;
-constexpr int LIST_BYTES = 2 * (4 + 4 * LIST);
-constexpr int AHEAD = 4;  // code tiles whose entries are looked for at the same time (transposed)
+// Where a code tile's residual entries are handed over: four words for each thread that converts 64 of its values, an
+// entry being column << 16 | value.
+constexpr uint32_t NO_ENTRY = 0xffffffffu, TOO_MANY = 0xfffffffeu;
+constexpr int SLOT_BYTES = 256 * 16;
+constexpr int AHEAD = 4;  // code tiles whose entries are fetched together
 
 template <int MODE, int BN>
 struct Shape {
     static constexpr int STAGE = A_BYTES + BN * 128;
     static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 6 : 12;
     static constexpr int STAGES = BN == 128 ? 5 : 4;
-    static constexpr int LISTS = MODE == GRADIENT ? 0 : 8;
+    static constexpr int SLOTS = MODE == GRADIENT ? 0 : 4;
     static constexpr int SUMS = MODE == GRADIENT ? 4 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
-    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2 * LISTS + 2 + 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + LISTS * LIST_BYTES + SUMS + BARS * 8;
+    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2 * SLOTS + 2;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SLOTS * SLOT_BYTES + SUMS + BARS * 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of one block");
     static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
 };
@@ -60,6 +62,7 @@ struct Args {
     V *out;
     long long ld_out;
     V *d_res;
+    const int *starts;    // transposed: [block of 128 columns][row] first residual entry not left of the block
     int groups_per_unit;  // gradient: groups that one block owns
 };
 
@@ -173,28 +176,32 @@ struct Window {
 #pragma unroll
         for (int j = 0; j < N; ++j) val[j] = from + j < end ? m.res_val[from + j] : from_float<V>(0.f);
     }
-    // calls f(column - k0, value) for the columns in [k0, k1), repeated ones added up; moves on while there may be more
-    template <typename F>
-    __device__ __forceinline__ void each(const Matrix<V> &m, int end, int k0, int k1, F f) {
+    // Entries with columns in [k0, k1) into a slot, repeated columns added up; moves on while there may be more.
+    __device__ __forceinline__ void hand_over(const Matrix<V> &m, int end, int k0, int k1, uint4 *slot) {
+        uint32_t *to = reinterpret_cast<uint32_t *>(slot);
+        *slot = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+        int n = 0;
         while (true) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const int k = col[j];
-                if (k < k0 || k >= k1) continue;
-                if (j > 0 && col[j - 1] == k) continue;  // not the first of its column
-                V v = val[j];
-                if (col[j + 1] == k) {
-                    float sum = to_float(v);
-                    for (int p = at + j + 1; p < end && m.res_col[p] == k; ++p) sum += to_float(m.res_val[p]);
-                    v = from_float<V>(sum);
+                if (k >= k0 && k < k1 && !(j > 0 && col[j - 1] == k)) {  // the first of its column
+                    V v = val[j];
+                    if (col[j + 1] == k) {
+                        float sum = to_float(v);
+                        for (int p = at + j + 1; p < end && m.res_col[p] == k; ++p) sum += to_float(m.res_val[p]);
+                        v = from_float<V>(sum);
+                    }
+                    if (n < 4) to[n] = (uint32_t)(k - k0) << 16 | *reinterpret_cast<const uint16_t *>(&v);
+                    ++n;
                 }
-                f(k - k0, v);
             }
-            if (col[N - 1] >= k1) return;
+            if (col[N - 1] >= k1) break;
             int next = at + N;
             while (next < end && m.res_col[next] == col[N - 1]) ++next;  // a column's entries stay together
             load(m, next, end);
         }
+        if (n > 4) to[3] = TOO_MANY;
     }
     __device__ __forceinline__ int first_not_below(long long k) const {
         int p = at;
@@ -220,37 +227,28 @@ __device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n
     }
 }
 
-// Entries of the 64 x 64 or 128 x 64 values of one A go into its list as they are found; the order does not matter, since
-// no two have the same place.
-template <typename V>
-__device__ __forceinline__ void list_entry(uint32_t *list, int place, V v) {
-    const uint32_t at = atomicAdd(list, 1u);
-    if (at < LIST) list[1 + at] = (uint32_t)place << 16 | *reinterpret_cast<uint16_t *>(&v);
-}
-__device__ __forceinline__ int place_in_tile(int row, int k) { return row * 64 + ((k / 8 ^ row & 7) << 3) + k % 8; }
-
 template <typename V, int MODE, int BN, bool TMA>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
                 const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
     using S = Shape<MODE, BN>;
-    constexpr int CODES = S::CODES ? S::CODES : 1, LISTS = S::LISTS ? S::LISTS : 1;
+    constexpr int CODES = S::CODES ? S::CODES : 1, SLOTS = S::SLOTS ? S::SLOTS : 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_shared;
     __shared__ volatile int failed;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
-    uint32_t *lists = reinterpret_cast<uint32_t *>(codes_at + S::CODES * CODE_TILE);
-    float *sums = reinterpret_cast<float *>(lists + S::LISTS * LIST_BYTES / 4);
+    uint4 *slots = reinterpret_cast<uint4 *>(codes_at + S::CODES * CODE_TILE);
+    float *sums = reinterpret_cast<float *>(slots + S::SLOTS * 256);
     const uint32_t bars = smem_addr(sums) + S::SUMS;
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (S::STAGES + s); };
     auto c_full = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
     auto c_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + S::CODES + s); };
-    auto l_full = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + s); };
-    auto l_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + S::LISTS + s); };
-    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES + 2 * S::LISTS), drained = done + 8, groups = done + 16;
+    auto s_full = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + s); };
+    auto s_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + S::SLOTS + s); };
+    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES + 2 * S::SLOTS), drained = done + 8;
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
 
     const Matrix<V> &m = g.m;
@@ -284,14 +282,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(c_full(s), 1);
             mbar_init(c_empty(s), 8);
         }
-        for (int s = 0; s < S::LISTS; ++s) {
-            mbar_init(l_full(s), 4);
-            mbar_init(l_empty(s), 8);
-            lists[s * LIST_BYTES / 4] = lists[s * LIST_BYTES / 4 + 1 + LIST] = 0;
+        for (int s = 0; s < S::SLOTS; ++s) {
+            mbar_init(s_full(s), 4);
+            mbar_init(s_empty(s), 8);
         }
         mbar_init(done, 1);
         mbar_init(drained, 16);
-        for (int j = 0; j < 4; ++j) mbar_init(groups + 8 * j, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_addr(&tmem_shared), COLUMNS);
@@ -414,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int n = group / 2; n < blocks; n += 2) {
             const Scales<V> now = next;
             if (n + 2 < blocks) next.load(m, row_at(n + 2), col_at(n + 2));
-            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES, ls = n % LISTS;
+            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES, ss = n % SLOTS;
             if (!(ok = warp_wait(c_full(cs), n / CODES & 1, polls))) break;
             uint4 c[2];
 #pragma unroll
@@ -434,33 +430,31 @@ __global__ void __launch_bounds__(THREADS, 1)
                     *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], sc, now.z[j]);
             }
             if (m.res_ptr) {
-                if (!(ok = warp_wait(l_full(ls), n / LISTS & 1, polls))) break;
-                uint32_t *list = lists + ls * LIST_BYTES / 4 + half * (1 + LIST);
-                const uint32_t count = *reinterpret_cast<volatile uint32_t *>(list);
-                auto add = [&](V *e, V v) { *e = from_float<V>(to_float(*e) + to_float(v)); };
+                if (!(ok = warp_wait(s_full(ss), n / SLOTS & 1, polls))) break;
+                const uint4 q = slots[ss * 256 + half * 128 + t];
                 __syncwarp();
-                if (lane == 0) mbar_arrive(groups + 8 * group);
-                if (!(ok = warp_wait(groups + 8 * group, n / 2 & 1, polls))) break;  // the group's values are all there
-                if (count <= LIST) {
-                    for (int e = t; e < (int)count; e += 128) {
-                        const uint16_t v = (uint16_t)list[1 + e];
-                        add(reinterpret_cast<V *>(tile_a) + (list[1 + e] >> 16), *reinterpret_cast<const V *>(&v));
+                if (lane == 0) mbar_arrive(s_empty(ss));
+                auto add = [&](int k, V v) {
+                    V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
+                    *e = from_float<V>(to_float(*e) + to_float(v));
+                };
+                if (q.w != TOO_MANY) {
+                    const uint32_t entry[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint16_t v = (uint16_t)entry[j];
+                        if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
                     }
-                } else {  // more than the list holds: every thread looks for its own row's
-                    const int i = row_at(n), k0 = col_at(n);
-                    if (i < m.n_rows) {
-                        int b, e;
-                        res_range(m, i, b, e);
-                        for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
-                            const int k = m.res_col[b] - k0;
-                            if (k < 0 || k >= 64 || k0 + k >= m.n_cols) break;
-                            add(reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2), m.res_val[b]);
-                        }
+                } else {  // this thread looks for its entries itself
+                    const int k0 = col_at(n), k1 = min(k0 + 64, m.n_cols);
+                    int b, e;
+                    res_range(m, row_at(n), b, e);
+                    for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
+                        const int k = m.res_col[b];
+                        if (k < k0 || k >= k1) break;
+                        add(k - k0, m.res_val[b]);
                     }
                 }
-                if (t == 0) *list = 0;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(l_empty(ls));
             }
             fence_async_shared();
             __syncwarp();
@@ -481,87 +475,51 @@ __global__ void __launch_bounds__(THREADS, 1)
             w.load(m, at, end);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int n = n0 + u, ls = n % LISTS, k0 = (block0 + n) * 128;
+                const int n = n0 + u, ss = n % SLOTS, k0 = (block0 + n) * 128;
                 if (n >= blocks || !ok) continue;
-                if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) continue;
-                uint32_t *list = lists + ls * LIST_BYTES / 4;
-                w.each(m, end, k0, min(k0 + 128, m.n_cols), [&](int k, V v) {
-                    list_entry(list + k / 64 * (1 + LIST), place_in_tile(t, k % 64), v);
-                });
+                if (!(ok = warp_wait(s_empty(ss), (n / SLOTS & 1) ^ 1, polls))) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w.hand_over(m, end, k0 + 64 * h, min(k0 + 64 * h + 64, m.n_cols), slots + ss * 256 + h * 128 + t);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(l_full(ls));
+                if (lane == 0) mbar_arrive(s_full(ss));
             }
             at = w.first_not_below(min((long long)(block0 + n0 + AHEAD) * 128, (long long)INT_MAX));
         }
         if (!ok) failed = 1;
     } else if (MODE == TRANSPOSED && warp >= FIND && m.res_ptr) {
-        // ---- residual: a thread looks up one row of each of AHEAD code tiles, all at the same time
-        const int t = threadIdx.x - 32 * FIND, k0 = line0, k1 = min(line0 + 128, m.n_cols);
+        // ---- residual: each thread has one row of every code tile; g.starts tells where its entries begin
+        const int t = threadIdx.x - 32 * FIND, k0 = line0;
+        const int *starts = g.starts + (long long)(line0 / 128) * m.n_rows;
         int begin[AHEAD], end[AHEAD];
-        auto rows = [&](int n0) {
+        auto ranges = [&](int n0) {
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const long long i = (block0 + n0 + u) * 128ll + t;
-                begin[u] = end[u] = 0;
-                if (n0 + u < blocks && i < m.n_rows) res_range(m, (int)i, begin[u], end[u]);
+                const bool real = n0 + u < blocks && i < m.n_rows;
+                begin[u] = real ? starts[i] : 0;
+                end[u] = real ? starts[m.n_rows + i] : 0;
             }
         };
-        rows(0);
+        ranges(0);
         bool ok = true;
         for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
-            int lo[AHEAD], hi[AHEAD], width = 0;
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                lo[u] = begin[u];
-                hi[u] = end[u];
-                width = max(width, hi[u] - lo[u]);
-            }
-            // the first entry not left of k0 lies in [lo, hi]; three probes a round leave a quarter of it
-            while (__any_sync(0xffffffffu, width > 0)) {
-                int c[AHEAD][3];
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        const int p = lo[u] + (int)((unsigned)(hi[u] - lo[u]) / 4 * (q + 1));
-                        c[u][q] = p < hi[u] ? m.res_col[p] : INT_MAX;
-                    }
-                width = 0;
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u) {
-                    const int quarter = (unsigned)(hi[u] - lo[u]) / 4, l = lo[u], h = hi[u];
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) {
-                        const int p = l + quarter * (q + 1);
-                        if (p < h && c[u][q] < k0) lo[u] = max(lo[u], p + 1);
-                    }
-#pragma unroll
-                    for (int q = 2; q >= 0; --q) {
-                        const int p = l + quarter * (q + 1);
-                        if (p >= lo[u] && p < h && c[u][q] >= k0) hi[u] = p;
-                    }
-                    width = max(width, hi[u] - lo[u]);
-                }
-            }
-            Window<V, 4> w[AHEAD];
+            Window<V, 3> w[AHEAD];
             int ends[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                ends[u] = end[u];
-                w[u].load(m, lo[u], end[u]);
-            }
-            rows(n0 + AHEAD);
+            for (int u = 0; u < AHEAD; ++u) w[u].load(m, begin[u], ends[u] = end[u]);
+            ranges(n0 + AHEAD);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int n = n0 + u, ls = n % LISTS;
+                const int n = n0 + u, ss = n % SLOTS;
                 if (n >= blocks || !ok) continue;
-                if (!(ok = warp_wait(l_empty(ls), (n / LISTS & 1) ^ 1, polls))) continue;
-                uint32_t *list = lists + ls * LIST_BYTES / 4 + t / 64 * (1 + LIST);
-                w[u].each(m, ends[u], k0, k1, [&](int k, V v) {
-                    list_entry(list, k / 64 * 4096 + place_in_tile(t % 64, k % 64), v);
-                });
+                if (!(ok = warp_wait(s_empty(ss), (n / SLOTS & 1) ^ 1, polls))) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w[u].hand_over(m, ends[u], k0 + 64 * h, min(k0 + 64 * h + 64, m.n_cols),
+                                   slots + ss * 256 + t / 64 * 128 + h * 64 + t % 64);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(l_full(ls));
+                if (lane == 0) mbar_arrive(s_full(ss));
             }
         }
         if (!ok) failed = 1;
@@ -679,6 +637,34 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 1) tmem_free(tmem, COLUMNS);
 }
 
+// starts[b][i] = first entry of row i with a column not below 128 b, for b = 0 .. blocks; 32 rows and 64 blocks of
+// columns at a time, so that both the entries and the results are touched in order.
+template <typename V>
+__global__ void __launch_bounds__(256) starts_kernel(Matrix<V> m, int blocks, int chunks, int *starts) {
+    __shared__ int part[64][33];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.x / chunks * 32, b0 = blockIdx.x % chunks * 64;
+    for (int r = warp; r < 32 && row0 + r < m.n_rows; r += 8) {
+        int begin, end;
+        res_range(m, row0 + r, begin, end);
+        begin = first_at_least(m.res_col, begin, end, min((long long)b0 * 128, (long long)INT_MAX));
+        int before = b0 - 1;  // block of the entry in front
+        bool more = true;
+        for (int e0 = begin; more; e0 += 32) {
+            const int e = e0 + lane;
+            // behind the last entry everything starts at the end
+            const int b = e < end ? min(max(m.res_col[e] / 128, b0 - 1), b0 + 63) : b0 + 63;
+            int left = __shfl_up_sync(0xffffffffu, b, 1);
+            if (lane == 0) left = before;
+            for (int k = left + 1; k <= b; ++k) part[k - b0][r] = min(e, end);
+            before = __shfl_sync(0xffffffffu, b, 31);
+            more = before < b0 + 63;
+        }
+    }
+    __syncthreads();
+    for (int k = warp; k < 64 && b0 + k <= blocks; k += 8)
+        if (row0 + lane < m.n_rows) starts[(long long)(b0 + k) * m.n_rows + row0 + lane] = part[k][lane];
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------
 
 using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -722,7 +708,13 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
     if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
     auto kernel = gemm_kernel<V, MODE, BN, TMA>;
     constexpr int bytes = Shape<MODE, BN>::SMEM;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<uint64_t> told{0};  // devices on which the kernel may have its shared memory
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device >= 64 || !(told.load() >> device & 1))) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && device < 64) told.fetch_or(1ull << device);
+    }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * g.splits));
@@ -736,6 +728,23 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, codes, a, b, g);
+}
+
+// From the device's stream-ordered pool, which keeps what is given back to it (as for the library's handles).
+cudaError_t pool_memory(void **p, size_t bytes, cudaStream_t s) {
+    static std::atomic<uint64_t> kept{0};  // devices whose pool has been told
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (device >= 64 || !(kept.load() >> device & 1)) {
+        cudaMemPool_t pool;
+        uint64_t all = UINT64_MAX;
+        if ((e = cudaDeviceGetDefaultMemPool(&pool, device)) != cudaSuccess ||
+            (e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all)) != cudaSuccess)
+            return e;
+        if (device < 64) kept.fetch_or(1ull << device);
+    }
+    return cudaMallocAsync(p, bytes, s);
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -785,14 +794,27 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (tma && !encode_vectors(&vectors, b, depth, n_vec, n_vec == 1 ? ceil_div(depth, 8) * 8 : ld_b, bn))
             return cudaErrorInvalidValue;
     }
-    const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
-    if (!tma) return launch<V, MODE, 128, false>(codes, codes, vectors, g, tiles, s);
-    switch (bn) {
-        case 32: return launch<V, MODE, 32, true>(codes, codes, vectors, g, tiles, s);
-        case 64: return launch<V, MODE, 64, true>(codes, codes, vectors, g, tiles, s);
-        case 128: return launch<V, MODE, 128, true>(codes, codes, vectors, g, tiles, s);
-        default: return launch<V, MODE, 256, true>(codes, codes, vectors, g, tiles, s);
+    int *starts = nullptr;
+    if (MODE == TRANSPOSED && m.res_ptr && depth > 0) {
+        const long long blocks = ceil_div(m.n_cols, 128), chunks = ceil_div(blocks + 1, 64);
+        const long long grid = ceil_div(m.n_rows, 32) * chunks;
+        if (grid > INT_MAX) return cudaErrorMemoryAllocation;
+        cudaError_t e = pool_memory((void **)&starts, sizeof(int) * (blocks + 1) * m.n_rows, s);
+        if (e != cudaSuccess) return e;
+        starts_kernel<<<(unsigned)grid, 256, 0, s>>>(m, (int)blocks, (int)chunks, starts);
+        g.starts = starts;
     }
+    const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
+    cudaError_t e = !tma        ? launch<V, MODE, 128, false>(codes, codes, vectors, g, tiles, s)
+                    : bn == 32  ? launch<V, MODE, 32, true>(codes, codes, vectors, g, tiles, s)
+                    : bn == 64  ? launch<V, MODE, 64, true>(codes, codes, vectors, g, tiles, s)
+                    : bn == 128 ? launch<V, MODE, 128, true>(codes, codes, vectors, g, tiles, s)
+                                : launch<V, MODE, 256, true>(codes, codes, vectors, g, tiles, s);
+    if (starts) {
+        const cudaError_t f = cudaFreeAsync(starts, s);
+        if (e == cudaSuccess) e = f;
+    }
+    return e;
 }
 
 }  // namespace
