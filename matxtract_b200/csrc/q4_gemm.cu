@@ -28,27 +28,24 @@ namespace {
 enum { PRODUCT, TRANSPOSED, GRADIENT };
 
 // Warps: 0 copies of x and dy, 1 tensor core issue, 2 copies of codes, 3 spare; then four groups of four warps that turn
-// codes into values and empty the tensor memory; then four warps that look for the residual's entries.
-constexpr int THREADS = 32 * 24;
-constexpr int CONVERT = 4, FIND = 20; // first warps of the latter
-constexpr int CODE_TILE = 128 * 64;   // bytes of 128 x 128 codes
+// codes into values and empty the tensor memory.
+constexpr int THREADS = 32 * 20;
+constexpr int CONVERT = 4;            // first warp of the latter
 constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
 constexpr int LOADERS = 64;           // threads that fetch x and dy where bulk copies cannot
-// Where a code tile's residual entries are handed over: four words for each thread that converts 64 of its values, an
-// entry being column << 16 | value.
+// A code tile: 128 rows x 128 columns of codes, then the residual's entries in it in slots of four words for each thread
+// that converts 64 of its values, an entry being column << 16 | value.
+constexpr int CODE_BYTES = 128 * 64, SLOT_BYTES = 256 * 16, CODE_TILE = CODE_BYTES + SLOT_BYTES;
 constexpr uint32_t NO_ENTRY = 0xffffffffu, TOO_MANY = 0xfffffffeu;
-constexpr int SLOT_BYTES = 256 * 16;
-constexpr int AHEAD = 4;  // code tiles whose entries are fetched together
 
 template <int MODE, int BN>
 struct Shape {
     static constexpr int STAGE = A_BYTES + BN * 128;
-    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 6 : 12;
+    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 5 : 8;
     static constexpr int STAGES = BN == 128 ? 5 : 4;
-    static constexpr int SLOTS = MODE == GRADIENT ? 0 : 4;
     static constexpr int SUMS = MODE == GRADIENT ? 4 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
-    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2 * SLOTS + 2;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SLOTS * SLOT_BYTES + SUMS + BARS * 8;
+    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SUMS + BARS * 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of one block");
     static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
 };
@@ -62,7 +59,7 @@ struct Args {
     V *out;
     long long ld_out;
     V *d_res;
-    const int *starts;    // transposed: [block of 128 columns][row] first residual entry not left of the block
+    const uint4 *slots;   // the residual's entries as code tiles take them, [row / 128][column / 128]; null: none
     int groups_per_unit;  // gradient: groups that one block owns
 };
 
@@ -118,20 +115,42 @@ template <typename V>
 struct Scales {
     V s[2];
     int z[2];
-    __device__ __forceinline__ void load(const Matrix<V> &m, int i, int k) {
+    __device__ __forceinline__ void load(const Matrix<V> &m, int i, int g0, int g1) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             s[j] = from_float<V>(0.f);
             z[j] = 8;
         }
-        if (i >= m.n_rows || k >= m.n_cols) return;
-        const int g0 = k / m.group, g1 = min(k + 32, m.n_cols - 1) / m.group;
+        if (i >= m.n_rows) return;
         const long long at = (long long)i * m.n_groups;
+        g0 = min(g0, m.n_groups - 1);  // behind the last column
+        g1 = min(g1, m.n_groups - 1);
         s[0] = m.scales[at + g0];
         s[1] = g1 == g0 ? s[0] : m.scales[at + g1];
         if (m.zeros) {
             z[0] = m.zeros[at + g0] & 15;
             z[1] = g1 == g0 ? z[0] : m.zeros[at + g1] & 15;
+        }
+    }
+};
+
+// The group of a column that moves on by a fixed number of 32s, without a division at every move.
+struct GroupOf {
+    int g, r, size, dg, dr;  // group, 32s into it, its 32s; the same of a move
+    __device__ __forceinline__ GroupOf(int column, int group, int move) {
+        size = group / 32;
+        g = column / group;
+        r = column / 32 - g * size;
+        dg = move / group;
+        dr = move / 32 - dg * size;
+    }
+    __device__ __forceinline__ int second() const { return g + (r + 1 >= size); }  // of the next 32 columns
+    __device__ __forceinline__ void move() {
+        g += dg;
+        r += dr;
+        if (r >= size) {
+            r -= size;
+            ++g;
         }
     }
 };
@@ -163,54 +182,6 @@ struct Cursor {
     }
 };
 
-// N neighbouring entries of a row in registers, loaded together, with the column behind them.  (Entries that
-// move up one by one as they are used would wait for the newest load at every move.)
-template <typename V, int N>
-struct Window {
-    int at, col[N + 1];
-    V val[N];
-    __device__ __forceinline__ void load(const Matrix<V> &m, int from, int end) {
-        at = from;
-#pragma unroll
-        for (int j = 0; j < N + 1; ++j) col[j] = from + j < end ? m.res_col[from + j] : INT_MAX;
-#pragma unroll
-        for (int j = 0; j < N; ++j) val[j] = from + j < end ? m.res_val[from + j] : from_float<V>(0.f);
-    }
-    // Entries with columns in [k0, k1) into a slot, repeated columns added up; moves on while there may be more.
-    __device__ __forceinline__ void hand_over(const Matrix<V> &m, int end, int k0, int k1, uint4 *slot) {
-        uint32_t *to = reinterpret_cast<uint32_t *>(slot);
-        *slot = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
-        int n = 0;
-        while (true) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int k = col[j];
-                if (k >= k0 && k < k1 && !(j > 0 && col[j - 1] == k)) {  // the first of its column
-                    V v = val[j];
-                    if (col[j + 1] == k) {
-                        float sum = to_float(v);
-                        for (int p = at + j + 1; p < end && m.res_col[p] == k; ++p) sum += to_float(m.res_val[p]);
-                        v = from_float<V>(sum);
-                    }
-                    if (n < 4) to[n] = (uint32_t)(k - k0) << 16 | *reinterpret_cast<const uint16_t *>(&v);
-                    ++n;
-                }
-            }
-            if (col[N - 1] >= k1) break;
-            int next = at + N;
-            while (next < end && m.res_col[next] == col[N - 1]) ++next;  // a column's entries stay together
-            load(m, next, end);
-        }
-        if (n > 4) to[3] = TOO_MANY;
-    }
-    __device__ __forceinline__ int first_not_below(long long k) const {
-        int p = at;
-#pragma unroll
-        for (int j = 0; j < N; ++j) p += col[j] < k;
-        return p;
-    }
-};
-
 // `rows` rows of 64 columns from (row, col) on into a swizzled tile, zero outside; `threads` threads
 template <typename V>
 __device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n_rows, long long n_cols, long long row,
@@ -232,23 +203,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
                 const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
     using S = Shape<MODE, BN>;
-    constexpr int CODES = S::CODES ? S::CODES : 1, SLOTS = S::SLOTS ? S::SLOTS : 1;
+    constexpr int CODES = S::CODES ? S::CODES : 1;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_shared;
     __shared__ volatile int failed;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
-    uint4 *slots = reinterpret_cast<uint4 *>(codes_at + S::CODES * CODE_TILE);
-    float *sums = reinterpret_cast<float *>(slots + S::SLOTS * 256);
+    float *sums = reinterpret_cast<float *>(codes_at + S::CODES * CODE_TILE);
     const uint32_t bars = smem_addr(sums) + S::SUMS;
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (S::STAGES + s); };
     auto c_full = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
     auto c_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + S::CODES + s); };
-    auto s_full = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + s); };
-    auto s_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + 2 * S::CODES + S::SLOTS + s); };
-    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES + 2 * S::SLOTS), drained = done + 8;
+    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES), drained = done + 8;
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
 
     const Matrix<V> &m = g.m;
@@ -281,10 +249,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int s = 0; s < S::CODES; ++s) {
             mbar_init(c_full(s), 1);
             mbar_init(c_empty(s), 8);
-        }
-        for (int s = 0; s < S::SLOTS; ++s) {
-            mbar_init(s_full(s), 4);
-            mbar_init(s_empty(s), 8);
         }
         mbar_init(done, 1);
         mbar_init(drained, 16);
@@ -385,16 +349,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (; n < blocks; ++n) {
             const int s = n % CODES;
             if (!(ok = mbar_wait(c_empty(s), (n / CODES & 1) ^ 1, polls))) break;
-            mbar_expect(c_full(s), CODE_TILE);
-            const int at = (block0 + n) * 128;
-            tma_load(smem_addr(codes_at) + s * CODE_TILE, &map_codes, (MODE == PRODUCT ? at : line0) / 2,
-                     MODE == PRODUCT ? line0 : at, c_full(s));
+            const int at = (block0 + n) * 128, row = MODE == PRODUCT ? line0 : at, col = MODE == PRODUCT ? at : line0;
+            const uint32_t to = smem_addr(codes_at) + s * CODE_TILE;
+            mbar_expect(c_full(s), g.slots ? CODE_TILE : CODE_BYTES);
+            tma_load(to, &map_codes, col / 2, row, c_full(s));
+            if (g.slots)
+                bulk_load(to + CODE_BYTES, g.slots + ((long long)(row / 128) * ((m.n_cols + 127) / 128) + col / 128) * 256,
+                          SLOT_BYTES, c_full(s));
         }
         if (!ok) {
             failed = 1;
             for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k % CODES), k / CODES & 1, polls);
         }
-    } else if (MODE != GRADIENT && warp >= CONVERT && warp < FIND) {  // ---- codes -> 16-bit values
+    } else if (MODE != GRADIENT && warp >= CONVERT) {  // ---- codes -> 16-bit values
         // group 0 and 1 take the two halves of the even code tiles, group 2 and 3 those of the odd ones
         const int group = (warp - CONVERT) / 4, half = group & 1, t = threadIdx.x - 32 * CONVERT - 128 * group;
         // this thread's 64 values: a row of the tile (product), or half of one of its half's 64 rows (transposed)
@@ -404,23 +371,28 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int out_block = MODE == PRODUCT ? 0 : t / 64 * 8192;
         auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + tile_row : (block0 + n) * 128 + tile_row; };
         auto col_at = [&](int n) { return (MODE == PRODUCT ? (block0 + n) * 128 : line0) + 64 * part; };
+        GroupOf at(col_at(group / 2), m.group, 256);
         Scales<V> next;
-        if (group / 2 < blocks) next.load(m, row_at(group / 2), col_at(group / 2));
+        if (group / 2 < blocks) next.load(m, row_at(group / 2), at.g, at.second());
         bool ok = true;
         for (int n = group / 2; n < blocks; n += 2) {
             const Scales<V> now = next;
-            if (n + 2 < blocks) next.load(m, row_at(n + 2), col_at(n + 2));
-            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES, ss = n % SLOTS;
+            if (n + 2 < blocks) {
+                if (MODE == PRODUCT) at.move();
+                next.load(m, row_at(n + 2), at.g, at.second());
+            }
+            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES;
             if (!(ok = warp_wait(c_full(cs), n / CODES & 1, polls))) break;
-            uint4 c[2];
+            uint4 c[2], entries;
+            const uint8_t *from = codes_at + cs * CODE_TILE;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                c[j] = *reinterpret_cast<const uint4 *>(codes_at + cs * CODE_TILE + tile_row * 64 +
-                                                        ((2 * part + j ^ tile_row >> 1 & 3) << 4));
+                c[j] = *reinterpret_cast<const uint4 *>(from + tile_row * 64 + ((2 * part + j ^ tile_row >> 1 & 3) << 4));
+            if (g.slots) entries = *reinterpret_cast<const uint4 *>(from + CODE_BYTES + (half * 128 + t) * 16);
             __syncwarp();
             if (lane == 0) mbar_arrive(c_empty(cs));
             if (!(ok = warp_wait(empty(s), (step / S::STAGES & 1) ^ 1, polls))) break;
-            uint8_t *tile_a = smem + s * S::STAGE, *a = tile_a + out_block + out_row * 128;
+            uint8_t *a = smem + s * S::STAGE + out_block + out_row * 128;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const typename Pair<V>::T sc = Pair<V>::both(now.s[j]);
@@ -429,17 +401,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int q = 0; q < 4; ++q)
                     *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], sc, now.z[j]);
             }
-            if (m.res_ptr) {
-                if (!(ok = warp_wait(s_full(ss), n / SLOTS & 1, polls))) break;
-                const uint4 q = slots[ss * 256 + half * 128 + t];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty(ss));
+            if (g.slots && entries.x != NO_ENTRY) {
                 auto add = [&](int k, V v) {
                     V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
                     *e = from_float<V>(to_float(*e) + to_float(v));
                 };
-                if (q.w != TOO_MANY) {
-                    const uint32_t entry[4] = {q.x, q.y, q.z, q.w};
+                if (entries.w != TOO_MANY) {
+                    const uint32_t entry[4] = {entries.x, entries.y, entries.z, entries.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint16_t v = (uint16_t)entry[j];
@@ -461,74 +429,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (lane == 0) mbar_arrive(full(s));
         }
         if (!ok) failed = 1;
-    } else if (MODE == PRODUCT && warp >= FIND && m.res_ptr) {
-        // ---- residual: each thread walks along one row, AHEAD code tiles at a time
-        const int t = threadIdx.x - 32 * FIND, i = line0 + t;
-        int at = 0, end = 0;
-        if (i < m.n_rows && blocks > 0) {
-            res_range(m, i, at, end);
-            at = first_at_least(m.res_col, at, end, block0 * 128);
-        }
-        Window<V, 8> w;
-        bool ok = true;
-        for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
-            w.load(m, at, end);
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int n = n0 + u, ss = n % SLOTS, k0 = (block0 + n) * 128;
-                if (n >= blocks || !ok) continue;
-                if (!(ok = warp_wait(s_empty(ss), (n / SLOTS & 1) ^ 1, polls))) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w.hand_over(m, end, k0 + 64 * h, min(k0 + 64 * h + 64, m.n_cols), slots + ss * 256 + h * 128 + t);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_full(ss));
-            }
-            at = w.first_not_below(min((long long)(block0 + n0 + AHEAD) * 128, (long long)INT_MAX));
-        }
-        if (!ok) failed = 1;
-    } else if (MODE == TRANSPOSED && warp >= FIND && m.res_ptr) {
-        // ---- residual: each thread has one row of every code tile; g.starts tells where its entries begin
-        const int t = threadIdx.x - 32 * FIND, k0 = line0;
-        const int *starts = g.starts + (long long)(line0 / 128) * m.n_rows;
-        int begin[AHEAD], end[AHEAD];
-        auto ranges = [&](int n0) {
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const long long i = (block0 + n0 + u) * 128ll + t;
-                const bool real = n0 + u < blocks && i < m.n_rows;
-                begin[u] = real ? starts[i] : 0;
-                end[u] = real ? starts[m.n_rows + i] : 0;
-            }
-        };
-        ranges(0);
-        bool ok = true;
-        for (int n0 = 0; n0 < blocks && ok; n0 += AHEAD) {
-            Window<V, 3> w[AHEAD];
-            int ends[AHEAD];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) w[u].load(m, begin[u], ends[u] = end[u]);
-            ranges(n0 + AHEAD);
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int n = n0 + u, ss = n % SLOTS;
-                if (n >= blocks || !ok) continue;
-                if (!(ok = warp_wait(s_empty(ss), (n / SLOTS & 1) ^ 1, polls))) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w[u].hand_over(m, ends[u], k0 + 64 * h, min(k0 + 64 * h + 64, m.n_cols),
-                                   slots + ss * 256 + t / 64 * 128 + h * 64 + t % 64);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_full(ss));
-            }
-        }
-        if (!ok) failed = 1;
     }
     __syncwarp();
 
     // ---- D leaves tensor memory: each group of four warps holds the four quarters of its rows, and every fourth 32 columns
     const int group = (warp - CONVERT) / 4, row = warp % 4 * 32 + lane;
-    const bool drains = warp >= CONVERT && warp < FIND;
+    const bool drains = warp >= CONVERT;
     const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
     if (MODE != GRADIENT) {
         const int line = line0 + row, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
@@ -637,32 +543,58 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 1) tmem_free(tmem, COLUMNS);
 }
 
-// starts[b][i] = first entry of row i with a column not below 128 b, for b = 0 .. blocks; 32 rows and 64 blocks of
-// columns at a time, so that both the entries and the results are touched in order.
-template <typename V>
-__global__ void __launch_bounds__(256) starts_kernel(Matrix<V> m, int blocks, int chunks, int *starts) {
-    __shared__ int part[64][33];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.x / chunks * 32, b0 = blockIdx.x % chunks * 64;
+// The residual's entries into the slots of the code tiles, 32 rows and 4096 columns at a time: collected in shared memory,
+// then written in order.  A segment of 64 columns with more than four entries, or with a repeated column, is marked.
+template <typename V, int MODE>
+__global__ void __launch_bounds__(256) slots_kernel(Matrix<V> m, int chunks, uint4 *slots) {
+    __shared__ uint4 part[64][32];  // [segment][row]
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int row0 = blockIdx.x / chunks * 32, k0 = blockIdx.x % chunks * 4096;
+    for (int j = threadIdx.x; j < 64 * 32; j += 256)
+        part[j / 32][j % 32] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+    __syncthreads();
+    const int k1 = min((long long)m.n_cols, k0 + 4096ll);
     for (int r = warp; r < 32 && row0 + r < m.n_rows; r += 8) {
         int begin, end;
         res_range(m, row0 + r, begin, end);
-        begin = first_at_least(m.res_col, begin, end, min((long long)b0 * 128, (long long)INT_MAX));
-        int before = b0 - 1;  // block of the entry in front
-        bool more = true;
-        for (int e0 = begin; more; e0 += 32) {
-            const int e = e0 + lane;
-            // behind the last entry everything starts at the end
-            const int b = e < end ? min(max(m.res_col[e] / 128, b0 - 1), b0 + 63) : b0 + 63;
-            int left = __shfl_up_sync(0xffffffffu, b, 1);
-            if (lane == 0) left = before;
-            for (int k = left + 1; k <= b; ++k) part[k - b0][r] = min(e, end);
-            before = __shfl_sync(0xffffffffu, b, 31);
-            more = before < b0 + 63;
+        begin = first_at_least(m.res_col, begin, end, k0);
+        int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
+        for (int e0 = begin; e0 < end; e0 += 32) {
+            const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
+            const bool mine = k >= k0 && k < k1;
+            const int segment = mine ? (k - k0) / 64 : 64;
+            int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
+            if (lane == 0) {
+                left = segment_before;
+                column = column_before;
+            }
+            const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
+            const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
+            uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
+            if (mine && rank < 4) {
+                const V v = m.res_val[e];
+                to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
+            }
+            __syncwarp();
+            if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
+            __syncwarp();
+            segment_before = __shfl_sync(0xffffffffu, segment, 31);
+            column_before = __shfl_sync(0xffffffffu, k, 31);
+            run = __shfl_sync(0xffffffffu, rank, 31) + 1;
+            if (segment_before == 64) break;
         }
     }
     __syncthreads();
-    for (int k = warp; k < 64 && b0 + k <= blocks; k += 8)
-        if (row0 + lane < m.n_rows) starts[(long long)(b0 + k) * m.n_rows + row0 + lane] = part[k][lane];
+    const long long tiles = (m.n_cols + 127) / 128;
+    const int i = row0 + lane;
+    for (int j = warp; j < 64 && k0 + 64 * j < m.n_cols; j += 8) {
+        const int in_tile = MODE == PRODUCT ? j % 2 * 128 + i % 128 : i % 128 / 64 * 128 + j % 2 * 64 + i % 64;
+        slots[((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile] = part[j][lane];
+        // the second half of a last tile that has no columns there
+        if (j % 2 == 0 && k0 + 64 * (j + 1) >= m.n_cols)
+            slots[((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile + (MODE == PRODUCT ? 128 : 64)] =
+                make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+    }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
@@ -794,15 +726,15 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (tma && !encode_vectors(&vectors, b, depth, n_vec, n_vec == 1 ? ceil_div(depth, 8) * 8 : ld_b, bn))
             return cudaErrorInvalidValue;
     }
-    int *starts = nullptr;
-    if (MODE == TRANSPOSED && m.res_ptr && depth > 0) {
-        const long long blocks = ceil_div(m.n_cols, 128), chunks = ceil_div(blocks + 1, 64);
-        const long long grid = ceil_div(m.n_rows, 32) * chunks;
-        if (grid > INT_MAX) return cudaErrorMemoryAllocation;
-        cudaError_t e = pool_memory((void **)&starts, sizeof(int) * (blocks + 1) * m.n_rows, s);
+    uint4 *slots = nullptr;
+    if (m.res_ptr && depth > 0) {
+        // whole tiles of 128 rows: rows behind the last have empty slots
+        const long long rows = ceil_div(m.n_rows, 128), cols = ceil_div(m.n_cols, 128), chunks = ceil_div(m.n_cols, 4096);
+        if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
+        cudaError_t e = pool_memory((void **)&slots, SLOT_BYTES * rows * cols, s);
         if (e != cudaSuccess) return e;
-        starts_kernel<<<(unsigned)grid, 256, 0, s>>>(m, (int)blocks, (int)chunks, starts);
-        g.starts = starts;
+        slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 256, 0, s>>>(m, (int)chunks, slots);
+        g.slots = slots;
     }
     const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
     cudaError_t e = !tma        ? launch<V, MODE, 128, false>(codes, codes, vectors, g, tiles, s)
@@ -810,8 +742,8 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
                     : bn == 64  ? launch<V, MODE, 64, true>(codes, codes, vectors, g, tiles, s)
                     : bn == 128 ? launch<V, MODE, 128, true>(codes, codes, vectors, g, tiles, s)
                                 : launch<V, MODE, 256, true>(codes, codes, vectors, g, tiles, s);
-    if (starts) {
-        const cudaError_t f = cudaFreeAsync(starts, s);
+    if (slots) {
+        const cudaError_t f = cudaFreeAsync(slots, s);
         if (e == cudaSuccess) e = f;
     }
     return e;

@@ -55,6 +55,12 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, i
         "l"(map), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+// `bytes` bytes in a row; both addresses and the size are multiples of 16
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 // what ordinary stores put into shared memory becomes visible to the tensor cores' reads
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
