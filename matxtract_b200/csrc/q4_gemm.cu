@@ -27,12 +27,11 @@ namespace {
 
 enum { PRODUCT, TRANSPOSED, GRADIENT };
 
-// Warps: 0 copies of x and dy, 1 tensor core issue, 2 copies of codes, 3 spare; then four groups of four warps that turn
+// Warps: 0 copies of x and dy, 1 tensor core issue, 2 copies of codes, 3 none; then four groups of four warps that turn
 // codes into values and empty the tensor memory.
 constexpr int THREADS = 32 * 20;
 constexpr int CONVERT = 4;            // first warp of the latter
 constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
-constexpr int LOADERS = 64;           // threads that fetch x and dy where bulk copies cannot
 // A code tile: 128 rows x 128 columns of codes, then the residual's entries in it in slots of four words for each thread
 // that converts 64 of its values, an entry being column << 16 | value.
 constexpr int CODE_BYTES = 128 * 64, SLOT_BYTES = 256 * 16, CODE_TILE = CODE_BYTES + SLOT_BYTES;
@@ -54,8 +53,6 @@ template <typename V>
 struct Args {
     Matrix<V> m;
     int n_vec, tiles_m, splits;
-    const V *a, *b;  // dy and x as operands A and B, for the loads that bulk copies cannot do
-    long long ld_a, ld_b;
     V *out;
     long long ld_out;
     V *d_res;
@@ -182,23 +179,7 @@ struct Cursor {
     }
 };
 
-// `rows` rows of 64 columns from (row, col) on into a swizzled tile, zero outside; `threads` threads
-template <typename V>
-__device__ void plain_tile(uint8_t *dst, const V *src, long long ld, long long n_rows, long long n_cols, long long row,
-                           long long col, int rows, int thread, int threads) {
-    for (int c = thread; c < rows * 8; c += threads) {
-        const int r = c / 8, j = c % 8;
-        V v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const long long k = col + j * 8 + e;
-            v[e] = row + r < n_rows && k < n_cols ? src[(row + r) * ld + k] : from_float<V>(0.f);
-        }
-        *reinterpret_cast<uint4 *>(dst + r * 128 + ((j ^ r & 7) << 4)) = *reinterpret_cast<uint4 *>(v);
-    }
-}
-
-template <typename V, int MODE, int BN, bool TMA>
+template <typename V, int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
                 const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
@@ -243,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (threadIdx.x == 0) {
         failed = 0;
         for (int s = 0; s < S::STAGES; ++s) {
-            mbar_init(full(s), (TMA ? 1 : LOADERS / 32) + (MODE == GRADIENT ? 0 : 4));
+            mbar_init(full(s), MODE == GRADIENT ? 1 : 5);
             mbar_init(empty(s), 1);
         }
         for (int s = 0; s < S::CODES; ++s) {
@@ -260,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
 
-    if (TMA && warp == 0 && lane == 0) {  // ---- x and dy through bulk copies
+    if (warp == 0 && lane == 0) {  // ---- x and dy through bulk copies
         int n = 0;
         bool ok = true;
         for (int turn = 0; turn < turns && ok; ++turn) {
@@ -285,31 +266,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int k = max(0, n - S::STAGES); k < n; ++k)
                 mbar_wait(full(k % S::STAGES), k / S::STAGES & 1, polls);
         }
-    } else if (!TMA && (warp == 0 || warp == 3)) {  // ---- the same with ordinary loads, where rows lie on any border
-        const int t = (warp == 3) * 32 + lane;
-        int n = 0;
-        bool ok = true;
-        for (int turn = 0; turn < turns && ok; ++turn) {
-            for (int step = 0; step < steps; ++step, ++n) {
-                const int s = n % S::STAGES;
-                if (!(ok = warp_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
-                uint8_t *a = smem + s * S::STAGE, *b = a + A_BYTES;
-                if (MODE == GRADIENT) {
-                    for (int j = 0; j < 2; ++j)
-                        plain_tile(a + j * 8192, g.a, g.ld_a, g.n_vec, m.n_rows, step * 64ll, line0 + 64ll * j, 64, t,
-                                   LOADERS);
-                    for (int j = 0; j < BN / 64; ++j)
-                        plain_tile(b + j * 8192, g.b, g.ld_b, g.n_vec, m.n_cols, step * 64ll,
-                                   col0 + (long long)turn * BN + 64 * j, 64, t, LOADERS);
-                } else {
-                    plain_tile(b, g.b, g.ld_b, g.n_vec, depth, col0, block0 * 128ll + step * 64, BN, t, LOADERS);
-                }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full(s));
-            }
-        }
-        if (!ok) failed = 1;
     } else if (warp == 1 && elect_one()) {  // ---- tensor cores
         constexpr bool BF16 = !std::is_same<V, __half>::value;
         constexpr uint32_t idesc = mma_shape(BF16, BN, MODE != PRODUCT, MODE == GRADIENT);
@@ -599,6 +555,41 @@ __global__ void __launch_bounds__(256) slots_kernel(Matrix<V> m, int chunks, uin
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// From the device's stream-ordered pool, which keeps what is given back to it (as for the library's handles).
+cudaError_t pool_memory(void **p, size_t bytes, cudaStream_t s) {
+    static std::atomic<uint64_t> kept{0};  // devices whose pool has been told
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (device >= 64 || !(kept.load() >> device & 1)) {
+        cudaMemPool_t pool;
+        uint64_t all = UINT64_MAX;
+        if ((e = cudaDeviceGetDefaultMemPool(&pool, device)) != cudaSuccess ||
+            (e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all)) != cudaSuccess)
+            return e;
+        if (device < 64) kept.fetch_or(1ull << device);
+    }
+    return cudaMallocAsync(p, bytes, s);
+}
+
+// Buffers of one call, given back to the pool in the stream's order when the call returns.
+struct Workspace {
+    cudaStream_t s;
+    void *held[3] = {};
+    int n = 0;
+    explicit Workspace(cudaStream_t s) : s(s) {}
+    ~Workspace() {
+        while (n > 0) cudaFreeAsync(held[--n], s);
+    }
+    cudaError_t take(void **p, size_t bytes) {
+        const cudaError_t e = pool_memory(p, bytes, s);
+        if (e == cudaSuccess) held[n++] = *p;
+        return e;
+    }
+};
+
 using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -630,15 +621,45 @@ bool encode_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long 
                   p, cols, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// rows that bulk copies can fetch: base and distance on 16-byte borders
+// to[r][c] = from[r][c]
 template <typename V>
-bool bulk_rows(const V *p, long long ld, int rows) { return (uintptr_t)p % 16 == 0 && (ld % 8 == 0 || rows == 1); }
+__global__ void align_kernel(const V *from, long long ld, V *to, long long ld_to, long long rows, int cols) {
+    const long long stride = (long long)gridDim.y * blockDim.y;
+    const long long c = ((long long)blockIdx.x * 32 + threadIdx.x) * 8;
+    for (long long r = (long long)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += stride) {
+        if (c >= cols) continue;
+        V v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? from[r * ld + c + j] : from_float<V>(0.f);
+        *reinterpret_cast<uint4 *>(to + r * ld_to + c) = *reinterpret_cast<uint4 *>(v);
+    }
+}
 
-template <typename V, int MODE, int BN, bool TMA>
+// The tensor map of `rows` vectors.  Bulk copies want rows on 16-byte borders: others are copied to such rows first
+// (2048 x 8192 values: 13 us; fetching them value by value inside the kernel took several times the product's time).
+template <typename V>
+cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work,
+                        cudaStream_t s) {
+    if (rows == 1) ld = ceil_div(cols, 8) * 8;
+    if ((uintptr_t)p % 16 || ld % 8) {
+        V *copy = nullptr;
+        const long long ld_copy = ceil_div(cols, 8) * 8;
+        cudaError_t e = work.take((void **)&copy, sizeof(V) * ld_copy * rows);
+        if (e != cudaSuccess) return e;
+        const dim3 block(32, 8), grid((unsigned)ceil_div(ld_copy, 256), (unsigned)std::min<long long>(ceil_div(rows, 8), 65535));
+        align_kernel<<<grid, block, 0, s>>>(p, ld, copy, ld_copy, rows, cols);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        p = copy;
+        ld = ld_copy;
+    }
+    return encode_vectors(map, p, cols, rows, ld, box_rows) ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename V, int MODE, int BN>
 cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtensorMap &b, const Args<V> &g,
                    long long tiles, cudaStream_t s) {
     if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
-    auto kernel = gemm_kernel<V, MODE, BN, TMA>;
+    auto kernel = gemm_kernel<V, MODE, BN>;
     constexpr int bytes = Shape<MODE, BN>::SMEM;
     static std::atomic<uint64_t> told{0};  // devices on which the kernel may have its shared memory
     int device = 0;
@@ -661,25 +682,6 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, codes, a, b, g);
 }
-
-// From the device's stream-ordered pool, which keeps what is given back to it (as for the library's handles).
-cudaError_t pool_memory(void **p, size_t bytes, cudaStream_t s) {
-    static std::atomic<uint64_t> kept{0};  // devices whose pool has been told
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    if (device >= 64 || !(kept.load() >> device & 1)) {
-        cudaMemPool_t pool;
-        uint64_t all = UINT64_MAX;
-        if ((e = cudaDeviceGetDefaultMemPool(&pool, device)) != cudaSuccess ||
-            (e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all)) != cudaSuccess)
-            return e;
-        if (device < 64) kept.fetch_or(1ull << device);
-    }
-    return cudaMallocAsync(p, bytes, s);
-}
-
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // Width of a tile and number of blocks that share its contraction: the choice with the least time by a model in clocks.
 // Measured on 2048 to 8192 rows and columns, 16 to 2048 vectors: a code tile takes 1020 to 1520 clocks (nearly the same
@@ -706,47 +708,41 @@ void plan(int lines, int depth, int n_vec, int &bn, int &splits) {
 template <typename V, int MODE>
 cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, V *out, long long ld_out, cudaStream_t s) {
     const int lines = MODE == PRODUCT ? m.n_rows : m.n_cols, depth = MODE == PRODUCT ? m.n_cols : m.n_rows;
-    const bool tma = bulk_rows(b, ld_b, n_vec) && depth > 0;
     Args<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.b = b;
-    g.ld_b = ld_b;
     g.out = out;
     g.ld_out = ld_out;
     g.tiles_m = (int)ceil_div(lines, 128);
-    int bn = 128;
-    g.splits = 1;
-    if (tma) plan(lines, depth, n_vec, bn, g.splits);
+    int bn = 0;
+    plan(lines, depth, n_vec, bn, g.splits);
     CUtensorMap codes = {}, vectors = {};
+    Workspace work(s);
     if (depth > 0) {
         if (!encode(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, m.codes, ceil_div(m.n_cols, 32) * 16, m.n_rows, m.code_ld, 64,
                     128, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
-        if (tma && !encode_vectors(&vectors, b, depth, n_vec, n_vec == 1 ? ceil_div(depth, 8) * 8 : ld_b, bn))
-            return cudaErrorInvalidValue;
-    }
-    uint4 *slots = nullptr;
-    if (m.res_ptr && depth > 0) {
-        // whole tiles of 128 rows: rows behind the last have empty slots
-        const long long rows = ceil_div(m.n_rows, 128), cols = ceil_div(m.n_cols, 128), chunks = ceil_div(m.n_cols, 4096);
-        if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
-        cudaError_t e = pool_memory((void **)&slots, SLOT_BYTES * rows * cols, s);
+        cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn, work, s);
         if (e != cudaSuccess) return e;
-        slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 256, 0, s>>>(m, (int)chunks, slots);
-        g.slots = slots;
+        if (m.res_ptr) {
+            // whole tiles of 128 rows: rows behind the last have empty slots
+            const long long rows = ceil_div(m.n_rows, 128), cols = ceil_div(m.n_cols, 128);
+            const long long chunks = ceil_div(m.n_cols, 4096);
+            uint4 *slots = nullptr;
+            if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
+            if ((e = work.take((void **)&slots, SLOT_BYTES * rows * cols)) != cudaSuccess) return e;
+            slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 256, 0, s>>>(m, (int)chunks, slots);
+            if ((e = cudaGetLastError()) != cudaSuccess) return e;
+            g.slots = slots;
+        }
     }
     const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
-    cudaError_t e = !tma        ? launch<V, MODE, 128, false>(codes, codes, vectors, g, tiles, s)
-                    : bn == 32  ? launch<V, MODE, 32, true>(codes, codes, vectors, g, tiles, s)
-                    : bn == 64  ? launch<V, MODE, 64, true>(codes, codes, vectors, g, tiles, s)
-                    : bn == 128 ? launch<V, MODE, 128, true>(codes, codes, vectors, g, tiles, s)
-                                : launch<V, MODE, 256, true>(codes, codes, vectors, g, tiles, s);
-    if (slots) {
-        const cudaError_t f = cudaFreeAsync(slots, s);
-        if (e == cudaSuccess) e = f;
+    switch (bn) {
+        case 32: return launch<V, MODE, 32>(codes, codes, vectors, g, tiles, s);
+        case 64: return launch<V, MODE, 64>(codes, codes, vectors, g, tiles, s);
+        case 128: return launch<V, MODE, 128>(codes, codes, vectors, g, tiles, s);
+        default: return launch<V, MODE, 256>(codes, codes, vectors, g, tiles, s);
     }
-    return e;
 }
 
 }  // namespace
@@ -765,25 +761,22 @@ cudaError_t product_t_many(const Matrix<V> &m, int n_vec, const V *dy, long long
 template <typename V>
 cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy,
                       V *d_scales, V *d_res, cudaStream_t s) {
-    const bool tma = n_vec > 0 && bulk_rows(x, ld_x, n_vec) && bulk_rows(dy, ld_dy, n_vec);
     Args<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.a = dy;
-    g.ld_a = ld_dy;
-    g.b = x;
-    g.ld_b = ld_x;
     g.out = d_scales;
     g.d_res = m.res_ptr ? d_res : nullptr;
     g.tiles_m = (int)ceil_div(m.n_rows, 128);
     g.splits = 1;
     g.groups_per_unit = std::max(1, 256 / m.group);
     CUtensorMap a = {}, b = {};
-    if (tma && (!encode_vectors(&a, dy, m.n_rows, n_vec, n_vec == 1 ? ceil_div(m.n_rows, 8) * 8 : ld_dy, 64) ||
-                !encode_vectors(&b, x, m.n_cols, n_vec, n_vec == 1 ? ceil_div(m.n_cols, 8) * 8 : ld_x, 64)))
-        return cudaErrorInvalidValue;
-    const long long tiles = g.tiles_m * ceil_div(m.n_groups, g.groups_per_unit);
-    return tma ? launch<V, GRADIENT, 256, true>(a, a, b, g, tiles, s) : launch<V, GRADIENT, 256, false>(a, a, b, g, tiles, s);
+    Workspace work(s);
+    if (n_vec > 0) {
+        cudaError_t e = map_vectors(&a, dy, m.n_rows, n_vec, ld_dy, 64, work, s);
+        if (e == cudaSuccess) e = map_vectors(&b, x, m.n_cols, n_vec, ld_x, 64, work, s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch<V, GRADIENT, 256>(a, a, b, g, g.tiles_m * ceil_div(m.n_groups, g.groups_per_unit), s);
 }
 
 cudaError_t waits_ran_out(int *flag, cudaStream_t s) {
