@@ -20,6 +20,7 @@
 #include "q4.h"
 #include "q4_gemm.h"
 #include "q4_ptx.cuh"
+#include "q4_values.cuh"
 
 namespace mx {
 namespace q4 {
@@ -62,39 +63,6 @@ struct Args {
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
 
-template <typename V>
-struct Pair;
-template <>
-struct Pair<__half> {
-    using T = __half2;
-    // 1024 + c is exact in the type; so is (1024 + 16 c) / 16
-    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) {
-        const uint32_t base = 0x6400u | z, low = 0xD400u | z << 4;  // 1024 + z, -(64 + z)
-        const T zz = bits(base | base << 16), zl = bits(low | low << 16), sixteenth = bits(0x2C002C00u);
-        p[0] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
-        p[1] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
-        w >>= 8;
-        p[2] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
-        p[3] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
-    }
-    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
-    static __device__ __forceinline__ T both(__half v) { return __half2half2(v); }
-};
-template <>
-struct Pair<__nv_bfloat16> {
-    using T = __nv_bfloat162;
-    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) {  // 128 + c is exact in the type
-        const uint32_t base = 0x4300u | z;
-        const T zz = bits(base | base << 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __hsub2(bits((w >> 4 * j & 0x000F000Fu) | 0x43004300u), zz);
-    }
-    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
-    static __device__ __forceinline__ T both(__nv_bfloat16 v) { return __bfloat162bfloat162(v); }
-};
-template <typename T>
-__device__ __forceinline__ uint32_t raw(T v) { return *reinterpret_cast<uint32_t *>(&v); }
-
 // eight codes -> eight values in order; codes j and j + 4 sit in one register until the end
 template <typename V>
 __device__ __forceinline__ uint4 values(uint32_t w, typename Pair<V>::T s, int z) {
@@ -127,27 +95,6 @@ struct Scales {
         if (m.zeros) {
             z[0] = m.zeros[at + g0] & 15;
             z[1] = g1 == g0 ? z[0] : m.zeros[at + g1] & 15;
-        }
-    }
-};
-
-// The group of a column that moves on by a fixed number of 32s, without a division at every move.
-struct GroupOf {
-    int g, r, size, dg, dr;  // group, 32s into it, its 32s; the same of a move
-    __device__ __forceinline__ GroupOf(int column, int group, int move) {
-        size = group / 32;
-        g = column / group;
-        r = column / 32 - g * size;
-        dg = move / group;
-        dr = move / 32 - dg * size;
-    }
-    __device__ __forceinline__ int second() const { return g + (r + 1 >= size); }  // of the next 32 columns
-    __device__ __forceinline__ void move() {
-        g += dg;
-        r += dr;
-        if (r >= size) {
-            r -= size;
-            ++g;
         }
     }
 };
@@ -661,13 +608,7 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
     if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
     auto kernel = gemm_kernel<V, MODE, BN>;
     constexpr int bytes = Shape<MODE, BN>::SMEM;
-    static std::atomic<uint64_t> told{0};  // devices on which the kernel may have its shared memory
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess && (device >= 64 || !(told.load() >> device & 1))) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess && device < 64) told.fetch_or(1ull << device);
-    }
+    const cudaError_t e = allow_smem<V, gemm_kernel<V, MODE, BN>>(bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * g.splits));

@@ -1,0 +1,88 @@
+// Codes -> 16-bit values, and small things that the product kernels share.
+#pragma once
+#include <limits.h>
+
+#include <atomic>
+
+#include "q4.h"
+
+namespace mx {
+namespace q4 {
+
+// c - z of a register's codes, two to a register, exact: p[j] holds those in bits 4 j (low half) and 16 + 4 j (high half),
+// whose zero points are z0 and z1.
+template <typename V>
+struct Pair;
+template <>
+struct Pair<__half> {
+    using T = __half2;
+    // 1024 + c is exact in the type; so is (1024 + 16 c) / 16
+    static __device__ __forceinline__ void steps(uint32_t w, int z0, int z1, T (&p)[4]) {
+        const uint32_t both = z0 | z1 << 16;
+        const T zz = bits(0x64006400u | both), zl = bits(0xD400D400u | both << 4), sixteenth = bits(0x2C002C00u);
+        p[0] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
+        p[1] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+        w >>= 8;
+        p[2] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
+        p[3] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+    }
+    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
+    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) { steps(w, z, z, p); }
+    static __device__ __forceinline__ T two(__half a, __half b) { return __halves2half2(a, b); }
+    static __device__ __forceinline__ T both(__half v) { return __half2half2(v); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    using T = __nv_bfloat162;
+    static __device__ __forceinline__ void steps(uint32_t w, int z0, int z1, T (&p)[4]) {  // 128 + c is exact in the type
+        const T zz = bits(0x43004300u | z0 | z1 << 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __hsub2(bits((w >> 4 * j & 0x000F000Fu) | 0x43004300u), zz);
+    }
+    static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
+    static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) { steps(w, z, z, p); }
+    static __device__ __forceinline__ T two(__nv_bfloat16 a, __nv_bfloat16 b) { return __halves2bfloat162(a, b); }
+    static __device__ __forceinline__ T both(__nv_bfloat16 v) { return __bfloat162bfloat162(v); }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t raw(T v) { return *reinterpret_cast<uint32_t *>(&v); }
+
+// The group of a column that moves on by a fixed number of 32s, without a division at every move.
+struct GroupOf {
+    int g, r, size, dg, dr;  // group, 32s into it, its 32s; the same of a move
+    __device__ __forceinline__ GroupOf(int column, int group, int move) {
+        size = group / 32;
+        g = column / group;
+        r = column / 32 - g * size;
+        dg = move / group;
+        dr = move / 32 - dg * size;
+    }
+    __device__ __forceinline__ int second() const { return g + (r + 1 >= size); }  // of the next 32 columns
+    // of the 32s that lie `n` < 4 further on
+    __device__ __forceinline__ int after(int n) const {
+        return g + (size == 1 ? n : size == 2 ? (r + n) / 2 : r + n >= size);
+    }
+    __device__ __forceinline__ void move() {
+        g += dg;
+        r += dr;
+        if (r >= size) {
+            r -= size;
+            ++g;
+        }
+    }
+};
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked once a device.
+template <typename V, auto KERNEL>
+cudaError_t allow_smem(size_t bytes) {
+    static std::atomic<uint64_t> told{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && told.load() >> device & 1)) return e;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 64) told.fetch_or(1ull << device);
+    return e;
+}
+
+}  // namespace q4
+}  // namespace mx
