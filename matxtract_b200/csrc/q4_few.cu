@@ -46,6 +46,18 @@ __device__ __forceinline__ uint4 eight(const V *x, int k, int end, bool wide) {
     return *reinterpret_cast<uint4 *>(v);
 }
 
+// BYTES (8 or 16) into shared memory, of which `size` are read and the others 0
+template <int BYTES>
+__device__ __forceinline__ void copy(uint32_t to, const void *from, int size) {
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void close_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>  // waits for this thread's copies but those of the LATER last groups
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
+
 // The 32 codes that a lane has of one row of 128 columns.  S is the width that shares a scale: the four lanes of a row
 // have neighbouring quarters of every S columns, so that one mma never mixes two groups.  Word w begins at column
 // place<S>(w, quarter).
@@ -53,25 +65,21 @@ template <int S>
 __device__ __forceinline__ int place(int w, int quarter) {
     return S == 128 ? 32 * quarter + 8 * w : S == 64 ? 64 * (w / 2) + 16 * quarter + 8 * (w % 2) : 32 * w + 8 * quarter;
 }
+// from 64 bytes of the row in shared memory
 template <int S>
-__device__ __forceinline__ void row_codes(uint32_t (&c)[4], const uint8_t *row, int k, int quarter, int row_bytes) {
+__device__ __forceinline__ void row_codes(uint32_t (&c)[4], const uint8_t *row, int quarter) {
     if (S == 128) {
-        const int at = k / 2 + 16 * quarter;
-        const uint4 v = at < row_bytes ? __ldg(reinterpret_cast<const uint4 *>(row + at)) : make_uint4(0, 0, 0, 0);
+        const uint4 v = *reinterpret_cast<const uint4 *>(row + 16 * quarter);
         c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
     } else if (S == 64) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int at = k / 2 + 32 * j + 8 * quarter;
-            const uint2 v = at < row_bytes ? __ldg(reinterpret_cast<const uint2 *>(row + at)) : make_uint2(0, 0);
+            const uint2 v = *reinterpret_cast<const uint2 *>(row + 32 * j + 8 * quarter);
             c[2 * j] = v.x, c[2 * j + 1] = v.y;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = k / 2 + 16 * j + 4 * quarter;
-            c[j] = at < row_bytes ? __ldg(reinterpret_cast<const uint32_t *>(row + at)) : 0;
-        }
+        for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const uint32_t *>(row + 16 * j + 4 * quarter);
     }
 }
 
@@ -85,6 +93,7 @@ struct Few {
     V *out;
     long long ld_out;
     V *d_res;
+    const int *starts;  // transposed: [block of 256 columns][row] first residual entry not left of the block
 };
 
 // d[tile] += steps of 16 rows x 8 columns (one word of two rows) times the vectors' values at those columns
@@ -103,11 +112,65 @@ __device__ __forceinline__ void word_product(float (&d)[NT][4], uint32_t up, uin
     }
 }
 
+// A warp's pieces of 16 rows x 128 columns on their way through shared memory, DEPTH at a time: the codes (64 bytes a
+// row) and the vectors' values at those columns.  Loads into registers two pieces ahead ran at 1.7 TB/s, since a wait
+// for any of them waited for the newest.
+template <typename V, int S, int NT, int DEPTH>
+struct Pieces {
+    const Few<V> &g;
+    const uint8_t *up, *low;  // rows `line` and `line` + 8
+    uint8_t *ring;
+    int line, quarter, row_bytes, slot_bytes;
+    __device__ __forceinline__ Pieces(const Few<V> &g, int row0, uint8_t *smem, int warp, int lane)
+        : g(g), line(lane / 4), quarter(lane % 4) {
+        const Matrix<V> &m = g.m;
+        row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16);
+        up = m.codes + min(row0 + line, m.n_rows - 1) * m.code_ld;  // the last row again: its results are not used
+        low = m.codes + min(row0 + line + 8, m.n_rows - 1) * m.code_ld;
+        slot_bytes = bytes(g.n_vec) / DEPTH;
+        ring = smem + warp * bytes(g.n_vec);
+    }
+    static __host__ __device__ int bytes(int n_vec) { return DEPTH * (1024 + 256 * n_vec); }  // of a warp
+    // n: the piece's number in the warp's order; k, k1: its columns, and where they end
+    __device__ __forceinline__ void fetch(int n, int k, int k1) {
+        const uint32_t to = smem_addr(ring) + n % DEPTH * slot_bytes;
+        const int at = k / 2 + 16 * quarter, valid = at < row_bytes ? 16 : 0;
+        copy<16>(to + line * 64 + 16 * quarter, up + (valid ? at : 0), valid);
+        copy<16>(to + 512 + line * 64 + 16 * quarter, low + (valid ? at : 0), valid);
+        if (g.wide_x) {
+#pragma unroll
+            for (int t = line; t < 8 * NT; t += 8)
+                if (t < g.n_vec)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = k + 8 * (4 * quarter + j), size = min(max(k1 - c, 0), 8) * 2;
+                        copy<16>(to + 1024 + t * 256 + ((4 * quarter + j ^ t) & 15) * 16, g.x + t * g.ld_x + (size ? c : 0), size);
+                    }
+        }
+    }
+    static __device__ __forceinline__ void arrived() {  // the oldest of DEPTH pieces
+        wait_copies<DEPTH - 1>();
+        __syncwarp();
+    }
+    __device__ __forceinline__ const uint8_t *slot(int n) const { return ring + n % DEPTH * slot_bytes; }
+    __device__ __forceinline__ void values_of(uint4 (&x)[NT], int n, int w, int k, int k1) const {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int t = 8 * j + line, c = place<S>(w, quarter);
+            x[j] = make_uint4(0, 0, 0, 0);
+            if (t >= g.n_vec) continue;
+            x[j] = g.wide_x ? *reinterpret_cast<const uint4 *>(slot(n) + 1024 + t * 256 + ((c / 8 ^ t) & 15) * 16)
+                            : eight(g.x + t * g.ld_x, k + c, k1, false);
+        }
+    }
+};
+
 // y = W x for up to 8 NT vectors.  A block has 16 rows; its warps take the 128-column pieces in turn, and the blocks of
 // a cluster (where there are too few rows to occupy the GPU) take contiguous parts of them; the parts are added in the
 // order of warps and ranks.
-template <typename V, int S, int NT>
-__global__ void __launch_bounds__(THREADS) product_few_kernel(const Few<V> g) {
+template <typename V, int S, int NT, int DEPTH>
+__global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_constant__ Few<V> g) {
+    extern __shared__ uint4 smem[];
     __shared__ float part[WARPS][8 * NT][17];
     __shared__ float sum[8 * NT][16];
     const Matrix<V> &m = g.m;
@@ -115,112 +178,99 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const Few<V> g) {
     const int rank = g.splits > 1 ? (int)cluster_rank() : 0, row0 = blockIdx.x / g.splits * 16;
     const int pieces = (int)(((long long)m.n_cols + 127) / 128);
     const int from = (int)((long long)pieces * rank / g.splits), to = (int)((long long)pieces * (rank + 1) / g.splits);
-    const int row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16);
-    const int i0 = min(row0 + line, m.n_rows - 1), i1 = min(row0 + line + 8, m.n_rows - 1);  // the last row again: unused
-    const uint8_t *up = m.codes + i0 * m.code_ld, *low = m.codes + i1 * m.code_ld;
-    const long long s_up = (long long)i0 * m.n_groups, s_low = (long long)i1 * m.n_groups;
+    const long long s_up = (long long)min(row0 + line, m.n_rows - 1) * m.n_groups;
+    const long long s_low = (long long)min(row0 + line + 8, m.n_rows - 1) * m.n_groups;
     constexpr int SEGMENTS = 128 / S;
-
-    // the residual's first entries of this warp's two rows are on their way while the codes are worked on
-    int begin[2] = {0, 0}, end[2] = {0, 0};
-    const bool has_residual = m.res_ptr && rank == 0;
-    if (has_residual)
-        for (int j = 0; j < 2; ++j)
-            if (row0 + 2 * warp + j < m.n_rows) res_range(m, row0 + 2 * warp + j, begin[j], end[j]);
-
-    float total[NT][4] = {};
-    GroupOf at((from + warp) * 128, m.group, WARPS * 128);
-    struct Piece {
-        uint32_t up[4], low[4];
-        V s_up[SEGMENTS], s_low[SEGMENTS];
+    Pieces<V, S, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
+    const int count = from + warp < to ? (to - from - warp - 1) / WARPS + 1 : 0;
+    auto column = [&](int n) { return (from + warp + n * WARPS) * 128; };
+#pragma unroll
+    for (int n = 0; n < DEPTH - 1; ++n) {
+        if (n < count) ring.fetch(n, column(n), m.n_cols);
+        close_copies();
+    }
+    struct Scale {
+        V up[SEGMENTS], low[SEGMENTS];
         int z_up[SEGMENTS], z_low[SEGMENTS];
     };
-    auto fetch = [&](Piece &p, int piece) {
-        row_codes<S>(p.up, up, piece * 128, quarter, row_bytes);
-        row_codes<S>(p.low, low, piece * 128, quarter, row_bytes);
+    GroupOf at((from + warp) * 128, m.group, WARPS * 128);
+    auto scales = [&](Scale &p) {
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
             const int gr = min(at.after(j * (S / 32)), m.n_groups - 1);
-            p.s_up[j] = m.scales[s_up + gr];
-            p.s_low[j] = m.scales[s_low + gr];
+            p.up[j] = m.scales[s_up + gr];
+            p.low[j] = m.scales[s_low + gr];
             p.z_up[j] = m.zeros ? m.zeros[s_up + gr] & 15 : 8;
             p.z_low[j] = m.zeros ? m.zeros[s_low + gr] & 15 : 8;
         }
         at.move();
     };
-    auto work = [&](const Piece &p, int piece) {
-        uint4 x[4][NT];
+    Scale next;
+    if (count > 0) scales(next);
+
+    // the residual, while the first pieces are on their way: two rows a warp
+    float extra[2][8 * NT] = {};
+    if (m.res_ptr && rank == 0) {
+        int begin[2] = {0, 0}, end[2] = {0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int j = 0; j < 2; ++j)
+            if (row0 + 2 * warp + j < m.n_rows) res_range(m, row0 + 2 * warp + j, begin[j], end[j]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int t = 8 * n + line;
-                x[w][n] = t < g.n_vec ? eight(g.x + t * g.ld_x, piece * 128 + place<S>(w, quarter), m.n_cols, g.wide_x)
-                                      : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 2; ++j)
+            for (int e = begin[j] + lane; e < end[j]; e += 32) {
+                const int k = m.res_col[e];
+                const float v = to_float(m.res_val[e]);
+                if (k < 0 || k >= m.n_cols) continue;
+#pragma unroll
+                for (int t = 0; t < 8 * NT; ++t)
+                    if (t < g.n_vec) extra[j][t] = fmaf(v, to_float(g.x[t * g.ld_x + k]), extra[j][t]);
             }
+    }
+
+    float total[NT][4] = {};
+    for (int n = 0; n < count; ++n) {
+        const Scale now = next;
+        if (n + DEPTH - 1 < count) ring.fetch(n + DEPTH - 1, column(n + DEPTH - 1), m.n_cols);
+        close_copies();
+        if (n + 1 < count) scales(next);
+        ring.arrived();
+        uint32_t a[4], b[4];
+        row_codes<S>(a, ring.slot(n) + line * 64, quarter);
+        row_codes<S>(b, ring.slot(n) + 512 + line * 64, quarter);
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
             float d[NT][4] = {};
 #pragma unroll
-            for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w)
-                word_product<V, NT>(d, p.up[w], p.low[w], p.z_up[j], p.z_low[j], x[w]);
-            const float a = to_float(p.s_up[j]), b = to_float(p.s_low[j]);
+            for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w) {
+                uint4 x[NT];
+                ring.values_of(x, n, w, column(n), m.n_cols);
+                word_product<V, NT>(d, a[w], b[w], now.z_up[j], now.z_low[j], x);
+            }
+            const float u = to_float(now.up[j]), l = to_float(now.low[j]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                total[n][0] = fmaf(a, d[n][0], total[n][0]);
-                total[n][1] = fmaf(a, d[n][1], total[n][1]);
-                total[n][2] = fmaf(b, d[n][2], total[n][2]);
-                total[n][3] = fmaf(b, d[n][3], total[n][3]);
+            for (int q = 0; q < NT; ++q) {
+                total[q][0] = fmaf(u, d[q][0], total[q][0]);
+                total[q][1] = fmaf(u, d[q][1], total[q][1]);
+                total[q][2] = fmaf(l, d[q][2], total[q][2]);
+                total[q][3] = fmaf(l, d[q][3], total[q][3]);
             }
         }
-    };
-    // two pieces ahead
-    Piece p[3];
-    int piece = from + warp;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (piece + WARPS * j < to) fetch(p[j], piece + WARPS * j);
-    int first[2];
-    V value[2];
-    if (has_residual)
-        for (int j = 0; j < 2; ++j)
-            if (begin[j] + lane < end[j]) {
-                first[j] = m.res_col[begin[j] + lane];
-                value[j] = m.res_val[begin[j] + lane];
-            }
-    while (piece < to) {
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            if (piece < to) {
-                if (piece + 2 * WARPS < to) fetch(p[(j + 2) % 3], piece + 2 * WARPS);
-                work(p[j], piece);
-            }
-            piece += WARPS;
-        }
+        __syncwarp();  // the slot is free again
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) part[warp][8 * n + 2 * quarter + j % 2][line + 8 * (j / 2)] = total[n][j];
-    if (has_residual) {
+    if (m.res_ptr && rank == 0) {
         __syncwarp();
-        for (int j = 0; j < 2; ++j) {
-            float r[8 * NT] = {};
-            for (int e = begin[j] + lane; e < end[j]; e += 32) {
-                const int k = e < begin[j] + 32 ? first[j] : m.res_col[e];
-                if (k < 0 || k >= m.n_cols) continue;
-                const float v = to_float(e < begin[j] + 32 ? value[j] : m.res_val[e]);
 #pragma unroll
-                for (int t = 0; t < 8 * NT; ++t)
-                    if (t < g.n_vec) r[t] = fmaf(v, to_float(g.x[t * g.ld_x + k]), r[t]);
-            }
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int t = 0; t < 8 * NT; ++t) {
                 if (t >= g.n_vec) break;
-                for (int d = 16; d; d /= 2) r[t] += __shfl_xor_sync(0xffffffffu, r[t], d);
-                if (lane == 0) part[warp][t][2 * warp + j] += r[t];
+                for (int d = 16; d; d /= 2) extra[j][t] += __shfl_xor_sync(0xffffffffu, extra[j][t], d);
+                if (lane == 0) part[warp][t][2 * warp + j] += extra[j][t];
             }
-        }
     }
     __syncthreads();
     const int row = threadIdx.x % 16, t = threadIdx.x / 16;
@@ -249,76 +299,29 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const Few<V> g) {
 
 // Gradients from up to 8 NT vectors.  A block has 16 rows and a part of the groups, a warp whole groups of them: the
 // sums over a group's columns for each vector are the product's, then they are weighed with dy instead of the scale.
-// S = 0: one group at a time, in pieces of 128 columns; else 128 / S groups at a time.
-template <typename V, int S, int NT>
-__global__ void __launch_bounds__(THREADS) grad_few_kernel(const Few<V> g) {
+// S = 0: one group after the other, in pieces of 128 columns; else a piece has 128 / S groups.
+template <typename V, int S, int NT, int DEPTH>
+__global__ void __launch_bounds__(THREADS) grad_few_kernel(const __grid_constant__ Few<V> g) {
+    extern __shared__ uint4 smem[];
     const Matrix<V> &m = g.m;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
     const int row0 = blockIdx.x / g.splits * 16, rank = blockIdx.x % g.splits;
-    const int row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16);
     const bool real0 = row0 + line < m.n_rows, real1 = row0 + line + 8 < m.n_rows;
     const int i0 = min(row0 + line, m.n_rows - 1), i1 = min(row0 + line + 8, m.n_rows - 1);
-    if (g.out) {
-        const uint8_t *up = m.codes + i0 * m.code_ld, *low = m.codes + i1 * m.code_ld;
-        const long long s_up = (long long)i0 * m.n_groups, s_low = (long long)i1 * m.n_groups;
-        float dy[NT][4];
+    constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH;
+    const int units = (m.n_groups + SEGMENTS - 1) / SEGMENTS, first = rank * WARPS + warp, stride = g.splits * WARPS;
+    const int per_unit = S ? 1 : (m.group + 127) / 128;
+    const int mine = g.out && first < units ? (units - first - 1) / stride + 1 : 0, count = mine * per_unit;
+    // of piece n: where its columns begin, and where its group's (or the matrix's) end
+    auto begin_of = [&](int n) { return (first + n / per_unit * stride) * SEGMENTS * m.group + n % per_unit * 128; };
+    auto end_of = [&](int n) {
+        return S ? m.n_cols : (int)min((long long)m.n_cols, ((long long)first + n / per_unit * stride + 1) * m.group);
+    };
+    Pieces<V, WIDTH, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = 8 * n + 2 * quarter + j % 2;
-                dy[n][j] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + (j < 2 ? i0 : i1)]) : 0.f;
-            }
-        constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH;
-        const int units = (m.n_groups + SEGMENTS - 1) / SEGMENTS;
-        for (int u = rank * WARPS + warp; u < units; u += g.splits * WARPS) {
-            const int k0 = u * SEGMENTS * m.group;
-            const int k1 = S ? m.n_cols : (int)min((long long)m.n_cols, (long long)k0 + m.group);
-            float d[SEGMENTS][NT][4] = {};
-            int z_up[SEGMENTS], z_low[SEGMENTS];
-#pragma unroll
-            for (int j = 0; j < SEGMENTS; ++j) {
-                const int gr = min(u * SEGMENTS + j, m.n_groups - 1);
-                z_up[j] = m.zeros ? m.zeros[s_up + gr] & 15 : 8;
-                z_low[j] = m.zeros ? m.zeros[s_low + gr] & 15 : 8;
-            }
-            for (int k = k0; k < (S ? k0 + 1 : k1); k += 128) {
-                uint32_t a[4], b[4];
-                row_codes<WIDTH>(a, up, k, quarter, row_bytes);
-                row_codes<WIDTH>(b, low, k, quarter, row_bytes);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint4 x[NT];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const int t = 8 * n + line;
-                        x[n] = t < g.n_vec ? eight(g.x + t * g.ld_x, k + place<WIDTH>(w, quarter), k1, g.wide_x)
-                                           : make_uint4(0, 0, 0, 0);
-                    }
-                    const int j = w / (WIDTH / 32);
-                    word_product<V, NT>(d[j], a[w], b[w], z_up[j], z_low[j], x);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < SEGMENTS; ++j) {
-                float e0 = 0.f, e1 = 0.f;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    e0 = fmaf(dy[n][0], d[j][n][0], fmaf(dy[n][1], d[j][n][1], e0));
-                    e1 = fmaf(dy[n][2], d[j][n][2], fmaf(dy[n][3], d[j][n][3], e1));
-                }
-#pragma unroll
-                for (int x = 1; x < 4; x *= 2) {
-                    e0 += __shfl_xor_sync(0xffffffffu, e0, x);
-                    e1 += __shfl_xor_sync(0xffffffffu, e1, x);
-                }
-                const int gr = u * SEGMENTS + j;
-                if (quarter == 0 && gr < m.n_groups) {
-                    if (real0) g.out[s_up + gr] = from_float<V>(e0);
-                    if (real1) g.out[s_low + gr] = from_float<V>(e1);
-                }
-            }
-        }
+    for (int n = 0; n < DEPTH - 1; ++n) {
+        if (n < count) ring.fetch(n, begin_of(n), end_of(n));
+        close_copies();
     }
     if (g.d_res && rank == 0) {
         for (int r = 2 * warp; r < 2 * warp + 2 && row0 + r < m.n_rows; ++r) {
@@ -339,90 +342,197 @@ __global__ void __launch_bounds__(THREADS) grad_few_kernel(const Few<V> g) {
             }
         }
     }
+    const long long s_up = (long long)i0 * m.n_groups, s_low = (long long)i1 * m.n_groups;
+    float dy[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = 8 * n + 2 * quarter + j % 2;
+            dy[n][j] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + (j < 2 ? i0 : i1)]) : 0.f;
+        }
+    float d[SEGMENTS][NT][4] = {};
+    int next_up[SEGMENTS], next_low[SEGMENTS];
+    auto zeros = [&](int n) {
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) {
+            const int gr = min((first + n / per_unit * stride) * SEGMENTS + j, m.n_groups - 1);
+            next_up[j] = m.zeros ? m.zeros[s_up + gr] & 15 : 8;
+            next_low[j] = m.zeros ? m.zeros[s_low + gr] & 15 : 8;
+        }
+    };
+    if (count > 0) zeros(0);
+    for (int n = 0; n < count; ++n) {
+        int z_up[SEGMENTS], z_low[SEGMENTS];
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) {
+            z_up[j] = next_up[j];
+            z_low[j] = next_low[j];
+        }
+        if (n + DEPTH - 1 < count) ring.fetch(n + DEPTH - 1, begin_of(n + DEPTH - 1), end_of(n + DEPTH - 1));
+        close_copies();
+        if (n + 1 < count) zeros(n + 1);
+        ring.arrived();
+        uint32_t a[4], b[4];
+        row_codes<WIDTH>(a, ring.slot(n) + line * 64, quarter);
+        row_codes<WIDTH>(b, ring.slot(n) + 512 + line * 64, quarter);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint4 x[NT];
+            ring.values_of(x, n, w, begin_of(n), end_of(n));
+            word_product<V, NT>(d[w / (WIDTH / 32)], a[w], b[w], z_up[w / (WIDTH / 32)], z_low[w / (WIDTH / 32)], x);
+        }
+        __syncwarp();  // the slot is free again
+        if (n % per_unit != per_unit - 1) continue;
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) {
+            float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+            for (int q = 0; q < NT; ++q) {
+                e0 = fmaf(dy[q][0], d[j][q][0], fmaf(dy[q][1], d[j][q][1], e0));
+                e1 = fmaf(dy[q][2], d[j][q][2], fmaf(dy[q][3], d[j][q][3], e1));
+                d[j][q][0] = d[j][q][1] = d[j][q][2] = d[j][q][3] = 0.f;
+            }
+#pragma unroll
+            for (int x = 1; x < 4; x *= 2) {
+                e0 += __shfl_xor_sync(0xffffffffu, e0, x);
+                e1 += __shfl_xor_sync(0xffffffffu, e1, x);
+            }
+            const int gr = (first + n / per_unit * stride) * SEGMENTS + j;
+            if (quarter == 0 && gr < m.n_groups) {
+                if (real0) g.out[s_up + gr] = from_float<V>(e0);
+                if (real1) g.out[s_low + gr] = from_float<V>(e1);
+            }
+        }
+    }
+}
+
+// starts[b][i] = first entry of row i with a column not below 256 b, for b = 0 .. blocks; 32 rows and 64 blocks of
+// columns at a time, so that both the entries and the results are touched in order.
+template <typename V>
+__global__ void __launch_bounds__(256) starts_kernel(Matrix<V> m, int blocks, int chunks, int *starts) {
+    __shared__ int part[64][33];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int row0 = blockIdx.x / chunks * 32, b0 = blockIdx.x % chunks * 64;
+    for (int r = warp; r < 32 && row0 + r < m.n_rows; r += 8) {
+        int begin, end;
+        res_range(m, row0 + r, begin, end);
+        begin = first_at_least(m.res_col, begin, end, (int)min(b0 * 256ll, (long long)INT_MAX));
+        int before = b0 - 1;  // block of the entry in front
+        for (int e = begin + lane; before < b0 + 63; e += 32) {
+            // behind the last entry everything starts at the end
+            const int b = e < end ? min(max(m.res_col[e] / 256, b0 - 1), b0 + 63) : b0 + 63;
+            int left = __shfl_up_sync(0xffffffffu, b, 1);
+            if (lane == 0) left = before;
+            for (int k = left + 1; k <= b; ++k) part[k - b0][r] = min(e, end);
+            before = __shfl_sync(0xffffffffu, b, 31);
+        }
+    }
+    __syncthreads();
+    for (int k = warp; k < 64 && b0 + k <= blocks; k += 8)
+        if (row0 + lane < m.n_rows) starts[(long long)(b0 + k) * m.n_rows + row0 + lane] = part[k][lane];
 }
 
 // dx = dy W for up to 8 vectors.  A block has 256 columns, its warps take 16 rows at a time; the contraction runs over
 // rows, whose scales differ, so the values are s (c - z), rounded once to the type.  The blocks of a cluster share the
 // rows.  A lane holds 32 columns of four rows; two rows' codes of a column are brought into one register.
 constexpr int COLS = 256, VEC = 8, VEC_STRIDE = 268, WARP_PART = VEC * VEC_STRIDE;
+constexpr int T_DEPTH = 4, T_SLOT = 2048 + 256;  // steps of a warp under way; bytes of one: codes, dy
+constexpr int T_SMEM = WARPS * (T_DEPTH * T_SLOT > 4 * WARP_PART ? T_DEPTH * T_SLOT : 4 * WARP_PART);
 __device__ __forceinline__ int part_at(int t, int k) { return t * VEC_STRIDE + k + k / 32; }
 
 template <typename V>
-__global__ void __launch_bounds__(THREADS) product_t_few_kernel(const Few<V> g) {
-    extern __shared__ float parts[];  // [warp][vector][column], columns a little apart
+__global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_constant__ Few<V> g) {
+    extern __shared__ uint4 smem[];
+    float *parts = reinterpret_cast<float *>(smem);  // in the end: [warp][vector][column], columns a little apart
     const Matrix<V> &m = g.m;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
     const int rank = g.splits > 1 ? (int)cluster_rank() : 0, k0 = blockIdx.x / g.splits * COLS;
     const int steps = (int)(((long long)m.n_rows + 15) / 16);
     const int from = (int)((long long)steps * rank / g.splits), to = (int)((long long)steps * (rank + 1) / g.splits);
+    const int count = from + warp < to ? (to - from - warp - 1) / WARPS + 1 : 0;
     const int k = k0 + 32 * line, gr = min(k / m.group, m.n_groups - 1);
     const bool inside = k < m.n_cols;
-    float d[16][4] = {};
-    struct Rows {
-        uint32_t c[4][4];
-        V s[4];
-        int z[4];
-        uint2 dy;
-    };
-    auto fetch = [&](Rows &r, int step) {
-        const int i0 = step * 16 + 4 * quarter;
+    uint8_t *ring = reinterpret_cast<uint8_t *>(smem) + warp * T_DEPTH * T_SLOT + lane * 16;
+    auto rows_of = [&](int n) { return (from + warp + n * WARPS) * 16 + 4 * quarter; };
+    auto fetch = [&](int n) {
+        const uint32_t slot = smem_addr(ring) + n % T_DEPTH * T_SLOT;
+        const int i0 = rows_of(n);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int i = i0 + j;
-            const bool real = inside && i < m.n_rows;
-            const uint4 v = real ? __ldg(reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2)) : make_uint4(0, 0, 0, 0);
-            r.c[j][0] = v.x, r.c[j][1] = v.y, r.c[j][2] = v.z, r.c[j][3] = v.w;
-            r.s[j] = real ? m.scales[(long long)i * m.n_groups + gr] : from_float<V>(0.f);
-            r.z[j] = real && m.zeros ? m.zeros[(long long)i * m.n_groups + gr] & 15 : 8;
+            const bool real = inside && i0 + j < m.n_rows;
+            copy<16>(slot + 512 * j, m.codes + (real ? (i0 + j) * m.code_ld + k / 2 : 0), real ? 16 : 0);
         }
-        r.dy = make_uint2(0, 0);
-        if (line < g.n_vec) {
-            const V *p = g.dy + line * g.ld_dy + i0;
-            if (g.wide_dy && i0 + 4 <= m.n_rows) {
-                r.dy = __ldg(reinterpret_cast<const uint2 *>(p));
-            } else {
-                V v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = i0 + j < m.n_rows ? p[j] : from_float<V>(0.f);
-                r.dy = *reinterpret_cast<uint2 *>(v);
-            }
+        if (g.wide_dy && line < g.n_vec) {
+            const int size = min(max(m.n_rows - i0, 0), 4) * 2;
+            copy<8>(slot + 2048 - lane * 8, g.dy + line * g.ld_dy + (size ? i0 : 0), size);
         }
     };
-    auto work = [&](const Rows &r) {
-        typename Pair<V>::T s[2] = {Pair<V>::two(r.s[0], r.s[1]), Pair<V>::two(r.s[2], r.s[3])};
+#pragma unroll
+    for (int n = 0; n < T_DEPTH - 1; ++n) {
+        if (n < count) fetch(n);
+        close_copies();
+    }
+    V scale[4];
+    int z[4];
+    auto scales = [&](int n) {
+        const int i0 = rows_of(n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool real = inside && i0 + j < m.n_rows;
+            scale[j] = real ? m.scales[(long long)(i0 + j) * m.n_groups + gr] : from_float<V>(0.f);
+            z[j] = real && m.zeros ? m.zeros[(long long)(i0 + j) * m.n_groups + gr] & 15 : 8;
+        }
+    };
+    if (count > 0) scales(0);
+    float d[16][4] = {};
+    for (int n = 0; n < count; ++n) {
+        const typename Pair<V>::T s0 = Pair<V>::two(scale[0], scale[1]), s1 = Pair<V>::two(scale[2], scale[3]);
+        const int z0 = z[0], z1 = z[1], z2 = z[2], z3 = z[3];
+        if (n + T_DEPTH - 1 < count) fetch(n + T_DEPTH - 1);
+        close_copies();
+        if (n + 1 < count) scales(n + 1);
+        wait_copies<T_DEPTH - 1>();
+        const uint8_t *slot = ring + n % T_DEPTH * T_SLOT;
+        uint2 dy = make_uint2(0, 0);
+        if (line < g.n_vec) {
+            if (g.wide_dy) {
+                dy = *reinterpret_cast<const uint2 *>(slot + 2048 - lane * 8);
+            } else {
+                const V *p = g.dy + line * g.ld_dy + rows_of(n);
+                V v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = rows_of(n) + j < m.n_rows ? p[j] : from_float<V>(0.f);
+                dy = *reinterpret_cast<uint2 *>(v);
+            }
+        }
+        uint32_t c[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(slot + 512 * j);
+            c[j][0] = v.x, c[j][1] = v.y, c[j][2] = v.z, c[j][3] = v.w;
+        }
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // columns 8 w + 4 h .. + 3
                 typename Pair<V>::T p[4], q[4];
                 const int pick = h ? 0x7632 : 0x5410;
-                Pair<V>::steps(__byte_perm(r.c[0][w], r.c[1][w], pick), r.z[0], r.z[1], p);
-                Pair<V>::steps(__byte_perm(r.c[2][w], r.c[3][w], pick), r.z[2], r.z[3], q);
+                Pair<V>::steps(__byte_perm(c[0][w], c[1][w], pick), z0, z1, p);
+                Pair<V>::steps(__byte_perm(c[2][w], c[3][w], pick), z2, z3, q);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    p[j] = __hmul2(p[j], s[0]);
-                    q[j] = __hmul2(q[j], s[1]);
+                    p[j] = __hmul2(p[j], s0);
+                    q[j] = __hmul2(q[j], s1);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {  // columns + 2 j and + 2 j + 1
                     const uint32_t a[4] = {raw(p[2 * j]), raw(p[2 * j + 1]), raw(q[2 * j]), raw(q[2 * j + 1])};
-                    mma16<V>(d[4 * w + 2 * h + j], a, r.dy.x, r.dy.y);
+                    mma16<V>(d[4 * w + 2 * h + j], a, dy.x, dy.y);
                 }
             }
-    };
-    Rows r[2];
-    int step = from + warp;
-    if (step < to) fetch(r[0], step);
-    while (step < to) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (step < to) {
-                if (step + WARPS < to) fetch(r[j ^ 1], step + WARPS);
-                work(r[j]);
-            }
-            step += WARPS;
-        }
     }
+    __syncthreads();  // every ring is empty
     float *mine = parts + warp * WARP_PART;
 #pragma unroll
     for (int c = 0; c < 16; ++c)
@@ -431,33 +541,42 @@ __global__ void __launch_bounds__(THREADS) product_t_few_kernel(const Few<V> g) 
     if (m.res_ptr) {
         // a lane a row; lanes whose entries meet in a column add one after the other, lower rows first
         __syncwarp();
-        const int k1 = (int)min((long long)m.n_cols, (long long)k0 + COLS);
-        for (int i0 = from * 16 + 32 * warp; i0 < min(to * 16, m.n_rows); i0 += 32 * WARPS) {
+        const int k1 = (int)min((long long)m.n_cols, (long long)k0 + COLS), last = min(to * 16, m.n_rows);
+        const int *starts = g.starts + (long long)(k0 / COLS) * m.n_rows;
+        for (int i0 = from * 16 + 32 * warp; i0 < last; i0 += 32 * WARPS) {
             const int i = i0 + lane;
-            int at = 0, end = 0;
+            int at = i < last ? starts[i] : 0;
+            const int end = i < last ? starts[m.n_rows + i] : 0;
             float dy[VEC];
-            if (i < min(to * 16, m.n_rows)) {
-                res_range(m, i, at, end);
-                at = first_at_least(m.res_col, at, end, k0);
-            }
 #pragma unroll
             for (int t = 0; t < VEC; ++t) dy[t] = at < end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
-            while (true) {
-                const int c = at < end ? m.res_col[at] : INT_MAX;
-                const bool hit = c < k1;
-                if (!__any_sync(0xffffffffu, hit)) break;
-                const float v = hit ? to_float(m.res_val[at]) : 0.f;
-                const unsigned same = __match_any_sync(0xffffffffu, hit ? c : -1 - lane);
-                const int turn = __popc(same & ((1u << lane) - 1));
-                const int turns = __reduce_max_sync(0xffffffffu, turn);
-                for (int n = 0; n <= turns; ++n) {
-                    if (hit && turn == n && c >= k0)
+            while (__any_sync(0xffffffffu, at < end)) {
+                constexpr int TOGETHER = 4;
+                int col[TOGETHER];
+                V val[TOGETHER];
 #pragma unroll
-                        for (int t = 0; t < VEC; ++t)
-                            if (t < g.n_vec) mine[part_at(t, c - k0)] += v * dy[t];
-                    __syncwarp();
+                for (int j = 0; j < TOGETHER; ++j) {
+                    col[j] = at + j < end ? m.res_col[at + j] : INT_MAX;
+                    val[j] = at + j < end ? m.res_val[at + j] : from_float<V>(0.f);
                 }
-                at += hit;
+#pragma unroll
+                for (int j = 0; j < TOGETHER; ++j) {
+                    const bool hit = col[j] >= k0 && col[j] < k1;
+                    if (!__any_sync(0xffffffffu, hit)) continue;
+                    const float v = to_float(val[j]);
+                    const unsigned same = __match_any_sync(0xffffffffu, hit ? col[j] : -1 - lane);
+                    const int turn = __popc(same & ((1u << lane) - 1));
+                    const int turns = __reduce_max_sync(0xffffffffu, turn);
+                    for (int n = 0; n <= turns; ++n) {
+                        if (hit && turn == n) {
+#pragma unroll
+                            for (int t = 0; t < VEC; ++t)
+                                if (t < g.n_vec) mine[part_at(t, col[j] - k0)] += v * dy[t];
+                        }
+                        __syncwarp();
+                    }
+                }
+                at += TOGETHER;
             }
         }
     }
@@ -496,7 +615,7 @@ bool on_border(const V *p, long long ld, int n_vec, int values) {
 }
 
 template <typename V>
-cudaError_t run(void (*kernel)(Few<V>), long long blocks, int cluster, size_t smem, const Few<V> &g, cudaStream_t s) {
+cudaError_t run(void (*kernel)(const Few<V>), long long blocks, int cluster, size_t smem, const Few<V> &g, cudaStream_t s) {
     if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -519,18 +638,32 @@ int parts_of(long long blocks, long long pieces) {
     return n;
 }
 
-template <typename V, int NT>
-cudaError_t product_by_width(const Few<V> &g, long long blocks, cudaStream_t s) {
-    auto kernel = g.m.group % 128 == 0  ? product_few_kernel<V, 128, NT>
-                  : g.m.group % 64 == 0 ? product_few_kernel<V, 64, NT>
-                                        : product_few_kernel<V, 32, NT>;
-    return run<V>(kernel, blocks * g.splits, g.splits, 0, g, s);
+template <typename V, auto KERNEL>
+cudaError_t run_ring(const Few<V> &g, long long blocks, int cluster, int warp_bytes, cudaStream_t s) {
+    const cudaError_t e = allow_smem<V, KERNEL>(WARPS * 4 * (1024 + 256 * 16));
+    return e == cudaSuccess ? run<V>(KERNEL, blocks, cluster, WARPS * warp_bytes, g, s) : e;
 }
 
-template <typename V, int NT>
-cudaError_t grad_by_width(const Few<V> &g, long long blocks, cudaStream_t s) {
-    auto kernel = g.m.group == 64 ? grad_few_kernel<V, 64, NT> : g.m.group == 32 ? grad_few_kernel<V, 32, NT> : grad_few_kernel<V, 0, NT>;
-    return run<V>(kernel, blocks * g.splits, 1, 0, g, s);
+// Pieces under way: 8 a warp for one or two vectors, 4 for more, whose values take more room (two blocks an SM, one for
+// more than 8 vectors).
+template <typename V, int S>
+cudaError_t product_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
+    blocks *= g.splits;
+    if (g.n_vec <= 2)
+        return run_ring<V, product_few_kernel<V, S, 1, 8>>(g, blocks, g.splits, Pieces<V, S, 1, 8>::bytes(g.n_vec), s);
+    if (g.n_vec <= 8)
+        return run_ring<V, product_few_kernel<V, S, 1, 4>>(g, blocks, g.splits, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
+    return run_ring<V, product_few_kernel<V, S, 2, 4>>(g, blocks, g.splits, Pieces<V, S, 2, 4>::bytes(g.n_vec), s);
+}
+
+template <typename V, int S>
+cudaError_t grad_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
+    blocks *= g.splits;
+    if (g.n_vec <= 2)
+        return run_ring<V, grad_few_kernel<V, S, 1, 8>>(g, blocks, 1, Pieces<V, S, 1, 8>::bytes(g.n_vec), s);
+    if (g.n_vec <= 8)
+        return run_ring<V, grad_few_kernel<V, S, 1, 4>>(g, blocks, 1, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
+    return run_ring<V, grad_few_kernel<V, S, 2, 4>>(g, blocks, 1, Pieces<V, S, 2, 4>::bytes(g.n_vec), s);
 }
 
 }  // namespace
@@ -548,7 +681,9 @@ cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V
     g.wide_x = on_border(x, ld_x, n_vec, 8);
     g.out = y;
     g.ld_out = ld_y;
-    return n_vec <= 8 ? product_by_width<V, 1>(g, blocks, s) : product_by_width<V, 2>(g, blocks, s);
+    return m.group % 128 == 0  ? product_of_width<V, 128>(g, blocks, s)
+           : m.group % 64 == 0 ? product_of_width<V, 64>(g, blocks, s)
+                               : product_of_width<V, 32>(g, blocks, s);
 }
 
 template <typename V>
@@ -565,9 +700,18 @@ cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_d
     g.wide_dy = on_border(dy, ld_dy, n_vec, 4);
     g.out = dx;
     g.ld_out = ld_dx;
-    constexpr size_t smem = sizeof(float) * WARPS * WARP_PART;
-    const cudaError_t e = allow_smem<V, product_t_few_kernel<V>>(smem);
-    return e == cudaSuccess ? run<V>(product_t_few_kernel<V>, blocks * g.splits, g.splits, smem, g, s) : e;
+    Workspace work(s);
+    cudaError_t e = allow_smem<V, product_t_few_kernel<V>>(T_SMEM);
+    if (e == cudaSuccess && m.res_ptr && m.n_rows > 0) {
+        const long long chunks = ceil_div(blocks + 1, 64), grid = ceil_div(m.n_rows, 32) * chunks;
+        int *starts = nullptr;
+        if (grid > INT_MAX) return cudaErrorMemoryAllocation;
+        if ((e = work.take((void **)&starts, sizeof(int) * (blocks + 1) * m.n_rows)) != cudaSuccess) return e;
+        starts_kernel<<<(unsigned)grid, 256, 0, s>>>(m, (int)blocks, (int)chunks, starts);
+        e = cudaGetLastError();
+        g.starts = starts;
+    }
+    return e == cudaSuccess ? run<V>(product_t_few_kernel<V>, blocks * g.splits, g.splits, T_SMEM, g, s) : e;
 }
 
 template <typename V>
@@ -586,7 +730,9 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
     g.ld_dy = ld_dy;
     g.out = d_scales;
     g.d_res = m.res_ptr ? d_res : nullptr;
-    return n_vec <= 8 ? grad_by_width<V, 1>(g, blocks, s) : grad_by_width<V, 2>(g, blocks, s);
+    return m.group == 64   ? grad_of_width<V, 64>(g, blocks, s)
+           : m.group == 32 ? grad_of_width<V, 32>(g, blocks, s)
+                           : grad_of_width<V, 0>(g, blocks, s);
 }
 
 #define INSTANTIATE(V)                                                                                                \

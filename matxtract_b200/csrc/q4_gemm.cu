@@ -502,41 +502,6 @@ __global__ void __launch_bounds__(256) slots_kernel(Matrix<V> m, int chunks, uin
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
-// From the device's stream-ordered pool, which keeps what is given back to it (as for the library's handles).
-cudaError_t pool_memory(void **p, size_t bytes, cudaStream_t s) {
-    static std::atomic<uint64_t> kept{0};  // devices whose pool has been told
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    if (device >= 64 || !(kept.load() >> device & 1)) {
-        cudaMemPool_t pool;
-        uint64_t all = UINT64_MAX;
-        if ((e = cudaDeviceGetDefaultMemPool(&pool, device)) != cudaSuccess ||
-            (e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all)) != cudaSuccess)
-            return e;
-        if (device < 64) kept.fetch_or(1ull << device);
-    }
-    return cudaMallocAsync(p, bytes, s);
-}
-
-// Buffers of one call, given back to the pool in the stream's order when the call returns.
-struct Workspace {
-    cudaStream_t s;
-    void *held[3] = {};
-    int n = 0;
-    explicit Workspace(cudaStream_t s) : s(s) {}
-    ~Workspace() {
-        while (n > 0) cudaFreeAsync(held[--n], s);
-    }
-    cudaError_t take(void **p, size_t bytes) {
-        const cudaError_t e = pool_memory(p, bytes, s);
-        if (e == cudaSuccess) held[n++] = *p;
-        return e;
-    }
-};
-
 using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
