@@ -113,54 +113,65 @@ __device__ __forceinline__ void word_product(float (&d)[NT][4], uint32_t up, uin
 }
 
 // A warp's pieces of 16 rows x 128 columns on their way through shared memory, DEPTH at a time: the codes (64 bytes a
-// row) and the vectors' values at those columns.  Loads into registers two pieces ahead ran at 1.7 TB/s, since a wait
-// for any of them waited for the newest.
+// row) and the vectors' values at those columns (256 bytes a vector, the sixteens of bytes in an order that keeps the
+// reads below apart).  Every address is a lane's constant plus the piece's: with the addresses worked out at each use
+// the kernel issued 470 instructions a piece and was bound by that (44 us for 16384 x 8192, one vector).
 template <typename V, int S, int NT, int DEPTH>
 struct Pieces {
     const Few<V> &g;
-    const uint8_t *up, *low;  // rows `line` and `line` + 8
-    uint8_t *ring;
-    int line, quarter, row_bytes, slot_bytes;
+    const uint8_t *up, *low;  // this lane's 16 bytes of rows `line` and `line` + 8 in a piece at column 0
+    const V *x;               // and its 16 bytes of the vectors
+    uint32_t ring, to;        // the ring, and where the next piece goes
+    const uint8_t *from;      // where the oldest one is
+    int line, quarter, row_bytes, slot_bytes, place_x[4];
     __device__ __forceinline__ Pieces(const Few<V> &g, int row0, uint8_t *smem, int warp, int lane)
         : g(g), line(lane / 4), quarter(lane % 4) {
         const Matrix<V> &m = g.m;
-        row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16);
-        up = m.codes + min(row0 + line, m.n_rows - 1) * m.code_ld;  // the last row again: its results are not used
-        low = m.codes + min(row0 + line + 8, m.n_rows - 1) * m.code_ld;
+        row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16) - 16 * quarter;
+        up = m.codes + min(row0 + line, m.n_rows - 1) * m.code_ld + 16 * quarter;  // the last row again: not used
+        low = m.codes + min(row0 + line + 8, m.n_rows - 1) * m.code_ld + 16 * quarter;
+        x = g.x + lane / 16 * g.ld_x + lane % 16 * 8;
         slot_bytes = bytes(g.n_vec) / DEPTH;
-        ring = smem + warp * bytes(g.n_vec);
+        from = smem + warp * bytes(g.n_vec);
+        ring = to = smem_addr(from);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) place_x[w] = 1024 + line * 256 + ((place<S>(w, quarter) / 8 ^ line) & 15) * 16;
     }
     static __host__ __device__ int bytes(int n_vec) { return DEPTH * (1024 + 256 * n_vec); }  // of a warp
-    // n: the piece's number in the warp's order; k, k1: its columns, and where they end
-    __device__ __forceinline__ void fetch(int n, int k, int k1) {
-        const uint32_t to = smem_addr(ring) + n % DEPTH * slot_bytes;
-        const int at = k / 2 + 16 * quarter, valid = at < row_bytes ? 16 : 0;
-        copy<16>(to + line * 64 + 16 * quarter, up + (valid ? at : 0), valid);
-        copy<16>(to + 512 + line * 64 + 16 * quarter, low + (valid ? at : 0), valid);
+    // k, k1: the piece's columns, and where they end
+    __device__ __forceinline__ void fetch(int lane, int k, int k1) {
+        const bool inside = k / 2 < row_bytes;
+        const int at = inside ? k / 2 : 0, size = inside ? 16 : 0;
+        copy<16>(to + lane * 16, up + at, size);
+        copy<16>(to + 512 + lane * 16, low + at, size);
         if (g.wide_x) {
+            const int c = k + lane % 16 * 8, valid = min(max(k1 - c, 0), 8) * 2;
+            const V *at_x = x + (valid ? k : 0);
 #pragma unroll
-            for (int t = line; t < 8 * NT; t += 8)
-                if (t < g.n_vec)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int c = k + 8 * (4 * quarter + j), size = min(max(k1 - c, 0), 8) * 2;
-                        copy<16>(to + 1024 + t * 256 + ((4 * quarter + j ^ t) & 15) * 16, g.x + t * g.ld_x + (size ? c : 0), size);
-                    }
+            for (int t = lane / 16; t < 8 * NT; t += 2) {
+                if (t < g.n_vec) copy<16>(to + 1024 + t * 256 + ((lane ^ t) & 15) * 16, at_x, valid);
+                at_x += 2 * g.ld_x;
+            }
         }
+        to += slot_bytes;
+        if (to == ring + DEPTH * slot_bytes) to = ring;
     }
     static __device__ __forceinline__ void arrived() {  // the oldest of DEPTH pieces
         wait_copies<DEPTH - 1>();
         __syncwarp();
     }
-    __device__ __forceinline__ const uint8_t *slot(int n) const { return ring + n % DEPTH * slot_bytes; }
-    __device__ __forceinline__ void values_of(uint4 (&x)[NT], int n, int w, int k, int k1) const {
+    __device__ __forceinline__ void free(int n) {  // the oldest piece is used up
+        __syncwarp();
+        from += slot_bytes;
+        if (n % DEPTH == DEPTH - 1) from -= DEPTH * slot_bytes;
+    }
+    __device__ __forceinline__ void values_of(uint4 (&v)[NT], int w, int k, int k1) const {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int t = 8 * j + line, c = place<S>(w, quarter);
-            x[j] = make_uint4(0, 0, 0, 0);
-            if (t >= g.n_vec) continue;
-            x[j] = g.wide_x ? *reinterpret_cast<const uint4 *>(slot(n) + 1024 + t * 256 + ((c / 8 ^ t) & 15) * 16)
-                            : eight(g.x + t * g.ld_x, k + c, k1, false);
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (8 * j + line >= g.n_vec) continue;
+            v[j] = g.wide_x ? *reinterpret_cast<const uint4 *>(from + (place_x[w] ^ (8 * j) * 16) + 2048 * j)
+                            : eight(g.x + (8 * j + line) * g.ld_x, k + place<S>(w, quarter), k1, false);
         }
     }
 };
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_const
     auto column = [&](int n) { return (from + warp + n * WARPS) * 128; };
 #pragma unroll
     for (int n = 0; n < DEPTH - 1; ++n) {
-        if (n < count) ring.fetch(n, column(n), m.n_cols);
+        if (n < count) ring.fetch(lane, column(n), m.n_cols);
         close_copies();
     }
     struct Scale {
@@ -194,14 +205,19 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_const
         int z_up[SEGMENTS], z_low[SEGMENTS];
     };
     GroupOf at((from + warp) * 128, m.group, WARPS * 128);
+    const V *scale_up = m.scales + s_up, *scale_low = m.scales + s_low;
+    const uint8_t *zero_up = m.zeros + s_up, *zero_low = m.zeros + s_low;
     auto scales = [&](Scale &p) {
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
-            const int gr = min(at.after(j * (S / 32)), m.n_groups - 1);
-            p.up[j] = m.scales[s_up + gr];
-            p.low[j] = m.scales[s_low + gr];
-            p.z_up[j] = m.zeros ? m.zeros[s_up + gr] & 15 : 8;
-            p.z_low[j] = m.zeros ? m.zeros[s_low + gr] & 15 : 8;
+            const int gr = j == 0 ? at.g : min(at.after(j * (S / 32)), m.n_groups - 1);
+            p.up[j] = scale_up[gr];
+            p.low[j] = scale_low[gr];
+            p.z_up[j] = p.z_low[j] = 8;
+            if (m.zeros) {
+                p.z_up[j] = zero_up[gr] & 15;
+                p.z_low[j] = zero_low[gr] & 15;
+            }
         }
         at.move();
     };
@@ -230,20 +246,20 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_const
     float total[NT][4] = {};
     for (int n = 0; n < count; ++n) {
         const Scale now = next;
-        if (n + DEPTH - 1 < count) ring.fetch(n + DEPTH - 1, column(n + DEPTH - 1), m.n_cols);
+        if (n + DEPTH - 1 < count) ring.fetch(lane, column(n + DEPTH - 1), m.n_cols);
         close_copies();
         if (n + 1 < count) scales(next);
         ring.arrived();
         uint32_t a[4], b[4];
-        row_codes<S>(a, ring.slot(n) + line * 64, quarter);
-        row_codes<S>(b, ring.slot(n) + 512 + line * 64, quarter);
+        row_codes<S>(a, ring.from + line * 64, quarter);
+        row_codes<S>(b, ring.from + 512 + line * 64, quarter);
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
             float d[NT][4] = {};
 #pragma unroll
             for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w) {
                 uint4 x[NT];
-                ring.values_of(x, n, w, column(n), m.n_cols);
+                ring.values_of(x, w, column(n), m.n_cols);
                 word_product<V, NT>(d, a[w], b[w], now.z_up[j], now.z_low[j], x);
             }
             const float u = to_float(now.up[j]), l = to_float(now.low[j]);
@@ -255,7 +271,7 @@ __global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_const
                 total[q][3] = fmaf(l, d[q][3], total[q][3]);
             }
         }
-        __syncwarp();  // the slot is free again
+        ring.free(n);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -320,7 +336,7 @@ __global__ void __launch_bounds__(THREADS) grad_few_kernel(const __grid_constant
     Pieces<V, WIDTH, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
 #pragma unroll
     for (int n = 0; n < DEPTH - 1; ++n) {
-        if (n < count) ring.fetch(n, begin_of(n), end_of(n));
+        if (n < count) ring.fetch(lane, begin_of(n), end_of(n));
         close_copies();
     }
     if (g.d_res && rank == 0) {
@@ -369,20 +385,20 @@ __global__ void __launch_bounds__(THREADS) grad_few_kernel(const __grid_constant
             z_up[j] = next_up[j];
             z_low[j] = next_low[j];
         }
-        if (n + DEPTH - 1 < count) ring.fetch(n + DEPTH - 1, begin_of(n + DEPTH - 1), end_of(n + DEPTH - 1));
+        if (n + DEPTH - 1 < count) ring.fetch(lane, begin_of(n + DEPTH - 1), end_of(n + DEPTH - 1));
         close_copies();
         if (n + 1 < count) zeros(n + 1);
         ring.arrived();
         uint32_t a[4], b[4];
-        row_codes<WIDTH>(a, ring.slot(n) + line * 64, quarter);
-        row_codes<WIDTH>(b, ring.slot(n) + 512 + line * 64, quarter);
+        row_codes<WIDTH>(a, ring.from + line * 64, quarter);
+        row_codes<WIDTH>(b, ring.from + 512 + line * 64, quarter);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             uint4 x[NT];
-            ring.values_of(x, n, w, begin_of(n), end_of(n));
+            ring.values_of(x, w, begin_of(n), end_of(n));
             word_product<V, NT>(d[w / (WIDTH / 32)], a[w], b[w], z_up[w / (WIDTH / 32)], z_low[w / (WIDTH / 32)], x);
         }
-        __syncwarp();  // the slot is free again
+        ring.free(n);
         if (n % per_unit != per_unit - 1) continue;
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
