@@ -36,16 +36,6 @@ __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// values k .. k + 7 of a vector, 0 from `end` on; `wide`: k is on a 16-byte border
-template <typename V>
-__device__ __forceinline__ uint4 eight(const V *x, int k, int end, bool wide) {
-    if (wide && k + 8 <= end) return __ldg(reinterpret_cast<const uint4 *>(x + k));
-    V v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < end ? x[k + j] : from_float<V>(0.f);
-    return *reinterpret_cast<uint4 *>(v);
-}
-
 // BYTES (8 or 16) into shared memory, of which `size` are read and the others 0
 template <int BYTES>
 __device__ __forceinline__ void copy(uint32_t to, const void *from, int size) {
@@ -89,69 +79,54 @@ struct Few {
     int n_vec, splits;
     const V *x, *dy;
     long long ld_x, ld_dy;
-    bool wide_x, wide_dy;
     V *out;
     long long ld_out;
     V *d_res;
     const int *starts;  // transposed: [block of 256 columns][row] first residual entry not left of the block
 };
 
-// d[tile] += steps of 16 rows x 8 columns (one word of two rows) times the vectors' values at those columns
-template <typename V, int NT>
-__device__ __forceinline__ void word_product(float (&d)[NT][4], uint32_t up, uint32_t low, int z_up, int z_low,
-                                             const uint4 (&x)[NT]) {
-    typename Pair<V>::T p[4], q[4];
-    Pair<V>::steps(up, z_up, p);
-    Pair<V>::steps(low, z_low, q);
-    // codes j and j + 4 share a register; the vectors' values are paired alike
-    const uint32_t a0[4] = {raw(p[0]), raw(q[0]), raw(p[1]), raw(q[1])}, a1[4] = {raw(p[2]), raw(q[2]), raw(p[3]), raw(q[3])};
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        mma16<V>(d[n], a0, __byte_perm(x[n].x, x[n].z, 0x5410), __byte_perm(x[n].x, x[n].z, 0x7632));
-        mma16<V>(d[n], a1, __byte_perm(x[n].y, x[n].w, 0x5410), __byte_perm(x[n].y, x[n].w, 0x7632));
-    }
-}
-
-// A warp's pieces of 16 rows x 128 columns on their way through shared memory, DEPTH at a time: the codes (64 bytes a
+// A warp's pieces of 32 rows x 128 columns on their way through shared memory, DEPTH at a time: the codes (64 bytes a
 // row) and the vectors' values at those columns (256 bytes a vector, the sixteens of bytes in an order that keeps the
-// reads below apart).  Every address is a lane's constant plus the piece's: with the addresses worked out at each use
-// the kernel issued 470 instructions a piece and was bound by that (44 us for 16384 x 8192, one vector).
+// reads below apart).  What bounds the product of one vector is the ALU pipe, which takes the codes apart: every address
+// is a lane's constant plus the piece's, and 32 rows share what the vectors cost (with 16 rows and the addresses worked
+// out at each use: 470 instructions for 1 KB of codes, 44 us for 16384 x 8192).
 template <typename V, int S, int NT, int DEPTH>
 struct Pieces {
-    const Few<V> &g;
-    const uint8_t *up, *low;  // this lane's 16 bytes of rows `line` and `line` + 8 in a piece at column 0
-    const V *x;               // and its 16 bytes of the vectors
-    uint32_t ring, to;        // the ring, and where the next piece goes
-    const uint8_t *from;      // where the oldest one is
-    int line, quarter, row_bytes, slot_bytes, place_x[4];
+    const uint8_t *rows[4];  // this lane's 16 bytes of rows `line` + 8 j in a piece at column 0
+    const V *x;              // and its 16 bytes of the vectors
+    long long ld_x;
+    uint32_t ring, to;       // the ring, and where the next piece goes
+    const uint8_t *from;     // where the oldest one is
+    int lane, n_vec, row_bytes, slot_bytes, place_x[4];
     __device__ __forceinline__ Pieces(const Few<V> &g, int row0, uint8_t *smem, int warp, int lane)
-        : g(g), line(lane / 4), quarter(lane % 4) {
+        : x(g.x + lane / 16 * g.ld_x + lane % 16 * 8), ld_x(2 * g.ld_x), lane(lane), n_vec(g.n_vec) {
         const Matrix<V> &m = g.m;
+        const int line = lane / 4, quarter = lane % 4;
         row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16) - 16 * quarter;
-        up = m.codes + min(row0 + line, m.n_rows - 1) * m.code_ld + 16 * quarter;  // the last row again: not used
-        low = m.codes + min(row0 + line + 8, m.n_rows - 1) * m.code_ld + 16 * quarter;
-        x = g.x + lane / 16 * g.ld_x + lane % 16 * 8;
-        slot_bytes = bytes(g.n_vec) / DEPTH;
-        from = smem + warp * bytes(g.n_vec);
-        ring = to = smem_addr(from);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) place_x[w] = 1024 + line * 256 + ((place<S>(w, quarter) / 8 ^ line) & 15) * 16;
+        for (int j = 0; j < 4; ++j)  // behind the last row the last row again: its results are not used
+            rows[j] = m.codes + min(row0 + line + 8 * j, m.n_rows - 1) * m.code_ld + 16 * quarter;
+        slot_bytes = bytes(n_vec) / DEPTH;
+        from = smem + warp * bytes(n_vec);
+        ring = to = smem_addr(from);
+        const int t = min(line, n_vec - 1);  // the columns of a product behind the last vector are not used
+#pragma unroll
+        for (int w = 0; w < 4; ++w) place_x[w] = 2048 + t * 256 + ((place<S>(w, quarter) / 8 ^ t) & 15) * 16;
     }
-    static __host__ __device__ int bytes(int n_vec) { return DEPTH * (1024 + 256 * n_vec); }  // of a warp
+    static __host__ __device__ int bytes(int n_vec) { return DEPTH * (2048 + 256 * n_vec); }  // of a warp
     // k, k1: the piece's columns, and where they end
-    __device__ __forceinline__ void fetch(int lane, int k, int k1) {
+    __device__ __forceinline__ void fetch(int k, int k1) {
         const bool inside = k / 2 < row_bytes;
         const int at = inside ? k / 2 : 0, size = inside ? 16 : 0;
-        copy<16>(to + lane * 16, up + at, size);
-        copy<16>(to + 512 + lane * 16, low + at, size);
-        if (g.wide_x) {
-            const int c = k + lane % 16 * 8, valid = min(max(k1 - c, 0), 8) * 2;
-            const V *at_x = x + (valid ? k : 0);
 #pragma unroll
-            for (int t = lane / 16; t < 8 * NT; t += 2) {
-                if (t < g.n_vec) copy<16>(to + 1024 + t * 256 + ((lane ^ t) & 15) * 16, at_x, valid);
-                at_x += 2 * g.ld_x;
-            }
+        for (int j = 0; j < 4; ++j) copy<16>(to + 512 * j + lane * 16, rows[j] + at, size);
+        const int valid = min(max(k1 - k - lane % 16 * 8, 0), 8) * 2;
+        const V *at_x = x + (valid ? k : 0);
+#pragma unroll
+        for (int j = 0; j < 4 * NT; ++j) {
+            const int t = lane / 16 + 2 * j;
+            if (t < n_vec) copy<16>(to + 2048 + t * 256 + ((lane ^ t) & 15) * 16, at_x, valid);
+            at_x += ld_x;
         }
         to += slot_bytes;
         if (to == ring + DEPTH * slot_bytes) to = ring;
@@ -160,187 +135,221 @@ struct Pieces {
         wait_copies<DEPTH - 1>();
         __syncwarp();
     }
-    __device__ __forceinline__ void free(int n) {  // the oldest piece is used up
+    __device__ __forceinline__ void free() {  // the oldest piece is used up
         __syncwarp();
         from += slot_bytes;
-        if (n % DEPTH == DEPTH - 1) from -= DEPTH * slot_bytes;
+        if (smem_addr(from) == ring + DEPTH * slot_bytes) from -= DEPTH * slot_bytes;
     }
-    __device__ __forceinline__ void values_of(uint4 (&v)[NT], int w, int k, int k1) const {
+    // word w of the oldest piece's columns, of the vectors 8 j + line; codes j and j + 4 of a word share a register, and
+    // the vectors' values are paired alike
+    __device__ __forceinline__ void values_of(uint32_t (&v)[NT][4], int w) const {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            v[j] = make_uint4(0, 0, 0, 0);
-            if (8 * j + line >= g.n_vec) continue;
-            v[j] = g.wide_x ? *reinterpret_cast<const uint4 *>(from + (place_x[w] ^ (8 * j) * 16) + 2048 * j)
-                            : eight(g.x + (8 * j + line) * g.ld_x, k + place<S>(w, quarter), k1, false);
+            // 8 vectors on: 2048 bytes, and the other half of the order; behind the last vector anything will do
+            const int at = j == 0 || 8 * j + lane / 4 < n_vec ? (place_x[w] ^ 128 * j) + 2048 * j : place_x[w];
+            const uint4 u = *reinterpret_cast<const uint4 *>(from + at);
+            v[j][0] = __byte_perm(u.x, u.z, 0x5410);
+            v[j][1] = __byte_perm(u.x, u.z, 0x7632);
+            v[j][2] = __byte_perm(u.y, u.w, 0x5410);
+            v[j][3] = __byte_perm(u.y, u.w, 0x7632);
         }
     }
 };
 
-// y = W x for up to 8 NT vectors.  A block has 16 rows; its warps take the 128-column pieces in turn, and the blocks of
+// d += 16 rows x 8 columns (a word of the upper and of the lower eight rows) times the vectors' values
+template <typename V, int NT>
+__device__ __forceinline__ void word_product(float (&d)[NT][4], uint32_t up, uint32_t low, int z_up, int z_low,
+                                             const uint32_t (&x)[NT][4]) {
+    typename Pair<V>::T p[4], q[4];
+    Pair<V>::steps(up, z_up, p);
+    Pair<V>::steps(low, z_low, q);
+    const uint32_t a0[4] = {raw(p[0]), raw(q[0]), raw(p[1]), raw(q[1])}, a1[4] = {raw(p[2]), raw(q[2]), raw(p[3]), raw(q[3])};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        mma16<V>(d[n], a0, x[n][0], x[n][1]);
+        mma16<V>(d[n], a1, x[n][2], x[n][3]);
+    }
+}
+
+// Scales (bits 0-15) and zero points (from bit 16) of a piece's 32 rows, a lane a row, in its SEGMENTS groups.
+template <int SEGMENTS>
+struct Numbers {
+    uint32_t v[SEGMENTS];
+};
+
+constexpr int ROWS = 32;
+
+// y = W x for up to 8 NT vectors.  A block has 32 rows; its warps take the 128-column pieces in turn, and the blocks of
 // a cluster (where there are too few rows to occupy the GPU) take contiguous parts of them; the parts are added in the
 // order of warps and ranks.
 template <typename V, int S, int NT, int DEPTH>
-__global__ void __launch_bounds__(THREADS) product_few_kernel(const __grid_constant__ Few<V> g) {
+__global__ void __launch_bounds__(THREADS, 2) product_few_kernel(const __grid_constant__ Few<V> g) {
     extern __shared__ uint4 smem[];
-    __shared__ float part[WARPS][8 * NT][17];
-    __shared__ float sum[8 * NT][16];
+    __shared__ float part[WARPS][8 * NT][ROWS + 1];
+    __shared__ float sum[8 * NT][ROWS];
     const Matrix<V> &m = g.m;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
-    const int rank = g.splits > 1 ? (int)cluster_rank() : 0, row0 = blockIdx.x / g.splits * 16;
+    const int rank = g.splits > 1 ? (int)cluster_rank() : 0, row0 = blockIdx.x / g.splits * ROWS;
     const int pieces = (int)(((long long)m.n_cols + 127) / 128);
     const int from = (int)((long long)pieces * rank / g.splits), to = (int)((long long)pieces * (rank + 1) / g.splits);
-    const long long s_up = (long long)min(row0 + line, m.n_rows - 1) * m.n_groups;
-    const long long s_low = (long long)min(row0 + line + 8, m.n_rows - 1) * m.n_groups;
     constexpr int SEGMENTS = 128 / S;
     Pieces<V, S, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
-    const int count = from + warp < to ? (to - from - warp - 1) / WARPS + 1 : 0;
-    auto column = [&](int n) { return (from + warp + n * WARPS) * 128; };
+    int ahead = from + warp;  // the piece to fetch next
 #pragma unroll
     for (int n = 0; n < DEPTH - 1; ++n) {
-        if (n < count) ring.fetch(lane, column(n), m.n_cols);
+        if (ahead < to) ring.fetch(ahead * 128, m.n_cols);
         close_copies();
+        ahead += WARPS;
     }
-    struct Scale {
-        V up[SEGMENTS], low[SEGMENTS];
-        int z_up[SEGMENTS], z_low[SEGMENTS];
-    };
     GroupOf at((from + warp) * 128, m.group, WARPS * 128);
-    const V *scale_up = m.scales + s_up, *scale_low = m.scales + s_low;
-    const uint8_t *zero_up = m.zeros + s_up, *zero_low = m.zeros + s_low;
-    auto scales = [&](Scale &p) {
+    const long long my_row = (long long)min(row0 + lane, m.n_rows - 1) * m.n_groups;
+    const uint16_t *scales = reinterpret_cast<const uint16_t *>(m.scales) + my_row;
+    const uint8_t *zeros = m.zeros + my_row;
+    Numbers<SEGMENTS> next;
+    auto numbers = [&] {
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
             const int gr = j == 0 ? at.g : min(at.after(j * (S / 32)), m.n_groups - 1);
-            p.up[j] = scale_up[gr];
-            p.low[j] = scale_low[gr];
-            p.z_up[j] = p.z_low[j] = 8;
-            if (m.zeros) {
-                p.z_up[j] = zero_up[gr] & 15;
-                p.z_low[j] = zero_low[gr] & 15;
-            }
+            next.v[j] = scales[gr];
+            if (m.zeros) next.v[j] |= (uint32_t)(zeros[gr] & 15) << 16;
         }
         at.move();
     };
-    Scale next;
-    if (count > 0) scales(next);
+    if (from + warp < to) numbers();
 
-    // the residual, while the first pieces are on their way: two rows a warp
-    float extra[2][8 * NT] = {};
+    // the residual, while the first pieces are on their way: four rows a warp
     if (m.res_ptr && rank == 0) {
-        int begin[2] = {0, 0}, end[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (row0 + 2 * warp + j < m.n_rows) res_range(m, row0 + 2 * warp + j, begin[j], end[j]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            for (int e = begin[j] + lane; e < end[j]; e += 32) {
+        int begin = 0, end = 0;
+        if (lane < 4 && row0 + 4 * warp + lane < m.n_rows) res_range(m, row0 + 4 * warp + lane, begin, end);
+        for (int j = 0; j < 4; ++j) {
+            const int b = __shfl_sync(0xffffffffu, begin, j), e1 = __shfl_sync(0xffffffffu, end, j);
+            float extra[8 * NT] = {};
+            for (int e = b + lane; e < e1; e += 32) {
                 const int k = m.res_col[e];
                 const float v = to_float(m.res_val[e]);
                 if (k < 0 || k >= m.n_cols) continue;
 #pragma unroll
                 for (int t = 0; t < 8 * NT; ++t)
-                    if (t < g.n_vec) extra[j][t] = fmaf(v, to_float(g.x[t * g.ld_x + k]), extra[j][t]);
+                    if (t < g.n_vec) extra[t] = fmaf(v, to_float(g.x[t * g.ld_x + k]), extra[t]);
             }
-    }
-
-    float total[NT][4] = {};
-    for (int n = 0; n < count; ++n) {
-        const Scale now = next;
-        if (n + DEPTH - 1 < count) ring.fetch(lane, column(n + DEPTH - 1), m.n_cols);
-        close_copies();
-        if (n + 1 < count) scales(next);
-        ring.arrived();
-        uint32_t a[4], b[4];
-        row_codes<S>(a, ring.from + line * 64, quarter);
-        row_codes<S>(b, ring.from + 512 + line * 64, quarter);
-#pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            float d[NT][4] = {};
-#pragma unroll
-            for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w) {
-                uint4 x[NT];
-                ring.values_of(x, w, column(n), m.n_cols);
-                word_product<V, NT>(d, a[w], b[w], now.z_up[j], now.z_low[j], x);
-            }
-            const float u = to_float(now.up[j]), l = to_float(now.low[j]);
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-                total[q][0] = fmaf(u, d[q][0], total[q][0]);
-                total[q][1] = fmaf(u, d[q][1], total[q][1]);
-                total[q][2] = fmaf(l, d[q][2], total[q][2]);
-                total[q][3] = fmaf(l, d[q][3], total[q][3]);
-            }
-        }
-        ring.free(n);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[warp][8 * n + 2 * quarter + j % 2][line + 8 * (j / 2)] = total[n][j];
-    if (m.res_ptr && rank == 0) {
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
+            __syncwarp();
 #pragma unroll
             for (int t = 0; t < 8 * NT; ++t) {
                 if (t >= g.n_vec) break;
-                for (int d = 16; d; d /= 2) extra[j][t] += __shfl_xor_sync(0xffffffffu, extra[j][t], d);
-                if (lane == 0) part[warp][t][2 * warp + j] += extra[j][t];
+                for (int d = 16; d; d /= 2) extra[t] += __shfl_xor_sync(0xffffffffu, extra[t], d);
+                if (lane == 0) sum[t][4 * warp + j] = extra[t];
             }
+        }
     }
+
+    float total[2][NT][4] = {};
+    for (int piece = from + warp; piece < to; piece += WARPS) {
+        const Numbers<SEGMENTS> now = next;
+        if (ahead < to) ring.fetch(ahead * 128, m.n_cols);
+        close_copies();
+        ahead += WARPS;
+        if (piece + WARPS < to) numbers();
+        ring.arrived();
+        uint32_t c[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row_codes<S>(c[j], ring.from + 512 * j + line * 64, quarter);
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) {
+            float d[2][NT][4] = {};
+            int z[4] = {8, 8, 8, 8};
+            float s[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t v = __shfl_sync(0xffffffffu, now.v[j], line + 8 * r);
+                const uint16_t bits = (uint16_t)v;
+                s[r] = to_float(*reinterpret_cast<const V *>(&bits));
+                if (m.zeros) z[r] = v >> 16;
+            }
+#pragma unroll
+            for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w) {
+                uint32_t x[NT][4];
+                ring.values_of(x, w);
+                word_product<V, NT>(d[0], c[0][w], c[1][w], z[0], z[1], x);
+                word_product<V, NT>(d[1], c[2][w], c[3][w], z[2], z[3], x);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < NT; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) total[h][q][e] = fmaf(s[2 * h + e / 2], d[h][q][e], total[h][q][e]);
+        }
+        ring.free();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                part[warp][8 * n + 2 * quarter + j % 2][line + 8 * (j / 2) + 16 * h] = total[h][n][j];
     __syncthreads();
-    const int row = threadIdx.x % 16, t = threadIdx.x / 16;
-    if (t < 8 * NT) {
-        float s = 0.f;
+    const int row = lane;
+    for (int t = warp; t < g.n_vec; t += WARPS) {
+        float s = m.res_ptr && rank == 0 ? sum[t][row] : 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) s += part[w][t][row];
         if (g.splits > 1) {
             sum[t][row] = s;
-        } else if (t < g.n_vec && row0 + row < m.n_rows) {
+        } else if (row0 + row < m.n_rows) {
             g.out[t * g.ld_out + row0 + row] = from_float<V>(s);
         }
     }
     if (g.splits > 1) {
         __syncthreads();
         cluster_barrier();
-        if (rank == 0 && t < g.n_vec && row0 + row < m.n_rows) {
-            float s = 0.f;
-            for (int r = 0; r < g.splits; ++r) s += cluster_load(smem_addr(&sum[t][row]), r);
-            g.out[t * g.ld_out + row0 + row] = from_float<V>(s);
+        if (rank == 0) {
+            for (int t = warp; t < g.n_vec; t += WARPS) {
+                float s = 0.f;
+                for (int r = 0; r < g.splits; ++r) s += cluster_load(smem_addr(&sum[t][row]), r);
+                if (row0 + row < m.n_rows) g.out[t * g.ld_out + row0 + row] = from_float<V>(s);
+            }
         }
         __syncwarp();
         cluster_barrier();
     }
 }
 
-// Gradients from up to 8 NT vectors.  A block has 16 rows and a part of the groups, a warp whole groups of them: the
+// Gradients from up to 8 NT vectors.  A block has 32 rows and a part of the groups, a warp whole groups of them: the
 // sums over a group's columns for each vector are the product's, then they are weighed with dy instead of the scale.
 // S = 0: one group after the other, in pieces of 128 columns; else a piece has 128 / S groups.
 template <typename V, int S, int NT, int DEPTH>
-__global__ void __launch_bounds__(THREADS) grad_few_kernel(const __grid_constant__ Few<V> g) {
+__global__ void __launch_bounds__(THREADS, 2) grad_few_kernel(const __grid_constant__ Few<V> g) {
     extern __shared__ uint4 smem[];
     const Matrix<V> &m = g.m;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
-    const int row0 = blockIdx.x / g.splits * 16, rank = blockIdx.x % g.splits;
-    const bool real0 = row0 + line < m.n_rows, real1 = row0 + line + 8 < m.n_rows;
-    const int i0 = min(row0 + line, m.n_rows - 1), i1 = min(row0 + line + 8, m.n_rows - 1);
+    const int row0 = blockIdx.x / g.splits * ROWS, rank = blockIdx.x % g.splits;
     constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH;
-    const int units = (m.n_groups + SEGMENTS - 1) / SEGMENTS, first = rank * WARPS + warp, stride = g.splits * WARPS;
-    const int per_unit = S ? 1 : (m.group + 127) / 128;
-    const int mine = g.out && first < units ? (units - first - 1) / stride + 1 : 0, count = mine * per_unit;
-    // of piece n: where its columns begin, and where its group's (or the matrix's) end
-    auto begin_of = [&](int n) { return (first + n / per_unit * stride) * SEGMENTS * m.group + n % per_unit * 128; };
-    auto end_of = [&](int n) {
-        return S ? m.n_cols : (int)min((long long)m.n_cols, ((long long)first + n / per_unit * stride + 1) * m.group);
+    const int units = (m.n_groups + SEGMENTS - 1) / SEGMENTS, stride = g.splits * WARPS, width = SEGMENTS * m.group;
+    // a place in the warp's order of pieces: its unit, and where its columns begin and end
+    struct Place {
+        int unit, k, k1;
     };
+    auto enter = [&](int unit) {
+        const long long k = (long long)unit * width;
+        return Place{unit, (int)min(k, (long long)INT_MAX), (int)min((long long)m.n_cols, k + width)};
+    };
+    auto move = [&](Place &p) {
+        p.k += 128;
+        if (S || p.k >= p.k1) p = enter(p.unit + stride);
+    };
+    Place here = enter(g.out ? rank * WARPS + warp : units), ahead = here;
     Pieces<V, WIDTH, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
 #pragma unroll
     for (int n = 0; n < DEPTH - 1; ++n) {
-        if (n < count) ring.fetch(lane, begin_of(n), end_of(n));
+        if (ahead.unit < units) {
+            ring.fetch(ahead.k, ahead.k1);
+            move(ahead);
+        }
         close_copies();
     }
     if (g.d_res && rank == 0) {
-        for (int r = 2 * warp; r < 2 * warp + 2 && row0 + r < m.n_rows; ++r) {
+        for (int r = 4 * warp; r < 4 * warp + 4 && row0 + r < m.n_rows; ++r) {
             const int i = row0 + r;
             int begin, end;
             res_range(m, i, begin, end);
@@ -358,66 +367,77 @@ __global__ void __launch_bounds__(THREADS) grad_few_kernel(const __grid_constant
             }
         }
     }
-    const long long s_up = (long long)i0 * m.n_groups, s_low = (long long)i1 * m.n_groups;
-    float dy[NT][4];
+    long long of_row[4];
+    float dy[4][NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int r = 0; r < 4; ++r) {
+        const int i = min(row0 + line + 8 * r, m.n_rows - 1);
+        of_row[r] = (long long)i * m.n_groups;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int t = 8 * n + 2 * quarter + j % 2;
-            dy[n][j] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + (j < 2 ? i0 : i1)]) : 0.f;
-        }
-    float d[SEGMENTS][NT][4] = {};
-    int next_up[SEGMENTS], next_low[SEGMENTS];
-    auto zeros = [&](int n) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            const int gr = min((first + n / per_unit * stride) * SEGMENTS + j, m.n_groups - 1);
-            next_up[j] = m.zeros ? m.zeros[s_up + gr] & 15 : 8;
-            next_low[j] = m.zeros ? m.zeros[s_low + gr] & 15 : 8;
-        }
+            for (int j = 0; j < 2; ++j) {
+                const int t = 8 * n + 2 * quarter + j;
+                dy[r][n][j] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
+            }
+    }
+    const uint8_t *zeros = m.zeros + (long long)min(row0 + lane, m.n_rows - 1) * m.n_groups;
+    float d[SEGMENTS][2][NT][4] = {};
+    int next[SEGMENTS];
+    auto fetch_zeros = [&](int unit) {
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) next[j] = m.zeros ? zeros[min(unit * SEGMENTS + j, m.n_groups - 1)] & 15 : 8;
     };
-    if (count > 0) zeros(0);
-    for (int n = 0; n < count; ++n) {
-        int z_up[SEGMENTS], z_low[SEGMENTS];
+    if (here.unit < units) fetch_zeros(here.unit);
+    while (here.unit < units) {
+        int now[SEGMENTS];
 #pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            z_up[j] = next_up[j];
-            z_low[j] = next_low[j];
+        for (int j = 0; j < SEGMENTS; ++j) now[j] = next[j];
+        if (ahead.unit < units) {
+            ring.fetch(ahead.k, ahead.k1);
+            move(ahead);
         }
-        if (n + DEPTH - 1 < count) ring.fetch(lane, begin_of(n + DEPTH - 1), end_of(n + DEPTH - 1));
         close_copies();
-        if (n + 1 < count) zeros(n + 1);
+        const Place was = here;
+        move(here);
+        if (here.unit < units) fetch_zeros(here.unit);
         ring.arrived();
-        uint32_t a[4], b[4];
-        row_codes<WIDTH>(a, ring.from + line * 64, quarter);
-        row_codes<WIDTH>(b, ring.from + 512 + line * 64, quarter);
+        uint32_t c[4][4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint4 x[NT];
-            ring.values_of(x, w, begin_of(n), end_of(n));
-            word_product<V, NT>(d[w / (WIDTH / 32)], a[w], b[w], z_up[w / (WIDTH / 32)], z_low[w / (WIDTH / 32)], x);
-        }
-        ring.free(n);
-        if (n % per_unit != per_unit - 1) continue;
+        for (int j = 0; j < 4; ++j) row_codes<WIDTH>(c[j], ring.from + 512 * j + line * 64, quarter);
 #pragma unroll
         for (int j = 0; j < SEGMENTS; ++j) {
-            float e0 = 0.f, e1 = 0.f;
+            int z[4];
 #pragma unroll
-            for (int q = 0; q < NT; ++q) {
-                e0 = fmaf(dy[q][0], d[j][q][0], fmaf(dy[q][1], d[j][q][1], e0));
-                e1 = fmaf(dy[q][2], d[j][q][2], fmaf(dy[q][3], d[j][q][3], e1));
-                d[j][q][0] = d[j][q][1] = d[j][q][2] = d[j][q][3] = 0.f;
-            }
+            for (int r = 0; r < 4; ++r) z[r] = m.zeros ? __shfl_sync(0xffffffffu, now[j], line + 8 * r) : 8;
 #pragma unroll
-            for (int x = 1; x < 4; x *= 2) {
-                e0 += __shfl_xor_sync(0xffffffffu, e0, x);
-                e1 += __shfl_xor_sync(0xffffffffu, e1, x);
+            for (int w = j * (WIDTH / 32); w < (j + 1) * (WIDTH / 32); ++w) {
+                uint32_t x[NT][4];
+                ring.values_of(x, w);
+                word_product<V, NT>(d[j][0], c[0][w], c[1][w], z[0], z[1], x);
+                word_product<V, NT>(d[j][1], c[2][w], c[3][w], z[2], z[3], x);
             }
-            const int gr = (first + n / per_unit * stride) * SEGMENTS + j;
-            if (quarter == 0 && gr < m.n_groups) {
-                if (real0) g.out[s_up + gr] = from_float<V>(e0);
-                if (real1) g.out[s_low + gr] = from_float<V>(e1);
+        }
+        ring.free();
+        if (here.unit == was.unit) continue;  // more of the group to come
+#pragma unroll
+        for (int j = 0; j < SEGMENTS; ++j) {
+            const int gr = was.unit * SEGMENTS + j;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float e = 0.f;
+#pragma unroll
+                for (int q = 0; q < NT; ++q)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float &v = d[j][r / 2][q][2 * (r % 2) + t];
+                        e = fmaf(dy[r][q][t], 8 * q + 2 * quarter + t < g.n_vec ? v : 0.f, e);
+                        v = 0.f;
+                    }
+                e += __shfl_xor_sync(0xffffffffu, e, 1);
+                e += __shfl_xor_sync(0xffffffffu, e, 2);
+                if (quarter == 0 && gr < m.n_groups && row0 + line + 8 * r < m.n_rows)
+                    g.out[of_row[r] + gr] = from_float<V>(e);
             }
         }
     }
@@ -479,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
             const bool real = inside && i0 + j < m.n_rows;
             copy<16>(slot + 512 * j, m.codes + (real ? (i0 + j) * m.code_ld + k / 2 : 0), real ? 16 : 0);
         }
-        if (g.wide_dy && line < g.n_vec) {
+        if (line < g.n_vec) {
             const int size = min(max(m.n_rows - i0, 0), 4) * 2;
             copy<8>(slot + 2048 - lane * 8, g.dy + line * g.ld_dy + (size ? i0 : 0), size);
         }
@@ -510,18 +530,8 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
         if (n + 1 < count) scales(n + 1);
         wait_copies<T_DEPTH - 1>();
         const uint8_t *slot = ring + n % T_DEPTH * T_SLOT;
-        uint2 dy = make_uint2(0, 0);
-        if (line < g.n_vec) {
-            if (g.wide_dy) {
-                dy = *reinterpret_cast<const uint2 *>(slot + 2048 - lane * 8);
-            } else {
-                const V *p = g.dy + line * g.ld_dy + rows_of(n);
-                V v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = rows_of(n) + j < m.n_rows ? p[j] : from_float<V>(0.f);
-                dy = *reinterpret_cast<uint2 *>(v);
-            }
-        }
+        // behind the last vector anything will do
+        const uint2 dy = *reinterpret_cast<const uint2 *>(slot + 2048 - lane * 8);
         uint32_t c[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -625,9 +635,22 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
     cluster_barrier();
 }
 
+// sums over no vectors: 0 for every scale and every residual entry that there is
 template <typename V>
-bool on_border(const V *p, long long ld, int n_vec, int values) {
-    return (uintptr_t)p % (2 * values) == 0 && (ld % values == 0 || n_vec == 1);
+__global__ void no_gradient_kernel(Matrix<V> m, V *d_scales, V *d_res) {
+    const int warp = (blockIdx.x * THREADS + threadIdx.x) / 32, lane = threadIdx.x % 32;
+    if (warp >= m.n_rows) return;
+    if (d_scales)
+        for (int j = lane; j < m.n_groups; j += 32) d_scales[(long long)warp * m.n_groups + j] = from_float<V>(0.f);
+    if (!d_res) return;
+    int begin, end;
+    res_range(m, warp, begin, end);
+    for (int e = begin + lane; e < end; e += 32) d_res[e] = from_float<V>(0.f);
+}
+template <typename V>
+cudaError_t no_gradient(const Matrix<V> &m, V *d_scales, V *d_res, cudaStream_t s) {
+    no_gradient_kernel<<<(unsigned)ceil_div(m.n_rows, WARPS), THREADS, 0, s>>>(m, d_scales, d_res);
+    return cudaGetLastError();
 }
 
 template <typename V>
@@ -656,30 +679,30 @@ int parts_of(long long blocks, long long pieces) {
 
 template <typename V, auto KERNEL>
 cudaError_t run_ring(const Few<V> &g, long long blocks, int cluster, int warp_bytes, cudaStream_t s) {
-    const cudaError_t e = allow_smem<V, KERNEL>(WARPS * 4 * (1024 + 256 * 16));
+    const cudaError_t e = allow_smem<V, KERNEL>(WARPS * 3 * (2048 + 256 * 8));
     return e == cudaSuccess ? run<V>(KERNEL, blocks, cluster, WARPS * warp_bytes, g, s) : e;
 }
 
-// Pieces under way: 8 a warp for one or two vectors, 4 for more, whose values take more room (two blocks an SM, one for
-// more than 8 vectors).
+// Pieces under way: four a warp for one or two vectors, three or two for more, whose values take more room, so that two
+// blocks fit an SM.
 template <typename V, int S>
 cudaError_t product_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
     blocks *= g.splits;
     if (g.n_vec <= 2)
-        return run_ring<V, product_few_kernel<V, S, 1, 8>>(g, blocks, g.splits, Pieces<V, S, 1, 8>::bytes(g.n_vec), s);
-    if (g.n_vec <= 8)
         return run_ring<V, product_few_kernel<V, S, 1, 4>>(g, blocks, g.splits, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
-    return run_ring<V, product_few_kernel<V, S, 2, 4>>(g, blocks, g.splits, Pieces<V, S, 2, 4>::bytes(g.n_vec), s);
+    if (g.n_vec <= 8)
+        return run_ring<V, product_few_kernel<V, S, 1, 3>>(g, blocks, g.splits, Pieces<V, S, 1, 3>::bytes(g.n_vec), s);
+    return run_ring<V, product_few_kernel<V, S, 2, 2>>(g, blocks, g.splits, Pieces<V, S, 2, 2>::bytes(g.n_vec), s);
 }
 
 template <typename V, int S>
 cudaError_t grad_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
     blocks *= g.splits;
     if (g.n_vec <= 2)
-        return run_ring<V, grad_few_kernel<V, S, 1, 8>>(g, blocks, 1, Pieces<V, S, 1, 8>::bytes(g.n_vec), s);
-    if (g.n_vec <= 8)
         return run_ring<V, grad_few_kernel<V, S, 1, 4>>(g, blocks, 1, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
-    return run_ring<V, grad_few_kernel<V, S, 2, 4>>(g, blocks, 1, Pieces<V, S, 2, 4>::bytes(g.n_vec), s);
+    if (g.n_vec <= 8)
+        return run_ring<V, grad_few_kernel<V, S, 1, 3>>(g, blocks, 1, Pieces<V, S, 1, 3>::bytes(g.n_vec), s);
+    return run_ring<V, grad_few_kernel<V, S, 2, 2>>(g, blocks, 1, Pieces<V, S, 2, 2>::bytes(g.n_vec), s);
 }
 
 }  // namespace
@@ -687,16 +710,16 @@ cudaError_t grad_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
 template <typename V>
 cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
     if (n_vec > 16) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
-    const long long blocks = ((long long)m.n_rows + 15) / 16;
+    const long long blocks = ceil_div(m.n_rows, ROWS);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, ((long long)m.n_cols + 127) / 128);
-    g.x = x;
-    g.ld_x = ld_x;
-    g.wide_x = on_border(x, ld_x, n_vec, 8);
+    g.splits = parts_of(blocks, ceil_div(m.n_cols, 128));
     g.out = y;
     g.ld_out = ld_y;
+    Workspace work(s);
+    cudaError_t e = aligned_rows(x, ld_x, m.n_cols, n_vec, work, &g.x, &g.ld_x);
+    if (e != cudaSuccess) return e;
     return m.group % 128 == 0  ? product_of_width<V, 128>(g, blocks, s)
            : m.group % 64 == 0 ? product_of_width<V, 64>(g, blocks, s)
                                : product_of_width<V, 32>(g, blocks, s);
@@ -706,18 +729,16 @@ template <typename V>
 cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
                       cudaStream_t s) {
     if (n_vec > VEC) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
-    const long long blocks = ((long long)m.n_cols + COLS - 1) / COLS;
+    const long long blocks = ceil_div(m.n_cols, COLS);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, ((long long)m.n_rows + 15) / 16);
-    g.dy = dy;
-    g.ld_dy = ld_dy;
-    g.wide_dy = on_border(dy, ld_dy, n_vec, 4);
+    g.splits = parts_of(blocks, ceil_div(m.n_rows, 16));
     g.out = dx;
     g.ld_out = ld_dx;
     Workspace work(s);
-    cudaError_t e = allow_smem<V, product_t_few_kernel<V>>(T_SMEM);
+    cudaError_t e = aligned_rows(dy, ld_dy, m.n_rows, n_vec, work, &g.dy, &g.ld_dy);
+    if (e == cudaSuccess) e = allow_smem<V, product_t_few_kernel<V>>(T_SMEM);
     if (e == cudaSuccess && m.res_ptr && m.n_rows > 0) {
         const long long chunks = ceil_div(blocks + 1, 64), grid = ceil_div(m.n_rows, 32) * chunks;
         int *starts = nullptr;
@@ -734,18 +755,19 @@ template <typename V>
 cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy, V *d_scales,
                  V *d_res, cudaStream_t s) {
     if (n_vec > 16) return grad_many(m, n_vec, x, ld_x, dy, ld_dy, d_scales, d_res, s);
-    const long long blocks = ((long long)m.n_rows + 15) / 16;
+    if (n_vec == 0) return no_gradient(m, d_scales, m.res_ptr ? d_res : nullptr, s);
+    const long long blocks = ceil_div(m.n_rows, ROWS);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, m.group <= 64 ? (m.n_groups * (long long)m.group + 127) / 128 : m.n_groups);
-    g.x = x;
-    g.ld_x = ld_x;
-    g.wide_x = on_border(x, ld_x, n_vec, 8);
+    g.splits = parts_of(blocks, m.group <= 64 ? ceil_div(m.n_groups * (long long)m.group, 128) : m.n_groups);
     g.dy = dy;
     g.ld_dy = ld_dy;
     g.out = d_scales;
     g.d_res = m.res_ptr ? d_res : nullptr;
+    Workspace work(s);
+    cudaError_t e = aligned_rows(x, ld_x, m.n_cols, n_vec, work, &g.x, &g.ld_x);
+    if (e != cudaSuccess) return e;
     return m.group == 64   ? grad_of_width<V, 64>(g, blocks, s)
            : m.group == 32 ? grad_of_width<V, 32>(g, blocks, s)
                            : grad_of_width<V, 0>(g, blocks, s);

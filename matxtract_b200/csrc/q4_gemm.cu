@@ -533,37 +533,11 @@ bool encode_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long 
                   p, cols, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// to[r][c] = from[r][c]
+// The tensor map of `rows` vectors.
 template <typename V>
-__global__ void align_kernel(const V *from, long long ld, V *to, long long ld_to, long long rows, int cols) {
-    const long long stride = (long long)gridDim.y * blockDim.y;
-    const long long c = ((long long)blockIdx.x * 32 + threadIdx.x) * 8;
-    for (long long r = (long long)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += stride) {
-        if (c >= cols) continue;
-        V v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? from[r * ld + c + j] : from_float<V>(0.f);
-        *reinterpret_cast<uint4 *>(to + r * ld_to + c) = *reinterpret_cast<uint4 *>(v);
-    }
-}
-
-// The tensor map of `rows` vectors.  Bulk copies want rows on 16-byte borders: others are copied to such rows first
-// (2048 x 8192 values: 13 us; fetching them value by value inside the kernel took several times the product's time).
-template <typename V>
-cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work,
-                        cudaStream_t s) {
-    if (rows == 1) ld = ceil_div(cols, 8) * 8;
-    if ((uintptr_t)p % 16 || ld % 8) {
-        V *copy = nullptr;
-        const long long ld_copy = ceil_div(cols, 8) * 8;
-        cudaError_t e = work.take((void **)&copy, sizeof(V) * ld_copy * rows);
-        if (e != cudaSuccess) return e;
-        const dim3 block(32, 8), grid((unsigned)ceil_div(ld_copy, 256), (unsigned)std::min<long long>(ceil_div(rows, 8), 65535));
-        align_kernel<<<grid, block, 0, s>>>(p, ld, copy, ld_copy, rows, cols);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-        p = copy;
-        ld = ld_copy;
-    }
+cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work) {
+    cudaError_t e = aligned_rows(p, ld, cols, rows, work, &p, &ld);
+    if (e != cudaSuccess) return e;
     return encode_vectors(map, p, cols, rows, ld, box_rows) ? cudaSuccess : cudaErrorInvalidValue;
 }
 
@@ -628,7 +602,7 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (!encode(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, m.codes, ceil_div(m.n_cols, 32) * 16, m.n_rows, m.code_ld, 64,
                     128, CU_TENSOR_MAP_SWIZZLE_64B))
             return cudaErrorInvalidValue;
-        cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn, work, s);
+        cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn, work);
         if (e != cudaSuccess) return e;
         if (m.res_ptr) {
             // whole tiles of 128 rows: rows behind the last have empty slots
@@ -678,8 +652,8 @@ cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x,
     CUtensorMap a = {}, b = {};
     Workspace work(s);
     if (n_vec > 0) {
-        cudaError_t e = map_vectors(&a, dy, m.n_rows, n_vec, ld_dy, 64, work, s);
-        if (e == cudaSuccess) e = map_vectors(&b, x, m.n_cols, n_vec, ld_x, 64, work, s);
+        cudaError_t e = map_vectors(&a, dy, m.n_rows, n_vec, ld_dy, 64, work);
+        if (e == cudaSuccess) e = map_vectors(&b, x, m.n_cols, n_vec, ld_x, 64, work);
         if (e != cudaSuccess) return e;
     }
     return launch<V, GRADIENT, 256>(a, a, b, g, g.tiles_m * ceil_div(m.n_groups, g.groups_per_unit), s);

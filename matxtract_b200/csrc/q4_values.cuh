@@ -2,6 +2,7 @@
 #pragma once
 #include <limits.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "q4.h"
@@ -106,6 +107,39 @@ struct Workspace {
         return e;
     }
 };
+
+// to[r][c] = from[r][c]
+template <typename V>
+__global__ void align_kernel(const V *from, long long ld, V *to, long long ld_to, long long rows, int cols) {
+    const long long stride = (long long)gridDim.y * blockDim.y;
+    const long long c = ((long long)blockIdx.x * 32 + threadIdx.x) * 8;
+    for (long long r = (long long)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += stride) {
+        if (c >= cols) continue;
+        V v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? from[r * ld + c + j] : from_float<V>(0.f);
+        *reinterpret_cast<uint4 *>(to + r * ld_to + c) = *reinterpret_cast<uint4 *>(v);
+    }
+}
+
+// Vectors that bulk and 16-byte copies can fetch: rows on 16-byte borders.  Others are copied to such rows first
+// (2048 x 8192 values: 13 us; fetching them value by value inside the kernel took several times the product's time).
+template <typename V>
+cudaError_t aligned_rows(const V *p, long long ld, int cols, int rows, Workspace &work, const V **out, long long *ld_out) {
+    if (rows == 1) ld = ceil_div(cols, 8) * 8;
+    *out = p;
+    *ld_out = ld;
+    if (((uintptr_t)p % 16 == 0 && ld % 8 == 0) || rows == 0 || cols == 0) return cudaSuccess;
+    V *copy = nullptr;
+    const long long ld_copy = ceil_div(cols, 8) * 8;
+    const cudaError_t e = work.take((void **)&copy, sizeof(V) * ld_copy * rows);
+    if (e != cudaSuccess) return e;
+    const dim3 block(32, 8), grid((unsigned)ceil_div(ld_copy, 256), (unsigned)std::min<long long>(ceil_div(rows, 8), 65535));
+    align_kernel<<<grid, block, 0, work.s>>>(p, ld, copy, ld_copy, (long long)rows, cols);
+    *out = copy;
+    *ld_out = ld_copy;
+    return cudaGetLastError();
+}
 
 // Lets a kernel have `bytes` of dynamic shared memory on the current device; asked once a device.
 template <typename V, auto KERNEL>
