@@ -10,6 +10,7 @@
 
 #include "q4.h"
 #include "q4_gemm.h"
+#include "q4_maps.h"
 #include "q4_ptx.cuh"
 #include "q4_values.cuh"
 
@@ -48,29 +49,11 @@ __device__ __forceinline__ void close_copies() { asm volatile("cp.async.commit_g
 template <int LATER>  // waits for this thread's copies but those of the LATER last groups
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
 
-// The 32 codes that a lane has of one row of 128 columns.  S is the width that shares a scale: the four lanes of a row
-// have neighbouring quarters of every S columns, so that one mma never mixes two groups.  Word w begins at column
-// place<S>(w, quarter).
+// Where a lane's words lie.  S is the width that shares a scale: the four lanes of a row have neighbouring quarters of
+// every S columns, so that one mma never mixes two groups.  Word w (eight codes) begins at column place<S>(w, quarter).
 template <int S>
 __device__ __forceinline__ int place(int w, int quarter) {
     return S == 128 ? 32 * quarter + 8 * w : S == 64 ? 64 * (w / 2) + 16 * quarter + 8 * (w % 2) : 32 * w + 8 * quarter;
-}
-// from 64 bytes of the row in shared memory
-template <int S>
-__device__ __forceinline__ void row_codes(uint32_t (&c)[4], const uint8_t *row, int quarter) {
-    if (S == 128) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(row + 16 * quarter);
-        c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
-    } else if (S == 64) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(row + 32 * j + 8 * quarter);
-            c[2 * j] = v.x, c[2 * j + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const uint32_t *>(row + 16 * j + 4 * quarter);
-    }
 }
 
 template <typename V>
@@ -79,81 +62,11 @@ struct Few {
     int n_vec, splits;
     const V *x, *dy;
     long long ld_x, ld_dy;
+    const V *turned;  // x as [column][vector], vectors filled up to 8 or 16; null for up to two vectors
     V *out;
     long long ld_out;
     V *d_res;
     const int *starts;  // transposed: [block of 256 columns][row] first residual entry not left of the block
-};
-
-// A warp's pieces of 32 rows x 128 columns on their way through shared memory, DEPTH at a time: the codes (64 bytes a
-// row) and the vectors' values at those columns (256 bytes a vector, the sixteens of bytes in an order that keeps the
-// reads below apart).  What bounds the product of one vector is the ALU pipe, which takes the codes apart: every address
-// is a lane's constant plus the piece's, and 32 rows share what the vectors cost (with 16 rows and the addresses worked
-// out at each use: 470 instructions for 1 KB of codes, 44 us for 16384 x 8192).
-template <typename V, int S, int NT, int DEPTH>
-struct Pieces {
-    const uint8_t *rows[4];  // this lane's 16 bytes of rows `line` + 8 j in a piece at column 0
-    const V *x;              // and its 16 bytes of the vectors
-    long long ld_x;
-    uint32_t ring, to;       // the ring, and where the next piece goes
-    const uint8_t *from;     // where the oldest one is
-    int lane, n_vec, row_bytes, slot_bytes, place_x[4];
-    __device__ __forceinline__ Pieces(const Few<V> &g, int row0, uint8_t *smem, int warp, int lane)
-        : x(g.x + lane / 16 * g.ld_x + lane % 16 * 8), ld_x(2 * g.ld_x), lane(lane), n_vec(g.n_vec) {
-        const Matrix<V> &m = g.m;
-        const int line = lane / 4, quarter = lane % 4;
-        row_bytes = (int)(((long long)m.n_cols + 31) / 32 * 16) - 16 * quarter;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)  // behind the last row the last row again: its results are not used
-            rows[j] = m.codes + min(row0 + line + 8 * j, m.n_rows - 1) * m.code_ld + 16 * quarter;
-        slot_bytes = bytes(n_vec) / DEPTH;
-        from = smem + warp * bytes(n_vec);
-        ring = to = smem_addr(from);
-        const int t = min(line, n_vec - 1);  // the columns of a product behind the last vector are not used
-#pragma unroll
-        for (int w = 0; w < 4; ++w) place_x[w] = 2048 + t * 256 + ((place<S>(w, quarter) / 8 ^ t) & 15) * 16;
-    }
-    static __host__ __device__ int bytes(int n_vec) { return DEPTH * (2048 + 256 * n_vec); }  // of a warp
-    // k, k1: the piece's columns, and where they end
-    __device__ __forceinline__ void fetch(int k, int k1) {
-        const bool inside = k / 2 < row_bytes;
-        const int at = inside ? k / 2 : 0, size = inside ? 16 : 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) copy<16>(to + 512 * j + lane * 16, rows[j] + at, size);
-        const int valid = min(max(k1 - k - lane % 16 * 8, 0), 8) * 2;
-        const V *at_x = x + (valid ? k : 0);
-#pragma unroll
-        for (int j = 0; j < 4 * NT; ++j) {
-            const int t = lane / 16 + 2 * j;
-            if (t < n_vec) copy<16>(to + 2048 + t * 256 + ((lane ^ t) & 15) * 16, at_x, valid);
-            at_x += ld_x;
-        }
-        to += slot_bytes;
-        if (to == ring + DEPTH * slot_bytes) to = ring;
-    }
-    static __device__ __forceinline__ void arrived() {  // the oldest of DEPTH pieces
-        wait_copies<DEPTH - 1>();
-        __syncwarp();
-    }
-    __device__ __forceinline__ void free() {  // the oldest piece is used up
-        __syncwarp();
-        from += slot_bytes;
-        if (smem_addr(from) == ring + DEPTH * slot_bytes) from -= DEPTH * slot_bytes;
-    }
-    // word w of the oldest piece's columns, of the vectors 8 j + line; codes j and j + 4 of a word share a register, and
-    // the vectors' values are paired alike
-    __device__ __forceinline__ void values_of(uint32_t (&v)[NT][4], int w) const {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            // 8 vectors on: 2048 bytes, and the other half of the order; behind the last vector anything will do
-            const int at = j == 0 || 8 * j + lane / 4 < n_vec ? (place_x[w] ^ 128 * j) + 2048 * j : place_x[w];
-            const uint4 u = *reinterpret_cast<const uint4 *>(from + at);
-            v[j][0] = __byte_perm(u.x, u.z, 0x5410);
-            v[j][1] = __byte_perm(u.x, u.z, 0x7632);
-            v[j][2] = __byte_perm(u.y, u.w, 0x5410);
-            v[j][3] = __byte_perm(u.y, u.w, 0x7632);
-        }
-    }
 };
 
 // d += 16 rows x 8 columns (a word of the upper and of the lower eight rows) times the vectors' values
@@ -171,275 +84,355 @@ __device__ __forceinline__ void word_product(float (&d)[NT][4], uint32_t up, uin
     }
 }
 
-// Scales (bits 0-15) and zero points (from bit 16) of a piece's 32 rows, a lane a row, in its SEGMENTS groups.
-template <int SEGMENTS>
-struct Numbers {
-    uint32_t v[SEGMENTS];
-};
-
-constexpr int ROWS = 32;
-
-// y = W x for up to 8 NT vectors.  A block has 32 rows; its warps take the 128-column pieces in turn, and the blocks of
-// a cluster (where there are too few rows to occupy the GPU) take contiguous parts of them; the parts are added in the
-// order of warps and ranks.
-template <typename V, int S, int NT, int DEPTH>
-__global__ void __launch_bounds__(THREADS, 2) product_few_kernel(const __grid_constant__ Few<V> g) {
-    extern __shared__ uint4 smem[];
-    __shared__ float part[WARPS][8 * NT][ROWS + 1];
-    __shared__ float sum[8 * NT][ROWS];
-    const Matrix<V> &m = g.m;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
-    const int rank = g.splits > 1 ? (int)cluster_rank() : 0, row0 = blockIdx.x / g.splits * ROWS;
-    const int pieces = (int)(((long long)m.n_cols + 127) / 128);
-    const int from = (int)((long long)pieces * rank / g.splits), to = (int)((long long)pieces * (rank + 1) / g.splits);
-    constexpr int SEGMENTS = 128 / S;
-    Pieces<V, S, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
-    int ahead = from + warp;  // the piece to fetch next
+// sum over the vectors of v times a residual entry's row (product: 1 term each) of the turned vectors
+template <typename V, int NT>
+__device__ __forceinline__ void turned_values(float (&x)[8 * NT], const V *at) {
 #pragma unroll
-    for (int n = 0; n < DEPTH - 1; ++n) {
-        if (ahead < to) ring.fetch(ahead * 128, m.n_cols);
-        close_copies();
-        ahead += WARPS;
-    }
-    GroupOf at((from + warp) * 128, m.group, WARPS * 128);
-    const long long my_row = (long long)min(row0 + lane, m.n_rows - 1) * m.n_groups;
-    const uint16_t *scales = reinterpret_cast<const uint16_t *>(m.scales) + my_row;
-    const uint8_t *zeros = m.zeros + my_row;
-    Numbers<SEGMENTS> next;
-    auto numbers = [&] {
+    for (int n = 0; n < NT; ++n) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(at) + n);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            const int gr = j == 0 ? at.g : min(at.after(j * (S / 32)), m.n_groups - 1);
-            next.v[j] = scales[gr];
-            if (m.zeros) next.v[j] |= (uint32_t)(zeros[gr] & 15) << 16;
+        for (int j = 0; j < 8; ++j) {
+            const uint16_t b = (uint16_t)(w[j / 2] >> 16 * (j % 2));
+            x[8 * n + j] = to_float(*reinterpret_cast<const V *>(&b));
         }
-        at.move();
-    };
-    if (from + warp < to) numbers();
-
-    // the residual, while the first pieces are on their way: four rows a warp
-    if (m.res_ptr && rank == 0) {
-        int begin = 0, end = 0;
-        if (lane < 4 && row0 + 4 * warp + lane < m.n_rows) res_range(m, row0 + 4 * warp + lane, begin, end);
-        for (int j = 0; j < 4; ++j) {
-            const int b = __shfl_sync(0xffffffffu, begin, j), e1 = __shfl_sync(0xffffffffu, end, j);
-            float extra[8 * NT] = {};
-            for (int e = b + lane; e < e1; e += 32) {
-                const int k = m.res_col[e];
-                const float v = to_float(m.res_val[e]);
-                if (k < 0 || k >= m.n_cols) continue;
-#pragma unroll
-                for (int t = 0; t < 8 * NT; ++t)
-                    if (t < g.n_vec) extra[t] = fmaf(v, to_float(g.x[t * g.ld_x + k]), extra[t]);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int t = 0; t < 8 * NT; ++t) {
-                if (t >= g.n_vec) break;
-                for (int d = 16; d; d /= 2) extra[t] += __shfl_xor_sync(0xffffffffu, extra[t], d);
-                if (lane == 0) sum[t][4 * warp + j] = extra[t];
-            }
-        }
-    }
-
-    float total[2][NT][4] = {};
-    for (int piece = from + warp; piece < to; piece += WARPS) {
-        const Numbers<SEGMENTS> now = next;
-        if (ahead < to) ring.fetch(ahead * 128, m.n_cols);
-        close_copies();
-        ahead += WARPS;
-        if (piece + WARPS < to) numbers();
-        ring.arrived();
-        uint32_t c[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) row_codes<S>(c[j], ring.from + 512 * j + line * 64, quarter);
-#pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            float d[2][NT][4] = {};
-            int z[4] = {8, 8, 8, 8};
-            float s[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t v = __shfl_sync(0xffffffffu, now.v[j], line + 8 * r);
-                const uint16_t bits = (uint16_t)v;
-                s[r] = to_float(*reinterpret_cast<const V *>(&bits));
-                if (m.zeros) z[r] = v >> 16;
-            }
-#pragma unroll
-            for (int w = j * (S / 32); w < (j + 1) * (S / 32); ++w) {
-                uint32_t x[NT][4];
-                ring.values_of(x, w);
-                word_product<V, NT>(d[0], c[0][w], c[1][w], z[0], z[1], x);
-                word_product<V, NT>(d[1], c[2][w], c[3][w], z[2], z[3], x);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int q = 0; q < NT; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) total[h][q][e] = fmaf(s[2 * h + e / 2], d[h][q][e], total[h][q][e]);
-        }
-        ring.free();
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                part[warp][8 * n + 2 * quarter + j % 2][line + 8 * (j / 2) + 16 * h] = total[h][n][j];
-    __syncthreads();
-    const int row = lane;
-    for (int t = warp; t < g.n_vec; t += WARPS) {
-        float s = m.res_ptr && rank == 0 ? sum[t][row] : 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) s += part[w][t][row];
-        if (g.splits > 1) {
-            sum[t][row] = s;
-        } else if (row0 + row < m.n_rows) {
-            g.out[t * g.ld_out + row0 + row] = from_float<V>(s);
-        }
-    }
-    if (g.splits > 1) {
-        __syncthreads();
-        cluster_barrier();
-        if (rank == 0) {
-            for (int t = warp; t < g.n_vec; t += WARPS) {
-                float s = 0.f;
-                for (int r = 0; r < g.splits; ++r) s += cluster_load(smem_addr(&sum[t][row]), r);
-                if (row0 + row < m.n_rows) g.out[t * g.ld_out + row0 + row] = from_float<V>(s);
-            }
-        }
-        __syncwarp();
-        cluster_barrier();
     }
 }
 
-// Gradients from up to 8 NT vectors.  A block has 32 rows and a part of the groups, a warp whole groups of them: the
-// sums over a group's columns for each vector are the product's, then they are weighed with dy instead of the scale.
-// S = 0: one group after the other, in pieces of 128 columns; else a piece has 128 / S groups.
-template <typename V, int S, int NT, int DEPTH>
-__global__ void __launch_bounds__(THREADS, 2) grad_few_kernel(const __grid_constant__ Few<V> g) {
-    extern __shared__ uint4 smem[];
+// One kernel for y = W x and for the gradients of W's numbers, for up to 8 NT vectors.  A block has 128 rows; a thread
+// of its own brings tiles of 128 rows x 128 columns of codes and the vectors' values at those columns into a ring of
+// shared memory; two groups of four warps, 32 rows a warp, take tiles in turn; three more warps see to the residual.
+//   product:  the blocks of a cluster take contiguous parts of a row's tiles, the parts are added in the order of groups
+//             and ranks.
+//   gradient: a warp takes whole units (a tile with 128 / S groups, or, S = 0, one group in tiles of 128 columns), whose
+//             sums for each vector are weighed with dy; the blocks of a row take units in turn.
+// What bounds it is the ALU pipe, which takes the codes apart (7 operations for 8 codes and as many again for all the
+// rest): tiles fetched by the converting warps themselves, 16 rows a warp, cost 470 instructions for 2048 codes and
+// 44 us for 16384 x 8192 and one vector.
+constexpr int STREAM_THREADS = 32 * 12, DEPTH = 8;
+constexpr int CODE_BYTES = 128 * 64;
+template <int NT>
+constexpr int stream_slot = CODE_BYTES + NT * 2048;
+template <int NT>
+constexpr int stream_smem = 1024 + DEPTH * stream_slot<NT> + 8 * NT * 128 * 4 + DEPTH * 16;
+constexpr int PART = 132;  // distance of two vectors' sums over 128 rows
+
+__device__ int wait_ran_out_few;
+
+template <typename V, int S, int NT, bool GRAD>
+__global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
+    stream_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_x,
+                  const __grid_constant__ Few<V> g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ volatile int failed;
+    constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH, SLOT = stream_slot<NT>;
     const Matrix<V> &m = g.m;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, line = lane / 4, quarter = lane % 4;
-    const int row0 = blockIdx.x / g.splits * ROWS, rank = blockIdx.x % g.splits;
-    constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH;
-    const int units = (m.n_groups + SEGMENTS - 1) / SEGMENTS, stride = g.splits * WARPS, width = SEGMENTS * m.group;
-    // a place in the warp's order of pieces: its unit, and where its columns begin and end
-    struct Place {
-        int unit, k, k1;
+    uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t base = smem_addr(smem);
+    float *extra = reinterpret_cast<float *>(smem + DEPTH * SLOT);  // [vector][row]: the residual's part, then sums
+    const uint32_t bars = smem_addr(extra + 8 * NT * 128);
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (DEPTH + s); };
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const int line = lane / 4, quarter = lane % 4;
+    const int rank = blockIdx.x % g.splits, row0 = blockIdx.x / g.splits * 128;
+
+    // the block's tiles
+    const int width = SEGMENTS * m.group, per_unit = S ? 1 : (m.group + 127) / 128;  // of a gradient's unit
+    const int pieces = (int)(((long long)m.n_cols + 127) / 128), units = (m.n_groups + SEGMENTS - 1) / SEGMENTS;
+    const int from = (int)((long long)pieces * rank / g.splits);
+    const int my_units = !GRAD || !g.out ? 0 : (units - rank + g.splits - 1) / g.splits;
+    const int tiles = GRAD ? my_units * per_unit : (int)((long long)pieces * (rank + 1) / g.splits) - from;
+    auto column = [&](int n) {
+        return GRAD ? (int)min((long long)(rank + n / per_unit * g.splits) * width + n % per_unit * 128, (long long)INT_MAX - 256)
+                    : (from + n) * 128;
     };
-    auto enter = [&](int unit) {
-        const long long k = (long long)unit * width;
-        return Place{unit, (int)min(k, (long long)INT_MAX), (int)min((long long)m.n_cols, k + width)};
-    };
-    auto move = [&](Place &p) {
-        p.k += 128;
-        if (S || p.k >= p.k1) p = enter(p.unit + stride);
-    };
-    Place here = enter(g.out ? rank * WARPS + warp : units), ahead = here;
-    Pieces<V, WIDTH, NT, DEPTH> ring(g, row0, reinterpret_cast<uint8_t *>(smem), warp, lane);
-#pragma unroll
-    for (int n = 0; n < DEPTH - 1; ++n) {
-        if (ahead.unit < units) {
-            ring.fetch(ahead.k, ahead.k1);
-            move(ahead);
+    const uint32_t polls = (1u << 22) + 64u * min(tiles, 1 << 24);
+
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < DEPTH; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 4);
         }
-        close_copies();
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (g.d_res && rank == 0) {
-        for (int r = 4 * warp; r < 4 * warp + 4 && row0 + r < m.n_rows; ++r) {
-            const int i = row0 + r;
-            int begin, end;
-            res_range(m, i, begin, end);
-            float dy[8 * NT];
+    __syncthreads();
+
+    float total[2][NT][4] = {};
+    if (warp < 8) {  // ---- the codes
+        const int group = warp / 4, lower = row0 + 32 * (warp % 4);
+        // this lane's places in a slot
+        const int swizzle = line >> 1 & 3;
+        int code_at[4], x_at[4];
 #pragma unroll
-            for (int t = 0; t < 8 * NT; ++t) dy[t] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
-            for (int e = begin + lane; e < end; e += 32) {
-                const int k = m.res_col[e];
-                if (k < 0 || k >= m.n_cols) continue;
-                float s = 0.f;
-#pragma unroll
-                for (int t = 0; t < 8 * NT; ++t)
-                    if (t < g.n_vec) s = fmaf(dy[t], to_float(g.x[t * g.ld_x + k]), s);
-                g.d_res[e] = from_float<V>(s);
-            }
+        for (int w = 0; w < 4; ++w) {
+            const int byte = place<WIDTH>(w, quarter) / 2, k = place<WIDTH>(w, quarter);
+            code_at[w] = (32 * (warp % 4) + line) * 64 + ((byte / 16 ^ swizzle) << 4) + byte % 16;
+            x_at[w] = CODE_BYTES + k / 64 * (NT * 1024) + line * 128 + ((k % 64 / 8 ^ line) << 4);
         }
-    }
-    long long of_row[4];
-    float dy[4][NT][2];
+        // scales and zero points: a lane a row, scale | zero << 16
+        const long long my_row = (long long)min(lower + lane, m.n_rows - 1) * m.n_groups;
+        const uint16_t *scales = reinterpret_cast<const uint16_t *>(m.scales) + my_row;
+        const uint8_t *zeros = m.zeros + my_row;
+        GroupOf at((from + group) * 128, m.group, 256);
+        uint32_t next[SEGMENTS] = {};
+        auto numbers = [&](int n) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = min(row0 + line + 8 * r, m.n_rows - 1);
-        of_row[r] = (long long)i * m.n_groups;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int t = 8 * n + 2 * quarter + j;
-                dy[r][n][j] = t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
+            for (int j = 0; j < SEGMENTS; ++j) {
+                const int gr = GRAD ? min((rank + n / per_unit * g.splits) * SEGMENTS + j, m.n_groups - 1)
+                                    : j == 0 ? at.g : min(at.after(j * (WIDTH / 32)), m.n_groups - 1);
+                next[j] = GRAD ? 0 : scales[gr];
+                if (m.zeros) next[j] |= (uint32_t)(zeros[gr] & 15) << 16;
             }
-    }
-    const uint8_t *zeros = m.zeros + (long long)min(row0 + lane, m.n_rows - 1) * m.n_groups;
-    float d[SEGMENTS][2][NT][4] = {};
-    int next[SEGMENTS];
-    auto fetch_zeros = [&](int unit) {
+            if (!GRAD) at.move();
+        };
+        float dy[4][NT][2];
+        if (GRAD) {
 #pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) next[j] = m.zeros ? zeros[min(unit * SEGMENTS + j, m.n_groups - 1)] & 15 : 8;
-    };
-    if (here.unit < units) fetch_zeros(here.unit);
-    while (here.unit < units) {
-        int now[SEGMENTS];
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) now[j] = next[j];
-        if (ahead.unit < units) {
-            ring.fetch(ahead.k, ahead.k1);
-            move(ahead);
-        }
-        close_copies();
-        const Place was = here;
-        move(here);
-        if (here.unit < units) fetch_zeros(here.unit);
-        ring.arrived();
-        uint32_t c[4][4];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row_codes<WIDTH>(c[j], ring.from + 512 * j + line * 64, quarter);
-#pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            int z[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) z[r] = m.zeros ? __shfl_sync(0xffffffffu, now[j], line + 8 * r) : 8;
-#pragma unroll
-            for (int w = j * (WIDTH / 32); w < (j + 1) * (WIDTH / 32); ++w) {
-                uint32_t x[NT][4];
-                ring.values_of(x, w);
-                word_product<V, NT>(d[j][0], c[0][w], c[1][w], z[0], z[1], x);
-                word_product<V, NT>(d[j][1], c[2][w], c[3][w], z[2], z[3], x);
-            }
-        }
-        ring.free();
-        if (here.unit == was.unit) continue;  // more of the group to come
-#pragma unroll
-        for (int j = 0; j < SEGMENTS; ++j) {
-            const int gr = was.unit * SEGMENTS + j;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float e = 0.f;
-#pragma unroll
-                for (int q = 0; q < NT; ++q)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        float &v = d[j][r / 2][q][2 * (r % 2) + t];
-                        e = fmaf(dy[r][q][t], 8 * q + 2 * quarter + t < g.n_vec ? v : 0.f, e);
-                        v = 0.f;
+                    for (int j = 0; j < 2; ++j) {
+                        const int t = 8 * n + 2 * quarter + j, i = lower + line + 8 * r;
+                        dy[r][n][j] = t < g.n_vec && i < m.n_rows ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
                     }
-                e += __shfl_xor_sync(0xffffffffu, e, 1);
-                e += __shfl_xor_sync(0xffffffffu, e, 2);
-                if (quarter == 0 && gr < m.n_groups && row0 + line + 8 * r < m.n_rows)
-                    g.out[of_row[r] + gr] = from_float<V>(e);
+        }
+        float d[SEGMENTS][2][NT][4] = {};
+        // the group's tiles: every second one, or (gradient) those of every second unit
+        const int step = GRAD && per_unit > 1 ? 1 : 2;
+        int n = GRAD ? group * per_unit : group;
+        if (n < tiles) numbers(n);
+        bool ok = true;
+        while (n < tiles) {
+            uint32_t now[SEGMENTS];
+#pragma unroll
+            for (int j = 0; j < SEGMENTS; ++j) now[j] = next[j];
+            const int was = n;
+            n += step;
+            const bool complete = !GRAD || per_unit == 1 || n % per_unit == 0;
+            if (step == 1 && complete) n += per_unit;  // the other group's unit
+            if (n < tiles) numbers(n);
+            const int slot = was % DEPTH;
+            if (!(ok = warp_wait(full(slot), was / DEPTH & 1, polls))) break;
+            const uint8_t *tile = smem + slot * SLOT;
+            uint32_t c[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (WIDTH == 128) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(tile + code_at[0] + 512 * j);
+                    c[j][0] = v.x, c[j][1] = v.y, c[j][2] = v.z, c[j][3] = v.w;
+                } else if (WIDTH == 64) {
+#pragma unroll
+                    for (int w = 0; w < 4; w += 2) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(tile + code_at[w] + 512 * j);
+                        c[j][w] = v.x, c[j][w + 1] = v.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) c[j][w] = *reinterpret_cast<const uint32_t *>(tile + code_at[w] + 512 * j);
+                }
+            }
+            // columns from `left` on belong to the next group (which begins on a multiple of 32)
+            const int left = GRAD && !S && complete ? m.group - (per_unit - 1) * 128 : 128;
+#pragma unroll
+            for (int j = 0; j < SEGMENTS; ++j) {
+                int z[4] = {8, 8, 8, 8};
+                float s[4];
+                if (!GRAD || m.zeros) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t v = __shfl_sync(0xffffffffu, now[j], line + 8 * r);
+                        const uint16_t b = (uint16_t)v;
+                        s[r] = to_float(*reinterpret_cast<const V *>(&b));
+                        if (m.zeros) z[r] = v >> 16;
+                    }
+                }
+                float(&e)[2][NT][4] = d[GRAD ? j : 0];
+                if (!GRAD) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) e[h][q][k] = 0.f;
+                }
+#pragma unroll
+                for (int w = j * (WIDTH / 32); w < (j + 1) * (WIDTH / 32); ++w) {
+                    // codes i and i + 4 of a word share a register; the vectors' values are paired alike
+                    uint32_t x[NT][4];
+#pragma unroll
+                    for (int q = 0; q < NT; ++q) {
+                        uint4 u = *reinterpret_cast<const uint4 *>(tile + x_at[w] + 1024 * q);
+                        if (GRAD && !S && left < 128 && place<WIDTH>(w, quarter) >= left) u = make_uint4(0, 0, 0, 0);
+                        x[q][0] = __byte_perm(u.x, u.z, 0x5410);
+                        x[q][1] = __byte_perm(u.x, u.z, 0x7632);
+                        x[q][2] = __byte_perm(u.y, u.w, 0x5410);
+                        x[q][3] = __byte_perm(u.y, u.w, 0x7632);
+                    }
+                    word_product<V, NT>(e[0], c[0][w], c[1][w], z[0], z[1], x);
+                    word_product<V, NT>(e[1], c[2][w], c[3][w], z[2], z[3], x);
+                }
+                if (!GRAD) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) total[h][q][k] = fmaf(s[2 * h + k / 2], e[h][q][k], total[h][q][k]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(slot));
+            if (GRAD && complete) {
+#pragma unroll
+                for (int j = 0; j < SEGMENTS; ++j) {
+                    const int gr = (rank + was / per_unit * g.splits) * SEGMENTS + j;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = 0.f;
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                float &v = d[j][r / 2][q][2 * (r % 2) + t];
+                                e = fmaf(dy[r][q][t], v, e);
+                                v = 0.f;
+                            }
+                        e += __shfl_xor_sync(0xffffffffu, e, 1);
+                        e += __shfl_xor_sync(0xffffffffu, e, 2);
+                        const int i = lower + line + 8 * r;
+                        if (quarter == 0 && gr < m.n_groups && i < m.n_rows)
+                            g.out[(long long)i * m.n_groups + gr] = from_float<V>(e);
+                    }
+                }
             }
         }
+        if (!ok) failed = 1;
+    } else if (warp == 8 && lane == 0) {  // ---- copies
+        bool ok = true;
+        int n = 0;
+        for (; n < tiles; ++n) {
+            const int slot = n % DEPTH, k = column(n);
+            if (!(ok = mbar_wait(empty(slot), (n / DEPTH & 1) ^ 1, polls))) break;
+            const uint32_t to = base + slot * SLOT;
+            mbar_expect(full(slot), SLOT);
+            tma_load(to, &map_codes, k / 2, row0, full(slot));
+            tma_load(to + CODE_BYTES, &map_x, k, 0, full(slot));
+            tma_load(to + CODE_BYTES + NT * 1024, &map_x, k + 64, 0, full(slot));
+        }
+        if (!ok) {
+            failed = 1;
+            for (int k = max(0, n - DEPTH); k < n; ++k) mbar_wait(full(k % DEPTH), k / DEPTH & 1, polls);
+        }
+    } else if (warp > 8) {  // ---- the residual: eight lanes a row, the ranks share the rows
+        const int first = 128 * rank / g.splits, last = 128 * (rank + 1) / g.splits;
+        if (!GRAD)
+            for (int j = threadIdx.x - 32 * 9; j < 8 * NT * 128; j += 96) extra[j] = 0.f;
+        asm volatile("bar.sync 1, 96;" ::: "memory");  // these three warps
+        if (m.res_ptr && (!GRAD || g.d_res)) {
+            for (int r0 = first + 4 * (warp - 9); r0 < last; r0 += 12) {
+                const int r = r0 + lane / 8, i = row0 + r;
+                int begin = 0, end = 0;
+                if (r < last && i < m.n_rows) res_range(m, i, begin, end);
+                float v[8 * NT] = {};
+                if (GRAD) {
+#pragma unroll
+                    for (int t = 0; t < 8 * NT; ++t) v[t] = begin < end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
+                }
+#pragma unroll 4
+                for (int e = begin + lane % 8; e < end; e += 8) {
+                    const int k = m.res_col[e];
+                    if (k < 0 || k >= m.n_cols) continue;
+                    float x[8 * NT];
+                    if (g.turned) {
+                        turned_values<V, NT>(x, g.turned + (long long)k * (8 * NT));
+                    } else {  // one or two vectors
+                        x[0] = to_float(g.x[k]);
+                        x[1] = g.n_vec > 1 ? to_float(g.x[g.ld_x + k]) : 0.f;
+                    }
+                    if (GRAD) {
+                        float s = fmaf(v[0], x[0], v[1] * x[1]);
+                        if (g.turned) {
+#pragma unroll
+                            for (int t = 2; t < 8 * NT; ++t) s = fmaf(v[t], x[t], s);
+                        }
+                        g.d_res[e] = from_float<V>(s);
+                    } else {
+                        const float a = to_float(m.res_val[e]);
+                        v[0] = fmaf(a, x[0], v[0]);
+                        v[1] = fmaf(a, x[1], v[1]);
+                        if (g.turned) {
+#pragma unroll
+                            for (int t = 2; t < 8 * NT; ++t) v[t] = fmaf(a, x[t], v[t]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (!GRAD) {
+#pragma unroll
+                    for (int t = 0; t < 8 * NT; ++t) {
+                        if (t >= g.n_vec) break;
+#pragma unroll
+                        for (int x = 1; x < 8; x *= 2) v[t] += __shfl_xor_sync(0xffffffffu, v[t], x);
+                        if (lane % 8 == 0 && r < last) extra[t * 128 + r] = v[t];
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (!GRAD) {
+        // the ring is used up: the two groups' sums go there, [group][vector][row]
+        float *part = reinterpret_cast<float *>(smem);
+        if (warp < 8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        part[(warp / 4 * 8 * NT + 8 * n + 2 * quarter + j % 2) * PART + 32 * (warp % 4) + line + 8 * (j / 2) +
+                             16 * h] = total[h][n][j];
+        }
+        __syncthreads();
+        const bool ok = !failed;
+        for (int j = threadIdx.x; j < 128 * g.n_vec; j += STREAM_THREADS) {
+            const int t = j / 128, r = j % 128;
+            const float s = extra[j] + part[t * PART + r] + part[(8 * NT + t) * PART + r];
+            if (g.splits > 1)
+                extra[j] = s;
+            else if (ok && row0 + r < m.n_rows)
+                g.out[t * g.ld_out + row0 + r] = from_float<V>(s);
+        }
+        if (g.splits > 1) {
+            __syncthreads();
+            cluster_barrier();
+            const int rows = 128 / g.splits;
+            for (int j = threadIdx.x; j < rows * g.n_vec; j += STREAM_THREADS) {
+                const int t = j / rows, r = rank * rows + j % rows;
+                float s = 0.f;
+                for (int q = 0; q < g.splits; ++q) s += cluster_load(smem_addr(extra + t * 128 + r), q);
+                if (ok && row0 + r < m.n_rows) g.out[t * g.ld_out + row0 + r] = from_float<V>(s);
+            }
+            __syncwarp();
+            cluster_barrier();
+        }
+    }
+    if (threadIdx.x == 0 && failed) wait_ran_out_few = 1;
+}
+
+// turned[k][t] = x[t][k], 0 for the vectors up to `filled`
+template <typename V>
+__global__ void turn_kernel(const V *x, long long ld, int n_vec, int n_cols, int filled, V *turned) {
+    const int k = blockIdx.x * THREADS + threadIdx.x;
+    if (k >= n_cols) return;
+    for (int t0 = 0; t0 < filled; t0 += 8) {
+        V v[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = t0 + t < n_vec ? x[(t0 + t) * ld + k] : from_float<V>(0.f);
+        *reinterpret_cast<uint4 *>(turned + (long long)k * filled + t0) = *reinterpret_cast<uint4 *>(v);
     }
 }
 
@@ -670,39 +663,53 @@ cudaError_t run(void (*kernel)(const Few<V>), long long blocks, int cluster, siz
     return cudaLaunchKernelEx(&cfg, kernel, g);
 }
 
-// as many parts of `pieces` as bring `blocks` to the GPU's 148 SMs, a power of two up to 8, a warp's share not below one
-int parts_of(long long blocks, long long pieces) {
+// as many parts of `pieces` as bring `blocks` to two on each of the GPU's 148 SMs, a power of two up to 8, a part not
+// smaller than `least`
+int parts_of(long long blocks, long long pieces, int least) {
     int n = 1;
-    while (n < 8 && blocks * n * 2 <= 2 * 148 && pieces >= 2 * n * WARPS) n *= 2;
+    while (n < 8 && blocks * n * 2 <= 2 * 148 && pieces >= 2ll * n * least) n *= 2;
     return n;
 }
 
-template <typename V, auto KERNEL>
-cudaError_t run_ring(const Few<V> &g, long long blocks, int cluster, int warp_bytes, cudaStream_t s) {
-    const cudaError_t e = allow_smem<V, KERNEL>(WARPS * 3 * (2048 + 256 * 8));
-    return e == cudaSuccess ? run<V>(KERNEL, blocks, cluster, WARPS * warp_bytes, g, s) : e;
+template <typename V, int S, int NT, bool GRAD>
+cudaError_t stream(const Few<V> &g, const CUtensorMap &codes, const CUtensorMap &x, cudaStream_t s) {
+    auto kernel = stream_kernel<V, S, NT, GRAD>;
+    const long long blocks = ceil_div(g.m.n_rows, 128) * g.splits;
+    if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
+    const cudaError_t e = allow_smem<V, stream_kernel<V, S, NT, GRAD>>(stream_smem<NT>);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(STREAM_THREADS);
+    cfg.dynamicSmemBytes = stream_smem<NT>;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = GRAD ? 1 : g.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = attr[0].val.clusterDim.x > 1;
+    return cudaLaunchKernelEx(&cfg, kernel, codes, x, g);
 }
 
-// Pieces under way: four a warp for one or two vectors, three or two for more, whose values take more room, so that two
-// blocks fit an SM.
-template <typename V, int S>
-cudaError_t product_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
-    blocks *= g.splits;
-    if (g.n_vec <= 2)
-        return run_ring<V, product_few_kernel<V, S, 1, 4>>(g, blocks, g.splits, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
-    if (g.n_vec <= 8)
-        return run_ring<V, product_few_kernel<V, S, 1, 3>>(g, blocks, g.splits, Pieces<V, S, 1, 3>::bytes(g.n_vec), s);
-    return run_ring<V, product_few_kernel<V, S, 2, 2>>(g, blocks, g.splits, Pieces<V, S, 2, 2>::bytes(g.n_vec), s);
-}
-
-template <typename V, int S>
-cudaError_t grad_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
-    blocks *= g.splits;
-    if (g.n_vec <= 2)
-        return run_ring<V, grad_few_kernel<V, S, 1, 4>>(g, blocks, 1, Pieces<V, S, 1, 4>::bytes(g.n_vec), s);
-    if (g.n_vec <= 8)
-        return run_ring<V, grad_few_kernel<V, S, 1, 3>>(g, blocks, 1, Pieces<V, S, 1, 3>::bytes(g.n_vec), s);
-    return run_ring<V, grad_few_kernel<V, S, 2, 2>>(g, blocks, 1, Pieces<V, S, 2, 2>::bytes(g.n_vec), s);
+// x with rows that can be fetched, its tensor map and the codes', and x turned where the residual's gathers want it
+template <typename V>
+cudaError_t stream_inputs(Few<V> &g, const V *x, long long ld_x, CUtensorMap &codes, CUtensorMap &map_x, bool gathers,
+                          Workspace &work) {
+    const Matrix<V> &m = g.m;
+    cudaError_t e = aligned_rows(x, ld_x, m.n_cols, g.n_vec, work, &g.x, &g.ld_x);
+    if (e != cudaSuccess || m.n_cols == 0) return e;
+    const int filled = g.n_vec <= 8 ? 8 : 16;
+    if (!encode_codes(&codes, m) || !encode_vectors(&map_x, g.x, m.n_cols, g.n_vec, g.ld_x, filled))
+        return cudaErrorInvalidValue;
+    if (gathers && g.n_vec > 2) {
+        V *turned = nullptr;
+        if ((e = work.take((void **)&turned, sizeof(V) * filled * m.n_cols)) != cudaSuccess) return e;
+        turn_kernel<<<(unsigned)ceil_div(m.n_cols, THREADS), THREADS, 0, work.s>>>(g.x, g.ld_x, g.n_vec, m.n_cols, filled, turned);
+        g.turned = turned;
+        e = cudaGetLastError();
+    }
+    return e;
 }
 
 }  // namespace
@@ -710,19 +717,22 @@ cudaError_t grad_of_width(const Few<V> &g, long long blocks, cudaStream_t s) {
 template <typename V>
 cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
     if (n_vec > 16) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
-    const long long blocks = ceil_div(m.n_rows, ROWS);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, ceil_div(m.n_cols, 128));
+    g.splits = parts_of(ceil_div(m.n_rows, 128), ceil_div(m.n_cols, 128), 2);
     g.out = y;
     g.ld_out = ld_y;
     Workspace work(s);
-    cudaError_t e = aligned_rows(x, ld_x, m.n_cols, n_vec, work, &g.x, &g.ld_x);
+    CUtensorMap codes = {}, map_x = {};
+    const cudaError_t e = stream_inputs(g, x, ld_x, codes, map_x, m.res_ptr != nullptr, work);
     if (e != cudaSuccess) return e;
-    return m.group % 128 == 0  ? product_of_width<V, 128>(g, blocks, s)
-           : m.group % 64 == 0 ? product_of_width<V, 64>(g, blocks, s)
-                               : product_of_width<V, 32>(g, blocks, s);
+    const bool one = n_vec <= 8;
+    if (m.group % 128 == 0)
+        return one ? stream<V, 128, 1, false>(g, codes, map_x, s) : stream<V, 128, 2, false>(g, codes, map_x, s);
+    if (m.group % 64 == 0)
+        return one ? stream<V, 64, 1, false>(g, codes, map_x, s) : stream<V, 64, 2, false>(g, codes, map_x, s);
+    return one ? stream<V, 32, 1, false>(g, codes, map_x, s) : stream<V, 32, 2, false>(g, codes, map_x, s);
 }
 
 template <typename V>
@@ -733,7 +743,7 @@ cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_d
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, ceil_div(m.n_rows, 16));
+    g.splits = parts_of(blocks, ceil_div(m.n_rows, 16), WARPS);
     g.out = dx;
     g.ld_out = ld_dx;
     Workspace work(s);
@@ -756,21 +766,28 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
                  V *d_res, cudaStream_t s) {
     if (n_vec > 16) return grad_many(m, n_vec, x, ld_x, dy, ld_dy, d_scales, d_res, s);
     if (n_vec == 0) return no_gradient(m, d_scales, m.res_ptr ? d_res : nullptr, s);
-    const long long blocks = ceil_div(m.n_rows, ROWS);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(blocks, m.group <= 64 ? ceil_div(m.n_groups * (long long)m.group, 128) : m.n_groups);
+    g.splits = parts_of(ceil_div(m.n_rows, 128), m.group <= 64 ? ceil_div(m.n_groups * (long long)m.group, 128) : m.n_groups, 2);
     g.dy = dy;
     g.ld_dy = ld_dy;
     g.out = d_scales;
     g.d_res = m.res_ptr ? d_res : nullptr;
     Workspace work(s);
-    cudaError_t e = aligned_rows(x, ld_x, m.n_cols, n_vec, work, &g.x, &g.ld_x);
+    CUtensorMap codes = {}, map_x = {};
+    const cudaError_t e = stream_inputs(g, x, ld_x, codes, map_x, g.d_res != nullptr, work);
     if (e != cudaSuccess) return e;
-    return m.group == 64   ? grad_of_width<V, 64>(g, blocks, s)
-           : m.group == 32 ? grad_of_width<V, 32>(g, blocks, s)
-                           : grad_of_width<V, 0>(g, blocks, s);
+    const bool one = n_vec <= 8;
+    if (m.group == 64) return one ? stream<V, 64, 1, true>(g, codes, map_x, s) : stream<V, 64, 2, true>(g, codes, map_x, s);
+    if (m.group == 32) return one ? stream<V, 32, 1, true>(g, codes, map_x, s) : stream<V, 32, 2, true>(g, codes, map_x, s);
+    return one ? stream<V, 0, 1, true>(g, codes, map_x, s) : stream<V, 0, 2, true>(g, codes, map_x, s);
+}
+
+cudaError_t waits_ran_out_few(int *flag, cudaStream_t s) {
+    void *p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_few);
+    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
 }
 
 #define INSTANTIATE(V)                                                                                                \

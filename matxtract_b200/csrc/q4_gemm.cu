@@ -19,6 +19,7 @@
 
 #include "q4.h"
 #include "q4_gemm.h"
+#include "q4_maps.h"
 #include "q4_ptx.cuh"
 #include "q4_values.cuh"
 
@@ -502,37 +503,6 @@ __global__ void __launch_bounds__(256) slots_kernel(Matrix<V> m, int chunks, uin
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                            const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-Encode encoder() {
-    static const Encode f = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
-            r != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<Encode>(p);
-    }();
-    return f;
-}
-
-bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t cols, uint64_t rows, uint64_t ld_bytes,
-            uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld_bytes};
-    const cuuint32_t box[2] = {box_cols, box_rows}, ones[2] = {1, 1};
-    return encoder() && encoder()(map, type, 2, const_cast<void *>(p), dims, strides, box, ones,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <typename V>
-bool encode_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows) {
-    return encode(map, std::is_same<V, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                  p, cols, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 // The tensor map of `rows` vectors.
 template <typename V>
 cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work) {
@@ -599,9 +569,7 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
     CUtensorMap codes = {}, vectors = {};
     Workspace work(s);
     if (depth > 0) {
-        if (!encode(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, m.codes, ceil_div(m.n_cols, 32) * 16, m.n_rows, m.code_ld, 64,
-                    128, CU_TENSOR_MAP_SWIZZLE_64B))
-            return cudaErrorInvalidValue;
+        if (!encode_codes(&codes, m)) return cudaErrorInvalidValue;
         cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn, work);
         if (e != cudaSuccess) return e;
         if (m.res_ptr) {
