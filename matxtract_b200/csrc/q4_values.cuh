@@ -10,6 +10,13 @@
 namespace mx {
 namespace q4 {
 
+// (v & mask) | base in one operation: written out, it became two, with a constant each
+__device__ __forceinline__ uint32_t pick(uint32_t v, uint32_t mask, uint32_t base) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(base));
+    return r;
+}
+
 // c - z of a register's codes, two to a register, exact: p[j] holds those in bits 4 j (low half) and 16 + 4 j (high half),
 // whose zero points are z0 and z1.
 template <typename V>
@@ -21,11 +28,11 @@ struct Pair<__half> {
     static __device__ __forceinline__ void steps(uint32_t w, int z0, int z1, T (&p)[4]) {
         const uint32_t both = z0 | z1 << 16;
         const T zz = bits(0x64006400u | both), zl = bits(0xD400D400u | both << 4), sixteenth = bits(0x2C002C00u);
-        p[0] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
-        p[1] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+        p[0] = __hsub2(bits(pick(w, 0x000F000Fu, 0x64006400u)), zz);
+        p[1] = __hfma2(bits(pick(w, 0x00F000F0u, 0x64006400u)), sixteenth, zl);
         w >>= 8;
-        p[2] = __hsub2(bits((w & 0x000F000Fu) | 0x64006400u), zz);
-        p[3] = __hfma2(bits((w & 0x00F000F0u) | 0x64006400u), sixteenth, zl);
+        p[2] = __hsub2(bits(pick(w, 0x000F000Fu, 0x64006400u)), zz);
+        p[3] = __hfma2(bits(pick(w, 0x00F000F0u, 0x64006400u)), sixteenth, zl);
     }
     static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
     static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) { steps(w, z, z, p); }
@@ -38,7 +45,7 @@ struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ void steps(uint32_t w, int z0, int z1, T (&p)[4]) {  // 128 + c is exact in the type
         const T zz = bits(0x43004300u | z0 | z1 << 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __hsub2(bits((w >> 4 * j & 0x000F000Fu) | 0x43004300u), zz);
+        for (int j = 0; j < 4; ++j) p[j] = __hsub2(bits(pick(w >> 4 * j, 0x000F000Fu, 0x43004300u)), zz);
     }
     static __device__ __forceinline__ T bits(uint32_t v) { return *reinterpret_cast<T *>(&v); }
     static __device__ __forceinline__ void steps(uint32_t w, int z, T (&p)[4]) { steps(w, z, z, p); }
