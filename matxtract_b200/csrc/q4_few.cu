@@ -332,42 +332,81 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             for (int j = threadIdx.x - 32 * 9; j < 8 * NT * 128; j += 96) extra[j] = 0.f;
         asm volatile("bar.sync 1, 96;" ::: "memory");  // these three warps
         if (m.res_ptr && (!GRAD || g.d_res)) {
-            for (int r0 = first + 4 * (warp - 9); r0 < last; r0 += 12) {
-                const int r = r0 + lane / 8, i = row0 + r;
-                int begin = 0, end = 0;
-                if (r < last && i < m.n_rows) res_range(m, i, begin, end);
+            // Everything here waits for memory three times in a row (where the row's entries are, the entries, the
+            // vectors), so a warp asks for all its rows' entries' places at once, and for the next four rows' entries
+            // while it works on four.
+            constexpr int TOGETHER = 6;  // entries a lane asks for at once: 48 of a row
+            struct Entries {
+                int begin, end, k[TOGETHER];
+                V a[TOGETHER];
+            };
+            auto row_of = [&](int n) { return first + 4 * (warp - 9) + 12 * (n / 4) + n % 4; };  // a warp's n-th row
+            int my_begin = 0, my_end = 0;  // of the row that is the lane's number
+            if (row_of(lane) < last && row0 + row_of(lane) < m.n_rows) res_range(m, row0 + row_of(lane), my_begin, my_end);
+            int their_begin = 0, their_end = 0;  // and 32 rows on
+            if (row_of(32 + lane) < last && row0 + row_of(32 + lane) < m.n_rows)
+                res_range(m, row0 + row_of(32 + lane), their_begin, their_end);
+            auto ask = [&](Entries &n, int from) {
+#pragma unroll
+                for (int u = 0; u < TOGETHER; ++u) {
+                    const int e = from + lane % 8 + 8 * u;
+                    n.k[u] = e < n.end ? m.res_col[e] : -1;
+                    if (!GRAD) n.a[u] = e < n.end ? m.res_val[e] : from_float<V>(0.f);
+                }
+            };
+            auto rows = [&](Entries &n, int round) {
+                const int at = 4 * round + lane / 8;
+                const int b0 = __shfl_sync(0xffffffffu, my_begin, at & 31), e0 = __shfl_sync(0xffffffffu, my_end, at & 31);
+                const int b1 = __shfl_sync(0xffffffffu, their_begin, at & 31), e1 = __shfl_sync(0xffffffffu, their_end, at & 31);
+                n.begin = at < 32 ? b0 : b1;
+                n.end = at < 32 ? e0 : e1;
+                ask(n, n.begin);
+            };
+            const int rounds = (last - first + 11) / 12;  // at most 11: 44 rows
+            Entries next;
+            rows(next, 0);
+            for (int round = 0; round < rounds; ++round) {
+                Entries now = next;
+                if (round + 1 < rounds) rows(next, round + 1);
+                const int r = row_of(4 * round + lane / 8), i = row0 + r;
                 float v[8 * NT] = {};
                 if (GRAD) {
 #pragma unroll
-                    for (int t = 0; t < 8 * NT; ++t) v[t] = begin < end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
+                    for (int t = 0; t < 8 * NT; ++t)
+                        v[t] = now.begin < now.end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
                 }
-#pragma unroll 4
-                for (int e = begin + lane % 8; e < end; e += 8) {
-                    const int k = m.res_col[e];
-                    if (k < 0 || k >= m.n_cols) continue;
-                    float x[8 * NT];
-                    if (g.turned) {
-                        turned_values<V, NT>(x, g.turned + (long long)k * (8 * NT));
-                    } else {  // one or two vectors
-                        x[0] = to_float(g.x[k]);
-                        x[1] = g.n_vec > 1 ? to_float(g.x[g.ld_x + k]) : 0.f;
-                    }
-                    if (GRAD) {
-                        float s = fmaf(v[0], x[0], v[1] * x[1]);
-                        if (g.turned) {
+                for (int from = now.begin;;) {
 #pragma unroll
-                            for (int t = 2; t < 8 * NT; ++t) s = fmaf(v[t], x[t], s);
-                        }
-                        g.d_res[e] = from_float<V>(s);
-                    } else {
-                        const float a = to_float(m.res_val[e]);
-                        v[0] = fmaf(a, x[0], v[0]);
-                        v[1] = fmaf(a, x[1], v[1]);
+                    for (int u = 0; u < TOGETHER; ++u) {
+                        const int k = now.k[u];
+                        if (k < 0 || k >= m.n_cols) continue;
+                        float x[8 * NT];
                         if (g.turned) {
+                            turned_values<V, NT>(x, g.turned + (long long)k * (8 * NT));
+                        } else {  // one or two vectors
+                            x[0] = to_float(g.x[k]);
+                            x[1] = g.n_vec > 1 ? to_float(g.x[g.ld_x + k]) : 0.f;
+                        }
+                        if (GRAD) {
+                            float s = fmaf(v[0], x[0], v[1] * x[1]);
+                            if (g.turned) {
 #pragma unroll
-                            for (int t = 2; t < 8 * NT; ++t) v[t] = fmaf(a, x[t], v[t]);
+                                for (int t = 2; t < 8 * NT; ++t) s = fmaf(v[t], x[t], s);
+                            }
+                            g.d_res[from + lane % 8 + 8 * u] = from_float<V>(s);
+                        } else {
+                            const float a = to_float(now.a[u]);
+                            v[0] = fmaf(a, x[0], v[0]);
+                            v[1] = fmaf(a, x[1], v[1]);
+                            if (g.turned) {
+#pragma unroll
+                                for (int t = 2; t < 8 * NT; ++t) v[t] = fmaf(a, x[t], v[t]);
+                            }
                         }
                     }
+                    from += 8 * TOGETHER;
+                    if (from >= now.end) break;
+                    ask(now, from);
                 }
                 __syncwarp();
                 if (!GRAD) {
