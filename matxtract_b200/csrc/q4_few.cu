@@ -104,8 +104,10 @@ __device__ __forceinline__ void turned_values(float (&x)[8 * NT], const V *at) {
 // shared memory; two groups of four warps, 32 rows a warp, take tiles in turn; three more warps see to the residual.
 //   product:  the blocks of a cluster take contiguous parts of a row's tiles, the parts are added in the order of groups
 //             and ranks.
-//   gradient: a warp takes whole units (a tile with 128 / S groups, or, S = 0, one group in tiles of 128 columns), whose
-//             sums for each vector are weighed with dy; the blocks of a row take units in turn.
+//   gradient: the sums of whole units (a tile with 128 / S groups, or, S = 0, one group in tiles of 128 columns) for each
+//             vector are weighed with dy; the blocks of a row take units in turn.  For S = 0 every warp has 16 rows and
+//             takes every tile: with units of several tiles taken in turn, a group of warps would meet a slot's barrier
+//             without having seen its last phase, which a wait for a parity cannot tell from the wanted one.
 // What bounds it is the ALU pipe, which takes the codes apart (7 operations for 8 codes and as many again for all the
 // rest): tiles fetched by the converting warps themselves, 16 rows a warp, cost 470 instructions for 2048 codes and
 // 44 us for 16384 x 8192 and one vector.
@@ -126,6 +128,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ volatile int failed;
     constexpr int WIDTH = S ? S : 128, SEGMENTS = 128 / WIDTH, SLOT = stream_slot<NT>;
+    constexpr bool ALL = GRAD && S == 0;  // every warp takes every tile
+    constexpr int H = ALL ? 1 : 2;        // 16 rows each
     const Matrix<V> &m = g.m;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
         failed = 0;
         for (int s = 0; s < DEPTH; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 4);
+            mbar_init(empty(s), ALL ? 8 : 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -161,14 +165,14 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
 
     float total[2][NT][4] = {};
     if (warp < 8) {  // ---- the codes
-        const int group = warp / 4, lower = row0 + 32 * (warp % 4);
+        const int group = ALL ? 0 : warp / 4, first_row = 16 * H * (ALL ? warp : warp % 4), lower = row0 + first_row;
         // this lane's places in a slot
         const int swizzle = line >> 1 & 3;
         int code_at[4], x_at[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int byte = place<WIDTH>(w, quarter) / 2, k = place<WIDTH>(w, quarter);
-            code_at[w] = (32 * (warp % 4) + line) * 64 + ((byte / 16 ^ swizzle) << 4) + byte % 16;
+            code_at[w] = (first_row + line) * 64 + ((byte / 16 ^ swizzle) << 4) + byte % 16;
             x_at[w] = CODE_BYTES + k / 64 * (NT * 1024) + line * 128 + ((k % 64 / 8 ^ line) << 4);
         }
         // scales and zero points: a lane a row, scale | zero << 16
@@ -187,10 +191,10 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             }
             if (!GRAD) at.move();
         };
-        float dy[4][NT][2];
+        float dy[2 * H][NT][2];
         if (GRAD) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 2 * H; ++r)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -199,10 +203,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                         dy[r][n][j] = t < g.n_vec && i < m.n_rows ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
                     }
         }
-        float d[SEGMENTS][2][NT][4] = {};
-        // the group's tiles: every second one, or (gradient) those of every second unit
-        const int step = GRAD && per_unit > 1 ? 1 : 2;
-        int n = GRAD ? group * per_unit : group;
+        float d[SEGMENTS][H][NT][4] = {};
+        int n = group;
         if (n < tiles) numbers(n);
         bool ok = true;
         while (n < tiles) {
@@ -210,16 +212,15 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
 #pragma unroll
             for (int j = 0; j < SEGMENTS; ++j) now[j] = next[j];
             const int was = n;
-            n += step;
-            const bool complete = !GRAD || per_unit == 1 || n % per_unit == 0;
-            if (step == 1 && complete) n += per_unit;  // the other group's unit
+            n += ALL ? 1 : 2;
+            const bool complete = !ALL || n % per_unit == 0;  // the unit's last tile
             if (n < tiles) numbers(n);
             const int slot = was % DEPTH;
             if (!(ok = warp_wait(full(slot), was / DEPTH & 1, polls))) break;
             const uint8_t *tile = smem + slot * SLOT;
-            uint32_t c[4][4];
+            uint32_t c[2 * H][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2 * H; ++j) {
                 if (WIDTH == 128) {
                     const uint4 v = *reinterpret_cast<const uint4 *>(tile + code_at[0] + 512 * j);
                     c[j][0] = v.x, c[j][1] = v.y, c[j][2] = v.z, c[j][3] = v.w;
@@ -235,24 +236,26 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                 }
             }
             // columns from `left` on belong to the next group (which begins on a multiple of 32)
-            const int left = GRAD && !S && complete ? m.group - (per_unit - 1) * 128 : 128;
+            const int left = ALL && complete ? m.group - (per_unit - 1) * 128 : 128;
 #pragma unroll
             for (int j = 0; j < SEGMENTS; ++j) {
-                int z[4] = {8, 8, 8, 8};
-                float s[4];
+                int z[2 * H];
+                float s[2 * H];
+#pragma unroll
+                for (int r = 0; r < 2 * H; ++r) z[r] = 8;
                 if (!GRAD || m.zeros) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
+                    for (int r = 0; r < 2 * H; ++r) {
                         const uint32_t v = __shfl_sync(0xffffffffu, now[j], line + 8 * r);
                         const uint16_t b = (uint16_t)v;
                         s[r] = to_float(*reinterpret_cast<const V *>(&b));
                         if (m.zeros) z[r] = v >> 16;
                     }
                 }
-                float(&e)[2][NT][4] = d[GRAD ? j : 0];
+                float(&e)[H][NT][4] = d[GRAD ? j : 0];
                 if (!GRAD) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < H; ++h)
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
 #pragma unroll
@@ -265,18 +268,18 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
 #pragma unroll
                     for (int q = 0; q < NT; ++q) {
                         uint4 u = *reinterpret_cast<const uint4 *>(tile + x_at[w] + 1024 * q);
-                        if (GRAD && !S && left < 128 && place<WIDTH>(w, quarter) >= left) u = make_uint4(0, 0, 0, 0);
+                        if (ALL && left < 128 && place<WIDTH>(w, quarter) >= left) u = make_uint4(0, 0, 0, 0);
                         x[q][0] = __byte_perm(u.x, u.z, 0x5410);
                         x[q][1] = __byte_perm(u.x, u.z, 0x7632);
                         x[q][2] = __byte_perm(u.y, u.w, 0x5410);
                         x[q][3] = __byte_perm(u.y, u.w, 0x7632);
                     }
                     word_product<V, NT>(e[0], c[0][w], c[1][w], z[0], z[1], x);
-                    word_product<V, NT>(e[1], c[2][w], c[3][w], z[2], z[3], x);
+                    if (H == 2) word_product<V, NT>(e[H - 1], c[2 * H - 2][w], c[2 * H - 1][w], z[2 * H - 2], z[2 * H - 1], x);
                 }
                 if (!GRAD) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < H; ++h)
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
 #pragma unroll
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                 for (int j = 0; j < SEGMENTS; ++j) {
                     const int gr = (rank + was / per_unit * g.splits) * SEGMENTS + j;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
+                    for (int r = 0; r < 2 * H; ++r) {
                         float e = 0.f;
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
@@ -808,7 +811,7 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
-    g.splits = parts_of(ceil_div(m.n_rows, 128), m.group <= 64 ? ceil_div(m.n_groups * (long long)m.group, 128) : m.n_groups, 2);
+    g.splits = parts_of(ceil_div(m.n_rows, 128), m.group == 32 || m.group == 64 ? ceil_div(m.n_cols, 128) : m.n_groups, 2);
     g.dy = dy;
     g.ld_dy = ld_dy;
     g.out = d_scales;
@@ -818,6 +821,7 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
     const cudaError_t e = stream_inputs(g, x, ld_x, codes, map_x, g.d_res != nullptr, work);
     if (e != cudaSuccess) return e;
     const bool one = n_vec <= 8;
+    if (m.group == 128) return one ? stream<V, 128, 1, true>(g, codes, map_x, s) : stream<V, 128, 2, true>(g, codes, map_x, s);
     if (m.group == 64) return one ? stream<V, 64, 1, true>(g, codes, map_x, s) : stream<V, 64, 2, true>(g, codes, map_x, s);
     if (m.group == 32) return one ? stream<V, 32, 1, true>(g, codes, map_x, s) : stream<V, 32, 2, true>(g, codes, map_x, s);
     return one ? stream<V, 0, 1, true>(g, codes, map_x, s) : stream<V, 0, 2, true>(g, codes, map_x, s);

@@ -117,6 +117,27 @@ def test_larger_matrices(n, k, t):
     check_grad(m, t, 3)
 
 
+@pytest.mark.parametrize("t", [1, 8, 16, 40])
+@pytest.mark.parametrize("group", [96, 128, 160, 256, 384, 1024, 1056, 4096])
+def test_wide_groups(group, t):
+    """Groups that take several tiles of the kernels, whole or not."""
+    m = make(140, 8256, group, torch.bfloat16, True, 0.002, group)
+    for _ in range(3):
+        check_product(m, t, 1)
+        check_product_t(m, t, 2)
+        check_grad(m, t, 3)
+
+
+@pytest.mark.parametrize("t", [17, 100, 200, 600])
+@pytest.mark.parametrize("n,k", [(200, 8200), (6000, 300), (1300, 5000)])
+def test_many_tiles(n, k, t):
+    """Contractions many times as long as what is under way at a time, in each width of tile."""
+    m = make(n, k, 128, torch.float16, True, 0.004, t)
+    for _ in range(3):
+        check_product(m, t, 1)
+        check_product_t(m, t, 2)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("t", [1, 7, 40, 150])
 @pytest.mark.parametrize("shift", [0, 1, 8])
