@@ -39,13 +39,19 @@ constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
 constexpr int CODE_BYTES = 128 * 64, SLOT_BYTES = 256 * 16, CODE_TILE = CODE_BYTES + SLOT_BYTES;
 constexpr uint32_t NO_ENTRY = 0xffffffffu, TOO_MANY = 0xfffffffeu;
 
+// Steps after which a barrier that tells of a step's (or a code tile's) end is used again.  A wait tells a phase from the
+// next by one bit, so whoever waits must see every phase: with four groups taking tiles of two steps in turn, a group
+// comes back to the same barrier after 8 steps, whatever the number of stages.
+constexpr int TURN = 8;
+
 template <int MODE, int BN>
 struct Shape {
     static constexpr int STAGE = A_BYTES + BN * 128;
     static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 5 : 8;
     static constexpr int STAGES = BN == 128 ? 5 : 4;
     static constexpr int SUMS = MODE == GRADIENT ? 4 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
-    static constexpr int BARS = 2 * STAGES + 2 * CODES + 2;
+    static constexpr int BARS = STAGES + 3 * TURN + 2;
+    static_assert(STAGES <= TURN && CODES <= TURN, "a barrier is not met again before its last phase was seen");
     static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SUMS + BARS * 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of one block");
     static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
@@ -76,26 +82,26 @@ __device__ __forceinline__ uint4 values(uint32_t w, typename Pair<V>::T s, int z
                       __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
 }
 
-// scale and zero point of the two halves of 64 columns
+// scales and zero points of a row's 128 columns, 32 at a time
 template <typename V>
 struct Scales {
-    V s[2];
-    int z[2];
-    __device__ __forceinline__ void load(const Matrix<V> &m, int i, int g0, int g1) {
+    V s[4];
+    int z[4];
+    __device__ __forceinline__ void load(const Matrix<V> &m, int i, const GroupOf &at) {
+        const bool real = i < m.n_rows;
+        const long long row = (long long)(real ? i : 0) * m.n_groups;
+        const int last = m.n_groups - 1;  // behind the last column
+        if (m.group % 128 == 0) {
+            const int g = min(at.g, last);
+            s[0] = s[1] = s[2] = s[3] = real ? m.scales[row + g] : from_float<V>(0.f);
+            z[0] = z[1] = z[2] = z[3] = m.zeros ? m.zeros[row + g] & 15 : 8;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            s[j] = from_float<V>(0.f);
-            z[j] = 8;
-        }
-        if (i >= m.n_rows) return;
-        const long long at = (long long)i * m.n_groups;
-        g0 = min(g0, m.n_groups - 1);  // behind the last column
-        g1 = min(g1, m.n_groups - 1);
-        s[0] = m.scales[at + g0];
-        s[1] = g1 == g0 ? s[0] : m.scales[at + g1];
-        if (m.zeros) {
-            z[0] = m.zeros[at + g0] & 15;
-            z[1] = g1 == g0 ? z[0] : m.zeros[at + g1] & 15;
+            for (int j = 0; j < 4; ++j) {
+                const int g = min(at.after(j), last);
+                s[j] = real ? m.scales[row + g] : from_float<V>(0.f);
+                z[j] = m.zeros ? m.zeros[row + g] & 15 : 8;
+            }
         }
     }
 };
@@ -141,11 +147,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
     float *sums = reinterpret_cast<float *>(codes_at + S::CODES * CODE_TILE);
     const uint32_t bars = smem_addr(sums) + S::SUMS;
-    auto full = [&](int s) { return bars + 8 * s; };
-    auto empty = [&](int s) { return bars + 8 * (S::STAGES + s); };
-    auto c_full = [&](int s) { return bars + 8 * (2 * S::STAGES + s); };
-    auto c_empty = [&](int s) { return bars + 8 * (2 * S::STAGES + S::CODES + s); };
-    const uint32_t done = bars + 8 * (2 * S::STAGES + 2 * S::CODES), drained = done + 8;
+    auto full = [&](int s) { return bars + 8 * s; };                                   // of a stage
+    auto empty = [&](int step) { return bars + 8 * (S::STAGES + step % TURN); };       // of a step
+    auto c_full = [&](int n) { return bars + 8 * (S::STAGES + TURN + n % TURN); };     // of a code tile
+    auto c_empty = [&](int n) { return bars + 8 * (S::STAGES + 2 * TURN + n % TURN); };
+    const uint32_t done = bars + 8 * (S::STAGES + 3 * TURN), drained = done + 8;
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
 
     const Matrix<V> &m = g.m;
@@ -171,13 +177,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int s = 0; s < S::STAGES; ++s) {
-            mbar_init(full(s), MODE == GRADIENT ? 1 : 5);
-            mbar_init(empty(s), 1);
-        }
-        for (int s = 0; s < S::CODES; ++s) {
-            mbar_init(c_full(s), 1);
-            mbar_init(c_empty(s), 8);
+        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), MODE == GRADIENT ? 1 : MODE == PRODUCT ? 5 : 3);
+        for (int n = 0; n < TURN; ++n) {
+            mbar_init(empty(n), 1);
+            mbar_init(c_full(n), 1);
+            mbar_init(c_empty(n), 4);
         }
         mbar_init(done, 1);
         mbar_init(drained, 16);
@@ -188,6 +192,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
+    // the stage of a step is free, the place of a code tile likewise, once what was there before is used up
+    auto stage_free = [&](int step) {
+        return step < S::STAGES || mbar_wait(empty(step - S::STAGES), (step - S::STAGES) / TURN & 1, polls);
+    };
+    auto place_free = [&](int n) { return n < CODES || mbar_wait(c_empty(n - CODES), (n - CODES) / TURN & 1, polls); };
 
     if (warp == 0 && lane == 0) {  // ---- x and dy through bulk copies
         int n = 0;
@@ -195,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int turn = 0; turn < turns && ok; ++turn) {
             for (int step = 0; step < steps; ++step, ++n) {
                 const int s = n % S::STAGES;
-                if (!(ok = mbar_wait(empty(s), (n / S::STAGES & 1) ^ 1, polls))) break;
+                if (!(ok = stage_free(n))) break;
                 const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
                 if (MODE == GRADIENT) {
                     mbar_expect(full(s), S::STAGE);
@@ -221,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint64_t db0 = MODE == GRADIENT ? operand(base + A_BYTES, 8192, 1024) : operand(base + A_BYTES, 16, 1024);
         // 16 of the depth, in 16 bytes: 32 bytes of each row, or 16 rows of 128 bytes
         constexpr uint32_t NEXT_A = (MODE == PRODUCT ? 32 : 2048) / 16, NEXT_B = (MODE == GRADIENT ? 2048 : 32) / 16;
-        int s = 0;
+        int s = 0, n = 0;
         uint32_t parity = 0;
         bool ok = true;
         for (int turn = 0; turn < turns && ok; ++turn) {
@@ -229,13 +238,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!(ok = mbar_wait(drained, (turn - 1) & 1, polls))) break;
                 tc_fence_after();
             }
-            for (int step = 0; step < steps; ++step) {
+            for (int step = 0; step < steps; ++step, ++n) {
                 if (!(ok = mbar_wait(full(s), parity, polls))) break;
                 tc_fence_after();
                 const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
-                tc_commit(empty(s));
+                tc_commit(empty(n));
                 if (++s == S::STAGES) {
                     s = 0;
                     parity ^= 1;
@@ -252,85 +261,96 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true;
         for (; n < blocks; ++n) {
             const int s = n % CODES;
-            if (!(ok = mbar_wait(c_empty(s), (n / CODES & 1) ^ 1, polls))) break;
+            if (!(ok = place_free(n))) break;
             const int at = (block0 + n) * 128, row = MODE == PRODUCT ? line0 : at, col = MODE == PRODUCT ? at : line0;
             const uint32_t to = smem_addr(codes_at) + s * CODE_TILE;
-            mbar_expect(c_full(s), g.slots ? CODE_TILE : CODE_BYTES);
-            tma_load(to, &map_codes, col / 2, row, c_full(s));
+            mbar_expect(c_full(n), g.slots ? CODE_TILE : CODE_BYTES);
+            tma_load(to, &map_codes, col / 2, row, c_full(n));
             if (g.slots)
                 bulk_load(to + CODE_BYTES, g.slots + ((long long)(row / 128) * ((m.n_cols + 127) / 128) + col / 128) * 256,
-                          SLOT_BYTES, c_full(s));
+                          SLOT_BYTES, c_full(n));
         }
         if (!ok) {
             failed = 1;
-            for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k % CODES), k / CODES & 1, polls);
+            for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k), k / TURN & 1, polls);
         }
     } else if (MODE != GRADIENT && warp >= CONVERT) {  // ---- codes -> 16-bit values
-        // group 0 and 1 take the two halves of the even code tiles, group 2 and 3 those of the odd ones
-        const int group = (warp - CONVERT) / 4, half = group & 1, t = threadIdx.x - 32 * CONVERT - 128 * group;
-        // this thread's 64 values: a row of the tile (product), or half of one of its half's 64 rows (transposed)
-        const int tile_row = MODE == PRODUCT ? t : 64 * half + t % 64;
-        const int part = MODE == PRODUCT ? half : t / 64;
+        // the groups take code tiles in turn; a thread has one row of 128 columns: of the product's tile 64 columns of
+        // each of two stages, of the transposed product's all 128 columns of one stage (rows 0-63 or 64-127 of the tile)
+        const int group = (warp - CONVERT) / 4, t = threadIdx.x - 32 * CONVERT - 128 * group;
         const int out_row = MODE == PRODUCT ? t : t % 64;
-        const int out_block = MODE == PRODUCT ? 0 : t / 64 * 8192;
-        auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + tile_row : (block0 + n) * 128 + tile_row; };
-        auto col_at = [&](int n) { return (MODE == PRODUCT ? (block0 + n) * 128 : line0) + 64 * part; };
-        GroupOf at(col_at(group / 2), m.group, 256);
+        auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + t : (block0 + n) * 128 + t; };
+        auto col_at = [&](int n) { return MODE == PRODUCT ? (block0 + n) * 128 : line0; };
+        GroupOf at(col_at(group), m.group, 512);
         Scales<V> next;
-        if (group / 2 < blocks) next.load(m, row_at(group / 2), at.g, at.second());
+        if (group < blocks) next.load(m, row_at(group), at);
         bool ok = true;
-        for (int n = group / 2; n < blocks; n += 2) {
+        for (int n = group; n < blocks && ok; n += 4) {
             const Scales<V> now = next;
-            if (n + 2 < blocks) {
+            if (n + 4 < blocks) {
                 if (MODE == PRODUCT) at.move();
-                next.load(m, row_at(n + 2), at.g, at.second());
+                next.load(m, row_at(n + 4), at);
             }
-            const int cs = n % CODES, step = 2 * n + half, s = step % S::STAGES;
-            if (!(ok = warp_wait(c_full(cs), n / CODES & 1, polls))) break;
-            uint4 c[2], entries;
+            const int cs = n % CODES;
+            if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
+            uint4 c[4], entries[2];
             const uint8_t *from = codes_at + cs * CODE_TILE;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                c[j] = *reinterpret_cast<const uint4 *>(from + tile_row * 64 + ((2 * part + j ^ tile_row >> 1 & 3) << 4));
-            if (g.slots) entries = *reinterpret_cast<const uint4 *>(from + CODE_BYTES + (half * 128 + t) * 16);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(c_empty(cs));
-            if (!(ok = warp_wait(empty(s), (step / S::STAGES & 1) ^ 1, polls))) break;
-            uint8_t *a = smem + s * S::STAGE + out_block + out_row * 128;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const typename Pair<V>::T sc = Pair<V>::both(now.s[j]);
-                const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], sc, now.z[j]);
+            for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const uint4 *>(from + t * 64 + ((j ^ t >> 1 & 3) << 4));
+            if (g.slots) {
+                const uint4 *slot = reinterpret_cast<const uint4 *>(from + CODE_BYTES) + (MODE == PRODUCT ? t : t / 64 * 128 + t % 64);
+                entries[0] = slot[0];
+                entries[1] = slot[MODE == PRODUCT ? 128 : 64];
             }
-            if (g.slots && entries.x != NO_ENTRY) {
-                auto add = [&](int k, V v) {
-                    V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
-                    *e = from_float<V>(to_float(*e) + to_float(v));
-                };
-                if (entries.w != TOO_MANY) {
-                    const uint32_t entry[4] = {entries.x, entries.y, entries.z, entries.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint16_t v = (uint16_t)entry[j];
-                        if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
-                    }
-                } else {  // this thread looks for its entries itself
-                    const int k0 = col_at(n), k1 = min(k0 + 64, m.n_cols);
-                    int b, e;
-                    res_range(m, row_at(n), b, e);
-                    for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
-                        const int k = m.res_col[b];
-                        if (k < k0 || k >= k1) break;
-                        add(k - k0, m.res_val[b]);
-                    }
-                }
-            }
+            // the loads are done before the place is given back: a bulk copy would overtake those still under way
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive(full(s));
+            if (lane == 0) mbar_arrive(c_empty(n));
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {  // 64 columns
+                const int step = 2 * n + (MODE == PRODUCT ? part : t / 64), s = step % S::STAGES;
+                if (MODE == PRODUCT || part == 0)
+                    if (!(ok = __all_sync(0xffffffffu, stage_free(step)))) break;
+                uint8_t *a = smem + s * S::STAGE + out_row * 128 + (MODE == PRODUCT ? 0 : part * 8192);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint4 v = c[2 * part + j];
+                    const typename Pair<V>::T sc = Pair<V>::both(now.s[2 * part + j]);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) =
+                            values<V>(w[q], sc, now.z[2 * part + j]);
+                }
+                if (g.slots && entries[part].x != NO_ENTRY) {
+                    auto add = [&](int k, V v) {
+                        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
+                        *e = from_float<V>(to_float(*e) + to_float(v));
+                    };
+                    if (entries[part].w != TOO_MANY) {
+                        const uint32_t entry[4] = {entries[part].x, entries[part].y, entries[part].z, entries[part].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint16_t v = (uint16_t)entry[j];
+                            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
+                        }
+                    } else {  // this thread looks for its entries itself
+                        const int k0 = col_at(n) + 64 * part, k1 = min(k0 + 64, m.n_cols);
+                        int b, e;
+                        res_range(m, row_at(n), b, e);
+                        for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
+                            const int k = m.res_col[b];
+                            if (k < k0 || k >= k1) break;
+                            add(k - k0, m.res_val[b]);
+                        }
+                    }
+                }
+                if (MODE == PRODUCT || part == 1) {
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full(s));
+                }
+            }
         }
         if (!ok) failed = 1;
     }
