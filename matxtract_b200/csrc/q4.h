@@ -31,6 +31,8 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 template <typename V>
 __device__ __forceinline__ V from_float(float v);
 template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }

@@ -70,18 +70,6 @@ struct Args {
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
 
-// eight codes -> eight values in order; codes j and j + 4 sit in one register until the end
-template <typename V>
-__device__ __forceinline__ uint4 values(uint32_t w, typename Pair<V>::T s, int z) {
-    typename Pair<V>::T p[4];
-    Pair<V>::steps(w, z, p);
-    uint32_t r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = raw(__hmul2(p[j], s));
-    return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410),
-                      __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
-}
-
 // scales and zero points of a row's 128 columns, 32 at a time
 template <typename V>
 struct Scales {

@@ -55,6 +55,18 @@ struct Pair<__nv_bfloat16> {
 template <typename T>
 __device__ __forceinline__ uint32_t raw(T v) { return *reinterpret_cast<uint32_t *>(&v); }
 
+// eight codes -> eight values in order; codes j and j + 4 sit in one register until the end
+template <typename V>
+__device__ __forceinline__ uint4 values(uint32_t w, typename Pair<V>::T s, int z) {
+    typename Pair<V>::T p[4];
+    Pair<V>::steps(w, z, p);
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = raw(__hmul2(p[j], s));
+    return make_uint4(__byte_perm(r[0], r[1], 0x5410), __byte_perm(r[2], r[3], 0x5410),
+                      __byte_perm(r[0], r[1], 0x7632), __byte_perm(r[2], r[3], 0x7632));
+}
+
 // The group of a column that moves on by a fixed number of 32s, without a division at every move.
 struct GroupOf {
     int g, r, size, dg, dr;  // group, 32s into it, its 32s; the same of a move
