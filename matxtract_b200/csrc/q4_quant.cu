@@ -40,26 +40,140 @@ struct Scale {
     }
 };
 
-// 8 neighbouring values of a row from column k on, 0 from column `end` on, not yet taken apart
+// 8 neighbouring values of a row, 16-bit ones two to a register and worked on two at a time as long as that is exact.
 template <typename W>
-struct Raw {
-    uint4 u[sizeof(W) / 2];
-    __device__ __forceinline__ void load(const W *row, int k, int end, bool wide) {
+struct Eight;
+template <>
+struct Eight<float> {
+    float v[8];
+    using Limit = float;
+    static __device__ __forceinline__ Limit limit(float threshold) { return threshold; }
+    __device__ __forceinline__ void load(const float *row, int k, int end, bool wide) {
         if (wide && k + 8 <= end) {
-#pragma unroll
-            for (int j = 0; j < (int)sizeof(W) / 2; ++j) u[j] = __ldg(reinterpret_cast<const uint4 *>(row + k) + j);
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(row + k)), b = __ldg(reinterpret_cast<const float4 *>(row + k) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         } else {
-            W v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + j < end ? row[k + j] : from_float<W>(0.f);
-#pragma unroll
-            for (int j = 0; j < (int)sizeof(W) / 2; ++j) u[j] = reinterpret_cast<const uint4 *>(v)[j];
+            for (int j = 0; j < 8; ++j) v[j] = k + j < end ? row[k + j] : 0.f;
         }
     }
-    __device__ __forceinline__ void values(float (&v)[8]) const {
-        const W *w = reinterpret_cast<const W *>(u);
+    __device__ __forceinline__ unsigned far(Limit t) const {  // a bit for each value above the threshold
+        unsigned m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float(w[j]);
+        for (int j = 0; j < 8; ++j) m |= (unsigned)(fabsf(v[j]) > t) << j;
+        return m;
+    }
+    __device__ __forceinline__ int count(Limit t) const { return __popc(far(t)); }
+    __device__ __forceinline__ void drop(Limit t) {  // those become 0
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) > t ? 0.f : v[j];
+    }
+    // lowest and highest value (or only the highest magnitude), a NaN spreading
+    struct Range {
+        float lo = 0.f, hi = 0.f;
+        bool nan = false;
+        template <bool ZEROS>
+        __device__ __forceinline__ void take(const Eight &e) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (ZEROS) lo = fminf(lo, e.v[j]);
+                hi = fmaxf(hi, ZEROS ? e.v[j] : fabsf(e.v[j]));
+                nan |= e.v[j] != e.v[j];
+            }
+        }
+        template <bool ZEROS>
+        __device__ __forceinline__ void share(int lanes) {
+            for (int d = lanes / 2; d; d /= 2) {
+                if (ZEROS) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+            }
+            const unsigned nans = __ballot_sync(0xffffffffu, nan);
+            nan = (nans >> (threadIdx.x % 32 & ~(lanes - 1)) & (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1)) != 0;
+        }
+        __device__ __forceinline__ float low() const { return lo; }
+        __device__ __forceinline__ float high() const { return hi; }
+        __device__ __forceinline__ bool is_nan() const { return nan; }
+    };
+    __device__ __forceinline__ float at(int j) const {  // no indexing: the values stay in registers
+        float r = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) r = i == j ? v[i] : r;
+        return r;
+    }
+    __device__ __forceinline__ void all(float (&f)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = v[j];
+    }
+};
+template <typename W>
+struct Eight {
+    using T = typename Pair<W>::T;
+    uint32_t u[4];
+    using Limit = T;
+    // values of the type are above the threshold where they are above the type's last value that is not
+    static __device__ __forceinline__ Limit limit(float threshold) { return Pair<W>::both(rounded_down(threshold, W())); }
+    static __device__ __forceinline__ __half rounded_down(float v, __half) { return __float2half_rd(v); }
+    static __device__ __forceinline__ __nv_bfloat16 rounded_down(float v, __nv_bfloat16) { return __float2bfloat16_rd(v); }
+    __device__ __forceinline__ void load(const W *row, int k, int end, bool wide) {
+        if (wide && k + 8 <= end) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + k));
+            u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w;
+        } else {
+            const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                u[j] = (k + 2 * j < end ? r[k + 2 * j] : 0u) | (k + 2 * j + 1 < end ? (uint32_t)r[k + 2 * j + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ uint32_t mask(int j, Limit t) const { return __hgt2_mask(__habs2(Pair<W>::bits(u[j])), t); }
+    __device__ __forceinline__ unsigned far(Limit t) const {
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m |= (mask(j, t) & 0x00020001u) << 2 * j;
+        return (m | m >> 16) & 0xff;  // bits 2 j of the low halves, 2 j + 1 of the high ones
+    }
+    __device__ __forceinline__ int count(Limit t) const { return __popc(far(t)); }
+    __device__ __forceinline__ void drop(Limit t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] &= ~mask(j, t);
+    }
+    struct Range {
+        T lo = Pair<W>::bits(0u), hi = Pair<W>::bits(0u);
+        template <bool ZEROS>
+        __device__ __forceinline__ void take(const Eight &e) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const T v = Pair<W>::bits(e.u[j]);
+                if (ZEROS) lo = __hmin2_nan(lo, v);
+                hi = __hmax2_nan(hi, ZEROS ? v : __habs2(v));
+            }
+        }
+        template <bool ZEROS>
+        __device__ __forceinline__ void share(int lanes) {
+            for (int d = lanes / 2; d; d /= 2) {
+                if (ZEROS) lo = __hmin2_nan(lo, Pair<W>::bits(__shfl_xor_sync(0xffffffffu, raw(lo), d)));
+                hi = __hmax2_nan(hi, Pair<W>::bits(__shfl_xor_sync(0xffffffffu, raw(hi), d)));
+            }
+        }
+        __device__ __forceinline__ float low() const { return fminf(to_float(lo.x), to_float(lo.y)); }
+        __device__ __forceinline__ float high() const { return fmaxf(to_float(hi.x), to_float(hi.y)); }
+        __device__ __forceinline__ bool is_nan() const {
+            const float a = to_float(lo.x) + to_float(lo.y), b = to_float(hi.x), c = to_float(hi.y);
+            return a != a || b != b || c != c;
+        }
+    };
+    __device__ __forceinline__ float at(int j) const {
+        const uint32_t w = j < 4 ? j < 2 ? u[0] : u[1] : j < 6 ? u[2] : u[3];
+        const uint16_t b = (uint16_t)(w >> 16 * (j & 1));
+        return to_float(*reinterpret_cast<const W *>(&b));
+    }
+    __device__ __forceinline__ void all(float (&f)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const T v = Pair<W>::bits(u[j]);
+            f[2 * j] = to_float(v.x);
+            f[2 * j + 1] = to_float(v.y);
+        }
     }
 };
 
@@ -72,17 +186,13 @@ __global__ void __launch_bounds__(32 * WARPS) count_kernel(int n_rows, int n_col
     if (piece >= (long long)n_rows * per_row) return;
     const W *row = w + piece / per_row * ld;
     const int k0 = (int)(piece % per_row) * PIECE + 8 * lane;
-    Raw<W> raw[CHUNKS];
+    Eight<W> v[CHUNKS];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) raw[c].load(row, k0 + c * CHUNK, n_cols, wide);
+    for (int c = 0; c < CHUNKS; ++c) v[c].load(row, k0 + c * CHUNK, n_cols, wide);
+    const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
     int n = 0;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-        float v[8];
-        raw[c].values(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) n += fabsf(v[j]) > threshold;
-    }
+    for (int c = 0; c < CHUNKS; ++c) n += v[c].count(limit);
     // what lies behind the last column counts as 0, which is above a negative threshold
     if (threshold < 0.f)
         for (int c = 0; c < CHUNKS; ++c) n -= 8 - min(max(n_cols - (k0 + c * CHUNK), 0), 8);
@@ -121,9 +231,9 @@ __device__ __forceinline__ int clamped(long long n) { return (int)min(n, (long l
 
 // Entries of eight neighbouring columns that go to the residual, lanes in order; `at`: the warp's place.
 template <typename V, typename W>
-__device__ __forceinline__ void hand_out(const Out<V> &o, const float (&v)[8], unsigned far, int k, long long &at) {
+__device__ __forceinline__ void hand_out(const Out<V> &o, const Eight<W> &v, unsigned far, int k, long long &at) {
+    if (!__any_sync(0xffffffffu, far)) return;
     const int n = __popc(far), lane = threadIdx.x % 32;
-    if (!__any_sync(0xffffffffu, n)) return;
     int before = n;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -131,20 +241,23 @@ __device__ __forceinline__ void hand_out(const Out<V> &o, const float (&v)[8], u
         if (lane >= d) before += u;
     }
     long long e = at + before - n;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (far >> j & 1) {
-            if (e < o.res_cap) {
-                o.res_col[e] = k + j;
-                o.res_val[e] = from_float<V>(v[j]);
-            }
-            ++e;
+    while (far) {
+        const int j = __ffs(far) - 1;
+        if (e < o.res_cap) {
+            o.res_col[e] = k + j;
+            o.res_val[e] = from_float<V>(v.at(j));
         }
+        ++e;
+        far &= far - 1;
+    }
+    __syncwarp();
     at += __shfl_sync(0xffffffffu, before, 31);
 }
 
-// One warp a piece, for groups of 32, 64, ... 2048 columns: SPAN chunks a group (1: up to 256 columns, lanes of one chunk).
-// Reading W is what bounds it; the division by the scale is a multiplication unless a value comes near a border.
+// One warp a piece, for groups of 32, 64, ... 2048 columns: SPAN chunks a group (1: up to 256 columns, lanes of one
+// chunk).  Reading W and the ALU are about equally far from bounding it: ranges are taken two values at a time, and a
+// quotient is a product with the reciprocal and one step of correction, which is the correctly rounded quotient where
+// that has few bits, at a border between two codes above all.
 template <typename V, typename W, bool ZEROS, int SPAN>
 __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, const W *w, long long ld, bool wide,
                                                               float threshold) {
@@ -153,101 +266,76 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
     if (piece >= (long long)o.n_rows * o.per_row) return;
     const int row = (int)(piece / o.per_row), start = (int)(piece % o.per_row) * PIECE;
     const W *from = w + row * ld;
-    uint8_t *codes = o.codes + row * o.code_ld;
+    uint8_t *codes = o.codes + row * o.code_ld + start / 2 + 4 * lane;
     const int lanes = SPAN > 1 ? 32 : o.group / 8;  // that share a group in a chunk
-    Raw<W> raw[CHUNKS];
+    Eight<W> v[CHUNKS];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) raw[c].load(from, start + c * CHUNK + 8 * lane, o.n_cols, wide);
+    for (int c = 0; c < CHUNKS; ++c) v[c].load(from, start + c * CHUNK + 8 * lane, o.n_cols, wide);
     const bool split = o.res_ptr != nullptr;
-    long long at = 0;
+    const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
     if (split) {
-        at = entries_before(piece, o.counts, o.sums);
+        long long at = entries_before(piece, o.counts, o.sums);
         if (lane == 0 && start + PIECE >= o.n_cols) o.res_ptr[row + 1] = clamped(at + o.counts[piece]);
         if (lane == 0 && piece == 0) o.res_ptr[0] = 0;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int k = start + c * CHUNK + 8 * lane;
+            hand_out<V, W>(o, v[c], v[c].far(limit) & (k + 8 <= o.n_cols ? 0xffu : (1u << max(o.n_cols - k, 0)) - 1), k, at);
+            v[c].drop(limit);
+        }
     }
 #pragma unroll
     for (int c0 = 0; c0 < CHUNKS; c0 += SPAN) {
         if (start + c0 * CHUNK >= o.n_cols) break;
-        float lo = 0.f, hi = 0.f;
-        bool nan = false;
+        typename Eight<W>::Range range;
 #pragma unroll
-        for (int c = c0; c < c0 + SPAN; ++c) {
-            float v[8];
-            raw[c].values(v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = split && fabsf(v[j]) > threshold ? 0.f : v[j];
-                if (ZEROS) {
-                    lo = fminf(lo, x);
-                    hi = fmaxf(hi, x);
-                } else {
-                    hi = fmaxf(hi, fabsf(x));
-                }
-                nan |= x != x;
-            }
-        }
-        for (int d = lanes / 2; d; d /= 2) {
-            if (ZEROS) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        }
-        // a NaN concerns the lanes of its own group
-        const unsigned nans = __ballot_sync(0xffffffffu, nan);
-        nan = (nans >> (lane & ~(lanes - 1)) & (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1)) != 0;
-        const Scale<V, ZEROS> g(lo, hi, nan);
+        for (int c = c0; c < c0 + SPAN; ++c) range.template take<ZEROS>(v[c]);
+        range.template share<ZEROS>(lanes);
+        const Scale<V, ZEROS> g(range.low(), range.high(), range.is_nan());
         const int k0 = start + c0 * CHUNK + 8 * lane;
         if (lane % lanes == 0 && k0 < o.n_cols) {
             const long long to = (long long)row * o.n_groups + k0 / o.group;
             o.scales[to] = g.stored;
             if (ZEROS) o.zeros[to] = (uint8_t)g.z;
         }
-        // a product with the reciprocal is off by 2^-22 of itself at most, where the scale was not rounded to few bits
+        // a scale that was rounded to few bits, or is none at all, takes the long way
         const bool quick = g.usable && g.s > 6.2e-5f;
-        const float inverse = quick ? 1.f / g.s : 0.f;
+        const float inverse = quick ? 1.f / g.s : 0.f, most = 15.f - g.z;
+        constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
+        // the eight codes are summed up in place: what the sum of the eight MAGICs and zero points comes to
+        const uint32_t offset = 0x11111111u * ((uint32_t)g.z - __float_as_uint(MAGIC));
 #pragma unroll
         for (int c = c0; c < c0 + SPAN; ++c) {
             const int k = k0 + (c - c0) * CHUNK;
-            float v[8];
-            raw[c].values(v);
-            unsigned far = 0;
-            if (split) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (fabsf(v[j]) > threshold && k + j < o.n_cols) far |= 1u << j;
-                hand_out<V, W>(o, v, far, k, at);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (far >> j & 1) v[j] = 0.f;
-            }
-            constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
-            const float base = MAGIC + g.z;
-            float q[8], worst = 0.f;
+            float f[8];
+            v[c].all(f);
+            uint32_t word = offset;
+            bool border = false;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float t = v[j] * inverse;
-                q[j] = __fadd_rn(t, MAGIC) - MAGIC;
-                worst = fmaxf(worst, fabsf(t - q[j]));
+                float t = f[j] * inverse;
+                t = fmaf(fmaf(-t, g.s, f[j]), inverse, t);
+                if (ZEROS) t = fminf(t, most);
+                const float q = __fadd_rn(t, MAGIC);
+                word += __float_as_uint(q) << 4 * j;
+                if (sizeof(W) == 4) border |= fabsf(t - __fadd_rn(q, -MAGIC)) == 0.5f;  // or only near it
             }
-            if (__any_sync(0xffffffffu, worst > 0.499f || !quick)) {
-                if (quick) {
+            if (__any_sync(0xffffffffu, border || !quick)) {
+                uint32_t exact = 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) q[j] = nearest_from(q[j], v[j], g.s);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[j] = g.usable ? nearest_quotient(v[j], g.s) : 0.f;
+                for (int j = 0; j < 8; ++j) {
+                    const float q = g.usable ? nearest_quotient(f[j], g.s) : 0.f;
+                    exact |= (uint32_t)fminf(fmaxf(q + g.z, ZEROS ? 0.f : 1.f), 15.f) << 4 * j;
                 }
+                word = exact;
             }
-            uint32_t word = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = fminf(fmaxf(q[j] + base, ZEROS ? MAGIC : MAGIC + 1.f), MAGIC + 15.f);
-                word |= (__float_as_uint(f) & 15u) << 4 * j;
-            }
+            uint8_t *to = codes + c * (CHUNK / 2);
             if (k + 8 <= o.n_cols) {
-                *reinterpret_cast<uint32_t *>(codes + k / 2) = word;
+                *reinterpret_cast<uint32_t *>(to) = word;
             } else {
                 // the last bytes; a half behind the last column is 0
                 for (int j = 0; j < 8 && k + j < o.n_cols; j += 2)
-                    codes[(k + j) / 2] = (uint8_t)(k + j + 1 < o.n_cols ? word >> 4 * j : word >> 4 * j & 15);
+                    to[j / 2] = (uint8_t)(k + j + 1 < o.n_cols ? word >> 4 * j : word >> 4 * j & 15);
             }
         }
     }
