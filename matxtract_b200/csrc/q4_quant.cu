@@ -2,6 +2,7 @@
 #include <math.h>
 
 #include "q4.h"
+#include "q4_gemm.h"
 #include "q4_values.cuh"
 
 namespace mx {
@@ -12,7 +13,6 @@ constexpr int WARPS = 8;
 // A warp's piece of a row: 8 chunks of 256 columns, 8 neighbouring columns a lane, all asked for at once.  Short pieces
 // fill the GPU with few rows too; their entries follow one another in the residual's order.
 constexpr int CHUNK = 256, CHUNKS = 8, PIECE = CHUNK * CHUNKS;
-constexpr int BLOCK = 256;  // pieces whose counts are summed up in one number
 
 // w / s to the nearest whole number, ties to even.  The quotient's own rounding can put it on the wrong side of a
 // border (w may have 24 bits), the remainder cannot: q * s has 4 + 11 bits, so that w - q * s is exact near a border.
@@ -26,17 +26,41 @@ __device__ __forceinline__ float nearest_quotient(float w, float s) {
     return nearest_from(rintf(fminf(fmaxf(w / s, -32.f), 32.f)), w, s);
 }
 
-// scale and zero point of a group whose values reach from lo <= 0 to hi >= 0
+__device__ __forceinline__ float reciprocal(float v) {  // to a step or two
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// a / b with about = 1 / b to a step or two: the remainder's share corrects the product.  A quotient of few bits, such as
+// the border between two codes, comes out exactly.
+__device__ __forceinline__ float quotient(float a, float b, float about) {
+    const float t = a * about;
+    return fmaf(fmaf(-t, b, a), about, t);
+}
+constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
+
+// Scale and zero point of a group whose values reach from lo <= 0 to hi >= 0.  `quick`: the scale is an ordinary number
+// of the type; one that was rounded to few bits, or is none at all, takes the long way.
 template <typename V, bool ZEROS>
 struct Scale {
     V stored;
-    float s, z;
-    bool usable;
+    float s, z, inverse;
+    bool usable, quick;
     __device__ __forceinline__ Scale(float lo, float hi, bool nan) {
-        stored = from_float<V>(nan ? nanf("") : ZEROS ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
+        // a division by a constant: with the rounded reciprocal and one correction the quotient is correctly rounded
+        const float reach = ZEROS ? hi - lo : fmaxf(hi, -lo), steps = ZEROS ? 15.f : 7.f;
+        stored = from_float<V>(quotient(reach, steps, 1.f / steps));
         s = to_float(stored);
-        usable = s > 0.f && s <= 3.4028235e38f;
-        z = ZEROS ? (usable ? fminf(nearest_quotient(-lo, s), 15.f) : 0.f) : 8.f;
+        quick = !nan && s > 6.2e-5f && s <= 3.4028235e38f;
+        usable = quick;
+        inverse = reciprocal(s);
+        z = ZEROS ? fminf(nearest_from(__fadd_rn(quotient(-lo, s, inverse), MAGIC) - MAGIC, -lo, s), 15.f) : 8.f;
+        if (!quick) {
+            stored = from_float<V>(nan ? nanf("") : reach / steps);
+            s = to_float(stored);
+            usable = s > 0.f && s <= 3.4028235e38f;
+            z = ZEROS ? (usable ? fminf(nearest_quotient(-lo, s), 15.f) : 0.f) : 8.f;
+        }
     }
 };
 
@@ -177,40 +201,34 @@ struct Eight {
     }
 };
 
-// counts[piece] = entries above the threshold, sums[b] = those of the pieces b BLOCK .. (b + 1) BLOCK - 1
-template <typename W>
-__global__ void __launch_bounds__(32 * WARPS) count_kernel(int n_rows, int n_cols, int per_row, const W *w, long long ld,
-                                                           bool wide, float threshold, int *counts, int *sums) {
-    const long long piece = (long long)blockIdx.x * WARPS + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
-    if (piece >= (long long)n_rows * per_row) return;
-    const W *row = w + piece / per_row * ld;
-    const int k0 = (int)(piece % per_row) * PIECE + 8 * lane;
-    Eight<W> v[CHUNKS];
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) v[c].load(row, k0 + c * CHUNK, n_cols, wide);
-    const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
-    int n = 0;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) n += v[c].count(limit);
-    // what lies behind the last column counts as 0, which is above a negative threshold
-    if (threshold < 0.f)
-        for (int c = 0; c < CHUNKS; ++c) n -= 8 - min(max(n_cols - (k0 + c * CHUNK), 0), 8);
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) {
-        counts[piece] = n;
-        if (n) atomicAdd(sums + piece / BLOCK, n);  // whole numbers: the order does not matter
-    }
+// Where a block's entries begin is only known when all blocks in front of it have counted theirs.  A block takes its
+// number when it starts (so that all in front of it have started, too), tells how many entries it has as soon as it has
+// its values, works on its codes, and then walks back over the blocks in front: it adds up what they have until it meets
+// one that knows its end.  W is read once; a counting pass in front took 31 us of 8192 x 8192 (2 bytes).
+// A block's word: entries << 2 | 1 (its own) or 2 (with all in front).
+__device__ __forceinline__ void tell(unsigned long long *word, long long n, int kind) {
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(word), "l"((unsigned long long)n << 2 | kind) : "memory");
 }
-
-// Entries in front of a warp's piece, for each warp of a block of neighbouring pieces.
-__device__ __forceinline__ long long entries_before(long long piece, const int *counts, const int *sums) {
+__device__ int wait_ran_out_quant;
+// entries in front of block `me`, for one warp; -1 when a block in front does not tell in time
+__device__ __forceinline__ long long entries_before(const unsigned long long *words, long long me) {
     const int lane = threadIdx.x % 32;
-    const long long block = piece / BLOCK;
     long long n = 0;
-    for (long long b = lane; b < block; b += 32) n += sums[b];
-    for (long long p = block * BLOCK + lane; p < piece; p += 32) n += counts[p];
-    for (int d = 16; d; d /= 2) n += __shfl_xor_sync(0xffffffffu, n, d);
+    for (long long end = me; end > 0; end -= 32) {  // lanes: the 32 blocks in front of `end`, the nearest first
+        const long long b = end - 1 - lane;
+        unsigned long long w = 2;  // in front of the first block: nothing, and that is all
+        if (b >= 0) {
+            w = 0;
+            for (unsigned polls = 0; polls < 1u << 22 && w == 0; ++polls)
+                asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(w) : "l"(words + b) : "memory");
+        }
+        if (__any_sync(0xffffffffu, w == 0)) return -1;
+        const unsigned whole = __ballot_sync(0xffffffffu, (w & 3) == 2);
+        long long mine = whole && lane > __ffs(whole) - 1 ? 0 : (long long)(w >> 2);
+        for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+        n += mine;
+        if (whole) break;
+    }
     return n;
 }
 
@@ -221,7 +239,7 @@ struct Out {
     long long code_ld;
     V *scales;
     uint8_t *zeros;
-    const int *counts, *sums;  // residual only
+    unsigned long long *words;  // residual only: the next block's number, then a word for each block
     int *res_ptr, *res_col;
     V *res_val;
     int res_cap;
@@ -229,30 +247,79 @@ struct Out {
 
 __device__ __forceinline__ int clamped(long long n) { return (int)min(n, (long long)INT_MAX); }
 
-// Entries of eight neighbouring columns that go to the residual, lanes in order; `at`: the warp's place.
+// Entries among eight neighbouring columns a lane, lanes in order: `far` has their bits, `at` is the warp's place.
 template <typename V, typename W>
-__device__ __forceinline__ void hand_out(const Out<V> &o, const Eight<W> &v, unsigned far, int k, long long &at) {
-    if (!__any_sync(0xffffffffu, far)) return;
+__device__ __forceinline__ void hand_out(const Out<V> &o, const W *row, unsigned far, int k, long long &at) {
+    const unsigned some = __ballot_sync(0xffffffffu, far != 0);
+    if (!some) return;
     const int n = __popc(far), lane = threadIdx.x % 32;
-    int before = n;
+    int before = __popc(some & ((1u << lane) - 1)), all = __popc(some);
+    if (__any_sync(0xffffffffu, n > 1)) {
+        before = n;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const int u = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += u;
+        for (int d = 1; d < 32; d *= 2) {
+            const int u = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += u;
+        }
+        all = __shfl_sync(0xffffffffu, before, 31);
+        before -= n;
     }
-    long long e = at + before - n;
+    long long e = at + before;
     while (far) {
-        const int j = __ffs(far) - 1;
+        const int c = k + __ffs(far) - 1;
         if (e < o.res_cap) {
-            o.res_col[e] = k + j;
-            o.res_val[e] = from_float<V>(v.at(j));
+            o.res_col[e] = c;
+            o.res_val[e] = from_float<V>(to_float(row[c]));  // read again: few are
         }
         ++e;
         far &= far - 1;
     }
     __syncwarp();
-    at += __shfl_sync(0xffffffffu, before, 31);
+    at += all;
 }
+
+// What the blocks of a kernel do together to place their entries.
+struct Places {
+    long long front;
+    int counts[WARPS];
+    unsigned block;
+    // the block's number, in the order in which blocks start
+    __device__ __forceinline__ unsigned number(unsigned long long *words) {
+        if (threadIdx.x == 0) block = (unsigned)atomicAdd(words, 1ull);
+        __syncthreads();
+        return block;
+    }
+    // a warp has n entries
+    __device__ __forceinline__ void count(unsigned long long *words, int n) {
+        if (threadIdx.x % 32 == 0) counts[threadIdx.x / 32] = n;
+        __syncthreads();
+        if (threadIdx.x == 0) tell(words + 1 + block, all(), block == 0 ? 2 : 1);
+    }
+    __device__ __forceinline__ int all() const {
+        int n = 0;
+        for (int w = 0; w < WARPS; ++w) n += counts[w];
+        return n;
+    }
+    // where the warp's entries begin; -1 when a block in front did not tell in time
+    __device__ __forceinline__ long long mine(unsigned long long *words) {
+        const int warp = threadIdx.x / 32;
+        if (warp == 0) {
+            const long long n = entries_before(words + 1, block);
+            if (threadIdx.x == 0) {
+                front = n;
+                if (n < 0)
+                    wait_ran_out_quant = 1;
+                else if (block > 0)
+                    tell(words + 1 + block, n + all(), 2);
+            }
+        }
+        __syncthreads();
+        long long at = front;
+        if (at >= 0)
+            for (int w = 0; w < warp; ++w) at += counts[w];
+        return at;
+    }
+};
 
 // One warp a piece, for groups of 32, 64, ... 2048 columns: SPAN chunks a group (1: up to 256 columns, lanes of one
 // chunk).  Reading W and the ALU are about equally far from bounding it: ranges are taken two values at a time, and a
@@ -261,28 +328,34 @@ __device__ __forceinline__ void hand_out(const Out<V> &o, const Eight<W> &v, uns
 template <typename V, typename W, bool ZEROS, int SPAN>
 __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, const W *w, long long ld, bool wide,
                                                               float threshold) {
-    const long long piece = (long long)blockIdx.x * WARPS + threadIdx.x / 32;
+    __shared__ Places places;
+    const bool split = o.res_ptr != nullptr;
+    const unsigned block = split ? places.number(o.words) : blockIdx.x;
+    const long long piece = (long long)block * WARPS + threadIdx.x / 32, pieces = (long long)o.n_rows * o.per_row;
     const int lane = threadIdx.x % 32;
-    if (piece >= (long long)o.n_rows * o.per_row) return;
-    const int row = (int)(piece / o.per_row), start = (int)(piece % o.per_row) * PIECE;
+    const bool real = piece < pieces;
+    if (!real && !split) return;
+    const int row = real ? (int)(piece / o.per_row) : 0, start = real ? (int)(piece % o.per_row) * PIECE : o.n_cols;
     const W *from = w + row * ld;
     uint8_t *codes = o.codes + row * o.code_ld + start / 2 + 4 * lane;
     const int lanes = SPAN > 1 ? 32 : o.group / 8;  // that share a group in a chunk
     Eight<W> v[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) v[c].load(from, start + c * CHUNK + 8 * lane, o.n_cols, wide);
-    const bool split = o.res_ptr != nullptr;
-    const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
+    unsigned far[CHUNKS / 4] = {};  // a byte for each chunk
     if (split) {
-        long long at = entries_before(piece, o.counts, o.sums);
-        if (lane == 0 && start + PIECE >= o.n_cols) o.res_ptr[row + 1] = clamped(at + o.counts[piece]);
-        if (lane == 0 && piece == 0) o.res_ptr[0] = 0;
+        const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
+        int n = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int k = start + c * CHUNK + 8 * lane;
-            hand_out<V, W>(o, v[c], v[c].far(limit) & (k + 8 <= o.n_cols ? 0xffu : (1u << max(o.n_cols - k, 0)) - 1), k, at);
+            const unsigned f = v[c].far(limit) & (k + 8 <= o.n_cols ? 0xffu : (1u << max(o.n_cols - k, 0)) - 1);
+            far[c / 4] |= f << 8 * (c % 4);
             v[c].drop(limit);
         }
+#pragma unroll
+        for (int c = 0; c < CHUNKS / 4; ++c) n += __popc(far[c]);
+        places.count(o.words, __reduce_add_sync(0xffffffffu, n));
     }
 #pragma unroll
     for (int c0 = 0; c0 < CHUNKS; c0 += SPAN) {
@@ -298,10 +371,7 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
             o.scales[to] = g.stored;
             if (ZEROS) o.zeros[to] = (uint8_t)g.z;
         }
-        // a scale that was rounded to few bits, or is none at all, takes the long way
-        const bool quick = g.usable && g.s > 6.2e-5f;
-        const float inverse = quick ? 1.f / g.s : 0.f, most = 15.f - g.z;
-        constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
+        const float most = 15.f - g.z;
         // the eight codes are summed up in place: what the sum of the eight MAGICs and zero points comes to
         const uint32_t offset = 0x11111111u * ((uint32_t)g.z - __float_as_uint(MAGIC));
 #pragma unroll
@@ -313,14 +383,13 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
             bool border = false;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float t = f[j] * inverse;
-                t = fmaf(fmaf(-t, g.s, f[j]), inverse, t);
+                float t = quotient(f[j], g.s, g.inverse);
                 if (ZEROS) t = fminf(t, most);
                 const float q = __fadd_rn(t, MAGIC);
                 word += __float_as_uint(q) << 4 * j;
-                if (sizeof(W) == 4) border |= fabsf(t - __fadd_rn(q, -MAGIC)) == 0.5f;  // or only near it
+                if (sizeof(W) == 4) border |= fabsf(t - __fadd_rn(q, -MAGIC)) > 0.4999f;  // 24 bits may lie just beside it
             }
-            if (__any_sync(0xffffffffu, border || !quick)) {
+            if (__any_sync(0xffffffffu, border || !g.quick)) {
                 uint32_t exact = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -339,25 +408,40 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
             }
         }
     }
+    if (split) {
+        long long at = places.mine(o.words);
+        if (at < 0 || !real) return;
+        const long long next = at + places.counts[threadIdx.x / 32];
+        if (lane == 0 && start + PIECE >= o.n_cols) o.res_ptr[row + 1] = clamped(next);
+        if (lane == 0 && piece == 0) o.res_ptr[0] = 0;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+            hand_out<V, W>(o, from, far[c / 4] >> 8 * (c % 4) & 0xff, start + c * CHUNK + 8 * lane, at);
+    }
 }
 
 // Any other group: one warp a row, 64 columns (2 a lane) at a time; a group is gone through twice, for its range and for
 // its codes.
 template <typename V, typename W, bool ZEROS>
 __global__ void quantize_any_kernel(const Out<V> o, const W *w, long long ld, float threshold) {
-    const int row = blockIdx.x * WARPS + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (row >= o.n_rows) return;
-    const W *wr = w + row * ld;
-    uint8_t *cr = o.codes + row * o.code_ld;
+    __shared__ Places places;
     const bool split = o.res_ptr != nullptr;
+    const unsigned block = split ? places.number(o.words) : blockIdx.x;
+    const int row = (int)min((long long)block * WARPS + threadIdx.x / 32, (long long)INT_MAX), lane = threadIdx.x % 32;
+    const bool real = row < o.n_rows;
+    const W *wr = w + (real ? row : 0) * ld;
+    uint8_t *cr = o.codes + (real ? row : 0) * o.code_ld;
     long long at = 0;
     if (split) {
-        at = entries_before((long long)row * o.per_row, o.counts, o.sums);
-        const long long next = entries_before((row + 1ll) * o.per_row, o.counts, o.sums);
-        if (lane == 0) {
-            o.res_ptr[row + 1] = clamped(next);
-            if (row == 0) o.res_ptr[0] = 0;
-        }
+        int n = 0;
+        for (int k = lane; real && k < o.n_cols; k += 32) n += fabsf(to_float(wr[k])) > threshold;
+        places.count(o.words, __reduce_add_sync(0xffffffffu, n));
+        at = places.mine(o.words);
+    }
+    if (!real || at < 0) return;
+    if (split && lane == 0) {
+        o.res_ptr[row + 1] = clamped(at + places.counts[threadIdx.x / 32]);
+        if (row == 0) o.res_ptr[0] = 0;
     }
     for (int g = 0; g < o.n_groups; ++g) {
         const int k0 = g * o.group, k1 = (int)min((long long)o.n_cols, (long long)k0 + o.group);
@@ -499,20 +583,14 @@ cudaError_t quantize_from(const mx_q4_matrix &m, const W *w, long long ld, float
     o.scales = static_cast<V *>(m.scales);
     o.zeros = static_cast<uint8_t *>(m.zeros);
     const bool wide = (uintptr_t)w % 16 == 0 && (m.n_rows == 1 || ld * sizeof(W) % 16 == 0);
-    const long long pieces = (long long)m.n_rows * o.per_row, blocks = ceil_div(pieces, BLOCK);
+    const long long pieces = (long long)m.n_rows * o.per_row;
     if (ceil_div(pieces, WARPS) > INT_MAX) return cudaErrorInvalidConfiguration;
     Workspace work(s);
     if (m.res_row_ptr) {
-        int *counts = nullptr;
-        cudaError_t e = work.take((void **)&counts, sizeof(int) * (pieces + blocks));
+        const size_t bytes = sizeof(unsigned long long) * (1 + ceil_div(pieces, WARPS));
+        cudaError_t e = work.take((void **)&o.words, bytes);
+        if (e == cudaSuccess) e = cudaMemsetAsync(o.words, 0, bytes, s);
         if (e != cudaSuccess) return e;
-        int *sums = counts + pieces;
-        if ((e = cudaMemsetAsync(sums, 0, sizeof(int) * blocks, s)) != cudaSuccess) return e;
-        count_kernel<<<(unsigned)ceil_div(pieces, WARPS), 32 * WARPS, 0, s>>>(m.n_rows, m.n_cols, o.per_row, w, ld, wide,
-                                                                              threshold, counts, sums);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-        o.counts = counts;
-        o.sums = sums;
         o.res_ptr = m.res_row_ptr;
         o.res_col = m.res_col_ind;
         o.res_val = static_cast<V *>(m.res_val);
@@ -539,6 +617,12 @@ cudaError_t expand(const Matrix<V> &m, V *w, long long ld, cudaStream_t s) {
     const bool wide = (uintptr_t)w % 16 == 0 && (m.n_rows == 1 || ld % 8 == 0);
     expand_kernel<<<(unsigned)blocks, 32 * WARPS, 0, s>>>(m, per_row, w, ld, wide);
     return cudaGetLastError();
+}
+
+cudaError_t waits_ran_out_quant(int *flag, cudaStream_t s) {
+    void *p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_quant);
+    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
 }
 
 #define INSTANTIATE(V)                                                                                              \
