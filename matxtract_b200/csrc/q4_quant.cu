@@ -10,9 +10,10 @@ namespace q4 {
 namespace {
 
 constexpr int WARPS = 8;
-// A warp's piece of a row: 8 chunks of 256 columns, 8 neighbouring columns a lane, all asked for at once.  Short pieces
-// fill the GPU with few rows too; their entries follow one another in the residual's order.
-constexpr int CHUNK = 256, CHUNKS = 8, PIECE = CHUNK * CHUNKS;
+// A warp's piece of a row: 4 chunks of 512 columns, 16 neighbouring columns a lane, all asked for at once.  Short pieces
+// fill the GPU with few rows too; their entries follow one another in the residual's order.  (With 8 columns a lane the
+// work on a group's scale, which all lanes do, was more than that on the codes.)
+constexpr int CHUNK = 512, CHUNKS = 4, PIECE = CHUNK * CHUNKS;
 
 // w / s to the nearest whole number, ties to even.  The quotient's own rounding can put it on the wrong side of a
 // border (w may have 24 bits), the remainder cannot: q * s has 4 + 11 bits, so that w - q * s is exact near a border.
@@ -235,6 +236,7 @@ __device__ __forceinline__ long long entries_before(const unsigned long long *wo
 template <typename V>
 struct Out {
     int n_rows, n_cols, group, n_groups, per_row;
+    int shift;  // where group is a power of two: its logarithm
     uint8_t *codes;
     long long code_ld;
     V *scales;
@@ -247,7 +249,7 @@ struct Out {
 
 __device__ __forceinline__ int clamped(long long n) { return (int)min(n, (long long)INT_MAX); }
 
-// Entries among eight neighbouring columns a lane, lanes in order: `far` has their bits, `at` is the warp's place.
+// Entries among sixteen neighbouring columns a lane, lanes in order: `far` has their bits, `at` is the warp's place.
 template <typename V, typename W>
 __device__ __forceinline__ void hand_out(const Out<V> &o, const W *row, unsigned far, int k, long long &at) {
     const unsigned some = __ballot_sync(0xffffffffu, far != 0);
@@ -321,7 +323,7 @@ struct Places {
     }
 };
 
-// One warp a piece, for groups of 32, 64, ... 2048 columns: SPAN chunks a group (1: up to 256 columns, lanes of one
+// One warp a piece, for groups of 32, 64, ... 2048 columns: SPAN chunks a group (1: up to 512 columns, lanes of one
 // chunk).  Reading W and the ALU are about equally far from bounding it: ranges are taken two values at a time, and a
 // quotient is a product with the reciprocal and one step of correction, which is the correctly rounded quotient where
 // that has few bits, at a border between two codes above all.
@@ -337,24 +339,28 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
     if (!real && !split) return;
     const int row = real ? (int)(piece / o.per_row) : 0, start = real ? (int)(piece % o.per_row) * PIECE : o.n_cols;
     const W *from = w + row * ld;
-    uint8_t *codes = o.codes + row * o.code_ld + start / 2 + 4 * lane;
-    const int lanes = SPAN > 1 ? 32 : o.group / 8;  // that share a group in a chunk
-    Eight<W> v[CHUNKS];
+    uint8_t *codes = o.codes + row * o.code_ld + start / 2 + 8 * lane;
+    const int lanes = SPAN > 1 ? 32 : o.group / 16;  // that share a group in a chunk
+    Eight<W> v[CHUNKS][2];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) v[c].load(from, start + c * CHUNK + 8 * lane, o.n_cols, wide);
-    unsigned far[CHUNKS / 4] = {};  // a byte for each chunk
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[c][h].load(from, start + c * CHUNK + 16 * lane + 8 * h, o.n_cols, wide);
+    unsigned far[CHUNKS / 2] = {};  // sixteen bits for each chunk
     if (split) {
         const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
         int n = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int k = start + c * CHUNK + 8 * lane;
-            const unsigned f = v[c].far(limit) & (k + 8 <= o.n_cols ? 0xffu : (1u << max(o.n_cols - k, 0)) - 1);
-            far[c / 4] |= f << 8 * (c % 4);
-            v[c].drop(limit);
+            const int k = start + c * CHUNK + 16 * lane;
+            const unsigned f = (v[c][0].far(limit) | v[c][1].far(limit) << 8) &
+                               (k + 16 <= o.n_cols ? 0xffffu : (1u << max(o.n_cols - k, 0)) - 1);
+            far[c / 2] |= f << 16 * (c % 2);
+            v[c][0].drop(limit);
+            v[c][1].drop(limit);
         }
 #pragma unroll
-        for (int c = 0; c < CHUNKS / 4; ++c) n += __popc(far[c]);
+        for (int c = 0; c < CHUNKS / 2; ++c) n += __popc(far[c]);
         places.count(o.words, __reduce_add_sync(0xffffffffu, n));
     }
 #pragma unroll
@@ -362,12 +368,15 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
         if (start + c0 * CHUNK >= o.n_cols) break;
         typename Eight<W>::Range range;
 #pragma unroll
-        for (int c = c0; c < c0 + SPAN; ++c) range.template take<ZEROS>(v[c]);
+        for (int c = c0; c < c0 + SPAN; ++c) {
+            range.template take<ZEROS>(v[c][0]);
+            range.template take<ZEROS>(v[c][1]);
+        }
         range.template share<ZEROS>(lanes);
         const Scale<V, ZEROS> g(range.low(), range.high(), range.is_nan());
-        const int k0 = start + c0 * CHUNK + 8 * lane;
+        const int k0 = start + c0 * CHUNK + 16 * lane;
         if (lane % lanes == 0 && k0 < o.n_cols) {
-            const long long to = (long long)row * o.n_groups + k0 / o.group;
+            const long long to = (long long)row * o.n_groups + (k0 >> o.shift);
             o.scales[to] = g.stored;
             if (ZEROS) o.zeros[to] = (uint8_t)g.z;
         }
@@ -377,34 +386,40 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
 #pragma unroll
         for (int c = c0; c < c0 + SPAN; ++c) {
             const int k = k0 + (c - c0) * CHUNK;
-            float f[8];
-            v[c].all(f);
-            uint32_t word = offset;
-            bool border = false;
+            uint32_t word[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float t = quotient(f[j], g.s, g.inverse);
-                if (ZEROS) t = fminf(t, most);
-                const float q = __fadd_rn(t, MAGIC);
-                word += __float_as_uint(q) << 4 * j;
-                if (sizeof(W) == 4) border |= fabsf(t - __fadd_rn(q, -MAGIC)) > 0.4999f;  // 24 bits may lie just beside it
-            }
-            if (__any_sync(0xffffffffu, border || !g.quick)) {
-                uint32_t exact = 0;
+            for (int h = 0; h < 2; ++h) {
+                float f[8];
+                v[c][h].all(f);
+                word[h] = offset;
+                bool border = false;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float q = g.usable ? nearest_quotient(f[j], g.s) : 0.f;
-                    exact |= (uint32_t)fminf(fmaxf(q + g.z, ZEROS ? 0.f : 1.f), 15.f) << 4 * j;
+                    float t = quotient(f[j], g.s, g.inverse);
+                    if (ZEROS) t = fminf(t, most);
+                    const float q = __fadd_rn(t, MAGIC);
+                    word[h] += __float_as_uint(q) << 4 * j;
+                    if (sizeof(W) == 4) border |= fabsf(t - __fadd_rn(q, -MAGIC)) > 0.4999f;  // 24 bits may lie just beside it
                 }
-                word = exact;
+                if (__any_sync(0xffffffffu, border || !g.quick)) {
+                    uint32_t exact = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float q = g.usable ? nearest_quotient(f[j], g.s) : 0.f;
+                        exact |= (uint32_t)fminf(fmaxf(q + g.z, ZEROS ? 0.f : 1.f), 15.f) << 4 * j;
+                    }
+                    word[h] = exact;
+                }
             }
             uint8_t *to = codes + c * (CHUNK / 2);
-            if (k + 8 <= o.n_cols) {
-                *reinterpret_cast<uint32_t *>(to) = word;
+            if (k + 16 <= o.n_cols) {
+                *reinterpret_cast<uint2 *>(to) = make_uint2(word[0], word[1]);
             } else {
                 // the last bytes; a half behind the last column is 0
-                for (int j = 0; j < 8 && k + j < o.n_cols; j += 2)
-                    to[j / 2] = (uint8_t)(k + j + 1 < o.n_cols ? word >> 4 * j : word >> 4 * j & 15);
+                for (int j = 0; j < 16 && k + j < o.n_cols; j += 2) {
+                    const uint32_t w8 = word[j / 8] >> 4 * (j % 8);
+                    to[j / 2] = (uint8_t)(k + j + 1 < o.n_cols ? w8 : w8 & 15);
+                }
             }
         }
     }
@@ -416,7 +431,7 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
         if (lane == 0 && piece == 0) o.res_ptr[0] = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
-            hand_out<V, W>(o, from, far[c / 4] >> 8 * (c % 4) & 0xff, start + c * CHUNK + 8 * lane, at);
+            hand_out<V, W>(o, from, far[c / 2] >> 16 * (c % 2) & 0xffff, start + c * CHUNK + 16 * lane, at);
     }
 }
 
@@ -493,9 +508,11 @@ __global__ void quantize_any_kernel(const Out<V> o, const W *w, long long ld, fl
     }
 }
 
-// One warp a piece: the codes' values first, then the entries of the residual on top of them.
+// One warp a piece, 8 neighbouring columns a lane, so that a warp's stores are one run of 512 bytes: the codes' values
+// first, then the entries of the residual on top of them.
 template <typename V>
 __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per_row, V *w, long long ld, bool wide) {
+    constexpr int STEPS = PIECE / 256;
     const long long piece = (long long)blockIdx.x * WARPS + threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (piece >= (long long)m.n_rows * per_row) return;
@@ -503,13 +520,15 @@ __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per
     const uint8_t *codes = m.codes + row * m.code_ld;
     const V *scales = m.scales + (long long)row * m.n_groups;
     V *to = w + row * ld;
-    uint32_t c[CHUNKS];
-    V s[CHUNKS];
-    int z[CHUNKS];
-    GroupOf at(start + 8 * lane, m.group, CHUNK);
+    int begin = 0, end = 0;
+    if (m.res_ptr) res_range(m, row, begin, end);
+    uint32_t c[STEPS];
+    V s[STEPS];
+    int z[STEPS];
+    GroupOf at(start + 8 * lane, m.group, 256);
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-        const int k = start + j * CHUNK + 8 * lane;
+    for (int j = 0; j < STEPS; ++j) {
+        const int k = start + j * 256 + 8 * lane;
         c[j] = 0;
         s[j] = from_float<V>(0.f);
         z[j] = 8;
@@ -520,11 +539,12 @@ __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per
         }
         at.move();
     }
-    int begin = 0, end = 0;
-    if (m.res_ptr) res_range(m, row, begin, end);
+    int early[2];  // the first entries' columns are on their way meanwhile
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-        const int k = start + j * CHUNK + 8 * lane;
+    for (int j = 0; j < 2; ++j) early[j] = begin + 32 * j + lane < end ? m.res_col[begin + 32 * j + lane] : -1;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+        const int k = start + j * 256 + 8 * lane;
         const uint4 v = values<V>(c[j], Pair<V>::both(s[j]), z[j]);
         if (wide && k + 8 <= m.n_cols) {
             *reinterpret_cast<uint4 *>(to + k) = v;
@@ -538,8 +558,8 @@ __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per
     if (begin >= end) return;
     __syncwarp();
     const int stop = min(m.n_cols, start + PIECE);
-    for (int i = begin + lane; i < end; i += 32) {
-        const int k = m.res_col[i];
+    for (int i = begin + lane, n = 0; i < end; i += 32, ++n) {
+        const int k = n == 0 ? early[0] : n == 1 ? early[1] : m.res_col[i];
         if (k < start || k >= stop || (i > begin && m.res_col[i - 1] == k)) continue;
         const int g = k / m.group, code = codes[k / 2] >> 4 * (k & 1) & 15;
         float v = to_float(scales[g]) * (float)(code - zero_of(m, row, g));
@@ -556,10 +576,10 @@ cudaError_t quantize_as(const Out<V> &o, const W *w, long long ld, bool wide, fl
         case 32:
         case 64:
         case 128:
-        case 256: quantize_kernel<V, W, ZEROS, 1><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
-        case 512: quantize_kernel<V, W, ZEROS, 2><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
-        case 1024: quantize_kernel<V, W, ZEROS, 4><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
-        case 2048: quantize_kernel<V, W, ZEROS, 8><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
+        case 256:
+        case 512: quantize_kernel<V, W, ZEROS, 1><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
+        case 1024: quantize_kernel<V, W, ZEROS, 2><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
+        case 2048: quantize_kernel<V, W, ZEROS, 4><<<grid, threads, 0, s>>>(o, w, ld, wide, threshold); break;
         default:
             quantize_any_kernel<V, W, ZEROS><<<(unsigned)ceil_div(o.n_rows, WARPS), threads, 0, s>>>(o, w, ld, threshold);
     }
@@ -578,6 +598,7 @@ cudaError_t quantize_from(const mx_q4_matrix &m, const W *w, long long ld, float
     o.group = m.group;
     o.n_groups = (int)ceil_div(m.n_cols, m.group);
     o.per_row = (int)ceil_div(m.n_cols, PIECE);
+    while ((1 << o.shift) < m.group) ++o.shift;
     o.codes = static_cast<uint8_t *>(m.codes);
     o.code_ld = m.code_ld;
     o.scales = static_cast<V *>(m.scales);
