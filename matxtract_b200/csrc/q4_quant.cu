@@ -249,9 +249,10 @@ struct Out {
 
 __device__ __forceinline__ int clamped(long long n) { return (int)min(n, (long long)INT_MAX); }
 
-// Entries among sixteen neighbouring columns a lane, lanes in order: `far` has their bits, `at` is the warp's place.
-template <typename V, typename W>
-__device__ __forceinline__ void hand_out(const Out<V> &o, const W *row, unsigned far, int k, long long &at) {
+// Entries among sixteen neighbouring columns a lane, lanes in order: calls put(place, column of the sixteen) for each of
+// the bits of `far`; `at` is the warp's place.
+template <typename F>
+__device__ __forceinline__ void in_order(unsigned far, long long &at, F put) {
     const unsigned some = __ballot_sync(0xffffffffu, far != 0);
     if (!some) return;
     const int n = __popc(far), lane = threadIdx.x % 32;
@@ -268,12 +269,7 @@ __device__ __forceinline__ void hand_out(const Out<V> &o, const W *row, unsigned
     }
     long long e = at + before;
     while (far) {
-        const int c = k + __ffs(far) - 1;
-        if (e < o.res_cap) {
-            o.res_col[e] = c;
-            o.res_val[e] = from_float<V>(to_float(row[c]));  // read again: few are
-        }
-        ++e;
+        put(e++, __ffs(far) - 1);
         far &= far - 1;
     }
     __syncwarp();
@@ -328,13 +324,16 @@ struct Places {
 // quotient is a product with the reciprocal and one step of correction, which is the correctly rounded quotient where
 // that has few bits, at a border between two codes above all.
 template <typename V, typename W, bool ZEROS, int SPAN>
-__global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, const W *w, long long ld, bool wide,
-                                                              float threshold) {
+__global__ void __launch_bounds__(32 * WARPS, sizeof(W) == 2 ? 4 : 2)
+    quantize_kernel(const Out<V> o, const W *w, long long ld, bool wide, float threshold) {
     __shared__ Places places;
+    constexpr int KEPT = 256;  // entries of a piece that wait for their place here, column of the piece << 16 | value
+    __shared__ uint32_t kept[WARPS][KEPT];
     const bool split = o.res_ptr != nullptr;
-    const unsigned block = split ? places.number(o.words) : blockIdx.x;
-    const long long piece = (long long)block * WARPS + threadIdx.x / 32, pieces = (long long)o.n_rows * o.per_row;
     const int lane = threadIdx.x % 32;
+    const long long pieces = (long long)o.n_rows * o.per_row;
+    const unsigned block = split ? places.number(o.words) : blockIdx.x;
+    const long long piece = (long long)block * WARPS + threadIdx.x / 32;
     const bool real = piece < pieces;
     if (!real && !split) return;
     const int row = real ? (int)(piece / o.per_row) : 0, start = real ? (int)(piece % o.per_row) * PIECE : o.n_cols;
@@ -347,21 +346,26 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
 #pragma unroll
         for (int h = 0; h < 2; ++h) v[c][h].load(from, start + c * CHUNK + 16 * lane + 8 * h, o.n_cols, wide);
     unsigned far[CHUNKS / 2] = {};  // sixteen bits for each chunk
+    int mine = 0;                   // entries of the warp
     if (split) {
         const typename Eight<W>::Limit limit = Eight<W>::limit(threshold);
-        int n = 0;
+        long long at = 0;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int k = start + c * CHUNK + 16 * lane;
             const unsigned f = (v[c][0].far(limit) | v[c][1].far(limit) << 8) &
                                (k + 16 <= o.n_cols ? 0xffffu : (1u << max(o.n_cols - k, 0)) - 1);
             far[c / 2] |= f << 16 * (c % 2);
+            in_order(f, at, [&](long long e, int j) {
+                const V x = from_float<V>(j < 8 ? v[c][0].at(j) : v[c][1].at(j - 8));
+                if (e < KEPT)
+                    kept[threadIdx.x / 32][e] = (uint32_t)(c * CHUNK + 16 * lane + j) << 16 | *reinterpret_cast<const uint16_t *>(&x);
+            });
             v[c][0].drop(limit);
             v[c][1].drop(limit);
         }
-#pragma unroll
-        for (int c = 0; c < CHUNKS / 2; ++c) n += __popc(far[c]);
-        places.count(o.words, __reduce_add_sync(0xffffffffu, n));
+        mine = (int)at;
+        places.count(o.words, mine);
     }
 #pragma unroll
     for (int c0 = 0; c0 < CHUNKS; c0 += SPAN) {
@@ -423,15 +427,31 @@ __global__ void __launch_bounds__(32 * WARPS) quantize_kernel(const Out<V> o, co
             }
         }
     }
-    if (split) {
-        long long at = places.mine(o.words);
-        if (at < 0 || !real) return;
-        const long long next = at + places.counts[threadIdx.x / 32];
-        if (lane == 0 && start + PIECE >= o.n_cols) o.res_ptr[row + 1] = clamped(next);
-        if (lane == 0 && piece == 0) o.res_ptr[0] = 0;
+    if (!split) return;
+    long long at = places.mine(o.words);
+    if (at < 0) return;  // the whole block
+    if (real && lane == 0) {
+        if (start + PIECE >= o.n_cols) o.res_ptr[row + 1] = clamped(at + mine);
+        if (piece == 0) o.res_ptr[0] = 0;
+    }
+    if (mine <= KEPT) {
+        for (int i = lane; i < mine; i += 32)
+            if (at + i < o.res_cap) {
+                const uint32_t e = kept[threadIdx.x / 32][i];
+                const uint16_t x = (uint16_t)e;
+                o.res_col[at + i] = start + (e >> 16);
+                o.res_val[at + i] = *reinterpret_cast<const V *>(&x);
+            }
+    } else {  // more than were kept: their values are read again
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
-            hand_out<V, W>(o, from, far[c / 2] >> 16 * (c % 2) & 0xffff, start + c * CHUNK + 16 * lane, at);
+            in_order(far[c / 2] >> 16 * (c % 2) & 0xffff, at, [&](long long e, int j) {
+                const int k = start + c * CHUNK + 16 * lane + j;
+                if (e < o.res_cap) {
+                    o.res_col[e] = k;
+                    o.res_val[e] = from_float<V>(to_float(from[k]));
+                }
+            });
     }
 }
 
