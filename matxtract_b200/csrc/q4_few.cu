@@ -66,7 +66,6 @@ struct Few {
     V *out;
     long long ld_out;
     V *d_res;
-    const int *starts;  // transposed: [block of 256 columns][row] first residual entry not left of the block
 };
 
 // d += 16 rows x 8 columns (a word of the upper and of the lower eight rows) times the vectors' values
@@ -454,8 +453,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             const int rows = 128 / g.splits;
             for (int j = threadIdx.x; j < rows * g.n_vec; j += STREAM_THREADS) {
                 const int t = j / rows, r = rank * rows + j % rows;
-                float s = 0.f;
-                for (int q = 0; q < g.splits; ++q) s += cluster_load(smem_addr(extra + t * 128 + r), q);
+                const float s = cluster_sum(smem_addr(extra + t * 128 + r), g.splits);
                 if (ok && row0 + r < m.n_rows) g.out[t * g.ld_out + row0 + r] = from_float<V>(s);
             }
             __syncwarp();
@@ -478,33 +476,7 @@ __global__ void turn_kernel(const V *x, long long ld, int n_vec, int n_cols, int
     }
 }
 
-// starts[b][i] = first entry of row i with a column not below 256 b, for b = 0 .. blocks; 32 rows and 64 blocks of
-// columns at a time, so that both the entries and the results are touched in order.
-template <typename V>
-__global__ void __launch_bounds__(256) starts_kernel(Matrix<V> m, int blocks, int chunks, int *starts) {
-    __shared__ int part[64][33];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int row0 = blockIdx.x / chunks * 32, b0 = blockIdx.x % chunks * 64;
-    for (int r = warp; r < 32 && row0 + r < m.n_rows; r += 8) {
-        int begin, end;
-        res_range(m, row0 + r, begin, end);
-        begin = first_at_least(m.res_col, begin, end, (int)min(b0 * 256ll, (long long)INT_MAX));
-        int before = b0 - 1;  // block of the entry in front
-        for (int e = begin + lane; before < b0 + 63; e += 32) {
-            // behind the last entry everything starts at the end
-            const int b = e < end ? min(max(m.res_col[e] / 256, b0 - 1), b0 + 63) : b0 + 63;
-            int left = __shfl_up_sync(0xffffffffu, b, 1);
-            if (lane == 0) left = before;
-            for (int k = left + 1; k <= b; ++k) part[k - b0][r] = min(e, end);
-            before = __shfl_sync(0xffffffffu, b, 31);
-        }
-    }
-    __syncthreads();
-    for (int k = warp; k < 64 && b0 + k <= blocks; k += 8)
-        if (row0 + lane < m.n_rows) starts[(long long)(b0 + k) * m.n_rows + row0 + lane] = part[k][lane];
-}
-
-// dx = dy W for up to 8 vectors.  A block has 256 columns, its warps take 16 rows at a time; the contraction runs over
+// dx = dy W for up to 8 vectors and no residual.  A block has 256 columns, its warps take 16 rows at a time; the contraction runs over
 // rows, whose scales differ, so the values are s (c - z), rounded once to the type.  The blocks of a cluster share the
 // rows.  A lane holds 32 columns of four rows; two rows' codes of a column are brought into one register.
 constexpr int COLS = 256, VEC = 8, VEC_STRIDE = 268, WARP_PART = VEC * VEC_STRIDE;
@@ -599,48 +571,6 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
     for (int c = 0; c < 16; ++c)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mine[part_at(2 * quarter + j % 2, 32 * line + 2 * c + j / 2)] = d[c][j];
-    if (m.res_ptr) {
-        // a lane a row; lanes whose entries meet in a column add one after the other, lower rows first
-        __syncwarp();
-        const int k1 = (int)min((long long)m.n_cols, (long long)k0 + COLS), last = min(to * 16, m.n_rows);
-        const int *starts = g.starts + (long long)(k0 / COLS) * m.n_rows;
-        for (int i0 = from * 16 + 32 * warp; i0 < last; i0 += 32 * WARPS) {
-            const int i = i0 + lane;
-            int at = i < last ? starts[i] : 0;
-            const int end = i < last ? starts[m.n_rows + i] : 0;
-            float dy[VEC];
-#pragma unroll
-            for (int t = 0; t < VEC; ++t) dy[t] = at < end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
-            while (__any_sync(0xffffffffu, at < end)) {
-                constexpr int TOGETHER = 4;
-                int col[TOGETHER];
-                V val[TOGETHER];
-#pragma unroll
-                for (int j = 0; j < TOGETHER; ++j) {
-                    col[j] = at + j < end ? m.res_col[at + j] : INT_MAX;
-                    val[j] = at + j < end ? m.res_val[at + j] : from_float<V>(0.f);
-                }
-#pragma unroll
-                for (int j = 0; j < TOGETHER; ++j) {
-                    const bool hit = col[j] >= k0 && col[j] < k1;
-                    if (!__any_sync(0xffffffffu, hit)) continue;
-                    const float v = to_float(val[j]);
-                    const unsigned same = __match_any_sync(0xffffffffu, hit ? col[j] : -1 - lane);
-                    const int turn = __popc(same & ((1u << lane) - 1));
-                    const int turns = __reduce_max_sync(0xffffffffu, turn);
-                    for (int n = 0; n <= turns; ++n) {
-                        if (hit && turn == n) {
-#pragma unroll
-                            for (int t = 0; t < VEC; ++t)
-                                if (t < g.n_vec) mine[part_at(t, col[j] - k0)] += v * dy[t];
-                        }
-                        __syncwarp();
-                    }
-                }
-                at += TOGETHER;
-            }
-        }
-    }
     __syncthreads();
     const int c = threadIdx.x;  // a column
     float s[VEC];
@@ -662,8 +592,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
     const int width = COLS / g.splits;
     for (int j = threadIdx.x; j < width * g.n_vec; j += THREADS) {
         const int t = j / width, col = rank * width + j % width;
-        float total = 0.f;
-        for (int q = 0; q < g.splits; ++q) total += cluster_load(smem_addr(parts + part_at(t, col)), q);
+        const float total = cluster_sum(smem_addr(parts + part_at(t, col)), g.splits);
         if (k0 + col < m.n_cols) g.out[t * g.ld_out + k0 + col] = from_float<V>(total);
     }
     __syncwarp();
@@ -758,7 +687,8 @@ cudaError_t stream_inputs(Few<V> &g, const V *x, long long ld_x, CUtensorMap &co
 
 template <typename V>
 cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
-    if (n_vec > 16) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
+    // 16 vectors, 4096 x 4096: 16.5 us here (one block an SM then), 10.2 us there; 8 vectors: 7 and 10
+    if (n_vec > 8) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
@@ -769,18 +699,17 @@ cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V
     CUtensorMap codes = {}, map_x = {};
     const cudaError_t e = stream_inputs(g, x, ld_x, codes, map_x, m.res_ptr != nullptr, work);
     if (e != cudaSuccess) return e;
-    const bool one = n_vec <= 8;
-    if (m.group % 128 == 0)
-        return one ? stream<V, 128, 1, false>(g, codes, map_x, s) : stream<V, 128, 2, false>(g, codes, map_x, s);
-    if (m.group % 64 == 0)
-        return one ? stream<V, 64, 1, false>(g, codes, map_x, s) : stream<V, 64, 2, false>(g, codes, map_x, s);
-    return one ? stream<V, 32, 1, false>(g, codes, map_x, s) : stream<V, 32, 2, false>(g, codes, map_x, s);
+    return m.group % 128 == 0  ? stream<V, 128, 1, false>(g, codes, map_x, s)
+           : m.group % 64 == 0 ? stream<V, 64, 1, false>(g, codes, map_x, s)
+                               : stream<V, 32, 1, false>(g, codes, map_x, s);
 }
 
 template <typename V>
 cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
                       cudaStream_t s) {
-    if (n_vec > VEC) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
+    // The residual's entries meet in columns: where there are some, the tiles that they are put into are faster even for
+    // one vector (4096 x 4096: 19 us there, 28 us with a search and ordered additions here).
+    if (n_vec > VEC || m.res_ptr) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
     const long long blocks = ceil_div(m.n_cols, COLS);
     Few<V> g = {};
     g.m = m;
@@ -791,15 +720,6 @@ cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_d
     Workspace work(s);
     cudaError_t e = aligned_rows(dy, ld_dy, m.n_rows, n_vec, work, &g.dy, &g.ld_dy);
     if (e == cudaSuccess) e = allow_smem<V, product_t_few_kernel<V>>(T_SMEM);
-    if (e == cudaSuccess && m.res_ptr && m.n_rows > 0) {
-        const long long chunks = ceil_div(blocks + 1, 64), grid = ceil_div(m.n_rows, 32) * chunks;
-        int *starts = nullptr;
-        if (grid > INT_MAX) return cudaErrorMemoryAllocation;
-        if ((e = work.take((void **)&starts, sizeof(int) * (blocks + 1) * m.n_rows)) != cudaSuccess) return e;
-        starts_kernel<<<(unsigned)grid, 256, 0, s>>>(m, (int)blocks, (int)chunks, starts);
-        e = cudaGetLastError();
-        g.starts = starts;
-    }
     return e == cudaSuccess ? run<V>(product_t_few_kernel<V>, blocks * g.splits, g.splits, T_SMEM, g, s) : e;
 }
 

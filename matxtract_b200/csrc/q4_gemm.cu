@@ -384,8 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int j = group; j < width; j += 4) {
                     const int c = rank * width + j;
                     const uint32_t at = base + (c * 128 + row) * 4;
-                    float sum = 0.f;
-                    for (int p = 0; p < g.splits; ++p) sum += cluster_load(at, p);
+                    const float sum = cluster_sum(at, g.splits);
                     if (line < lines && col0 + c < col_end) g.out[(col0 + c) * g.ld_out + line] = from_float<V>(sum);
                 }
             }

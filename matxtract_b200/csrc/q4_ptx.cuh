@@ -130,8 +130,20 @@ __device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
     uint32_t a;
     float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
     return v;
+}
+
+// the sum over the `n` <= 8 blocks of a cluster, in the order of their ranks, all asked for at once
+__device__ __forceinline__ float cluster_sum(uint32_t addr, int n) {
+    float v[8], sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        if (r < n) v[r] = cluster_load(addr, r);
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        if (r < n) sum += v[r];
+    return sum;
 }
 
 }  // namespace q4
