@@ -454,57 +454,69 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 1) tmem_free(tmem, COLUMNS);
 }
 
-// The residual's entries into the slots of the code tiles, 32 rows and 4096 columns at a time: collected in shared memory,
-// then written in order.  A segment of 64 columns with more than four entries, or with a repeated column, is marked.
+// First entry of [begin, end) whose column is at least k, for a whole warp: 32 places are looked at together.
+__device__ __forceinline__ int warp_first_at_least(const int *col, int begin, int end, int k) {
+    const int lane = threadIdx.x % 32;
+    while (end - begin > 32) {
+        const int step = (end - begin + 31) / 32, p = min(begin + (lane + 1) * step, end) - 1;  // the last of each part
+        const unsigned below = __ballot_sync(0xffffffffu, col[p] < k);
+        const int parts = below == 0xffffffffu ? 32 : __ffs(~below) - 1;  // that lie in front of k altogether
+        const int from = min(begin + parts * step, end);
+        end = min(from + step, end);
+        begin = from;
+    }
+    const bool below = begin + lane < end && col[begin + lane] < k;
+    return begin + __popc(__ballot_sync(0xffffffffu, below));
+}
+
+// The residual's entries into the slots of the code tiles, 32 rows (a warp each) and 4096 columns at a time: collected in
+// shared memory, then written in order.  A segment of 64 columns with more than four entries, or with a repeated column,
+// is marked.  (With four rows a warp, one after the other, it waited for memory 13 us of 8192 x 8192.)
 template <typename V, int MODE>
-__global__ void __launch_bounds__(256) slots_kernel(Matrix<V> m, int chunks, uint4 *slots) {
+__global__ void __launch_bounds__(1024) slots_kernel(Matrix<V> m, int chunks, uint4 *slots) {
     __shared__ uint4 part[64][32];  // [segment][row]
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32, r = threadIdx.x / 32;
     const int row0 = blockIdx.x / chunks * 32, k0 = blockIdx.x % chunks * 4096;
-    for (int j = threadIdx.x; j < 64 * 32; j += 256)
+    int begin = 0, end = 0;
+    if (row0 + r < m.n_rows) res_range(m, row0 + r, begin, end);
+    for (int j = threadIdx.x; j < 64 * 32; j += 1024)
         part[j / 32][j % 32] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
     __syncthreads();
     const int k1 = min((long long)m.n_cols, k0 + 4096ll);
-    for (int r = warp; r < 32 && row0 + r < m.n_rows; r += 8) {
-        int begin, end;
-        res_range(m, row0 + r, begin, end);
-        begin = first_at_least(m.res_col, begin, end, k0);
-        int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
-        for (int e0 = begin; e0 < end; e0 += 32) {
-            const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
-            const bool mine = k >= k0 && k < k1;
-            const int segment = mine ? (k - k0) / 64 : 64;
-            int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
-            if (lane == 0) {
-                left = segment_before;
-                column = column_before;
-            }
-            const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
-            const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
-            uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
-            if (mine && rank < 4) {
-                const V v = m.res_val[e];
-                to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
-            }
-            __syncwarp();
-            if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
-            __syncwarp();
-            segment_before = __shfl_sync(0xffffffffu, segment, 31);
-            column_before = __shfl_sync(0xffffffffu, k, 31);
-            run = __shfl_sync(0xffffffffu, rank, 31) + 1;
-            if (segment_before == 64) break;
+    if (k0 > 0) begin = warp_first_at_least(m.res_col, begin, end, k0);
+    int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
+    for (int e0 = begin; e0 < end; e0 += 32) {
+        const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
+        const V v = e < end ? m.res_val[e] : from_float<V>(0.f);
+        const bool mine = k >= k0 && k < k1;
+        const int segment = mine ? (k - k0) / 64 : 64;
+        int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
+        if (lane == 0) {
+            left = segment_before;
+            column = column_before;
         }
+        const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
+        const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
+        uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
+        if (mine && rank < 4) to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
+        __syncwarp();
+        if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
+        __syncwarp();
+        segment_before = __shfl_sync(0xffffffffu, segment, 31);
+        column_before = __shfl_sync(0xffffffffu, k, 31);
+        run = __shfl_sync(0xffffffffu, rank, 31) + 1;
+        if (segment_before == 64) break;
     }
     __syncthreads();
     const long long tiles = (m.n_cols + 127) / 128;
     const int i = row0 + lane;
-    for (int j = warp; j < 64 && k0 + 64 * j < m.n_cols; j += 8) {
+    for (int j = r; j < 64 && k0 + 64 * j < m.n_cols; j += 32) {
         const int in_tile = MODE == PRODUCT ? j % 2 * 128 + i % 128 : i % 128 / 64 * 128 + j % 2 * 64 + i % 64;
-        slots[((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile] = part[j][lane];
+        uint4 *to = slots + ((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile;
+        *to = part[j][lane];
         // the second half of a last tile that has no columns there
         if (j % 2 == 0 && k0 + 64 * (j + 1) >= m.n_cols)
-            slots[((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile + (MODE == PRODUCT ? 128 : 64)] =
-                make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+            to[MODE == PRODUCT ? 128 : 64] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
     }
 }
 
@@ -586,7 +598,7 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
             uint4 *slots = nullptr;
             if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
             if ((e = work.take((void **)&slots, SLOT_BYTES * rows * cols)) != cudaSuccess) return e;
-            slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 256, 0, s>>>(m, (int)chunks, slots);
+            slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 1024, 0, s>>>(m, (int)chunks, slots);
             if ((e = cudaGetLastError()) != cudaSuccess) return e;
             g.slots = slots;
         }
