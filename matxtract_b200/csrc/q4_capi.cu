@@ -185,7 +185,7 @@ int mx_q4_check(const mx_q4_matrix *m, void *stream) {
     OnDevice on(m->device);
     if (on.status != MX_OK) return on.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int *flag = nullptr, bad = 0, late[3] = {0, 0, 0};
+    int *flag = nullptr, bad = 0, late[4] = {0, 0, 0, 0};
     cudaError_t e = cudaMallocAsync((void **)&flag, sizeof(int), s);
     if (e != cudaSuccess) return done(e);
     e = cudaMemsetAsync(flag, 0, sizeof(int), s);
@@ -198,11 +198,12 @@ int mx_q4_check(const mx_q4_matrix *m, void *stream) {
     if (e == cudaSuccess) e = waits_ran_out(&late[0], s);
     if (e == cudaSuccess) e = waits_ran_out_few(&late[1], s);
     if (e == cudaSuccess) e = waits_ran_out_quant(&late[2], s);
+    if (e == cudaSuccess) e = waits_ran_out_grad(&late[3], s);
     cudaError_t f = cudaFreeAsync(flag, s);
     if (e == cudaSuccess) e = f;
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return done(e);
-    return late[0] || late[1] || late[2] ? MX_ERR_TIMEOUT : bad ? MX_ERR_INVALID : MX_OK;
+    return late[0] || late[1] || late[2] || late[3] ? MX_ERR_TIMEOUT : bad ? MX_ERR_INVALID : MX_OK;
 }
 
 }  // extern "C"

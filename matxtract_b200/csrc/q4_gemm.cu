@@ -1,14 +1,12 @@
-// Products of a 4-bit matrix with many vectors, and the gradients of its numbers, on the fifth-generation tensor cores.
+// Products of a 4-bit matrix with many vectors on the fifth-generation tensor cores.
 //
-// One block computes D[128 x BN] in tensor memory, contraction 64 deep a stage:
-//   product    D[i][t] = sum_k W[i][k] x[t][k]     A = W's rows, depth-major         B = x's rows, depth-major
-//   transposed D[k][t] = sum_i W[i][k] dy[t][i]    A = W's columns, line-major       B = dy's rows, depth-major
-//   gradient   D[i][k] = sum_t dy[t][i] x[t][k]    A = dy's columns, line-major      B = x's columns, line-major
+// One block computes D[128 x BN] in tensor memory, contraction 64 deep a step:
+//   product    D[i][t] = sum_k W[i][k] x[t][k]     A = W's rows, depth-major      B = x's rows, depth-major
+//   transposed D[k][t] = sum_i W[i][k] dy[t][i]    A = W's columns, line-major    B = dy's rows, depth-major
 // x and dy come through tiled bulk copies.  W is made on the way: its codes come through a ring of their own (128 rows x
-// 128 columns = 8 KB each) and two groups of four warps turn them into 16-bit values s * (c - z), rounded once, add the
+// 128 columns = 8 KB each) and four groups of four warps turn them into 16-bit values s * (c - z), rounded once, add the
 // residual's entries that fall into the tile, and store them in the operand's swizzled layout; in this form a tile of W
-// has the same bytes for the product and its transpose, only the operand descriptor differs.  The gradient keeps D and
-// reduces it against the codes in the epilogue: G is never stored.
+// has the same bytes for the product and its transpose, only the operand descriptor differs.
 // Where there are fewer tiles than SMs, up to four blocks of a cluster share a tile's contraction and add their parts
 // through distributed shared memory, in the order of their ranks.
 #include <limits.h>
@@ -27,7 +25,7 @@ namespace mx {
 namespace q4 {
 namespace {
 
-enum { PRODUCT, TRANSPOSED, GRADIENT };
+enum { PRODUCT, TRANSPOSED };
 
 // Warps: 0 copies of x and dy, 1 tensor core issue, 2 copies of codes, 3 none; then four groups of four warps that turn
 // codes into values and empty the tensor memory.
@@ -47,14 +45,13 @@ constexpr int TURN = 8;
 template <int MODE, int BN>
 struct Shape {
     static constexpr int STAGE = A_BYTES + BN * 128;
-    static constexpr int CODES = MODE == GRADIENT ? 0 : BN == 256 ? 2 : BN == 128 ? 5 : 8;
+    static constexpr int CODES = BN == 256 ? 2 : BN == 128 ? 5 : 8;
     static constexpr int STAGES = BN == 128 ? 5 : 4;
-    static constexpr int SUMS = MODE == GRADIENT ? 4 * 8 * 128 * 4 : 0;  // parts of the scales' gradients
-    static constexpr int BARS = STAGES + 3 * TURN + 2;
+    static constexpr int BARS = STAGES + 3 * TURN + 1;
     static_assert(STAGES <= TURN && CODES <= TURN, "a barrier is not met again before its last phase was seen");
-    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + SUMS + BARS * 8;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + BARS * 8;
     static_assert(SMEM <= 227 * 1024, "shared memory of one block");
-    static_assert(MODE == GRADIENT || STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
+    static_assert(STAGES * STAGE >= 128 * BN * 4, "room for the parts of a split contraction");
 };
 
 template <typename V>
@@ -63,9 +60,7 @@ struct Args {
     int n_vec, tiles_m, splits;
     V *out;
     long long ld_out;
-    V *d_res;
-    const uint4 *slots;   // the residual's entries as code tiles take them, [row / 128][column / 128]; null: none
-    int groups_per_unit;  // gradient: groups that one block owns
+    const uint4 *slots;  // the residual's entries as code tiles take them, [row / 128][column / 128]; null: none
 };
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
@@ -94,52 +89,24 @@ struct Scales {
     }
 };
 
-// entries of one row, columns ascending, the next two already loaded
-template <typename V>
-struct Cursor {
-    int at = 0, end = 0, col[2];
-    V val[2];
-    __device__ __forceinline__ void fetch(const Matrix<V> &m, int j) {
-        const int p = at + j;
-        col[j] = p < end ? m.res_col[p] : 0x7fffffff;
-        val[j] = p < end ? m.res_val[p] : from_float<V>(0.f);
-    }
-    __device__ __forceinline__ void start(const Matrix<V> &m, int i, int k) {
-        at = end = 0;
-        if (m.res_ptr && i < m.n_rows) {
-            res_range(m, i, at, end);
-            at = first_at_least(m.res_col, at, end, k);
-        }
-        fetch(m, 0);
-        fetch(m, 1);
-    }
-    __device__ __forceinline__ void next(const Matrix<V> &m) {
-        ++at;
-        col[0] = col[1];
-        val[0] = val[1];
-        fetch(m, 1);
-    }
-};
-
 template <typename V, int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_a,
-                const __grid_constant__ CUtensorMap map_b, const Args<V> g) {
+    gemm_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ Args<V> g) {
     using S = Shape<MODE, BN>;
-    constexpr int CODES = S::CODES ? S::CODES : 1;
+    constexpr int CODES = S::CODES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_shared;
     __shared__ volatile int failed;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
-    float *sums = reinterpret_cast<float *>(codes_at + S::CODES * CODE_TILE);
-    const uint32_t bars = smem_addr(sums) + S::SUMS;
+    const uint32_t bars = smem_addr(codes_at + CODES * CODE_TILE);
     auto full = [&](int s) { return bars + 8 * s; };                                   // of a stage
     auto empty = [&](int step) { return bars + 8 * (S::STAGES + step % TURN); };       // of a step
     auto c_full = [&](int n) { return bars + 8 * (S::STAGES + TURN + n % TURN); };     // of a code tile
     auto c_empty = [&](int n) { return bars + 8 * (S::STAGES + 2 * TURN + n % TURN); };
-    const uint32_t done = bars + 8 * (S::STAGES + 3 * TURN), drained = done + 8;
+    const uint32_t done = bars + 8 * (S::STAGES + 3 * TURN);
     constexpr uint32_t COLUMNS = BN < 32 ? 32 : BN;
 
     const Matrix<V> &m = g.m;
@@ -147,32 +114,24 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int rank = g.splits > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / g.splits;
     const int line0 = tile % g.tiles_m * 128;  // first row of D: a row of W, or a column for the transposed product
-    const int unit = tile / g.tiles_m;
+    const int col0 = tile / g.tiles_m * BN, col_end = min(g.n_vec, col0 + BN);
 
-    // what is contracted, in steps of 64: columns, rows or vectors
-    const int depth = MODE == PRODUCT ? m.n_cols : MODE == TRANSPOSED ? m.n_rows : g.n_vec;
+    // what is contracted, columns or rows of W, in steps of 64
+    const int depth = MODE == PRODUCT ? m.n_cols : m.n_rows;
     const int blocks128 = (int)(((long long)depth + 127) / 128);
     const int block0 = (int)((long long)blocks128 * rank / g.splits);
-    const int blocks = (int)((long long)blocks128 * (rank + 1) / g.splits) - block0;
-    const int steps = MODE == GRADIENT ? (depth + 63) / 64 : 2 * blocks;
-    // columns of D: vectors, or for the gradient the columns of a whole number of groups, in turns of BN
-    const int col0 = MODE == GRADIENT ? unit * g.groups_per_unit * m.group : unit * BN;
-    const int col_end = MODE == GRADIENT
-                            ? (int)min((long long)m.n_cols, col0 + (long long)g.groups_per_unit * m.group)
-                            : min(g.n_vec, col0 + BN);
-    const int turns = MODE == GRADIENT ? (col_end - col0 + BN - 1) / BN : 1;
+    const int blocks = (int)((long long)blocks128 * (rank + 1) / g.splits) - block0, steps = 2 * blocks;
     const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
 
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), MODE == GRADIENT ? 1 : MODE == PRODUCT ? 5 : 3);
+        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), MODE == PRODUCT ? 5 : 3);
         for (int n = 0; n < TURN; ++n) {
             mbar_init(empty(n), 1);
             mbar_init(c_full(n), 1);
             mbar_init(c_empty(n), 4);
         }
         mbar_init(done, 1);
-        mbar_init(drained, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_addr(&tmem_shared), COLUMNS);
@@ -186,25 +145,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     auto place_free = [&](int n) { return n < CODES || mbar_wait(c_empty(n - CODES), (n - CODES) / TURN & 1, polls); };
 
-    if (warp == 0 && lane == 0) {  // ---- x and dy through bulk copies
+    if (warp == 0 && lane == 0) {  // ---- x or dy
         int n = 0;
         bool ok = true;
-        for (int turn = 0; turn < turns && ok; ++turn) {
-            for (int step = 0; step < steps; ++step, ++n) {
-                const int s = n % S::STAGES;
-                if (!(ok = stage_free(n))) break;
-                const uint32_t a = base + s * S::STAGE, b = a + A_BYTES;
-                if (MODE == GRADIENT) {
-                    mbar_expect(full(s), S::STAGE);
-                    for (int j = 0; j < 2; ++j)
-                        tma_load(a + j * 8192, &map_a, line0 + 64 * j, step * 64, full(s));
-                    for (int j = 0; j < BN / 64; ++j)
-                        tma_load(b + j * 8192, &map_b, col0 + turn * BN + 64 * j, step * 64, full(s));
-                } else {
-                    mbar_expect(full(s), BN * 128);
-                    tma_load(b, &map_b, block0 * 128 + step * 64, col0, full(s));
-                }
-            }
+        for (; n < steps; ++n) {
+            const int s = n % S::STAGES;
+            if (!(ok = stage_free(n))) break;
+            mbar_expect(full(s), BN * 128);
+            tma_load(base + s * S::STAGE + A_BYTES, &map_b, block0 * 128 + n * 64, col0, full(s));
         }
         if (!ok) {  // nothing of this block may still be on its way when it ends
             failed = 1;
@@ -212,39 +160,29 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mbar_wait(full(k % S::STAGES), k / S::STAGES & 1, polls);
         }
     } else if (warp == 1 && elect_one()) {  // ---- tensor cores
-        constexpr bool BF16 = !std::is_same<V, __half>::value;
-        constexpr uint32_t idesc = mma_shape(BF16, BN, MODE != PRODUCT, MODE == GRADIENT);
+        constexpr uint32_t idesc = mma_shape(!std::is_same<V, __half>::value, BN, MODE == TRANSPOSED, false);
         const uint64_t da0 = MODE == PRODUCT ? operand(base, 16, 1024) : operand(base, 8192, 1024);
-        const uint64_t db0 = MODE == GRADIENT ? operand(base + A_BYTES, 8192, 1024) : operand(base + A_BYTES, 16, 1024);
+        const uint64_t db0 = operand(base + A_BYTES, 16, 1024);
         // 16 of the depth, in 16 bytes: 32 bytes of each row, or 16 rows of 128 bytes
-        constexpr uint32_t NEXT_A = (MODE == PRODUCT ? 32 : 2048) / 16, NEXT_B = (MODE == GRADIENT ? 2048 : 32) / 16;
-        int s = 0, n = 0;
+        constexpr uint32_t NEXT_A = (MODE == PRODUCT ? 32 : 2048) / 16, NEXT_B = 32 / 16;
+        int s = 0;
         uint32_t parity = 0;
         bool ok = true;
-        for (int turn = 0; turn < turns && ok; ++turn) {
-            if (turn > 0) {
-                if (!(ok = mbar_wait(drained, (turn - 1) & 1, polls))) break;
-                tc_fence_after();
-            }
-            for (int step = 0; step < steps; ++step, ++n) {
-                if (!(ok = mbar_wait(full(s), parity, polls))) break;
-                tc_fence_after();
-                const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
+        for (int n = 0; n < steps; ++n) {
+            if (!(ok = mbar_wait(full(s), parity, polls))) break;
+            tc_fence_after();
+            const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
-                tc_commit(empty(n));
-                if (++s == S::STAGES) {
-                    s = 0;
-                    parity ^= 1;
-                }
+            for (int j = 0; j < 4; ++j) tc_mma(tmem, da + NEXT_A * j, db + NEXT_B * j, idesc, n > 0 || j > 0);
+            tc_commit(empty(n));
+            if (++s == S::STAGES) {
+                s = 0;
+                parity ^= 1;
             }
-            if (ok) tc_commit(done);
         }
-        if (!ok) {
-            failed = 1;
-            tc_commit(done);
-        }
-    } else if (MODE != GRADIENT && warp == 2 && lane == 0) {  // ---- codes
+        if (!ok) failed = 1;
+        tc_commit(done);
+    } else if (warp == 2 && lane == 0) {  // ---- codes
         int n = 0;
         bool ok = true;
         for (; n < blocks; ++n) {
@@ -262,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             failed = 1;
             for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k), k / TURN & 1, polls);
         }
-    } else if (MODE != GRADIENT && warp >= CONVERT) {  // ---- codes -> 16-bit values
+    } else if (warp >= CONVERT) {  // ---- codes -> 16-bit values
         // the groups take code tiles in turn; a thread has one row of 128 columns: of the product's tile 64 columns of
         // each of two stages, of the transposed product's all 128 columns of one stage (rows 0-63 or 64-127 of the tile)
         const int group = (warp - CONVERT) / 4, t = threadIdx.x - 32 * CONVERT - 128 * group;
@@ -348,104 +286,47 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int group = (warp - CONVERT) / 4, row = warp % 4 * 32 + lane;
     const bool drains = warp >= CONVERT;
     const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
-    if (MODE != GRADIENT) {
-        const int line = line0 + row, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
-        bool ok = false;
-        if (drains) {
-            ok = __all_sync(0xffffffffu, warp_wait(done, 0, polls) && !failed);
-            if (!ok) failed = 1;
-            tc_fence_after();
-        }
-        float v[32];
-        if (ok) {
-            for (int c = 32 * group; c < BN; c += 128) {
-                if (steps > 0) {
-                    tmem_load32(quarter + c, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                }
-                if (g.splits == 1) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (line < lines && col0 + c + j < col_end)
-                            g.out[(col0 + c + j) * g.ld_out + line] = from_float<V>(v[j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) reinterpret_cast<float *>(smem)[(c + j) * 128 + row] = v[j];
-                }
-            }
-        }
-        if (g.splits > 1) {
-            __syncwarp();
-            cluster_barrier();
-            if (ok) {
-                const int width = BN / g.splits;
-                for (int j = group; j < width; j += 4) {
-                    const int c = rank * width + j;
-                    const uint32_t at = base + (c * 128 + row) * 4;
-                    const float sum = cluster_sum(at, g.splits);
-                    if (line < lines && col0 + c < col_end) g.out[(col0 + c) * g.ld_out + line] = from_float<V>(sum);
-                }
-            }
-            __syncwarp();
-            cluster_barrier();
-        }
-    } else if (drains) {
-        const int i = line0 + row;
-        const bool real = i < m.n_rows;
-        float *mine = sums + group * 8 * 128 + row;  // [group of the unit][row], one for each four warps
-        for (int j = 0; j < 8; ++j) mine[j * 128] = 0.f;
-        Cursor<V> cursor;
-        bool ok = true;
-        for (int turn = 0; turn < turns; ++turn) {
-            if (!(ok = __all_sync(0xffffffffu, warp_wait(done, turn & 1, polls) && !failed))) break;
-            tc_fence_after();
-            const int from = col0 + turn * BN + group * (BN / 4), to = min(from + BN / 4, col_end);
-            if (g.d_res) cursor.start(m, i, from);
-            for (int k = from; k < to; k += 32) {
-                float v[32];
-                if (steps > 0) {
-                    tmem_load32(quarter + (k - col0 - turn * BN), v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                }
-                if (real && g.out) {
-                    // codes behind the last column take part with G = 0
-                    const uint4 c = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
-                    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-                    const float z = 8388608.f + zero_of(m, i, k / m.group);
-                    float part = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)  // c - z through 2^23 + c, exact
-                        part = fmaf(__uint_as_float(0x4B000000u | (w[j / 8] >> 4 * (j % 8) & 15)) - z, v[j], part);
-                    mine[(k - col0) / m.group * 128] += part;
-                }
-                if (real && g.d_res) {
-                    while (cursor.col[0] < min(k + 32, to)) {
-                        const int d = cursor.col[0] - k;
-                        float e = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) e = j == d ? v[j] : e;
-                        if (d >= 0) g.d_res[cursor.at] = from_float<V>(e);
-                        cursor.next(m);
-                    }
-                }
-                __syncwarp();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(drained);
-        }
+    const int line = line0 + row, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
+    bool ok = false;
+    if (drains) {
+        ok = __all_sync(0xffffffffu, warp_wait(done, 0, polls) && !failed);
         if (!ok) failed = 1;
-        asm volatile("bar.sync 1, 512;" ::: "memory");  // the sixteen warps of the epilogue
-        if (ok && real && g.out && group == 0) {
-            const int g0 = col0 / m.group, n = min(g.groups_per_unit, m.n_groups - g0);
-            for (int j = 0; j < n; ++j)
-                g.out[(long long)i * m.n_groups + g0 + j] =
-                    from_float<V>(mine[j * 128] + mine[(8 + j) * 128] + mine[(16 + j) * 128] + mine[(24 + j) * 128]);
+        tc_fence_after();
+    }
+    float v[32];
+    if (ok) {
+        for (int c = 32 * group; c < BN; c += 128) {
+            if (steps > 0) {
+                tmem_load32(quarter + c, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.f;
+            }
+            if (g.splits == 1) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (line < lines && col0 + c + j < col_end)
+                        g.out[(col0 + c + j) * g.ld_out + line] = from_float<V>(v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) reinterpret_cast<float *>(smem)[(c + j) * 128 + row] = v[j];
+            }
         }
+    }
+    if (g.splits > 1) {
+        __syncwarp();
+        cluster_barrier();
+        if (ok) {
+            const int width = BN / g.splits;
+            for (int j = group; j < width; j += 4) {
+                const int c = rank * width + j;
+                const uint32_t at = base + (c * 128 + row) * 4;
+                const float sum = cluster_sum(at, g.splits);
+                if (line < lines && col0 + c < col_end) g.out[(col0 + c) * g.ld_out + line] = from_float<V>(sum);
+            }
+        }
+        __syncwarp();
+        cluster_barrier();
     }
     tc_fence_before();
     __syncthreads();
@@ -522,16 +403,8 @@ __global__ void __launch_bounds__(1024) slots_kernel(Matrix<V> m, int chunks, ui
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-// The tensor map of `rows` vectors.
-template <typename V>
-cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work) {
-    cudaError_t e = aligned_rows(p, ld, cols, rows, work, &p, &ld);
-    if (e != cudaSuccess) return e;
-    return encode_vectors(map, p, cols, rows, ld, box_rows) ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 template <typename V, int MODE, int BN>
-cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtensorMap &b, const Args<V> &g,
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &b, const Args<V> &g,
                    long long tiles, cudaStream_t s) {
     if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
     auto kernel = gemm_kernel<V, MODE, BN>;
@@ -549,7 +422,7 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &a, const CUtenso
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, codes, a, b, g);
+    return cudaLaunchKernelEx(&cfg, kernel, codes, b, g);
 }
 
 // Width of a tile and number of blocks that share its contraction: the choice with the least time by a model in clocks.
@@ -605,10 +478,10 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
     }
     const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
     switch (bn) {
-        case 32: return launch<V, MODE, 32>(codes, codes, vectors, g, tiles, s);
-        case 64: return launch<V, MODE, 64>(codes, codes, vectors, g, tiles, s);
-        case 128: return launch<V, MODE, 128>(codes, codes, vectors, g, tiles, s);
-        default: return launch<V, MODE, 256>(codes, codes, vectors, g, tiles, s);
+        case 32: return launch<V, MODE, 32>(codes, vectors, g, tiles, s);
+        case 64: return launch<V, MODE, 64>(codes, vectors, g, tiles, s);
+        case 128: return launch<V, MODE, 128>(codes, vectors, g, tiles, s);
+        default: return launch<V, MODE, 256>(codes, vectors, g, tiles, s);
     }
 }
 
@@ -625,27 +498,6 @@ cudaError_t product_t_many(const Matrix<V> &m, int n_vec, const V *dy, long long
     return tiles_of<V, TRANSPOSED>(m, n_vec, dy, ld_dy, dx, ld_dx, s);
 }
 
-template <typename V>
-cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy,
-                      V *d_scales, V *d_res, cudaStream_t s) {
-    Args<V> g = {};
-    g.m = m;
-    g.n_vec = n_vec;
-    g.out = d_scales;
-    g.d_res = m.res_ptr ? d_res : nullptr;
-    g.tiles_m = (int)ceil_div(m.n_rows, 128);
-    g.splits = 1;
-    g.groups_per_unit = std::max(1, 256 / m.group);
-    CUtensorMap a = {}, b = {};
-    Workspace work(s);
-    if (n_vec > 0) {
-        cudaError_t e = map_vectors(&a, dy, m.n_rows, n_vec, ld_dy, 64, work);
-        if (e == cudaSuccess) e = map_vectors(&b, x, m.n_cols, n_vec, ld_x, 64, work);
-        if (e != cudaSuccess) return e;
-    }
-    return launch<V, GRADIENT, 256>(a, a, b, g, g.tiles_m * ceil_div(m.n_groups, g.groups_per_unit), s);
-}
-
 cudaError_t waits_ran_out(int *flag, cudaStream_t s) {
     void *p = nullptr;
     cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out);
@@ -655,9 +507,7 @@ cudaError_t waits_ran_out(int *flag, cudaStream_t s) {
 #define INSTANTIATE(V)                                                                                             \
     template cudaError_t product_many<V>(const Matrix<V> &, int, const V *, long long, V *, long long, cudaStream_t); \
     template cudaError_t product_t_many<V>(const Matrix<V> &, int, const V *, long long, V *, long long,           \
-                                           cudaStream_t);                                                         \
-    template cudaError_t grad_many<V>(const Matrix<V> &, int, const V *, long long, const V *, long long, V *, V *, \
-                                      cudaStream_t);
+                                           cudaStream_t);
 INSTANTIATE(__half)
 INSTANTIATE(__nv_bfloat16)
 

@@ -16,6 +16,7 @@ cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x,
 // *flag = whether a bounded wait of an earlier call on the current device ended without its barrier (async copy)
 cudaError_t waits_ran_out(int *flag, cudaStream_t s);
 cudaError_t waits_ran_out_few(int *flag, cudaStream_t s);
+cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s);
 cudaError_t waits_ran_out_quant(int *flag, cudaStream_t s);
 
 }  // namespace q4

@@ -1,0 +1,292 @@
+// Gradients of a 4-bit matrix's own numbers from many vectors, on the fifth-generation tensor cores.
+//
+//   G[i][k] = sum_t dy[t][i] x[t][k]      A = dy's columns, B = x's columns, both line-major
+//   d_scales[i][g] = sum over the group's k of (c - z)[i][k] G[i][k],   d_res[e] = G[row of e][column of e]
+//
+// G is never stored: it stays in tensor memory and is reduced against the codes from there.  A pair of blocks computes 256
+// rows x 256 columns of it: each brings its 128 rows' dy and half of the columns' x into its shared memory, so that a
+// step's operands cross the L2 and the shared memories half as often as with a block on its own.  The pairs go on from
+// tile to tile, and the tensor memory holds two, so that one is reduced while the next is computed.
+#include <limits.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "q4.h"
+#include "q4_gemm.h"
+#include "q4_maps.h"
+#include "q4_ptx.cuh"
+#include "q4_values.cuh"
+
+namespace mx {
+namespace q4 {
+namespace {
+
+// Warps: 0 copies, 1 tensor core issue (of block 0), 2 and 3 none; then four groups of four that reduce.
+constexpr int REDUCE = 4, THREADS = 32 * 20;
+constexpr int HALF = 128 * 64 * 2;  // bytes of 128 lines x 64 deep: a block's part of A, and of B
+constexpr int STAGE = 2 * HALF, STAGES = 6, COLS = 256;
+constexpr int SUMS = 4 * 8 * 128;  // parts of the scales' gradients: [group of warps][group of the unit][row]
+constexpr int BARS = 2 * STAGES + 5;
+constexpr int SMEM = 1024 + STAGES * STAGE + 2 * SUMS * 4 + BARS * 8;
+static_assert(SMEM <= 227 * 1024, "shared memory of one block");
+
+template <typename V>
+struct Args {
+    Matrix<V> m;
+    int n_vec, tiles_m, units, groups_per_unit;
+    V *d_scales, *d_res;
+};
+
+__device__ int wait_ran_out_grad;
+
+// entries of one row, columns ascending, the next two already loaded
+template <typename V>
+struct Cursor {
+    int at = 0, end = 0, col[2];
+    V val[2];
+    __device__ __forceinline__ void fetch(const Matrix<V> &m, int j) {
+        const int p = at + j;
+        col[j] = p < end ? m.res_col[p] : 0x7fffffff;
+        val[j] = p < end ? m.res_val[p] : from_float<V>(0.f);
+    }
+    __device__ __forceinline__ void start(const Matrix<V> &m, int i, int k) {
+        at = end = 0;
+        if (m.res_ptr && i < m.n_rows) {
+            res_range(m, i, at, end);
+            at = first_at_least(m.res_col, at, end, k);
+        }
+        fetch(m, 0);
+        fetch(m, 1);
+    }
+    __device__ __forceinline__ void next(const Matrix<V> &m) {
+        ++at;
+        col[0] = col[1];
+        val[0] = val[1];
+        fetch(m, 1);
+    }
+};
+
+template <typename V>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    gradient_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x,
+                    const __grid_constant__ Args<V> g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_shared;
+    __shared__ volatile int failed;
+    uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t base = smem_addr(smem);
+    float *sums = reinterpret_cast<float *>(smem + STAGES * STAGE);
+    const uint32_t bars = smem_addr(sums + 2 * SUMS);
+    auto full = [&](int s) { return bars + 8 * s; };               // block 0's: both blocks' parts of a stage are there
+    auto empty = [&](int s) { return bars + 8 * (STAGES + s); };   // each block's: the stage is used up
+    auto done = [&](int b) { return bars + 8 * (2 * STAGES + b); };         // each block's: D is complete
+    auto drained = [&](int b) { return bars + 8 * (2 * STAGES + 2 + b); };  // block 0's: both blocks have taken it
+    const uint32_t together = bars + 8 * (2 * STAGES + 4);                  // the sixteen warps that reduce
+
+    const Matrix<V> &m = g.m;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const int steps = (g.n_vec + 63) / 64, tiles = g.tiles_m * g.units, pairs = gridDim.x / 2;
+    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
+    // A tile: 256 rows, of which this block has 128, and a unit: the columns of a whole number of groups, in turns of 256.
+    struct Tile {
+        int line0, col0, col_end, turns;
+    };
+    auto tile_at = [&](int n) {
+        Tile t;
+        const int unit = n / g.tiles_m;
+        t.line0 = n % g.tiles_m * 256 + 128 * (int)rank;
+        t.col0 = unit * g.groups_per_unit * m.group;
+        t.col_end = (int)min((long long)m.n_cols, t.col0 + (long long)g.groups_per_unit * m.group);
+        t.turns = (t.col_end - t.col0 + COLS - 1) / COLS;
+        return t;
+    };
+
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(done(b), 1);
+            mbar_init(drained(b), 32);
+        }
+        mbar_init(together, 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(smem_addr(&tmem_shared), 2 * COLS);
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // the other block's barriers are there, too
+    tc_fence_after();
+    const uint32_t tmem = tmem_shared;
+
+    if (warp == 0 && lane == 0) {  // ---- this block's parts of x and dy
+        int n = 0;
+        bool ok = true;
+        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs) {
+            const Tile t = tile_at(at);
+            for (int turn = 0; turn < t.turns && ok; ++turn) {
+                const int col = t.col0 + turn * COLS + 128 * (int)rank;
+                for (int step = 0; step < steps; ++step, ++n) {
+                    const int s = n % STAGES;
+                    if (!(ok = mbar_wait(empty(s), (n / STAGES & 1) ^ 1, polls))) break;
+                    if (rank == 0) mbar_expect(full(s), 2 * STAGE);
+                    const uint32_t to = base + s * STAGE, bar = in_block(full(s), 0);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        tma_load_pair(to + j * (HALF / 2), &map_dy, t.line0 + 64 * j, step * 64, bar);
+                        tma_load_pair(to + HALF + j * (HALF / 2), &map_x, col + 64 * j, step * 64, bar);
+                    }
+                }
+            }
+        }
+        if (!ok) failed = 1;
+        // nothing may be on its way to this block when it ends
+        if (!ok && rank == 0)
+            for (int k = max(0, n - STAGES); k < n; ++k) mbar_wait(full(k % STAGES), k / STAGES & 1, polls);
+    } else if (rank == 0 && warp == 1 && elect_one()) {  // ---- tensor cores of both blocks
+        constexpr uint32_t idesc = mma_shape(!std::is_same<V, __half>::value, COLS, true, true, 256);
+        const uint64_t da0 = operand(base, HALF / 2, 1024), db0 = operand(base + HALF, HALF / 2, 1024);
+        int s = 0, u = 0;
+        uint32_t parity = 0;
+        bool ok = true;
+        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs) {
+            const Tile t = tile_at(at);
+            for (int turn = 0; turn < t.turns && ok; ++turn, ++u) {
+                const int b = u & 1;
+                if (u >= 2) {
+                    if (!(ok = mbar_wait_cluster(drained(b), (u / 2 - 1) & 1, polls))) break;
+                    tc_fence_after();
+                }
+                for (int step = 0; step < steps; ++step) {
+                    if (!(ok = mbar_wait_cluster(full(s), parity, polls))) break;
+                    tc_fence_after();
+                    const uint64_t da = da0 + (uint32_t)(s * STAGE / 16), db = db0 + (uint32_t)(s * STAGE / 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)  // 16 rows of 128 bytes
+                        tc_mma_pair(tmem + b * COLS, da + 128 * j, db + 128 * j, idesc, step > 0 || j > 0);
+                    tc_commit_pair(empty(s));
+                    if (++s == STAGES) {
+                        s = 0;
+                        parity ^= 1;
+                    }
+                }
+                if (ok) tc_commit_pair(done(b));
+            }
+        }
+        if (!ok) failed = 1;
+    } else if (warp >= REDUCE) {
+        const int group = (warp - REDUCE) / 4, row = warp % 4 * 32 + lane;
+        const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+        int u = 0, count = 0;
+        bool ok = true;
+        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs, ++count) {
+            const Tile t = tile_at(at);
+            const int i = t.line0 + row;
+            const bool real = i < m.n_rows;
+            // this thread's sums, one set for each four warps; the sets change places from tile to tile, so that one may
+            // still be read while the other is filled
+            float *mine = sums + (count & 1) * SUMS + group * 8 * 128 + row;
+            for (int j = 0; j < 8; ++j) mine[j * 128] = 0.f;
+            Cursor<V> cursor;
+            for (int turn = 0; turn < t.turns; ++turn, ++u) {
+                const int b = u & 1;
+                const int from = t.col0 + turn * COLS + group * (COLS / 4), to = min(from + COLS / 4, t.col_end);
+                if (g.d_res) cursor.start(m, i, from);
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(done(b), u / 2 & 1, polls) && !failed))) break;
+                tc_fence_after();
+                for (int k = from; k < to; k += 32) {
+                    float v[32];
+                    tmem_load32(quarter + b * COLS + (k - t.col0 - turn * COLS), v);
+                    if (real && g.d_scales) {
+                        // codes behind the last column take part with G = 0
+                        const uint4 c = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
+                        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+                        const int gr = k / m.group;
+                        const float z = 8388608.f + zero_of(m, i, gr);
+                        float part = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)  // c - z through 2^23 + c, exact
+                            part = fmaf(__uint_as_float(0x4B000000u | (w[j / 8] >> 4 * (j % 8) & 15)) - z, v[j], part);
+                        mine[(gr - t.col0 / m.group) * 128] += part;
+                    }
+                    if (real && g.d_res) {
+                        while (cursor.col[0] < min(k + 32, to)) {
+                            const int d = cursor.col[0] - k;
+                            float e = 0.f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) e = j == d ? v[j] : e;
+                            if (d >= 0) g.d_res[cursor.at] = from_float<V>(e);
+                            cursor.next(m);
+                        }
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(in_block(drained(b), 0));
+            }
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(together);
+            if (!(ok = warp_wait(together, count & 1, polls))) break;
+            if (real && g.d_scales && group == 0) {
+                const int g0 = t.col0 / m.group, n = min(g.groups_per_unit, m.n_groups - g0);
+                for (int j = 0; j < n; ++j)
+                    g.d_scales[(long long)i * m.n_groups + g0 + j] =
+                        from_float<V>(mine[j * 128] + mine[(8 + j) * 128] + mine[(16 + j) * 128] + mine[(24 + j) * 128]);
+            }
+        }
+        if (!ok) failed = 1;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // neither block ends while the other may still reach into it
+    tc_fence_after();
+    if (threadIdx.x == 0 && failed) wait_ran_out_grad = 1;
+    if (warp == 1) tmem_free_pair(tmem, 2 * COLS);
+}
+
+}  // namespace
+
+template <typename V>
+cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy,
+                      V *d_scales, V *d_res, cudaStream_t s) {
+    Args<V> g = {};
+    g.m = m;
+    g.n_vec = n_vec;
+    g.tiles_m = (int)ceil_div(m.n_rows, 256);
+    g.groups_per_unit = std::max(1, COLS / m.group);
+    g.units = (int)ceil_div(m.n_groups, g.groups_per_unit);
+    g.d_scales = d_scales;
+    g.d_res = m.res_ptr ? d_res : nullptr;
+    const long long tiles = (long long)g.tiles_m * g.units;
+    if (tiles > INT_MAX / 2) return cudaErrorInvalidConfiguration;
+    CUtensorMap map_dy = {}, map_x = {};
+    Workspace work(s);
+    cudaError_t e = map_vectors(&map_dy, dy, m.n_rows, n_vec, ld_dy, 64, work);
+    if (e == cudaSuccess) e = map_vectors(&map_x, x, m.n_cols, n_vec, ld_x, 64, work);
+    if (e == cudaSuccess) e = allow_smem<V, gradient_kernel<V>>(SMEM);
+    if (e != cudaSuccess) return e;
+    gradient_kernel<V><<<(unsigned)(2 * std::min<long long>(tiles, 74)), THREADS, SMEM, s>>>(map_dy, map_x, g);
+    return cudaGetLastError();
+}
+
+cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s) {
+    void *p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_grad);
+    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
+}
+
+#define INSTANTIATE(V)                                                                                              \
+    template cudaError_t grad_many<V>(const Matrix<V> &, int, const V *, long long, const V *, long long, V *, V *, \
+                                      cudaStream_t);
+INSTANTIATE(__half)
+INSTANTIATE(__nv_bfloat16)
+
+}  // namespace q4
+}  // namespace mx

@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "q4.h"
+#include "q4_values.cuh"
 
 namespace mx {
 namespace q4 {
@@ -40,6 +41,14 @@ template <typename V>
 bool encode_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows) {
     return encode(map, std::is_same<V, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                   p, cols, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The tensor map of `rows` vectors.
+template <typename V>
+cudaError_t map_vectors(CUtensorMap *map, const V *p, int cols, int rows, long long ld, int box_rows, Workspace &work) {
+    cudaError_t e = aligned_rows(p, ld, cols, rows, work, &p, &ld);
+    if (e != cudaSuccess) return e;
+    return encode_vectors(map, p, cols, rows, ld, box_rows) ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 // 128 rows x 128 columns of codes (64 bytes a row, in 64-byte swizzle)

@@ -111,10 +111,68 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32
     return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// instruction descriptor: 32-bit sums, both inputs f16 (0) or bf16 (1), 128 x n, which operands are line-major
-__host__ __device__ constexpr uint32_t mma_shape(int bf16, int n, bool a_lines, bool b_lines) {
+// instruction descriptor: 32-bit sums, both inputs f16 (0) or bf16 (1), m x n, which operands are line-major
+__host__ __device__ constexpr uint32_t mma_shape(int bf16, int n, bool a_lines, bool b_lines, int m = 128) {
     return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)a_lines << 15 | (uint32_t)b_lines << 16 |
-           (uint32_t)(n / 8) << 17 | (uint32_t)(128 / 16) << 24;
+           (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
+}
+
+// ---- a pair of blocks (the two of a cluster) on one tile: both take the same steps with the tensor memory, one thread of
+// block 0 issues; the operands' addresses hold in both blocks, A's lines and B's lines split between them ----
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t where, uint32_t columns) {  // one whole warp of each block
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t tmem, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+// D[256 x n] (+)= A * B; this block's lines of D are in its own tensor memory
+__device__ __forceinline__ void tc_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+// the barrier at this address gets an arrival in both blocks
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// an address of this block's shared memory in block `rank` of the cluster
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {  // of any block of the cluster
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// A wait for arrivals that come from the other block, too.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t polls) {
+#pragma unroll 1
+    for (uint32_t n = 0; n <= polls; ++n) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+// a tile into this block's shared memory that counts on the barrier of any block of the pair
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t cluster_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(cluster_bar), "r"(x), "r"(y)
+        : "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
