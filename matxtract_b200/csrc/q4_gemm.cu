@@ -65,22 +65,27 @@ struct Args {
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
 
-// scales and zero points of a row's 128 columns, 32 at a time
-template <typename V>
+// scales and zero points of N times 32 of a row's columns
+template <typename V, int N>
 struct Scales {
-    V s[4];
-    int z[4];
+    V s[N];
+    int z[N];
     __device__ __forceinline__ void load(const Matrix<V> &m, int i, const GroupOf &at) {
         const bool real = i < m.n_rows;
         const long long row = (long long)(real ? i : 0) * m.n_groups;
         const int last = m.n_groups - 1;  // behind the last column
-        if (m.group % 128 == 0) {
+        if (m.group % (32 * N) == 0) {
             const int g = min(at.g, last);
-            s[0] = s[1] = s[2] = s[3] = real ? m.scales[row + g] : from_float<V>(0.f);
-            z[0] = z[1] = z[2] = z[3] = m.zeros ? m.zeros[row + g] & 15 : 8;
+            const V scale = real ? m.scales[row + g] : from_float<V>(0.f);
+            const int zero = m.zeros ? m.zeros[row + g] & 15 : 8;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                s[j] = scale;
+                z[j] = zero;
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < N; ++j) {
                 const int g = min(at.after(j), last);
                 s[j] = real ? m.scales[row + g] : from_float<V>(0.f);
                 z[j] = m.zeros ? m.zeros[row + g] & 15 : 8;
@@ -88,6 +93,82 @@ struct Scales {
         }
     }
 };
+
+// 64 values of a row in the operand's layout, with the residual's entries among them: `a` is the row's 128 bytes in a
+// stage, whose sixteens are in an order that goes by the row.
+template <typename V>
+__device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4 (&c)[2], const V (&scale)[2], const int (&zero)[2],
+                                            bool slots, const uint4 &entries, const Matrix<V> &m, int row, int col) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const typename Pair<V>::T s = Pair<V>::both(scale[j]);
+        const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], s, zero[j]);
+    }
+    if (!slots || entries.x == NO_ENTRY) return;
+    auto add = [&](int k, V v) {
+        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
+        *e = from_float<V>(to_float(*e) + to_float(v));
+    };
+    if (entries.w != TOO_MANY) {
+        const uint32_t entry[4] = {entries.x, entries.y, entries.z, entries.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint16_t v = (uint16_t)entry[j];
+            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
+        }
+    } else {  // this thread looks for its entries itself
+        const int k1 = min(col + 64, m.n_cols);
+        int b, e;
+        res_range(m, row, b, e);
+        for (b = first_at_least(m.res_col, b, e, col); b < e; ++b) {
+            const int k = m.res_col[b];
+            if (k < col || k >= k1) break;
+            add(k - col, m.res_val[b]);
+        }
+    }
+}
+
+// A code tile -> 16-bit values in the operand's layout, by the four warps of a group.  A thread has one row of 128 columns:
+// of the product's tile 64 columns of each of two stages, of the transposed product's all 128 columns of one stage (rows
+// 0-63 or 64-127 of the tile).  `release`: the tile's place may be filled again; free(p), stage(p), arrive(p): of the
+// tile's stage p.
+template <typename V, int MODE, typename Release, typename Free, typename Stage, typename Arrive>
+__device__ __forceinline__ bool convert_tile(const Matrix<V> &m, const uint8_t *from, bool slots, const Scales<V, 4> &now,
+                                             int t, int row, int col, Release release, Free free, Stage stage,
+                                             Arrive arrive) {
+    const int lane = threadIdx.x % 32, out_row = MODE == PRODUCT ? t : t % 64;
+    uint4 c[2][2], entries[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j / 2][j % 2] = *reinterpret_cast<const uint4 *>(from + t * 64 + ((j ^ t >> 1 & 3) << 4));
+    if (slots) {
+        const uint4 *slot = reinterpret_cast<const uint4 *>(from + CODE_BYTES) + (MODE == PRODUCT ? t : t / 64 * 128 + t % 64);
+        entries[0] = slot[0];
+        entries[1] = slot[MODE == PRODUCT ? 128 : 64];
+    }
+    // the loads are done before the place is given back: a bulk copy would overtake those still under way
+    fence_async_shared();
+    __syncwarp();
+    if (lane == 0) release();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {  // 64 columns
+        const int part = MODE == PRODUCT ? half : t / 64;
+        if (MODE == PRODUCT || half == 0)
+            if (!free(part)) return false;
+        const V s[2] = {now.s[2 * half], now.s[2 * half + 1]};
+        const int z[2] = {now.z[2 * half], now.z[2 * half + 1]};
+        convert_row<V>(stage(part) + out_row * 128 + (MODE == PRODUCT ? 0 : half * 8192), out_row, c[half], s, z, slots,
+                       entries[half], m, row, col + 64 * half);
+        if (MODE == PRODUCT || half == 1) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) arrive(part);
+        }
+    }
+    return true;
+}
 
 template <typename V, int MODE, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -201,82 +282,28 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int k = max(0, n - CODES); k < n; ++k) mbar_wait(c_full(k), k / TURN & 1, polls);
         }
     } else if (warp >= CONVERT) {  // ---- codes -> 16-bit values
-        // the groups take code tiles in turn; a thread has one row of 128 columns: of the product's tile 64 columns of
-        // each of two stages, of the transposed product's all 128 columns of one stage (rows 0-63 or 64-127 of the tile)
+        // the groups take code tiles in turn
         const int group = (warp - CONVERT) / 4, t = threadIdx.x - 32 * CONVERT - 128 * group;
-        const int out_row = MODE == PRODUCT ? t : t % 64;
         auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + t : (block0 + n) * 128 + t; };
         auto col_at = [&](int n) { return MODE == PRODUCT ? (block0 + n) * 128 : line0; };
         GroupOf at(col_at(group), m.group, 512);
-        Scales<V> next;
+        Scales<V, 4> next;
         if (group < blocks) next.load(m, row_at(group), at);
         bool ok = true;
         for (int n = group; n < blocks && ok; n += 4) {
-            const Scales<V> now = next;
+            const Scales<V, 4> now = next;
             if (n + 4 < blocks) {
                 if (MODE == PRODUCT) at.move();
                 next.load(m, row_at(n + 4), at);
             }
-            const int cs = n % CODES;
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
-            uint4 c[4], entries[2];
-            const uint8_t *from = codes_at + cs * CODE_TILE;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const uint4 *>(from + t * 64 + ((j ^ t >> 1 & 3) << 4));
-            if (g.slots) {
-                const uint4 *slot = reinterpret_cast<const uint4 *>(from + CODE_BYTES) + (MODE == PRODUCT ? t : t / 64 * 128 + t % 64);
-                entries[0] = slot[0];
-                entries[1] = slot[MODE == PRODUCT ? 128 : 64];
-            }
-            // the loads are done before the place is given back: a bulk copy would overtake those still under way
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(c_empty(n));
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {  // 64 columns
-                const int step = 2 * n + (MODE == PRODUCT ? part : t / 64), s = step % S::STAGES;
-                if (MODE == PRODUCT || part == 0)
-                    if (!(ok = __all_sync(0xffffffffu, stage_free(step)))) break;
-                uint8_t *a = smem + s * S::STAGE + out_row * 128 + (MODE == PRODUCT ? 0 : part * 8192);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint4 v = c[2 * part + j];
-                    const typename Pair<V>::T sc = Pair<V>::both(now.s[2 * part + j]);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) =
-                            values<V>(w[q], sc, now.z[2 * part + j]);
-                }
-                if (g.slots && entries[part].x != NO_ENTRY) {
-                    auto add = [&](int k, V v) {
-                        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
-                        *e = from_float<V>(to_float(*e) + to_float(v));
-                    };
-                    if (entries[part].w != TOO_MANY) {
-                        const uint32_t entry[4] = {entries[part].x, entries[part].y, entries[part].z, entries[part].w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint16_t v = (uint16_t)entry[j];
-                            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
-                        }
-                    } else {  // this thread looks for its entries itself
-                        const int k0 = col_at(n) + 64 * part, k1 = min(k0 + 64, m.n_cols);
-                        int b, e;
-                        res_range(m, row_at(n), b, e);
-                        for (b = first_at_least(m.res_col, b, e, k0); b < e; ++b) {
-                            const int k = m.res_col[b];
-                            if (k < k0 || k >= k1) break;
-                            add(k - k0, m.res_val[b]);
-                        }
-                    }
-                }
-                if (MODE == PRODUCT || part == 1) {
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full(s));
-                }
-            }
+            const int cs = n % CODES;
+            ok = convert_tile<V, MODE>(
+                m, codes_at + cs * CODE_TILE, g.slots != nullptr, now, t, row_at(n), col_at(n),
+                [&] { mbar_arrive(c_empty(n)); },
+                [&](int part) { return __all_sync(0xffffffffu, stage_free(2 * n + part)); },
+                [&](int part) { return smem + (2 * n + part) % S::STAGES * S::STAGE; },
+                [&](int part) { mbar_arrive(full((2 * n + part) % S::STAGES)); });
         }
         if (!ok) failed = 1;
     }
@@ -333,6 +360,232 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     if (threadIdx.x == 0 && failed) wait_ran_out = 1;
     if (warp == 1) tmem_free(tmem, COLUMNS);
+}
+
+// The same for large products: a pair of blocks computes 256 lines x 256 vectors.  Each makes its own 128 lines of W and
+// brings half of the vectors, so that a step's vectors cross the L2 and the shared memories half as often.  The pairs go on
+// from tile to tile; the tensor memory holds two tiles, and four warps more write one while the next is computed.
+constexpr int PAIR_THREADS = 32 * 24, WRITE = 20;  // first of the writing warps
+struct PairShape {
+    static constexpr int STAGE = 2 * A_BYTES, STAGES = 6, CODES = 2, COLS = 256;
+    static constexpr int BARS = STAGES + 3 * TURN + 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + BARS * 8;
+    static_assert(SMEM <= 227 * 1024 && STAGES <= TURN && CODES <= TURN, "as above");
+};
+
+template <typename V, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ Args<V> g) {
+    using S = PairShape;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_shared;
+    __shared__ volatile int failed;
+    uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t base = smem_addr(smem);
+    uint8_t *codes_at = smem + S::STAGES * S::STAGE;
+    const uint32_t bars = smem_addr(codes_at + S::CODES * CODE_TILE);
+    auto full = [&](int s) { return bars + 8 * s; };                                // block 0's: of both blocks' stage
+    auto empty = [&](int step) { return bars + 8 * (S::STAGES + step % TURN); };    // each block's, of a step
+    auto c_full = [&](int n) { return bars + 8 * (S::STAGES + TURN + n % TURN); };  // of a code tile of its own
+    auto c_empty = [&](int n) { return bars + 8 * (S::STAGES + 2 * TURN + n % TURN); };
+    auto done = [&](int b) { return bars + 8 * (S::STAGES + 3 * TURN + b); };         // each block's: D is complete
+    auto drained = [&](int b) { return bars + 8 * (S::STAGES + 3 * TURN + 2 + b); };  // block 0's: both have written it
+
+    const Matrix<V> &m = g.m;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const int pairs = gridDim.x / 2, first = blockIdx.x / 2;
+    const int tiles = g.tiles_m * ((g.n_vec + S::COLS - 1) / S::COLS), mine = (tiles - first + pairs - 1) / pairs;
+    const int depth = MODE == PRODUCT ? m.n_cols : m.n_rows;
+    const int blocks = (int)(((long long)depth + 127) / 128), steps = 2 * blocks;
+    auto line_of = [&](int tile) { return tile % g.tiles_m * 256 + 128 * (int)rank; };
+    auto vector_of = [&](int tile) { return tile / g.tiles_m * S::COLS; };
+    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
+
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), 1 + 8);  // the copies, and a group's warps of each block
+        for (int n = 0; n < TURN; ++n) {
+            mbar_init(empty(n), 1);
+            mbar_init(c_full(n), 1);
+            mbar_init(c_empty(n), 8);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(done(b), 1);
+            mbar_init(drained(b), 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(smem_addr(&tmem_shared), 2 * S::COLS);
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // the other block's barriers are there, too
+    tc_fence_after();
+    const uint32_t tmem = tmem_shared;
+    // steps and code tiles are numbered on from tile to tile
+    auto stage_free = [&](int step) {
+        return step < S::STAGES || mbar_wait(empty(step - S::STAGES), (step - S::STAGES) / TURN & 1, polls);
+    };
+    auto place_free = [&](int n) {
+        return n < S::CODES || mbar_wait(c_empty(n - S::CODES), (n - S::CODES) / TURN & 1, polls);
+    };
+
+    if (warp == 0 && lane == 0) {  // ---- this block's half of x or dy
+        int n = 0;
+        bool ok = true;
+        for (int at = 0; at < mine && ok; ++at) {
+            const int vector = vector_of(first + at * pairs) + 128 * (int)rank;
+            for (int step = 0; step < steps; ++step, ++n) {
+                const int s = n % S::STAGES;
+                if (!(ok = stage_free(n))) break;
+                if (rank == 0) mbar_expect(full(s), 2 * A_BYTES);
+                tma_load_pair(base + s * S::STAGE + A_BYTES, &map_b, step * 64, vector, in_block(full(s), 0));
+            }
+        }
+        if (!ok) {  // nothing may still be on its way to this block when it ends
+            failed = 1;
+            for (int k = max(0, n - S::STAGES); k < n && rank == 0; ++k)
+                mbar_wait(full(k % S::STAGES), k / S::STAGES & 1, polls);
+        }
+    } else if (rank == 0 && warp == 1 && elect_one()) {  // ---- tensor cores of both blocks
+        constexpr uint32_t idesc = mma_shape(!std::is_same<V, __half>::value, S::COLS, MODE == TRANSPOSED, false, 256);
+        const uint64_t da0 = MODE == PRODUCT ? operand(base, 16, 1024) : operand(base, 8192, 1024);
+        const uint64_t db0 = operand(base + A_BYTES, 16, 1024);
+        constexpr uint32_t NEXT_A = (MODE == PRODUCT ? 32 : 2048) / 16, NEXT_B = 32 / 16;
+        int s = 0, n = 0;
+        uint32_t parity = 0;
+        bool ok = true;
+        for (int at = 0; at < mine && ok; ++at) {
+            const int b = at & 1;
+            if (at >= 2) {
+                if (!(ok = mbar_wait_cluster(drained(b), (at / 2 - 1) & 1, polls))) break;
+                tc_fence_after();
+            }
+            for (int step = 0; step < steps; ++step, ++n) {
+                if (!(ok = mbar_wait_cluster(full(s), parity, polls))) break;
+                tc_fence_after();
+                const uint64_t da = da0 + (uint32_t)(s * S::STAGE / 16), db = db0 + (uint32_t)(s * S::STAGE / 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    tc_mma_pair(tmem + b * S::COLS, da + NEXT_A * j, db + NEXT_B * j, idesc, step > 0 || j > 0);
+                tc_commit_pair(empty(n));
+                if (++s == S::STAGES) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+            if (ok) tc_commit_pair(done(b));
+        }
+        if (!ok) failed = 1;
+    } else if (warp == 2 && lane == 0) {  // ---- codes of this block's lines
+        int n = 0;
+        bool ok = true;
+        for (int at = 0; at < mine && ok; ++at) {
+            const int line0 = line_of(first + at * pairs);
+            for (int block = 0; block < blocks; ++block, ++n) {
+                if (!(ok = place_free(n))) break;
+                const int row = MODE == PRODUCT ? line0 : block * 128, col = MODE == PRODUCT ? block * 128 : line0;
+                const int tile_rows = (int)(((long long)m.n_rows + 127) / 128), tile_cols = (int)(((long long)m.n_cols + 127) / 128);
+                // the second block of the last pair may lie behind the last line altogether
+                const bool slots = g.slots && row / 128 < tile_rows && col / 128 < tile_cols;
+                const uint32_t to = smem_addr(codes_at) + n % S::CODES * CODE_TILE;
+                mbar_expect(c_full(n), slots ? CODE_TILE : CODE_BYTES);
+                tma_load(to, &map_codes, col / 2, row, c_full(n));
+                if (slots)
+                    bulk_load(to + CODE_BYTES, g.slots + ((long long)(row / 128) * tile_cols + col / 128) * 256, SLOT_BYTES,
+                              c_full(n));
+            }
+        }
+        if (!ok) {
+            failed = 1;
+            for (int k = max(0, n - S::CODES); k < n; ++k) mbar_wait(c_full(k), k / TURN & 1, polls);
+        }
+    } else if (warp >= CONVERT && warp < WRITE) {  // ---- codes -> 16-bit values
+        // Two groups share a code tile, a stage each, so that few stages are being filled at a time: groups 0 and 1 have the
+        // even tiles of all, 2 and 3 the odd ones.  (A group with both stages of a tile holds stages that others wait for:
+        // 270 us instead of 190 for 2048 vectors, 8192 x 8192.)  A thread has 64 values of a row.
+        const int group = (warp - CONVERT) / 4, half = group & 1, t = threadIdx.x - 32 * CONVERT - 128 * group;
+        const int tile_row = MODE == PRODUCT ? t : 64 * half + t % 64, part = MODE == PRODUCT ? half : t / 64;
+        const int out_row = MODE == PRODUCT ? t : t % 64, out_at = out_row * 128 + (MODE == PRODUCT ? 0 : part * 8192);
+        // a group's place: code tile n of all, code tile `block` of the pair's tile `at`
+        int at = 0, block = group / 2, line0 = 0;
+        auto settle = [&] {
+            while (block >= blocks && at < mine) {
+                block -= blocks;
+                ++at;
+            }
+            line0 = line_of(first + at * pairs);
+        };
+        settle();
+        auto row = [&] { return (MODE == PRODUCT ? line0 : block * 128) + tile_row; };
+        auto col = [&] { return (MODE == PRODUCT ? block * 128 : line0) + 64 * part; };
+        GroupOf of(col(), m.group, 256);
+        Scales<V, 2> next;
+        if (at < mine) next.load(m, row(), of);
+        bool ok = true;
+        for (int n = group / 2; at < mine && ok; n += 2) {
+            const Scales<V, 2> now = next;
+            const int this_row = row(), this_col = col();
+            const bool slots = g.slots && line0 < (MODE == PRODUCT ? m.n_rows : m.n_cols);
+            block += 2;
+            if (block < blocks) {
+                if (MODE == PRODUCT) of.move();
+            } else {
+                settle();
+                of = GroupOf(col(), m.group, 256);
+            }
+            if (at < mine) next.load(m, row(), of);
+            if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
+            const uint8_t *from = codes_at + n % S::CODES * CODE_TILE;
+            uint4 c[2], entries;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                c[j] = *reinterpret_cast<const uint4 *>(from + tile_row * 64 + ((2 * part + j ^ tile_row >> 1 & 3) << 4));
+            if (slots) entries = *reinterpret_cast<const uint4 *>(from + CODE_BYTES + (half * 128 + t) * 16);
+            fence_async_shared();  // as in convert_tile
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c_empty(n));
+            const int step = 2 * n + half, s = step % S::STAGES;
+            if (!(ok = __all_sync(0xffffffffu, stage_free(step)))) break;
+            convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, now.s, now.z, slots, entries, m, this_row, this_col);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(in_block(full(s), 0));
+        }
+        if (!ok) failed = 1;
+    } else if (warp >= WRITE) {  // ---- D leaves tensor memory
+        const int line = warp % 4 * 32 + lane, lines = MODE == PRODUCT ? m.n_rows : m.n_cols;
+        const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+        bool ok = true;
+        for (int at = 0; at < mine; ++at) {
+            const int b = at & 1, tile = first + at * pairs, to = line_of(tile) + line, t0 = vector_of(tile);
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(done(b), at / 2 & 1, polls) && !failed))) break;
+            tc_fence_after();
+            for (int c = 0; c < S::COLS && t0 + c < g.n_vec; c += 32) {
+                float v[32];
+                tmem_load32(quarter + b * S::COLS + c, v);
+                V *out = g.out + (long long)(t0 + c) * g.ld_out + to;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (to < lines && t0 + c + j < g.n_vec) *out = from_float<V>(v[j]);
+                    out += g.ld_out;
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(in_block(drained(b), 0));
+        }
+        if (!ok) failed = 1;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // neither block ends while the other may still reach into it
+    tc_fence_after();
+    if (threadIdx.x == 0 && failed) wait_ran_out = 1;
+    if (warp == 1) tmem_free_pair(tmem, 2 * S::COLS);
 }
 
 // First entry of [begin, end) whose column is at least k, for a whole warp: 32 places are looked at together.
@@ -426,16 +679,16 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &b, const Args<V>
 }
 
 // Width of a tile and number of blocks that share its contraction: the choice with the least time by a model in clocks.
-// Measured on 2048 to 8192 rows and columns, 16 to 2048 vectors: a code tile takes 1020 to 1520 clocks (nearly the same
+// Measured on 2048 to 8192 rows and columns, 16 to 2048 vectors: a code tile takes 800 to 1300 clocks (nearly the same
 // for 32 to 128 vectors: the conversion bounds it), a block 11,000 to 14,000 to begin and to end, adding up parts through
-// the cluster 30 a vector.
+// the cluster 30 a vector.  A pair of blocks (bn = 0) takes 1060 a code tile and does not pause between its tiles.
 void plan(int lines, int depth, int n_vec, int &bn, int &splits) {
     const long long m_tiles = ceil_div(lines, 128), blocks = std::max<long long>(ceil_div(depth, 128), 1);
     double best = 0;
     for (int w : {32, 64, 128, 256}) {
         for (int s = 1; s <= 4; s *= 2) {
             if (s > blocks) break;
-            const double per_block = w == 32 ? 1020 : w == 64 ? 1080 : w == 128 ? 1140 : 1520;
+            const double per_block = w == 32 ? 800 : w == 64 ? 850 : w == 128 ? 950 : 1300;
             const double waves = (double)ceil_div(m_tiles * ceil_div(n_vec, w) * s, 148);
             const double cost = waves * (ceil_div(blocks, s) * per_block + 12000 + (s > 1 ? 30 * w : 0));
             if (best == 0 || cost < best) {
@@ -444,6 +697,11 @@ void plan(int lines, int depth, int n_vec, int &bn, int &splits) {
                 splits = s;
             }
         }
+    }
+    const long long pair_tiles = ceil_div(lines, 256) * ceil_div(n_vec, 256);
+    if (ceil_div(pair_tiles, 74) * blocks * 1060.0 + 14000 < best && depth > 0) {
+        bn = 0;
+        splits = 1;
     }
 }
 
@@ -455,14 +713,14 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
     g.n_vec = n_vec;
     g.out = out;
     g.ld_out = ld_out;
-    g.tiles_m = (int)ceil_div(lines, 128);
     int bn = 0;
     plan(lines, depth, n_vec, bn, g.splits);
+    g.tiles_m = (int)ceil_div(lines, bn ? 128 : 256);
     CUtensorMap codes = {}, vectors = {};
     Workspace work(s);
     if (depth > 0) {
         if (!encode_codes(&codes, m)) return cudaErrorInvalidValue;
-        cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn, work);
+        cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn ? bn : 128, work);
         if (e != cudaSuccess) return e;
         if (m.res_ptr) {
             // whole tiles of 128 rows: rows behind the last have empty slots
@@ -475,6 +733,14 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
             if ((e = cudaGetLastError()) != cudaSuccess) return e;
             g.slots = slots;
         }
+    }
+    if (bn == 0) {
+        const long long tiles = g.tiles_m * ceil_div(n_vec, 256);
+        if (tiles > INT_MAX / 2) return cudaErrorInvalidConfiguration;
+        const cudaError_t e = allow_smem<V, pair_kernel<V, MODE>>(PairShape::SMEM);
+        if (e != cudaSuccess) return e;
+        pair_kernel<V, MODE><<<(unsigned)(2 * std::min<long long>(tiles, 74)), PAIR_THREADS, PairShape::SMEM, s>>>(codes, vectors, g);
+        return cudaGetLastError();
     }
     const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
     switch (bn) {

@@ -139,6 +139,18 @@ def test_many_tiles(n, k, t):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,k,group,density", [(4100, 1032, 128, 0.005), (1032, 4100, 32, 0.02), (8200, 520, 96, None),
+                                               (4224, 1024, 1024, 0.2), (520, 8200, 64, 0.005)])
+def test_large_products(n, k, group, density, dtype):
+    """Many tiles of many vectors, with last ones that are cut short in each direction."""
+    m = make(n, k, group, dtype, True, density, 5)
+    for t in (1030, 1500):
+        check_product(m, t, 1)
+        check_product_t(m, t, 2)
+        check_grad(m, t, 3)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("t", [1, 7, 40, 150])
 @pytest.mark.parametrize("shift", [0, 1, 8])
 def test_strided_vectors(t, dtype, shift):
