@@ -70,9 +70,9 @@ template <typename V, int N>
 struct Scales {
     V s[N];
     int z[N];
-    __device__ __forceinline__ void load(const Matrix<V> &m, int i, const GroupOf &at) {
-        const bool real = i < m.n_rows;
-        const long long row = (long long)(real ? i : 0) * m.n_groups;
+    // `row`: where the row's numbers begin; real: there is such a row
+    __device__ __forceinline__ void load(const Matrix<V> &m, bool real, long long row, const GroupOf &at) {
+        if (!real) row = 0;
         const int last = m.n_groups - 1;  // behind the last column
         if (m.group % (32 * N) == 0) {
             const int g = min(at.g, last);
@@ -288,13 +288,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto col_at = [&](int n) { return MODE == PRODUCT ? (block0 + n) * 128 : line0; };
         GroupOf at(col_at(group), m.group, 512);
         Scales<V, 4> next;
-        if (group < blocks) next.load(m, row_at(group), at);
+        long long numbers = (long long)row_at(group) * m.n_groups;  // of the row
+        if (group < blocks) next.load(m, row_at(group) < m.n_rows, numbers, at);
         bool ok = true;
         for (int n = group; n < blocks && ok; n += 4) {
             const Scales<V, 4> now = next;
             if (n + 4 < blocks) {
-                if (MODE == PRODUCT) at.move();
-                next.load(m, row_at(n + 4), at);
+                if (MODE == PRODUCT)
+                    at.move();
+                else
+                    numbers += 512ll * m.n_groups;
+                next.load(m, row_at(n + 4) < m.n_rows, numbers, at);
             }
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
             const int cs = n % CODES;
@@ -522,7 +526,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         auto col = [&] { return (MODE == PRODUCT ? block * 128 : line0) + 64 * part; };
         GroupOf of(col(), m.group, 256);
         Scales<V, 2> next;
-        if (at < mine) next.load(m, row(), of);
+        long long numbers = (long long)row() * m.n_groups;  // of the row
+        if (at < mine) next.load(m, row() < m.n_rows, numbers, of);
         bool ok = true;
         for (int n = group / 2; at < mine && ok; n += 2) {
             const Scales<V, 2> now = next;
@@ -530,12 +535,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             const bool slots = g.slots && line0 < (MODE == PRODUCT ? m.n_rows : m.n_cols);
             block += 2;
             if (block < blocks) {
-                if (MODE == PRODUCT) of.move();
+                if (MODE == PRODUCT)
+                    of.move();
+                else
+                    numbers += 256ll * m.n_groups;
             } else {
                 settle();
                 of = GroupOf(col(), m.group, 256);
+                numbers = (long long)row() * m.n_groups;
             }
-            if (at < mine) next.load(m, row(), of);
+            if (at < mine) next.load(m, row() < m.n_rows, numbers, of);
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
             const uint8_t *from = codes_at + n % S::CODES * CODE_TILE;
             uint4 c[2], entries;
@@ -551,7 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, now.s, now.z, slots, entries, m, this_row, this_col);
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(in_block(full(s), 0));
+            if (lane == 0) mbar_arrive_own_at(in_block(full(s), 0));
         }
         if (!ok) failed = 1;
     } else if (warp >= WRITE) {  // ---- D leaves tensor memory
