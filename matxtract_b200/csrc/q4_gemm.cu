@@ -32,9 +32,11 @@ enum { PRODUCT, TRANSPOSED };
 constexpr int THREADS = 32 * 20;
 constexpr int CONVERT = 4;            // first warp of the latter
 constexpr int A_BYTES = 128 * 128;    // 128 lines x 64 deep x 2 bytes
-// A code tile: 128 rows x 128 columns of codes, then the residual's entries in it in slots of four words for each thread
-// that converts 64 of its values, an entry being column << 16 | value.
+// A code tile: 128 rows x 128 columns of codes, then for each thread that converts 64 of its values the residual's entries
+// among them in slots of four words, an entry being column << 16 | value.  For pairs of blocks, scales and zero points of
+// its two 32s (two words) lie between them.
 constexpr int CODE_BYTES = 128 * 64, SLOT_BYTES = 256 * 16, CODE_TILE = CODE_BYTES + SLOT_BYTES;
+constexpr int NUMBER_BYTES = 256 * 8, PAIR_TILE = CODE_BYTES + NUMBER_BYTES + SLOT_BYTES;
 constexpr uint32_t NO_ENTRY = 0xffffffffu, TOO_MANY = 0xfffffffeu;
 
 // Steps after which a barrier that tells of a step's (or a code tile's) end is used again.  A wait tells a phase from the
@@ -60,8 +62,16 @@ struct Args {
     int n_vec, tiles_m, splits;
     V *out;
     long long ld_out;
-    const uint4 *slots;  // the residual's entries as code tiles take them, [row / 128][column / 128]; null: none
+    const uint8_t *sides;  // what follows a code tile's codes, [row / 128][column / 128][side_bytes]; null: nothing
+    int side_bytes;
+    bool slots;  // the residual's entries are among it
 };
+
+template <typename V>
+__device__ __forceinline__ V from_bits(uint32_t low) {
+    const uint16_t v = (uint16_t)low;
+    return *reinterpret_cast<const V *>(&v);
+}
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
 
@@ -115,10 +125,8 @@ __device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4
     if (entries.w != TOO_MANY) {
         const uint32_t entry[4] = {entries.x, entries.y, entries.z, entries.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint16_t v = (uint16_t)entry[j];
-            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, *reinterpret_cast<const V *>(&v));
-        }
+        for (int j = 0; j < 4; ++j)
+            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, from_bits<V>(entry[j]));
     } else {  // this thread looks for its entries itself
         const int k1 = min(col + 64, m.n_cols);
         int b, e;
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_expect(c_full(n), g.slots ? CODE_TILE : CODE_BYTES);
             tma_load(to, &map_codes, col / 2, row, c_full(n));
             if (g.slots)
-                bulk_load(to + CODE_BYTES, g.slots + ((long long)(row / 128) * ((m.n_cols + 127) / 128) + col / 128) * 256,
+                bulk_load(to + CODE_BYTES, g.sides + ((long long)(row / 128) * ((m.n_cols + 127) / 128) + col / 128) * SLOT_BYTES,
                           SLOT_BYTES, c_full(n));
         }
         if (!ok) {
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
             const int cs = n % CODES;
             ok = convert_tile<V, MODE>(
-                m, codes_at + cs * CODE_TILE, g.slots != nullptr, now, t, row_at(n), col_at(n),
+                m, codes_at + cs * CODE_TILE, g.slots, now, t, row_at(n), col_at(n),
                 [&] { mbar_arrive(c_empty(n)); },
                 [&](int part) { return __all_sync(0xffffffffu, stage_free(2 * n + part)); },
                 [&](int part) { return smem + (2 * n + part) % S::STAGES * S::STAGE; },
@@ -373,7 +381,7 @@ constexpr int PAIR_THREADS = 32 * 24, WRITE = 20;  // first of the writing warps
 struct PairShape {
     static constexpr int STAGE = 2 * A_BYTES, STAGES = 6, CODES = 2, COLS = 256;
     static constexpr int BARS = STAGES + 3 * TURN + 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * CODE_TILE + BARS * 8;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * PAIR_TILE + BARS * 8;
     static_assert(SMEM <= 227 * 1024 && STAGES <= TURN && CODES <= TURN, "as above");
 };
 
@@ -388,7 +396,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
-    const uint32_t bars = smem_addr(codes_at + S::CODES * CODE_TILE);
+    const uint32_t bars = smem_addr(codes_at + S::CODES * PAIR_TILE);
     auto full = [&](int s) { return bars + 8 * s; };                                // block 0's: of both blocks' stage
     auto empty = [&](int step) { return bars + 8 * (S::STAGES + step % TURN); };    // each block's, of a step
     auto c_full = [&](int n) { return bars + 8 * (S::STAGES + TURN + n % TURN); };  // of a code tile of its own
@@ -492,13 +500,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 const int row = MODE == PRODUCT ? line0 : block * 128, col = MODE == PRODUCT ? block * 128 : line0;
                 const int tile_rows = (int)(((long long)m.n_rows + 127) / 128), tile_cols = (int)(((long long)m.n_cols + 127) / 128);
                 // the second block of the last pair may lie behind the last line altogether
-                const bool slots = g.slots && row / 128 < tile_rows && col / 128 < tile_cols;
-                const uint32_t to = smem_addr(codes_at) + n % S::CODES * CODE_TILE;
-                mbar_expect(c_full(n), slots ? CODE_TILE : CODE_BYTES);
+                const bool sides = row / 128 < tile_rows && col / 128 < tile_cols;
+                const uint32_t to = smem_addr(codes_at) + n % S::CODES * PAIR_TILE;
+                mbar_expect(c_full(n), CODE_BYTES + (sides ? g.side_bytes : 0));
                 tma_load(to, &map_codes, col / 2, row, c_full(n));
-                if (slots)
-                    bulk_load(to + CODE_BYTES, g.slots + ((long long)(row / 128) * tile_cols + col / 128) * 256, SLOT_BYTES,
-                              c_full(n));
+                if (sides)
+                    bulk_load(to + CODE_BYTES, g.sides + ((long long)(row / 128) * tile_cols + col / 128) * g.side_bytes,
+                              g.side_bytes, c_full(n));
             }
         }
         if (!ok) {
@@ -513,51 +521,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const int tile_row = MODE == PRODUCT ? t : 64 * half + t % 64, part = MODE == PRODUCT ? half : t / 64;
         const int out_row = MODE == PRODUCT ? t : t % 64, out_at = out_row * 128 + (MODE == PRODUCT ? 0 : part * 8192);
         // a group's place: code tile n of all, code tile `block` of the pair's tile `at`
-        int at = 0, block = group / 2, line0 = 0;
-        auto settle = [&] {
+        int at = 0, block = group / 2;
+        bool ok = true;
+        for (int n = group / 2; ok; n += 2, block += 2) {
             while (block >= blocks && at < mine) {
                 block -= blocks;
                 ++at;
             }
-            line0 = line_of(first + at * pairs);
-        };
-        settle();
-        auto row = [&] { return (MODE == PRODUCT ? line0 : block * 128) + tile_row; };
-        auto col = [&] { return (MODE == PRODUCT ? block * 128 : line0) + 64 * part; };
-        GroupOf of(col(), m.group, 256);
-        Scales<V, 2> next;
-        long long numbers = (long long)row() * m.n_groups;  // of the row
-        if (at < mine) next.load(m, row() < m.n_rows, numbers, of);
-        bool ok = true;
-        for (int n = group / 2; at < mine && ok; n += 2) {
-            const Scales<V, 2> now = next;
-            const int this_row = row(), this_col = col();
-            const bool slots = g.slots && line0 < (MODE == PRODUCT ? m.n_rows : m.n_cols);
-            block += 2;
-            if (block < blocks) {
-                if (MODE == PRODUCT)
-                    of.move();
-                else
-                    numbers += 256ll * m.n_groups;
-            } else {
-                settle();
-                of = GroupOf(col(), m.group, 256);
-                numbers = (long long)row() * m.n_groups;
-            }
-            if (at < mine) next.load(m, row() < m.n_rows, numbers, of);
-            if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
-            const uint8_t *from = codes_at + n % S::CODES * CODE_TILE;
+            if (at >= mine || !(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
+            const int line0 = line_of(first + at * pairs);
+            const uint8_t *from = codes_at + n % S::CODES * PAIR_TILE, *side = from + CODE_BYTES;
             uint4 c[2], entries;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
                 c[j] = *reinterpret_cast<const uint4 *>(from + tile_row * 64 + ((2 * part + j ^ tile_row >> 1 & 3) << 4));
-            if (slots) entries = *reinterpret_cast<const uint4 *>(from + CODE_BYTES + (half * 128 + t) * 16);
+            const uint2 numbers = reinterpret_cast<const uint2 *>(side)[128 * half + t];
+            const bool slots = g.slots && line0 < (MODE == PRODUCT ? m.n_rows : m.n_cols);
+            if (slots) entries = reinterpret_cast<const uint4 *>(side + NUMBER_BYTES)[128 * half + t];
             fence_async_shared();  // as in convert_tile
             __syncwarp();
             if (lane == 0) mbar_arrive(c_empty(n));
             const int step = 2 * n + half, s = step % S::STAGES;
             if (!(ok = __all_sync(0xffffffffu, stage_free(step)))) break;
-            convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, now.s, now.z, slots, entries, m, this_row, this_col);
+            const V scale[2] = {from_bits<V>(numbers.x), from_bits<V>(numbers.x >> 16)};
+            const int zero[2] = {(int)(numbers.y & 0xffff), (int)(numbers.y >> 16)};
+            const int row = (MODE == PRODUCT ? line0 : block * 128) + tile_row;
+            const int col = (MODE == PRODUCT ? block * 128 : line0) + 64 * part;
+            convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, scale, zero, slots, entries, m, row, col);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive_own_at(in_block(full(s), 0));
@@ -612,54 +602,76 @@ __device__ __forceinline__ int warp_first_at_least(const int *col, int begin, in
     return begin + __popc(__ballot_sync(0xffffffffu, below));
 }
 
-// The residual's entries into the slots of the code tiles, 32 rows (a warp each) and 4096 columns at a time: collected in
-// shared memory, then written in order.  A segment of 64 columns with more than four entries, or with a repeated column,
-// is marked.  (With four rows a warp, one after the other, it waited for memory 13 us of 8192 x 8192.)
+// What follows the code tiles' codes: the residual's entries in slots, and scales and zero points (`numbers`) in the order
+// in which a tile's threads read them, so that they come with the codes; each block 32 rows (a warp each) x 4096 columns,
+// collected in shared memory and written in order.  A segment of 64 columns with more than four entries, or with a
+// repeated column, is marked.  (With four rows a warp, one after the other, it waited for memory 13 us of 8192 x 8192.)
 template <typename V, int MODE>
-__global__ void __launch_bounds__(1024) slots_kernel(Matrix<V> m, int chunks, uint4 *slots) {
+__global__ void __launch_bounds__(1024) sides_kernel(Matrix<V> m, int chunks, bool numbers, uint8_t *sides, int side_bytes) {
     __shared__ uint4 part[64][32];  // [segment][row]
+    __shared__ uint2 number[64][32];  // [segment][row, in an order that goes by the segment]
     const int lane = threadIdx.x % 32, r = threadIdx.x / 32;
     const int row0 = blockIdx.x / chunks * 32, k0 = blockIdx.x % chunks * 4096;
-    int begin = 0, end = 0;
-    if (row0 + r < m.n_rows) res_range(m, row0 + r, begin, end);
-    for (int j = threadIdx.x; j < 64 * 32; j += 1024)
-        part[j / 32][j % 32] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
-    __syncthreads();
-    const int k1 = min((long long)m.n_cols, k0 + 4096ll);
-    if (k0 > 0) begin = warp_first_at_least(m.res_col, begin, end, k0);
-    int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
-    for (int e0 = begin; e0 < end; e0 += 32) {
-        const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
-        const V v = e < end ? m.res_val[e] : from_float<V>(0.f);
-        const bool mine = k >= k0 && k < k1;
-        const int segment = mine ? (k - k0) / 64 : 64;
-        int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
-        if (lane == 0) {
-            left = segment_before;
-            column = column_before;
+    const long long tiles = ((long long)m.n_cols + 127) / 128;
+    const int segments = (int)min(64ll, 2 * tiles - k0 / 64);  // of whole tiles
+    const bool real = row0 + r < m.n_rows;
+    if (numbers) {
+        const long long from = (real ? row0 + r : 0) * (long long)m.n_groups;
+        for (int j = lane; j < segments; j += 32) {
+            uint2 w = make_uint2(0, 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int g = min((k0 + 64 * j + 32 * h) / m.group, m.n_groups - 1);
+                const V scale = real ? m.scales[from + g] : from_float<V>(0.f);  // rows behind the last add nothing
+                const uint32_t zero = m.zeros ? m.zeros[from + g] & 15 : 8;
+                w.x |= (uint32_t)*reinterpret_cast<const uint16_t *>(&scale) << 16 * h;
+                w.y |= zero << 16 * h;
+            }
+            number[j][(r ^ j) & 31] = w;
         }
-        const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
-        const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
-        uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
-        if (mine && rank < 4) to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
-        __syncwarp();
-        if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
-        __syncwarp();
-        segment_before = __shfl_sync(0xffffffffu, segment, 31);
-        column_before = __shfl_sync(0xffffffffu, k, 31);
-        run = __shfl_sync(0xffffffffu, rank, 31) + 1;
-        if (segment_before == 64) break;
+    }
+    if (m.res_ptr) {
+        for (int j = threadIdx.x; j < 64 * 32; j += 1024)
+            part[j / 32][j % 32] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+        __syncthreads();
+        int begin = 0, end = 0;
+        if (real) res_range(m, row0 + r, begin, end);
+        const int k1 = min((long long)m.n_cols, k0 + 4096ll);
+        if (k0 > 0) begin = warp_first_at_least(m.res_col, begin, end, k0);
+        int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
+        for (int e0 = begin; e0 < end; e0 += 32) {
+            const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
+            const V v = e < end ? m.res_val[e] : from_float<V>(0.f);
+            const bool mine = k >= k0 && k < k1;
+            const int segment = mine ? (k - k0) / 64 : 64;
+            int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
+            if (lane == 0) {
+                left = segment_before;
+                column = column_before;
+            }
+            const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
+            const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
+            uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
+            if (mine && rank < 4) to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
+            __syncwarp();
+            if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
+            __syncwarp();
+            segment_before = __shfl_sync(0xffffffffu, segment, 31);
+            column_before = __shfl_sync(0xffffffffu, k, 31);
+            run = __shfl_sync(0xffffffffu, rank, 31) + 1;
+            if (segment_before == 64) break;
+        }
     }
     __syncthreads();
-    const long long tiles = (m.n_cols + 127) / 128;
     const int i = row0 + lane;
-    for (int j = r; j < 64 && k0 + 64 * j < m.n_cols; j += 32) {
+    for (int j = r; j < segments; j += 32) {
         const int in_tile = MODE == PRODUCT ? j % 2 * 128 + i % 128 : i % 128 / 64 * 128 + j % 2 * 64 + i % 64;
-        uint4 *to = slots + ((long long)(i / 128) * tiles + k0 / 128 + j / 2) * 256 + in_tile;
-        *to = part[j][lane];
-        // the second half of a last tile that has no columns there
-        if (j % 2 == 0 && k0 + 64 * (j + 1) >= m.n_cols)
-            to[MODE == PRODUCT ? 128 : 64] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+        uint8_t *to = sides + ((long long)(i / 128) * tiles + k0 / 128 + j / 2) * side_bytes;
+        if (numbers) {
+            reinterpret_cast<uint2 *>(to)[in_tile] = number[j][(lane ^ j) & 31];
+            to += NUMBER_BYTES;
+        }
+        if (m.res_ptr) reinterpret_cast<uint4 *>(to)[in_tile] = part[j][lane];
     }
 }
 
@@ -731,16 +743,18 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (!encode_codes(&codes, m)) return cudaErrorInvalidValue;
         cudaError_t e = map_vectors(&vectors, b, depth, n_vec, ld_b, bn ? bn : 128, work);
         if (e != cudaSuccess) return e;
-        if (m.res_ptr) {
+        g.slots = m.res_ptr != nullptr;
+        g.side_bytes = (bn == 0 ? NUMBER_BYTES : 0) + (g.slots ? SLOT_BYTES : 0);
+        if (g.side_bytes > 0) {
             // whole tiles of 128 rows: rows behind the last have empty slots
             const long long rows = ceil_div(m.n_rows, 128), cols = ceil_div(m.n_cols, 128);
             const long long chunks = ceil_div(m.n_cols, 4096);
-            uint4 *slots = nullptr;
+            uint8_t *sides = nullptr;
             if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
-            if ((e = work.take((void **)&slots, SLOT_BYTES * rows * cols)) != cudaSuccess) return e;
-            slots_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 1024, 0, s>>>(m, (int)chunks, slots);
+            if ((e = work.take((void **)&sides, g.side_bytes * rows * cols)) != cudaSuccess) return e;
+            sides_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 1024, 0, s>>>(m, (int)chunks, bn == 0, sides, g.side_bytes);
             if ((e = cudaGetLastError()) != cudaSuccess) return e;
-            g.slots = slots;
+            g.sides = sides;
         }
     }
     if (bn == 0) {
