@@ -603,20 +603,27 @@ __device__ __forceinline__ int warp_first_at_least(const int *col, int begin, in
 }
 
 // What follows the code tiles' codes: the residual's entries in slots, and scales and zero points (`numbers`) in the order
-// in which a tile's threads read them, so that they come with the codes; each block 32 rows (a warp each) x 4096 columns,
+// in which a tile's threads read them, so that they come with the codes; each block 16 rows (a warp each) x 8192 columns,
 // collected in shared memory and written in order.  A segment of 64 columns with more than four entries, or with a
-// repeated column, is marked.  (With four rows a warp, one after the other, it waited for memory 13 us of 8192 x 8192.)
+// repeated column, is marked.  It waits for memory, a few loads after one another, so that all rows should be under way at
+// once (8192 x 8192: 13 us; by 32 rows x 4096 columns, in two turns, 17; four rows a warp, 13 us more).
+constexpr int SIDE_ROWS = 16, SIDE_SEGMENTS = 128;
+
 template <typename V, int MODE>
-__global__ void __launch_bounds__(1024) sides_kernel(Matrix<V> m, int chunks, bool numbers, uint8_t *sides, int side_bytes) {
-    __shared__ uint4 part[64][32];  // [segment][row]
-    __shared__ uint2 number[64][32];  // [segment][row, in an order that goes by the segment]
+__global__ void __launch_bounds__(32 * SIDE_ROWS)
+    sides_kernel(Matrix<V> m, int chunks, bool numbers, uint8_t *sides, int side_bytes) {
+    __shared__ uint4 part[SIDE_SEGMENTS][SIDE_ROWS];
+    __shared__ uint2 number[SIDE_SEGMENTS][SIDE_ROWS];  // a segment's rows are in an order that goes by the segment
     const int lane = threadIdx.x % 32, r = threadIdx.x / 32;
-    const int row0 = blockIdx.x / chunks * 32, k0 = blockIdx.x % chunks * 4096;
+    const int row0 = blockIdx.x / chunks * SIDE_ROWS, k0 = blockIdx.x % chunks * (64 * SIDE_SEGMENTS);
     const long long tiles = ((long long)m.n_cols + 127) / 128;
-    const int segments = (int)min(64ll, 2 * tiles - k0 / 64);  // of whole tiles
+    const int segments = (int)min((long long)SIDE_SEGMENTS, 2 * tiles - k0 / 64);  // of whole tiles
     const bool real = row0 + r < m.n_rows;
+    int begin = 0, end = 0;
+    if (real && m.res_ptr) res_range(m, row0 + r, begin, end);
     if (numbers) {
         const long long from = (real ? row0 + r : 0) * (long long)m.n_groups;
+#pragma unroll 4
         for (int j = lane; j < segments; j += 32) {
             uint2 w = make_uint2(0, 0);
 #pragma unroll
@@ -627,23 +634,21 @@ __global__ void __launch_bounds__(1024) sides_kernel(Matrix<V> m, int chunks, bo
                 w.x |= (uint32_t)*reinterpret_cast<const uint16_t *>(&scale) << 16 * h;
                 w.y |= zero << 16 * h;
             }
-            number[j][(r ^ j) & 31] = w;
+            number[j][(r ^ j) % SIDE_ROWS] = w;
         }
     }
     if (m.res_ptr) {
-        for (int j = threadIdx.x; j < 64 * 32; j += 1024)
-            part[j / 32][j % 32] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
+        for (int j = threadIdx.x; j < SIDE_SEGMENTS * SIDE_ROWS; j += 32 * SIDE_ROWS)
+            part[j / SIDE_ROWS][j % SIDE_ROWS] = make_uint4(NO_ENTRY, NO_ENTRY, NO_ENTRY, NO_ENTRY);
         __syncthreads();
-        int begin = 0, end = 0;
-        if (real) res_range(m, row0 + r, begin, end);
-        const int k1 = min((long long)m.n_cols, k0 + 4096ll);
+        const int k1 = min((long long)m.n_cols, k0 + 64ll * SIDE_SEGMENTS);
         if (k0 > 0) begin = warp_first_at_least(m.res_col, begin, end, k0);
         int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
         for (int e0 = begin; e0 < end; e0 += 32) {
             const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
             const V v = e < end ? m.res_val[e] : from_float<V>(0.f);
             const bool mine = k >= k0 && k < k1;
-            const int segment = mine ? (k - k0) / 64 : 64;
+            const int segment = mine ? (k - k0) / 64 : SIDE_SEGMENTS;
             int left = __shfl_up_sync(0xffffffffu, segment, 1), column = __shfl_up_sync(0xffffffffu, k, 1);
             if (lane == 0) {
                 left = segment_before;
@@ -651,7 +656,7 @@ __global__ void __launch_bounds__(1024) sides_kernel(Matrix<V> m, int chunks, bo
             }
             const unsigned heads = __ballot_sync(0xffffffffu, segment != left) & (0xffffffffu >> (31 - lane));
             const int rank = heads ? lane - (31 - __clz(heads)) : run + lane;
-            uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment & 63][r]);
+            uint32_t *to = reinterpret_cast<uint32_t *>(&part[segment % SIDE_SEGMENTS][r]);
             if (mine && rank < 4) to[rank] = (uint32_t)(k % 64) << 16 | *reinterpret_cast<const uint16_t *>(&v);
             __syncwarp();
             if (mine && (rank >= 4 || column == k)) to[3] = TOO_MANY;
@@ -659,19 +664,19 @@ __global__ void __launch_bounds__(1024) sides_kernel(Matrix<V> m, int chunks, bo
             segment_before = __shfl_sync(0xffffffffu, segment, 31);
             column_before = __shfl_sync(0xffffffffu, k, 31);
             run = __shfl_sync(0xffffffffu, rank, 31) + 1;
-            if (segment_before == 64) break;
+            if (segment_before == SIDE_SEGMENTS) break;
         }
     }
     __syncthreads();
-    const int i = row0 + lane;
-    for (int j = r; j < segments; j += 32) {
+    const int row = threadIdx.x % SIDE_ROWS, i = row0 + row;
+    for (int j = threadIdx.x / SIDE_ROWS; j < segments; j += 32) {
         const int in_tile = MODE == PRODUCT ? j % 2 * 128 + i % 128 : i % 128 / 64 * 128 + j % 2 * 64 + i % 64;
         uint8_t *to = sides + ((long long)(i / 128) * tiles + k0 / 128 + j / 2) * side_bytes;
         if (numbers) {
-            reinterpret_cast<uint2 *>(to)[in_tile] = number[j][(lane ^ j) & 31];
+            reinterpret_cast<uint2 *>(to)[in_tile] = number[j][(row ^ j) % SIDE_ROWS];
             to += NUMBER_BYTES;
         }
-        if (m.res_ptr) reinterpret_cast<uint4 *>(to)[in_tile] = part[j][lane];
+        if (m.res_ptr) reinterpret_cast<uint4 *>(to)[in_tile] = part[j][row];
     }
 }
 
@@ -748,11 +753,12 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (g.side_bytes > 0) {
             // whole tiles of 128 rows: rows behind the last have empty slots
             const long long rows = ceil_div(m.n_rows, 128), cols = ceil_div(m.n_cols, 128);
-            const long long chunks = ceil_div(m.n_cols, 4096);
+            const long long grid = rows * (128 / SIDE_ROWS) * ceil_div(m.n_cols, 64 * SIDE_SEGMENTS);
             uint8_t *sides = nullptr;
-            if (rows * 4 * chunks > INT_MAX) return cudaErrorMemoryAllocation;
+            if (grid > INT_MAX) return cudaErrorMemoryAllocation;
             if ((e = work.take((void **)&sides, g.side_bytes * rows * cols)) != cudaSuccess) return e;
-            sides_kernel<V, MODE><<<(unsigned)(rows * 4 * chunks), 1024, 0, s>>>(m, (int)chunks, bn == 0, sides, g.side_bytes);
+            sides_kernel<V, MODE><<<(unsigned)grid, 32 * SIDE_ROWS, 0, s>>>(
+                m, (int)ceil_div(m.n_cols, 64 * SIDE_SEGMENTS), bn == 0, sides, g.side_bytes);
             if ((e = cudaGetLastError()) != cudaSuccess) return e;
             g.sides = sides;
         }
