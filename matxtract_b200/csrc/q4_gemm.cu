@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 1) tmem_alloc(smem_addr(&tmem_shared), COLUMNS);
     tc_fence_before();
     __syncthreads();
+    front_is_done();
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
     // the stage of a step is free, the place of a code tile likewise, once what was there before is used up
@@ -433,6 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     cluster_barrier();  // the other block's barriers are there, too
+    front_is_done();
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
     // steps and code tiles are numbered on from tile to tile
@@ -614,6 +616,7 @@ __global__ void __launch_bounds__(32 * SIDE_ROWS)
     sides_kernel(Matrix<V> m, int chunks, bool numbers, uint8_t *sides, int side_bytes) {
     __shared__ uint4 part[SIDE_SEGMENTS][SIDE_ROWS];
     __shared__ uint2 number[SIDE_SEGMENTS][SIDE_ROWS];  // a segment's rows are in an order that goes by the segment
+    next_may_start();
     const int lane = threadIdx.x % 32, r = threadIdx.x / 32;
     const int row0 = blockIdx.x / chunks * SIDE_ROWS, k0 = blockIdx.x % chunks * (64 * SIDE_SEGMENTS);
     const long long tiles = ((long long)m.n_cols + 127) / 128;
@@ -685,23 +688,11 @@ __global__ void __launch_bounds__(32 * SIDE_ROWS)
 template <typename V, int MODE, int BN>
 cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &b, const Args<V> &g,
                    long long tiles, cudaStream_t s) {
-    if (tiles * g.splits > INT_MAX) return cudaErrorInvalidConfiguration;
     auto kernel = gemm_kernel<V, MODE, BN>;
     constexpr int bytes = Shape<MODE, BN>::SMEM;
     const cudaError_t e = allow_smem<V, gemm_kernel<V, MODE, BN>>(bytes);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * g.splits));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = g.splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, codes, b, g);
+    return launch_behind(kernel, tiles * g.splits, THREADS, bytes, g.splits, s, codes, b, g);
 }
 
 // Width of a tile and number of blocks that share its contraction: the choice with the least time by a model in clocks.
@@ -768,8 +759,8 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
         if (tiles > INT_MAX / 2) return cudaErrorInvalidConfiguration;
         const cudaError_t e = allow_smem<V, pair_kernel<V, MODE>>(PairShape::SMEM);
         if (e != cudaSuccess) return e;
-        pair_kernel<V, MODE><<<(unsigned)(2 * std::min<long long>(tiles, 74)), PAIR_THREADS, PairShape::SMEM, s>>>(codes, vectors, g);
-        return cudaGetLastError();
+        return launch_behind(pair_kernel<V, MODE>, 2 * std::min<long long>(tiles, 74), PAIR_THREADS, PairShape::SMEM, 0, s, codes,
+                             vectors, g);
     }
     const long long tiles = g.tiles_m * ceil_div(n_vec, bn);
     switch (bn) {

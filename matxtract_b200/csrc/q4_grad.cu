@@ -120,6 +120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     cluster_barrier();  // the other block's barriers are there, too
+    front_is_done();
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
 
@@ -272,8 +273,7 @@ cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x,
     if (e == cudaSuccess) e = map_vectors(&map_x, x, m.n_cols, n_vec, ld_x, 64, work);
     if (e == cudaSuccess) e = allow_smem<V, gradient_kernel<V>>(SMEM);
     if (e != cudaSuccess) return e;
-    gradient_kernel<V><<<(unsigned)(2 * std::min<long long>(tiles, 74)), THREADS, SMEM, s>>>(map_dy, map_x, g);
-    return cudaGetLastError();
+    return launch_behind(gradient_kernel<V>, 2 * std::min<long long>(tiles, 74), THREADS, SMEM, 0, s, map_dy, map_x, g);
 }
 
 cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s) {

@@ -127,9 +127,36 @@ struct Workspace {
     }
 };
 
+// A kernel that lays something out for the next one lets it start (`next_may_start`), so that its blocks set themselves up
+// meanwhile; they touch no memory of a caller's or of a kernel's in front before `front_is_done` has returned.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void front_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that calls front_is_done; cluster: blocks, 0 where the kernel says so itself.
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), long long blocks, int threads, int smem, int cluster, cudaStream_t s,
+                          const A &...args) {
+    if (blocks > INT_MAX) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // to[r][c] = from[r][c]
 template <typename V>
 __global__ void align_kernel(const V *from, long long ld, V *to, long long ld_to, long long rows, int cols) {
+    next_may_start();
     const long long stride = (long long)gridDim.y * blockDim.y;
     const long long c = ((long long)blockIdx.x * 32 + threadIdx.x) * 8;
     for (long long r = (long long)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += stride) {
