@@ -64,6 +64,7 @@ struct Args {
     long long ld_out;
     const uint8_t *sides;  // what follows a code tile's codes, [row / 128][column / 128][side_bytes]; null: nothing
     int side_bytes;
+    int wide;  // scales that may be loaded together: 1, 2, 4
     bool slots;  // the residual's entries are among it
 };
 
@@ -75,47 +76,63 @@ __device__ __forceinline__ V from_bits(uint32_t low) {
 
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
 
-// scales and zero points of N times 32 of a row's columns
-template <typename V, int N>
+// Scales and zero points of a row's 128 columns, by 32s.  A warp's lanes look at 32 rows, so that each load costs 32 accesses
+// to the L1, whose rate bounds it: neighbouring groups come together where the rows' numbers lie on such borders (`wide` of
+// them; 8192 x 8192, 16 vectors, groups of 32 with zero points: 36.5 -> 24.4 us).
+template <typename V>
 struct Scales {
-    V s[N];
-    int z[N];
-    // `row`: where the row's numbers begin; real: there is such a row
-    __device__ __forceinline__ void load(const Matrix<V> &m, bool real, long long row, const GroupOf &at) {
-        if (!real) row = 0;
+    uint2 s;     // four scales
+    uint32_t z;  // four zero points, a byte each
+    // `row`: where the row's numbers begin; real: there is such a row; at: the group of the first column, a multiple of 128
+    __device__ __forceinline__ void load(const Matrix<V> &m, int wide, bool real, long long row, const GroupOf &at) {
+        const V *scales = m.scales + row;
+        const uint8_t *zeros = m.zeros + row;
         const int last = m.n_groups - 1;  // behind the last column
-        if (m.group % (32 * N) == 0) {
-            const int g = min(at.g, last);
-            const V scale = real ? m.scales[row + g] : from_float<V>(0.f);
-            const int zero = m.zeros ? m.zeros[row + g] & 15 : 8;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                s[j] = scale;
-                z[j] = zero;
-            }
+        z = 0x08080808u;
+        s = make_uint2(0, 0);
+        if (!real) return;  // rows behind the last add nothing
+        const int g = min(at.g, last);
+        if (m.group % 128 == 0) {
+            s.x = s.y = twice(scales[g]);
+            if (m.zeros) z = zeros[g] * 0x01010101u;
+        } else if (m.group == 32 && wide == 4) {
+            s = *reinterpret_cast<const uint2 *>(scales + g);
+            if (m.zeros) z = *reinterpret_cast<const uint32_t *>(zeros + g);
+        } else if (m.group == 32 && wide == 2) {
+            const int h = min(g + 2, last - 1);
+            s.x = *reinterpret_cast<const uint32_t *>(scales + g);
+            s.y = *reinterpret_cast<const uint32_t *>(scales + h);
+            if (m.zeros) z = *reinterpret_cast<const uint16_t *>(zeros + g) | (uint32_t)*reinterpret_cast<const uint16_t *>(zeros + h) << 16;
+        } else if (m.group == 64 && wide >= 2) {
+            const uint32_t two = *reinterpret_cast<const uint32_t *>(scales + g);
+            s.x = __byte_perm(two, 0, 0x1010);
+            s.y = __byte_perm(two, 0, 0x3232);
+            if (m.zeros) z = __byte_perm(*reinterpret_cast<const uint16_t *>(zeros + g), 0, 0x1100);
         } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int g = min(at.after(j), last);
-                s[j] = real ? m.scales[row + g] : from_float<V>(0.f);
-                z[j] = m.zeros ? m.zeros[row + g] & 15 : 8;
-            }
+            const int g1 = min(at.after(1), last), g2 = min(at.after(2), last), g3 = min(at.after(3), last);
+            s.x = bits(scales[g]) | bits(scales[g1]) << 16;
+            s.y = bits(scales[g2]) | bits(scales[g3]) << 16;
+            if (m.zeros) z = zeros[g] | zeros[g1] << 8 | zeros[g2] << 16 | (uint32_t)zeros[g3] << 24;
         }
     }
+    static __device__ __forceinline__ uint32_t bits(V v) { return *reinterpret_cast<const uint16_t *>(&v); }
+    static __device__ __forceinline__ uint32_t twice(V v) { return bits(v) * 0x10001u; }
+    __device__ __forceinline__ uint2 half(int h) const { return make_uint2(h ? s.y : s.x, h ? z >> 16 : z); }
 };
 
 // 64 values of a row in the operand's layout, with the residual's entries among them: `a` is the row's 128 bytes in a
-// stage, whose sixteens are in an order that goes by the row.
+// stage, whose sixteens are in an order that goes by the row.  numbers: two scales, and two zero points in a byte each.
 template <typename V>
-__device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4 (&c)[2], const V (&scale)[2], const int (&zero)[2],
-                                            bool slots, const uint4 &entries, const Matrix<V> &m, int row, int col) {
+__device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4 (&c)[2], uint2 numbers, bool slots,
+                                            const uint4 &entries, const Matrix<V> &m, int row, int col) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const typename Pair<V>::T s = Pair<V>::both(scale[j]);
+        const typename Pair<V>::T s = Pair<V>::both(from_bits<V>(numbers.x >> 16 * j));
+        const int zero = numbers.y >> 8 * j & 15;
         const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], s, zero[j]);
+            *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], s, zero);
     }
     if (!slots || entries.x == NO_ENTRY) return;
     auto add = [&](int k, V v) {
@@ -144,7 +161,7 @@ __device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4
 // 0-63 or 64-127 of the tile).  `release`: the tile's place may be filled again; free(p), stage(p), arrive(p): of the
 // tile's stage p.
 template <typename V, int MODE, typename Release, typename Free, typename Stage, typename Arrive>
-__device__ __forceinline__ bool convert_tile(const Matrix<V> &m, const uint8_t *from, bool slots, const Scales<V, 4> &now,
+__device__ __forceinline__ bool convert_tile(const Matrix<V> &m, const uint8_t *from, bool slots, const Scales<V> &now,
                                              int t, int row, int col, Release release, Free free, Stage stage,
                                              Arrive arrive) {
     const int lane = threadIdx.x % 32, out_row = MODE == PRODUCT ? t : t % 64;
@@ -165,10 +182,8 @@ __device__ __forceinline__ bool convert_tile(const Matrix<V> &m, const uint8_t *
         const int part = MODE == PRODUCT ? half : t / 64;
         if (MODE == PRODUCT || half == 0)
             if (!free(part)) return false;
-        const V s[2] = {now.s[2 * half], now.s[2 * half + 1]};
-        const int z[2] = {now.z[2 * half], now.z[2 * half + 1]};
-        convert_row<V>(stage(part) + out_row * 128 + (MODE == PRODUCT ? 0 : half * 8192), out_row, c[half], s, z, slots,
-                       entries[half], m, row, col + 64 * half);
+        convert_row<V>(stage(part) + out_row * 128 + (MODE == PRODUCT ? 0 : half * 8192), out_row, c[half],
+                       now.half(half), slots, entries[half], m, row, col + 64 * half);
         if (MODE == PRODUCT || half == 1) {
             fence_async_shared();
             __syncwarp();
@@ -296,18 +311,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto row_at = [&](int n) { return MODE == PRODUCT ? line0 + t : (block0 + n) * 128 + t; };
         auto col_at = [&](int n) { return MODE == PRODUCT ? (block0 + n) * 128 : line0; };
         GroupOf at(col_at(group), m.group, 512);
-        Scales<V, 4> next;
+        Scales<V> next;
         long long numbers = (long long)row_at(group) * m.n_groups;  // of the row
-        if (group < blocks) next.load(m, row_at(group) < m.n_rows, numbers, at);
+        if (group < blocks) next.load(m, g.wide, row_at(group) < m.n_rows, numbers, at);
         bool ok = true;
         for (int n = group; n < blocks && ok; n += 4) {
-            const Scales<V, 4> now = next;
+            const Scales<V> now = next;
             if (n + 4 < blocks) {
                 if (MODE == PRODUCT)
                     at.move();
                 else
                     numbers += 512ll * m.n_groups;
-                next.load(m, row_at(n + 4) < m.n_rows, numbers, at);
+                next.load(m, g.wide, row_at(n + 4) < m.n_rows, numbers, at);
             }
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
             const int cs = n % CODES;
@@ -545,11 +560,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if (lane == 0) mbar_arrive(c_empty(n));
             const int step = 2 * n + half, s = step % S::STAGES;
             if (!(ok = __all_sync(0xffffffffu, stage_free(step)))) break;
-            const V scale[2] = {from_bits<V>(numbers.x), from_bits<V>(numbers.x >> 16)};
-            const int zero[2] = {(int)(numbers.y & 0xffff), (int)(numbers.y >> 16)};
             const int row = (MODE == PRODUCT ? line0 : block * 128) + tile_row;
             const int col = (MODE == PRODUCT ? block * 128 : line0) + 64 * part;
-            convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, scale, zero, slots, entries, m, row, col);
+            convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, numbers, slots, entries, m, row, col);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive_own_at(in_block(full(s), 0));
@@ -635,7 +648,7 @@ __global__ void __launch_bounds__(32 * SIDE_ROWS)
                 const V scale = real ? m.scales[from + g] : from_float<V>(0.f);  // rows behind the last add nothing
                 const uint32_t zero = m.zeros ? m.zeros[from + g] & 15 : 8;
                 w.x |= (uint32_t)*reinterpret_cast<const uint16_t *>(&scale) << 16 * h;
-                w.y |= zero << 16 * h;
+                w.y |= zero << 8 * h;
             }
             number[j][(r ^ j) % SIDE_ROWS] = w;
         }
@@ -730,6 +743,8 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
     g.n_vec = n_vec;
     g.out = out;
     g.ld_out = ld_out;
+    for (g.wide = 4; g.wide > 1; g.wide /= 2)
+        if (m.n_groups % g.wide == 0 && (uintptr_t)m.scales % (2 * g.wide) == 0 && (uintptr_t)m.zeros % g.wide == 0) break;
     int bn = 0;
     plan(lines, depth, n_vec, bn, g.splits);
     g.tiles_m = (int)ceil_div(lines, bn ? 128 : 256);
