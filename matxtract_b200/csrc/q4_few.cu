@@ -59,7 +59,7 @@ __device__ __forceinline__ int place(int w, int quarter) {
 template <typename V>
 struct Few {
     Matrix<V> m;
-    int n_vec, splits;
+    int n_vec, splits, wide;
     const V *x, *dy;
     long long ld_x, ld_dy;
     const V *turned;  // x as [column][vector], vectors filled up to 8 or 16; null for up to two vectors
@@ -118,6 +118,23 @@ template <int NT>
 constexpr int stream_smem = 1024 + DEPTH * stream_slot<NT> + 8 * NT * 128 * 4 + DEPTH * 16;
 constexpr int PART = 132;  // distance of two vectors' sums over 128 rows
 
+// sums over four neighbouring lanes: lane `quarter` gets that of the value quarter % N
+__device__ __forceinline__ float quarters(const float (&e)[1], int) {
+    const float s = e[0] + __shfl_xor_sync(0xffffffffu, e[0], 1);
+    return s + __shfl_xor_sync(0xffffffffu, s, 2);
+}
+__device__ __forceinline__ float quarters(const float (&e)[2], int quarter) {
+    const bool odd = quarter & 1;
+    const float s = (odd ? e[1] : e[0]) + __shfl_xor_sync(0xffffffffu, odd ? e[0] : e[1], 1);
+    return s + __shfl_xor_sync(0xffffffffu, s, 2);
+}
+__device__ __forceinline__ float quarters(const float (&e)[4], int quarter) {
+    const bool odd = quarter & 1, high = quarter & 2;
+    const float a = (odd ? e[1] : e[0]) + __shfl_xor_sync(0xffffffffu, odd ? e[0] : e[1], 1);
+    const float b = (odd ? e[3] : e[2]) + __shfl_xor_sync(0xffffffffu, odd ? e[2] : e[3], 1);
+    return (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 2);
+}
+
 __device__ int wait_ran_out_few;
 
 template <typename V, int S, int NT, bool GRAD>
@@ -174,21 +191,22 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             code_at[w] = (first_row + line) * 64 + ((byte / 16 ^ swizzle) << 4) + byte % 16;
             x_at[w] = CODE_BYTES + k / 64 * (NT * 1024) + line * 128 + ((k % 64 / 8 ^ line) << 4);
         }
-        // scales and zero points: a lane a row, scale | zero << 16
+        // scales and zero points: a lane a row
         const long long my_row = (long long)min(lower + lane, m.n_rows - 1) * m.n_groups;
-        const uint16_t *scales = reinterpret_cast<const uint16_t *>(m.scales) + my_row;
-        const uint8_t *zeros = m.zeros + my_row;
         GroupOf at((from + group) * 128, m.group, 256);
-        uint32_t next[SEGMENTS] = {};
+        Scales<V> next;
         auto numbers = [&](int n) {
-#pragma unroll
-            for (int j = 0; j < SEGMENTS; ++j) {
-                const int gr = GRAD ? min((rank + n / per_unit * g.splits) * SEGMENTS + j, m.n_groups - 1)
-                                    : j == 0 ? at.g : min(at.after(j * (WIDTH / 32)), m.n_groups - 1);
-                next[j] = GRAD ? 0 : scales[gr];
-                if (m.zeros) next[j] |= (uint32_t)(zeros[gr] & 15) << 16;
+            const int gr = (rank + n / per_unit * g.splits) * SEGMENTS;  // gradient
+            if (SEGMENTS == 1) {  // one word: scale, zero point << 16
+                next.s.x = GRAD ? 0 : Scales<V>::bits(m.scales[my_row + at.g]);
+                if (m.zeros) next.s.x |= (uint32_t)(m.zeros[my_row + (GRAD ? gr : at.g)] & 15) << 16;
+                if (!GRAD) at.move();
+            } else if (GRAD) {
+                if (m.zeros) next.load(m, g.wide, my_row, gr, [&](int j) { return gr + j / (4 / SEGMENTS); });
+            } else {
+                next.load(m, g.wide, my_row, at.g, [&](int j) { return at.after(j); });
+                at.move();
             }
-            if (!GRAD) at.move();
         };
         float dy[2 * H][NT][2];
         if (GRAD) {
@@ -207,9 +225,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
         if (n < tiles) numbers(n);
         bool ok = true;
         while (n < tiles) {
-            uint32_t now[SEGMENTS];
-#pragma unroll
-            for (int j = 0; j < SEGMENTS; ++j) now[j] = next[j];
+            const Scales<V> now = next;
+            uint32_t two[2 * H], four[2 * H];  // this lane's rows' scales and zero points
             const int was = n;
             n += ALL ? 1 : 2;
             const bool complete = !ALL || n % per_unit == 0;  // the unit's last tile
@@ -238,18 +255,21 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             const int left = ALL && complete ? m.group - (per_unit - 1) * 128 : 128;
 #pragma unroll
             for (int j = 0; j < SEGMENTS; ++j) {
+                const int n32 = j * (WIDTH / 32);
                 int z[2 * H];
                 float s[2 * H];
 #pragma unroll
-                for (int r = 0; r < 2 * H; ++r) z[r] = 8;
-                if (!GRAD || m.zeros) {
-#pragma unroll
-                    for (int r = 0; r < 2 * H; ++r) {
-                        const uint32_t v = __shfl_sync(0xffffffffu, now[j], line + 8 * r);
-                        const uint16_t b = (uint16_t)v;
-                        s[r] = to_float(*reinterpret_cast<const V *>(&b));
-                        if (m.zeros) z[r] = v >> 16;
+                for (int r = 0; r < 2 * H; ++r) {
+                    if (SEGMENTS == 1) {
+                        two[r] = !GRAD || m.zeros ? __shfl_sync(0xffffffffu, now.s.x, line + 8 * r) : 0;
+                        s[r] = GRAD ? 0.f : to_float(from_bits<V>(two[r]));
+                        z[r] = m.zeros ? two[r] >> 16 : 8;
+                        continue;
                     }
+                    if (!GRAD && n32 % 2 == 0) two[r] = __shfl_sync(0xffffffffu, n32 < 2 ? now.s.x : now.s.y, line + 8 * r);
+                    if (j == 0 && m.zeros) four[r] = __shfl_sync(0xffffffffu, now.z, line + 8 * r);
+                    s[r] = GRAD ? 0.f : to_float(from_bits<V>(two[r] >> 16 * (n32 % 2)));
+                    z[r] = m.zeros ? four[r] >> 8 * n32 & 15 : 8;
                 }
                 float(&e)[H][NT][4] = d[GRAD ? j : 0];
                 if (!GRAD) {
@@ -288,26 +308,27 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(slot));
             if (GRAD && complete) {
+                const int first_group = (rank + was / per_unit * g.splits) * SEGMENTS;
 #pragma unroll
-                for (int j = 0; j < SEGMENTS; ++j) {
-                    const int gr = (rank + was / per_unit * g.splits) * SEGMENTS + j;
+                for (int r = 0; r < 2 * H; ++r) {
+                    float e[SEGMENTS];
 #pragma unroll
-                    for (int r = 0; r < 2 * H; ++r) {
-                        float e = 0.f;
+                    for (int j = 0; j < SEGMENTS; ++j) {
+                        e[j] = 0.f;
 #pragma unroll
                         for (int q = 0; q < NT; ++q)
 #pragma unroll
                             for (int t = 0; t < 2; ++t) {
                                 float &v = d[j][r / 2][q][2 * (r % 2) + t];
-                                e = fmaf(dy[r][q][t], v, e);
+                                e[j] = fmaf(dy[r][q][t], v, e[j]);
                                 v = 0.f;
                             }
-                        e += __shfl_xor_sync(0xffffffffu, e, 1);
-                        e += __shfl_xor_sync(0xffffffffu, e, 2);
-                        const int i = lower + line + 8 * r;
-                        if (quarter == 0 && gr < m.n_groups && i < m.n_rows)
-                            g.out[(long long)i * m.n_groups + gr] = from_float<V>(e);
                     }
+                    // over the four lanes of a row, which end with a group each
+                    const float sum = quarters(e, quarter);
+                    const int i = lower + line + 8 * r, gr = first_group + quarter % SEGMENTS;
+                    if (quarter < SEGMENTS && gr < m.n_groups && i < m.n_rows)
+                        g.out[(long long)i * m.n_groups + gr] = from_float<V>(sum);
                 }
             }
         }
@@ -692,6 +713,7 @@ cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
+    g.wide = numbers_together(m);
     g.splits = parts_of(ceil_div(m.n_rows, 128), ceil_div(m.n_cols, 128), 2);
     g.out = y;
     g.ld_out = ld_y;
@@ -708,8 +730,10 @@ template <typename V>
 cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
                       cudaStream_t s) {
     // The residual's entries meet in columns: where there are some, the tiles that they are put into are faster even for
-    // one vector (4096 x 4096: 19 us there, 28 us with a search and ordered additions here).
-    if (n_vec > VEC || m.res_ptr) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
+    // one vector (4096 x 4096: 19 us there, 28 us with a search and ordered additions here).  Those also take the larger
+    // matrices (8 vectors, 2048 x 2048: 7.0 us here, 8.0 there; 4096 x 4096: 13.7 and 10.4, with groups of 32 and zero
+    // points 15.5 and 11.3), which few clusters of eight do not spread over the GPU.
+    if (n_vec > VEC || m.res_ptr || (long long)m.n_rows * m.n_cols > 1 << 22) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);
     const long long blocks = ceil_div(m.n_cols, COLS);
     Few<V> g = {};
     g.m = m;
@@ -731,6 +755,7 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
     Few<V> g = {};
     g.m = m;
     g.n_vec = n_vec;
+    g.wide = numbers_together(m);
     g.splits = parts_of(ceil_div(m.n_rows, 128), m.group == 32 || m.group == 64 ? ceil_div(m.n_cols, 128) : m.n_groups, 2);
     g.dy = dy;
     g.ld_dy = ld_dy;

@@ -68,57 +68,7 @@ struct Args {
     bool slots;  // the residual's entries are among it
 };
 
-template <typename V>
-__device__ __forceinline__ V from_bits(uint32_t low) {
-    const uint16_t v = (uint16_t)low;
-    return *reinterpret_cast<const V *>(&v);
-}
-
 __device__ int wait_ran_out;  // set when a bounded wait ended without its barrier
-
-// Scales and zero points of a row's 128 columns, by 32s.  A warp's lanes look at 32 rows, so that each load costs 32 accesses
-// to the L1, whose rate bounds it: neighbouring groups come together where the rows' numbers lie on such borders (`wide` of
-// them; 8192 x 8192, 16 vectors, groups of 32 with zero points: 36.5 -> 24.4 us).
-template <typename V>
-struct Scales {
-    uint2 s;     // four scales
-    uint32_t z;  // four zero points, a byte each
-    // `row`: where the row's numbers begin; real: there is such a row; at: the group of the first column, a multiple of 128
-    __device__ __forceinline__ void load(const Matrix<V> &m, int wide, bool real, long long row, const GroupOf &at) {
-        const V *scales = m.scales + row;
-        const uint8_t *zeros = m.zeros + row;
-        const int last = m.n_groups - 1;  // behind the last column
-        z = 0x08080808u;
-        s = make_uint2(0, 0);
-        if (!real) return;  // rows behind the last add nothing
-        const int g = min(at.g, last);
-        if (m.group % 128 == 0) {
-            s.x = s.y = twice(scales[g]);
-            if (m.zeros) z = zeros[g] * 0x01010101u;
-        } else if (m.group == 32 && wide == 4) {
-            s = *reinterpret_cast<const uint2 *>(scales + g);
-            if (m.zeros) z = *reinterpret_cast<const uint32_t *>(zeros + g);
-        } else if (m.group == 32 && wide == 2) {
-            const int h = min(g + 2, last - 1);
-            s.x = *reinterpret_cast<const uint32_t *>(scales + g);
-            s.y = *reinterpret_cast<const uint32_t *>(scales + h);
-            if (m.zeros) z = *reinterpret_cast<const uint16_t *>(zeros + g) | (uint32_t)*reinterpret_cast<const uint16_t *>(zeros + h) << 16;
-        } else if (m.group == 64 && wide >= 2) {
-            const uint32_t two = *reinterpret_cast<const uint32_t *>(scales + g);
-            s.x = __byte_perm(two, 0, 0x1010);
-            s.y = __byte_perm(two, 0, 0x3232);
-            if (m.zeros) z = __byte_perm(*reinterpret_cast<const uint16_t *>(zeros + g), 0, 0x1100);
-        } else {
-            const int g1 = min(at.after(1), last), g2 = min(at.after(2), last), g3 = min(at.after(3), last);
-            s.x = bits(scales[g]) | bits(scales[g1]) << 16;
-            s.y = bits(scales[g2]) | bits(scales[g3]) << 16;
-            if (m.zeros) z = zeros[g] | zeros[g1] << 8 | zeros[g2] << 16 | (uint32_t)zeros[g3] << 24;
-        }
-    }
-    static __device__ __forceinline__ uint32_t bits(V v) { return *reinterpret_cast<const uint16_t *>(&v); }
-    static __device__ __forceinline__ uint32_t twice(V v) { return bits(v) * 0x10001u; }
-    __device__ __forceinline__ uint2 half(int h) const { return make_uint2(h ? s.y : s.x, h ? z >> 16 : z); }
-};
 
 // 64 values of a row in the operand's layout, with the residual's entries among them: `a` is the row's 128 bytes in a
 // stage, whose sixteens are in an order that goes by the row.  numbers: two scales, and two zero points in a byte each.
@@ -313,7 +263,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         GroupOf at(col_at(group), m.group, 512);
         Scales<V> next;
         long long numbers = (long long)row_at(group) * m.n_groups;  // of the row
-        if (group < blocks) next.load(m, g.wide, row_at(group) < m.n_rows, numbers, at);
+        auto fetch = [&](int n) {
+            if (row_at(n) < m.n_rows)
+                next.load(m, g.wide, numbers, at.g, [&](int j) { return at.after(j); });
+            else
+                next = {};  // rows behind the last add nothing
+        };
+        if (group < blocks) fetch(group);
         bool ok = true;
         for (int n = group; n < blocks && ok; n += 4) {
             const Scales<V> now = next;
@@ -322,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     at.move();
                 else
                     numbers += 512ll * m.n_groups;
-                next.load(m, g.wide, row_at(n + 4) < m.n_rows, numbers, at);
+                fetch(n + 4);
             }
             if (!(ok = warp_wait(c_full(n), n / TURN & 1, polls))) break;
             const int cs = n % CODES;
@@ -743,8 +699,7 @@ cudaError_t tiles_of(const Matrix<V> &m, int n_vec, const V *b, long long ld_b, 
     g.n_vec = n_vec;
     g.out = out;
     g.ld_out = ld_out;
-    for (g.wide = 4; g.wide > 1; g.wide /= 2)
-        if (m.n_groups % g.wide == 0 && (uintptr_t)m.scales % (2 * g.wide) == 0 && (uintptr_t)m.zeros % g.wide == 0) break;
+    g.wide = numbers_together(m);
     int bn = 0;
     plan(lines, depth, n_vec, bn, g.splits);
     g.tiles_m = (int)ceil_div(lines, bn ? 128 : 256);

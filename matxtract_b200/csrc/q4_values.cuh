@@ -92,6 +92,62 @@ struct GroupOf {
     }
 };
 
+template <typename V>
+__device__ __forceinline__ V from_bits(uint32_t low) {
+    const uint16_t v = (uint16_t)low;
+    return *reinterpret_cast<const V *>(&v);
+}
+
+// Scales and zero points of 128 columns of a row (from a multiple of 128 on), by 32s.  A warp's lanes look at 32 rows, so
+// that each load costs 32 accesses to the L1, whose rate bounds it: neighbouring groups come together where the rows'
+// numbers lie on such borders (`wide` of them; groups of 32 with zero points, 8192 x 8192, 16 vectors: 36.5 -> 24.4 us,
+// 16384 x 8192, 1 vector: 57.6 -> 32.6).
+template <typename V>
+struct Scales {
+    uint2 s = {0, 0};          // four scales
+    uint32_t z = 0x08080808u;  // four zero points, a byte each
+    // row: where the row's numbers begin; g: the first column's group, after(n): that of the column 32 n further on
+    template <typename F>
+    __device__ __forceinline__ void load(const Matrix<V> &m, int wide, long long row, int g, F after) {
+        const V *scales = m.scales + row;
+        const uint8_t *zeros = m.zeros + row;
+        const int last = m.n_groups - 1;  // behind the last column
+        g = min(g, last);
+        if (m.group % 128 == 0) {
+            s.x = s.y = bits(scales[g]) * 0x10001u;
+            if (m.zeros) z = zeros[g] * 0x01010101u;
+        } else if (m.group == 32 && wide == 4) {
+            s = *reinterpret_cast<const uint2 *>(scales + g);
+            if (m.zeros) z = *reinterpret_cast<const uint32_t *>(zeros + g);
+        } else if (m.group == 32 && wide == 2) {
+            const int h = min(g + 2, last - 1);
+            s.x = *reinterpret_cast<const uint32_t *>(scales + g);
+            s.y = *reinterpret_cast<const uint32_t *>(scales + h);
+            if (m.zeros)
+                z = *reinterpret_cast<const uint16_t *>(zeros + g) | (uint32_t)*reinterpret_cast<const uint16_t *>(zeros + h) << 16;
+        } else if (m.group == 64 && wide >= 2) {
+            const uint32_t two = *reinterpret_cast<const uint32_t *>(scales + g);
+            s.x = __byte_perm(two, 0, 0x1010);
+            s.y = __byte_perm(two, 0, 0x3232);
+            if (m.zeros) z = __byte_perm(*reinterpret_cast<const uint16_t *>(zeros + g), 0, 0x1100);
+        } else {
+            const int g1 = min(after(1), last), g2 = min(after(2), last), g3 = min(after(3), last);
+            s.x = bits(scales[g]) | bits(scales[g1]) << 16;
+            s.y = bits(scales[g2]) | bits(scales[g3]) << 16;
+            if (m.zeros) z = zeros[g] | zeros[g1] << 8 | zeros[g2] << 16 | (uint32_t)zeros[g3] << 24;
+        }
+    }
+    static __device__ __forceinline__ uint32_t bits(V v) { return *reinterpret_cast<const uint16_t *>(&v); }
+    __device__ __forceinline__ uint2 half(int h) const { return make_uint2(h ? s.y : s.x, h ? z >> 16 : z); }
+};
+// how many (1, 2, 4) may be loaded together
+template <typename V>
+int numbers_together(const Matrix<V> &m) {
+    int n = 4;
+    while (n > 1 && (m.n_groups % n != 0 || (uintptr_t)m.scales % (2 * n) != 0 || (uintptr_t)m.zeros % n != 0)) n /= 2;
+    return n;
+}
+
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // From the device's stream-ordered pool, which keeps what is given back to it (as for the library's handles).
