@@ -184,6 +184,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
         int u = 0, count = 0;
         bool ok = true;
+        // This thread's codes in a turn's columns, 32 at a time, with their zero points and groups: asked for a turn ahead
+        // (64 vectors, 16384 x 8192: FIGURE).
+        struct Codes {
+            uint4 c[2];
+            float z[2];
+            int gr[2];
+        } next;
+        auto fetch = [&](const Tile &t, int turn) {
+            const int i = t.line0 + row, from = t.col0 + turn * COLS + group * (COLS / 4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = from + 32 * h;
+                if (!g.d_scales || i >= m.n_rows || k >= t.col_end) continue;
+                next.c[h] = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
+                next.gr[h] = k / m.group;
+                next.z[h] = 8388608.f + zero_of(m, i, next.gr[h]);
+            }
+        };
+        if (blockIdx.x / 2 < tiles) fetch(tile_at(blockIdx.x / 2), 0);
         for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs, ++count) {
             const Tile t = tile_at(at);
             const int i = t.line0 + row;
@@ -196,18 +215,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int turn = 0; turn < t.turns; ++turn, ++u) {
                 const int b = u & 1;
                 const int from = t.col0 + turn * COLS + group * (COLS / 4), to = min(from + COLS / 4, t.col_end);
+                const Codes now = next;
+                if (turn + 1 < t.turns)
+                    fetch(t, turn + 1);
+                else if (at + pairs < tiles)
+                    fetch(tile_at(at + pairs), 0);
                 if (g.d_res) cursor.start(m, i, from);
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(done(b), u / 2 & 1, polls) && !failed))) break;
                 tc_fence_after();
-                for (int k = from; k < to; k += 32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = from + 32 * h;
+                    if (k >= to) break;
                     float v[32];
                     tmem_load32(quarter + b * COLS + (k - t.col0 - turn * COLS), v);
                     if (real && g.d_scales) {
                         // codes behind the last column take part with G = 0
-                        const uint4 c = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
-                        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-                        const int gr = k / m.group;
-                        const float z = 8388608.f + zero_of(m, i, gr);
+                        const uint32_t w[4] = {now.c[h].x, now.c[h].y, now.c[h].z, now.c[h].w};
+                        const int gr = now.gr[h];
+                        const float z = now.z[h];
                         float part = 0.f;
 #pragma unroll
                         for (int j = 0; j < 32; ++j)  // c - z through 2^23 + c, exact
@@ -228,7 +254,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_at(in_block(drained(b), 0));
+                if (lane == 0) mbar_arrive_own_at(in_block(drained(b), 0));
             }
             if (!ok) break;
             __syncwarp();
