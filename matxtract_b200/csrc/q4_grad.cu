@@ -67,6 +67,50 @@ struct Cursor {
     }
 };
 
+// Two 32-bit numbers in one operation.
+__device__ __forceinline__ uint64_t two(uint32_t low, uint32_t high) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(low), "r"(high));
+    return r;
+}
+__device__ __forceinline__ uint64_t two(float low, float high) { return two(__float_as_uint(low), __float_as_uint(high)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float both(uint64_t v) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+    return __uint_as_float(a) + __uint_as_float(b);
+}
+
+// sum of (c - z) v over 32 columns.  A code that begins at bit b of a word becomes the number 2^(23 - b) + c where it
+// stands, from which 2^(23 - b) + z is taken, both exact: nine operations for eight codes, and one for two sums each.
+__device__ __forceinline__ float weighed(const uint4 &codes, float z, const float (&v)[32]) {
+    const float n0 = -8388608.f - z, n1 = -524288.f - z, n2 = -32768.f - z, n3 = -2048.f - z, n4 = -128.f - z;
+    const uint64_t n[4] = {two(n0, n1), two(n2, n3), two(n4, n2), two(n3, n4)};
+    const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint64_t sum[2] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t w = word[j], h = w >> 12;
+        const uint64_t c[4] = {two(pick(w, 0xF, 0x4B000000), pick(w, 0xF0, 0x49000000)),
+                               two(pick(w, 0xF00, 0x47000000), pick(w, 0xF000, 0x45000000)),
+                               two(pick(w, 0xF0000, 0x43000000), pick(h, 0xF00, 0x47000000)),
+                               two(pick(h, 0xF000, 0x45000000), pick(h, 0xF0000, 0x43000000))};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            sum[q % 2] = fma2(add2(c[q], n[q]), two(v[8 * j + 2 * q], v[8 * j + 2 * q + 1]), sum[q % 2]);
+    }
+    return both(add2(sum[0], sum[1]));
+}
+
 template <typename V>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     gradient_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x,
@@ -199,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (!g.d_scales || i >= m.n_rows || k >= t.col_end) continue;
                 next.c[h] = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
                 next.gr[h] = k / m.group;
-                next.z[h] = 8388608.f + zero_of(m, i, next.gr[h]);
+                next.z[h] = (float)zero_of(m, i, next.gr[h]);
             }
         };
         if (blockIdx.x / 2 < tiles) fetch(tile_at(blockIdx.x / 2), 0);
@@ -231,13 +275,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     tmem_load32(quarter + b * COLS + (k - t.col0 - turn * COLS), v);
                     if (real && g.d_scales) {
                         // codes behind the last column take part with G = 0
-                        const uint32_t w[4] = {now.c[h].x, now.c[h].y, now.c[h].z, now.c[h].w};
+                        const float part = weighed(now.c[h], now.z[h], v);
                         const int gr = now.gr[h];
-                        const float z = now.z[h];
-                        float part = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)  // c - z through 2^23 + c, exact
-                            part = fmaf(__uint_as_float(0x4B000000u | (w[j / 8] >> 4 * (j % 8) & 15)) - z, v[j], part);
                         mine[(gr - t.col0 / m.group) * 128] += part;
                     }
                     if (real && g.d_res) {
