@@ -22,11 +22,11 @@ namespace mx {
 namespace q4 {
 namespace {
 
-// Warps: 0 copies, 1 tensor core issue (of block 0), 2 and 3 none; then four groups of four that reduce.
+// Warps: 0 and 2 copies, 1 tensor core issue (of block 0), 3 none; then four groups of four that reduce.
 constexpr int REDUCE = 4, THREADS = 32 * 20;
 constexpr int HALF = 128 * 64 * 2;  // bytes of 128 lines x 64 deep: a block's part of A, and of B
 constexpr int STAGE = 2 * HALF, STAGES = 6, COLS = 256;
-constexpr int SUMS = 4 * 8 * 128;  // parts of the scales' gradients: [group of warps][group of the unit][row]
+constexpr int SUMS = 8 * 128;  // parts of the scales' gradients: [32 columns][row]
 constexpr int BARS = 2 * STAGES + 5;
 constexpr int SMEM = 1024 + STAGES * STAGE + 2 * SUMS * 4 + BARS * 8;
 static_assert(SMEM <= 227 * 1024, "shared memory of one block");
@@ -135,18 +135,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
     // A tile: 256 rows, of which this block has 128, and a unit: the columns of a whole number of groups, in turns of 256.
     struct Tile {
-        int line0, col0, col_end, turns;
+        int band, unit;
     };
-    auto tile_at = [&](int n) {
-        Tile t;
-        const int unit = n / g.tiles_m;
-        t.line0 = n % g.tiles_m * 256 + 128 * (int)rank;
-        t.col0 = unit * g.groups_per_unit * m.group;
-        t.col_end = (int)min((long long)m.n_cols, t.col0 + (long long)g.groups_per_unit * m.group);
-        t.turns = (t.col_end - t.col0 + COLS - 1) / COLS;
-        return t;
-    };
-
+    const int unit_cols = g.groups_per_unit * m.group;
+    auto line0 = [&](Tile t) { return t.band * 256 + 128 * (int)rank; };
+    auto col0 = [&](Tile t) { return t.unit * unit_cols; };
+    auto col_end = [&](Tile t) { return min(m.n_cols - col0(t), unit_cols) + col0(t); };
+    auto turns = [&](Tile t) { return (min(m.n_cols - col0(t), unit_cols) + COLS - 1) / COLS; };
     if (threadIdx.x == 0) {
         failed = 0;
         for (int s = 0; s < STAGES; ++s) {
@@ -161,6 +156,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc_pair(smem_addr(&tmem_shared), 2 * COLS);
+    const Tile first = {(int)(blockIdx.x / 2) % g.tiles_m, (int)(blockIdx.x / 2) / g.tiles_m};
+    const int bands_on = pairs % g.tiles_m, units_on = pairs / g.tiles_m;
+    auto go_on = [&](Tile &t) {  // to the pair's next tile
+        t.band += bands_on;
+        t.unit += units_on;
+        if (t.band >= g.tiles_m) {
+            t.band -= g.tiles_m;
+            ++t.unit;
+        }
+    };
     tc_fence_before();
     __syncthreads();
     cluster_barrier();  // the other block's barriers are there, too
@@ -168,23 +173,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_shared;
 
-    if (warp == 0 && lane == 0) {  // ---- this block's parts of x and dy
+    if ((warp == 0 || warp == 2) && lane == 0) {  // ---- this block's part of dy, or of x
+        // (one thread for both had no time to spare: with its loop a little longer, a step took 550 clocks instead of 500)
+        const bool of_dy = warp == 0;
+        const CUtensorMap *map = of_dy ? &map_dy : &map_x;
+        const uint32_t place = base + (of_dy ? 0 : HALF), bar = in_block(bars, 0);
         int n = 0;
         bool ok = true;
-        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs) {
-            const Tile t = tile_at(at);
-            for (int turn = 0; turn < t.turns && ok; ++turn) {
-                const int col = t.col0 + turn * COLS + 128 * (int)rank;
+        Tile t = first;
+        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs, go_on(t)) {
+            for (int turn = 0; turn < turns(t) && ok; ++turn) {
+                const int line = of_dy ? line0(t) : col0(t) + turn * COLS + 128 * (int)rank;
                 for (int step = 0; step < steps; ++step, ++n) {
                     const int s = n % STAGES;
                     if (!(ok = mbar_wait(empty(s), (n / STAGES & 1) ^ 1, polls))) break;
-                    if (rank == 0) mbar_expect(full(s), 2 * STAGE);
-                    const uint32_t to = base + s * STAGE, bar = in_block(full(s), 0);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        tma_load_pair(to + j * (HALF / 2), &map_dy, t.line0 + 64 * j, step * 64, bar);
-                        tma_load_pair(to + HALF + j * (HALF / 2), &map_x, col + 64 * j, step * 64, bar);
-                    }
+                    if (rank == 0 && of_dy) mbar_expect(full(s), 2 * STAGE);
+                    const uint32_t to = place + s * STAGE;
+                    tma_load_pair(to, map, line, step * 64, bar + 8 * s);
+                    tma_load_pair(to + HALF / 2, map, line + 64, step * 64, bar + 8 * s);
                 }
             }
         }
@@ -195,32 +201,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     } else if (rank == 0 && warp == 1 && elect_one()) {  // ---- tensor cores of both blocks
         constexpr uint32_t idesc = mma_shape(!std::is_same<V, __half>::value, COLS, true, true, 256);
         const uint64_t da0 = operand(base, HALF / 2, 1024), db0 = operand(base + HALF, HALF / 2, 1024);
-        int s = 0, u = 0;
+        int s = 0, all = 0;  // turns of all the pair's tiles
         uint32_t parity = 0;
         bool ok = true;
-        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs) {
-            const Tile t = tile_at(at);
-            for (int turn = 0; turn < t.turns && ok; ++turn, ++u) {
-                const int b = u & 1;
-                if (u >= 2) {
-                    if (!(ok = mbar_wait_cluster(drained(b), (u / 2 - 1) & 1, polls))) break;
-                    tc_fence_after();
-                }
-                for (int step = 0; step < steps; ++step) {
-                    if (!(ok = mbar_wait_cluster(full(s), parity, polls))) break;
-                    tc_fence_after();
-                    const uint64_t da = da0 + (uint32_t)(s * STAGE / 16), db = db0 + (uint32_t)(s * STAGE / 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)  // 16 rows of 128 bytes
-                        tc_mma_pair(tmem + b * COLS, da + 128 * j, db + 128 * j, idesc, step > 0 || j > 0);
-                    tc_commit_pair(empty(s));
-                    if (++s == STAGES) {
-                        s = 0;
-                        parity ^= 1;
-                    }
-                }
-                if (ok) tc_commit_pair(done(b));
+        Tile t = first;
+        for (int at = blockIdx.x / 2; at < tiles; at += pairs, go_on(t)) all += turns(t);
+        for (int u = 0; u < all && ok; ++u) {
+            const int b = u & 1;
+            if (u >= 2) {
+                if (!(ok = mbar_wait_cluster(drained(b), (u / 2 - 1) & 1, polls))) break;
+                tc_fence_after();
             }
+            for (int step = 0; step < steps; ++step) {
+                if (!(ok = mbar_wait_cluster(full(s), parity, polls))) break;
+                tc_fence_after();
+                const uint64_t da = da0 + (uint32_t)(s * STAGE / 16), db = db0 + (uint32_t)(s * STAGE / 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)  // 16 rows of 128 bytes
+                    tc_mma_pair(tmem + b * COLS, da + 128 * j, db + 128 * j, idesc, step > 0 || j > 0);
+                tc_commit_pair(empty(s));
+                if (++s == STAGES) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+            if (ok) tc_commit_pair(done(b));
         }
         if (!ok) failed = 1;
     } else if (warp >= REDUCE) {
@@ -228,57 +233,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
         int u = 0, count = 0;
         bool ok = true;
-        // This thread's codes in a turn's columns, 32 at a time, with their zero points and groups: asked for a turn ahead
-        // (64 vectors, 16384 x 8192: FIGURE).
+        // This thread's codes in a turn's columns, 32 at a time, with their zero points: asked for a turn ahead.
         struct Codes {
             uint4 c[2];
-            float z[2];
-            int gr[2];
+            int z;  // the second one's from bit 4 on
         } next;
-        auto fetch = [&](const Tile &t, int turn) {
-            const int i = t.line0 + row, from = t.col0 + turn * COLS + group * (COLS / 4);
+        // the group of the unit that they belong to: where there are more turns than one, there is only one
+        const int of = g.groups_per_unit > 1 ? 64 * group / m.group | (64 * group + 32) / m.group << 4 : 0;
+        auto fetch = [&](Tile t, int turn) {
+            const int i = line0(t) + row, from = col0(t) + turn * COLS + 64 * group;
+            next.z = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int k = from + 32 * h;
-                if (!g.d_scales || i >= m.n_rows || k >= t.col_end) continue;
+                if (!g.d_scales || i >= m.n_rows || k >= col_end(t)) continue;
                 next.c[h] = *reinterpret_cast<const uint4 *>(m.codes + i * m.code_ld + k / 2);
-                next.gr[h] = k / m.group;
-                next.z[h] = (float)zero_of(m, i, next.gr[h]);
+                next.z |= zero_of(m, i, t.unit * g.groups_per_unit + (of >> 4 * h & 15)) << 4 * h;
             }
         };
-        if (blockIdx.x / 2 < tiles) fetch(tile_at(blockIdx.x / 2), 0);
-        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs, ++count) {
-            const Tile t = tile_at(at);
-            const int i = t.line0 + row;
+        const int parts = min(m.group, COLS) / 32;  // of a group
+        Tile t = first, after = first;
+        if (blockIdx.x / 2 < tiles) fetch(t, 0);
+        for (int at = blockIdx.x / 2; at < tiles && ok; at += pairs, ++count, t = after) {
+            go_on(after);
+            const int i = line0(t) + row;
             const bool real = i < m.n_rows;
-            // this thread's sums, one set for each four warps; the sets change places from tile to tile, so that one may
-            // still be read while the other is filled
-            float *mine = sums + (count & 1) * SUMS + group * 8 * 128 + row;
-            for (int j = 0; j < 8; ++j) mine[j * 128] = 0.f;
+            // the parts change places from tile to tile, so that one may still be read while the other is filled
+            float *part = sums + (count & 1) * SUMS + row, sum[2] = {0.f, 0.f};
             Cursor<V> cursor;
-            for (int turn = 0; turn < t.turns; ++turn, ++u) {
+            for (int turn = 0; turn < turns(t); ++turn, ++u) {
                 const int b = u & 1;
-                const int from = t.col0 + turn * COLS + group * (COLS / 4), to = min(from + COLS / 4, t.col_end);
+                const int from = col0(t) + turn * COLS + 64 * group, to = min(from + 64, col_end(t));
                 const Codes now = next;
-                if (turn + 1 < t.turns)
+                if (turn + 1 < turns(t))
                     fetch(t, turn + 1);
                 else if (at + pairs < tiles)
-                    fetch(tile_at(at + pairs), 0);
+                    fetch(after, 0);
                 if (g.d_res) cursor.start(m, i, from);
-                if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(done(b), u / 2 & 1, polls) && !failed))) break;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(done(b), u / 2 & 1, polls) && !failed))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int k = from + 32 * h;
                     if (k >= to) break;
                     float v[32];
-                    tmem_load32(quarter + b * COLS + (k - t.col0 - turn * COLS), v);
-                    if (real && g.d_scales) {
-                        // codes behind the last column take part with G = 0
-                        const float part = weighed(now.c[h], now.z[h], v);
-                        const int gr = now.gr[h];
-                        mine[(gr - t.col0 / m.group) * 128] += part;
-                    }
+                    tmem_load32(quarter + b * COLS + (k - col0(t) - turn * COLS), v);
+                    // codes behind the last column take part with G = 0
+                    if (real && g.d_scales) sum[h] += weighed(now.c[h], (float)(now.z >> 4 * h & 15), v);
                     if (real && g.d_res) {
                         while (cursor.col[0] < min(k + 32, to)) {
                             const int d = cursor.col[0] - k;
@@ -296,14 +297,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (lane == 0) mbar_arrive_own_at(in_block(drained(b), 0));
             }
             if (!ok) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) part[(2 * group + h) * 128] = sum[h];
             __syncwarp();
             if (lane == 0) mbar_arrive(together);
             if (!(ok = warp_wait(together, count & 1, polls))) break;
-            if (real && g.d_scales && group == 0) {
-                const int g0 = t.col0 / m.group, n = min(g.groups_per_unit, m.n_groups - g0);
-                for (int j = 0; j < n; ++j)
-                    g.d_scales[(long long)i * m.n_groups + g0 + j] =
-                        from_float<V>(mine[j * 128] + mine[(8 + j) * 128] + mine[(16 + j) * 128] + mine[(24 + j) * 128]);
+            if (real && g.d_scales) {
+                const int g0 = t.unit * g.groups_per_unit, n = min(g.groups_per_unit, m.n_groups - g0);
+                for (int j = group; j < n; j += 4) {
+                    float s = 0.f;
+                    for (int p = j * parts; p < (j + 1) * parts; ++p) s += part[p * 128];
+                    g.d_scales[(long long)i * m.n_groups + g0 + j] = from_float<V>(s);
+                }
             }
         }
         if (!ok) failed = 1;
