@@ -26,7 +26,7 @@ namespace {
 constexpr int REDUCE = 4, THREADS = 32 * 20;
 constexpr int HALF = 128 * 64 * 2;  // bytes of 128 lines x 64 deep: a block's part of A, and of B
 constexpr int STAGE = 2 * HALF, STAGES = 6, COLS = 256;
-constexpr int SUMS = 8 * 128;  // parts of the scales' gradients: [32 columns][row]
+constexpr int PART = 136, SUMS = 8 * PART;  // parts of the scales' gradients: [32 columns][row], a little apart
 constexpr int BARS = 2 * STAGES + 5;
 constexpr int SMEM = 1024 + STAGES * STAGE + 2 * SUMS * 4 + BARS * 8;
 static_assert(SMEM <= 227 * 1024, "shared memory of one block");
@@ -259,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const int i = line0(t) + row;
             const bool real = i < m.n_rows;
             // the parts change places from tile to tile, so that one may still be read while the other is filled
-            float *part = sums + (count & 1) * SUMS + row, sum[2] = {0.f, 0.f};
+            float *part = sums + (count & 1) * SUMS, sum[2] = {0.f, 0.f};
             Cursor<V> cursor;
             for (int turn = 0; turn < turns(t); ++turn, ++u) {
                 const int b = u & 1;
@@ -298,15 +298,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
             if (!ok) break;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) part[(2 * group + h) * 128] = sum[h];
+            for (int h = 0; h < 2; ++h) part[(2 * group + h) * PART + row] = sum[h];
             __syncwarp();
             if (lane == 0) mbar_arrive(together);
             if (!(ok = warp_wait(together, count & 1, polls))) break;
-            if (real && g.d_scales) {
-                const int g0 = t.unit * g.groups_per_unit, n = min(g.groups_per_unit, m.n_groups - g0);
-                for (int j = group; j < n; j += 4) {
+            if (g.d_scales) {  // four threads a row
+                const int r = (threadIdx.x - 32 * REDUCE) / 4, i = line0(t) + r;
+                const int g0 = t.unit * g.groups_per_unit, n = i < m.n_rows ? min(g.groups_per_unit, m.n_groups - g0) : 0;
+                for (int j = threadIdx.x % 4; j < n; j += 4) {
                     float s = 0.f;
-                    for (int p = j * parts; p < (j + 1) * parts; ++p) s += part[p * 128];
+                    for (int p = j * parts; p < (j + 1) * parts; ++p) s += part[p * PART + r];
                     g.d_scales[(long long)i * m.n_groups + g0 + j] = from_float<V>(s);
                 }
             }
