@@ -44,11 +44,9 @@ __device__ int wait_ran_out_grad;
 template <typename V>
 struct Cursor {
     int at = 0, end = 0, col[2];
-    V val[2];
     __device__ __forceinline__ void fetch(const Matrix<V> &m, int j) {
         const int p = at + j;
         col[j] = p < end ? m.res_col[p] : 0x7fffffff;
-        val[j] = p < end ? m.res_val[p] : from_float<V>(0.f);
     }
     __device__ __forceinline__ void start(const Matrix<V> &m, int i, int k) {
         at = end = 0;
@@ -62,7 +60,6 @@ struct Cursor {
     __device__ __forceinline__ void next(const Matrix<V> &m) {
         ++at;
         col[0] = col[1];
-        val[0] = val[1];
         fetch(m, 1);
     }
 };
@@ -111,7 +108,7 @@ __device__ __forceinline__ float weighed(const uint4 &codes, float z, const floa
     return both(add2(sum[0], sum[1]));
 }
 
-template <typename V>
+template <typename V, bool RES>  // with the residual's gradient
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     gradient_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ Args<V> g) {
@@ -269,7 +266,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     fetch(t, turn + 1);
                 else if (at + pairs < tiles)
                     fetch(after, 0);
-                if (g.d_res) cursor.start(m, i, from);
+                if (RES) cursor.start(m, i, from);
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(done(b), u / 2 & 1, polls) && !failed))) break;
                 tc_fence_after();
 #pragma unroll
@@ -280,7 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     tmem_load32(quarter + b * COLS + (k - col0(t) - turn * COLS), v);
                     // codes behind the last column take part with G = 0
                     if (real && g.d_scales) sum[h] += weighed(now.c[h], (float)(now.z >> 4 * h & 15), v);
-                    if (real && g.d_res) {
+                    if (RES && real) {
                         while (cursor.col[0] < min(k + 32, to)) {
                             const int d = cursor.col[0] - k;
                             float e = 0.f;
@@ -323,6 +320,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (warp == 1) tmem_free_pair(tmem, 2 * COLS);
 }
 
+template <typename V, bool RES>
+cudaError_t launch(const CUtensorMap &map_dy, const CUtensorMap &map_x, const Args<V> &g, long long tiles, cudaStream_t s) {
+    const cudaError_t e = allow_smem<V, gradient_kernel<V, RES>>(SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_behind(gradient_kernel<V, RES>, 2 * std::min<long long>(tiles, 74), THREADS, SMEM, 0, s, map_dy, map_x, g);
+}
+
 }  // namespace
 
 template <typename V>
@@ -342,9 +346,9 @@ cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x,
     Workspace work(s);
     cudaError_t e = map_vectors(&map_dy, dy, m.n_rows, n_vec, ld_dy, 64, work);
     if (e == cudaSuccess) e = map_vectors(&map_x, x, m.n_cols, n_vec, ld_x, 64, work);
-    if (e == cudaSuccess) e = allow_smem<V, gradient_kernel<V>>(SMEM);
-    if (e != cudaSuccess) return e;
-    return launch_behind(gradient_kernel<V>, 2 * std::min<long long>(tiles, 74), THREADS, SMEM, 0, s, map_dy, map_x, g);
+    return e != cudaSuccess ? e
+           : g.d_res        ? launch<V, true>(map_dy, map_x, g, tiles, s)
+                            : launch<V, false>(map_dy, map_x, g, tiles, s);
 }
 
 cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s) {
