@@ -351,12 +351,15 @@ int mx_csr_spmv_static(int dtype, int n_rows, int n_cols, int nnz, const int *ro
  * (4-bit codes, one scale per `group` consecutive columns of a row) and a CSR residual of the entries that are too
  * large for the codes:
  *     W[i][k] = scales[i][k / group] * (codes[i][k] - zeros[i][k / group]) + R[i][k]
- * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls keep nothing between calls (a
- * workspace comes from the device's stream-ordered pool and goes back to it within the call), are asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured
- * into a graph (mx_q4_check excepted) and leave the calling thread's current device as it was.  Calls on different
- * streams are independent of each other as far as their buffers are.  Results do not depend on anything but the
- * inputs: no sum is taken in an order that varies.  n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do
- * not overlap inputs.
+ * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls keep nothing between calls, are
+ * asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured into a graph
+ * (mx_q4_check excepted) and leave the calling thread's current device as it was.  A workspace comes from the device's
+ * stream-ordered pool and goes back to it within the call: for a product at most three quarters of the codes' bytes and
+ * a copy of vectors that are not on 16-byte borders.  Calls on different streams are independent of each other as far
+ * as their buffers are.  Results do not depend on anything but the inputs: no sum is taken in an order that varies.
+ * n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do not overlap inputs.  A result that a scale, a
+ * residual value or a vector's value enters which is not finite is itself infinite or NaN, not always the one of the
+ * two that the formula gives.
  *
  * codes: row i starts at codes + i * code_ld; two codes a byte, even column in the low half.  The base is 16-byte
  *   aligned, code_ld a multiple of 16 and at least (n_cols + 1) / 2; the buffer has n_rows * code_ld bytes.  What the
@@ -387,8 +390,8 @@ typedef struct {
  * MX_FP16, MX_BF16 or MX_FP32; ld_w elements from row to row).  With a residual, entries with |w| > threshold go there
  * (rounded to dtype) and count as 0 for the codes; without one, threshold is ignored.  Per group, over the entries that
  * stay:  without zeros  s = max|w| / 7, code = 8 + w / s;  with zeros  s = (max(w, 0) - min(w, 0)) / 15,
- * zero = -min(w, 0) / s, code = zero + w / s.  s is taken in 32 bits and rounded to dtype first, the quotients by the rounded s to the
- * nearest whole number, ties to even; codes are clamped to 1..15 (0..15 with zeros).  A group whose s is 0 gets
+ * zero = -min(w, 0) / s, code = zero + w / s.  s is taken in 32 bits and rounded to dtype first, the quotients by the
+ * rounded s to the nearest whole number, ties to even; codes are clamped to 1..15 (0..15 with zeros).  A group whose s is 0 gets
  * codes = zero; one that holds a NaN gets s = NaN, one that holds an infinity s = infinity.
  * res_row_ptr always receives the true counts: where res_row_ptr[n_rows] > res_cap the residual did not fit, and the
  * entries behind res_cap are lost (quantise again with more room).  Buffer parts behind the last entry stay untouched. */
@@ -396,9 +399,11 @@ int mx_q4_quantize(const mx_q4_matrix *m, int w_dtype, const void *w, long long 
 /* w[i][k] = W[i][k], dense row-major in the matrix's dtype, rounded once. */
 int mx_q4_expand(const mx_q4_matrix *m, void *w, long long ld_w, void *stream);
 /* y[t][i] = sum_k W[i][k] x[t][k] for n_vec vectors (rows of x and y, ld_x and ld_y elements apart): what mx_spmv is
- * for a sparse matrix.  Sums in 32 bits, rounded once at the end. */
+ * for a sparse matrix.  Sums in 32 bits, rounded once at the end; for more than 8 vectors W[i][k] is rounded to dtype
+ * before it is multiplied (and is infinite where it leaves dtype's range, as in mx_q4_expand). */
 int mx_q4_product(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, void *y, long long ld_y, void *stream);
-/* dx[t][k] = sum_i W[i][k] dy[t][i]: the product with the transposed matrix, which is also the gradient of x. */
+/* dx[t][k] = sum_i W[i][k] dy[t][i]: the product with the transposed matrix, which is also the gradient of x.  W[i][k]
+ * is rounded to dtype before it is multiplied, for any number of vectors. */
 int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long ld_dy, void *dx, long long ld_dx,
                     void *stream);
 /* Gradients of the matrix's own numbers, G[i][k] = sum_t dy[t][i] x[t][k] (never stored):
@@ -408,9 +413,8 @@ int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long 
 int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, const void *dy, long long ld_dy,
                void *d_scales, void *d_res_val, void *stream);
 /* Checks the residual once, on the device: res_row_ptr starts at 0, never decreases and ends inside res_cap, columns lie
- * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  MX_ERR_TIMEOUT when a bounded
- * wait inside an earlier mx_q4_* kernel on this GPU ran out (its results are then not complete).  Synchronises the
- * stream. */
+ * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  MX_ERR_TIMEOUT when a bounded wait inside an
+ * earlier mx_q4_* kernel on this GPU ran out (its results are then not complete).  Synchronises the stream. */
 int mx_q4_check(const mx_q4_matrix *m, void *stream);
 
 #ifdef __cplusplus

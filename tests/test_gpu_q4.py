@@ -419,6 +419,111 @@ def test_they_work_together():
     check_grad(m, t, 0, x, dy)
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("group", [32, 64, 96])
+@pytest.mark.parametrize("k", [128, 416, 448, 480, 512])
+def test_numbers_on_any_border(k, group, shift):
+    """Rows of scales and zero points of any length, from an address of any alignment."""
+    n, groups = 150, -(-k // group)
+    m = make(n, k, group, torch.float16, True, 0.01, k)
+    for name in ("scales", "zeros"):
+        room = torch.empty(n * groups + shift, dtype=m[name].dtype, device="cuda")
+        moved = room[shift:].view(n, groups)
+        moved.copy_(m[name])
+        m[name] = moved
+    for t in (1, 8, 12, 40, 130):
+        check_product(m, t, 1)
+        check_product_t(m, t, 2)
+        check_grad(m, t, 3)
+
+
+def test_calls_behind_one_another():
+    """Calls that start while the one in front still runs see what it writes: vectors and workspaces of each are made anew."""
+    n, k = 517, 1037  # rows on no 16-byte border: every call copies its vectors first
+    m = make(n, k, 64, torch.bfloat16, True, 0.01, 23)
+    q = matrix(m)
+    for t in (3, 30, 300):
+        x0 = normal(1, t, k, dtype=torch.bfloat16, scale=0.1)
+
+        def chain(pause):
+            x, seen = x0.clone(), []
+            for _ in range(6):
+                y, ds = torch.empty(t, n, dtype=torch.bfloat16, device="cuda"), torch.empty_like(m["scales"])
+                dv = torch.zeros_like(m["residual"][2])
+                for call in (lambda: q.product(x, y), lambda: q.grad(x, y, ds, dv), lambda: q.product_t(y, x)):
+                    call()
+                    if pause:
+                        torch.cuda.synchronize()
+                x = x / x.float().abs().max().to(torch.bfloat16)
+                seen += [y, ds, dv, x]
+            torch.cuda.synchronize()
+            return seen
+
+        for a, b in zip(chain(True), chain(False)):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_changed_numbers_count():
+    """Nothing of a matrix is kept from one call for the next."""
+    m = make(300, 640, 32, torch.float16, True, 0.02, 24)
+    q = matrix(m)
+    for t in (2, 40, 1100):
+        x, y = normal(t, t, 640, dtype=torch.float16), torch.empty(t, 300, dtype=torch.float16, device="cuda")
+        q.product(x, y)
+        m["scales"].mul_(2)
+        m["codes"].copy_(m["codes"].flip(0))
+        m["residual"][2].mul_(-1)
+        check_product(m, t, t, x, y)
+        check_product_t(m, t, t)
+        check_grad(m, t, t)
+
+
+def test_codes_of_more_than_two_gigabytes():
+    """The last rows of a matrix whose codes and values lie further off than 32 bits count."""
+    n, k, last, dtype = 70000, 65536, 96, torch.bfloat16
+    m = make(1, 64, 128, dtype, True, None, 25)
+    codes = torch.randint(0, 2 ** 31 - 1, (n, k // 8), dtype=torch.int32, device="cuda").view(torch.uint8)
+    scales = torch.rand(n, k // 128, device="cuda").add_(0.01).to(dtype)
+    zeros = torch.randint(0, 16, (n, k // 128), dtype=torch.uint8, device="cuda")
+    ptr = torch.arange(0, 2 * n + 2, 2, dtype=torch.int32, device="cuda")
+    col = torch.randint(0, k // 2, (n, 2), dtype=torch.int32, device="cuda")
+    col[:, 1] += k // 2
+    val = normal(26, 2 * n, dtype=dtype)
+    m.update(n=n, k=k, codes=codes, scales=scales, zeros=zeros, residual=(ptr, col.view(-1), val))
+    end = dict(m, n=last, codes=codes[-last:], scales=scales[-last:], zeros=zeros[-last:],
+               residual=(ptr[: last + 1], col.view(-1)[-2 * last:], val[-2 * last:]))
+    q, w = matrix(m), dense64(end)
+    for t in (2, 40, 300):
+        x, y = normal(t, t, k, dtype=dtype), torch.empty(t, n, dtype=dtype, device="cuda")
+        q.product(x, y)
+        xd = x.double()
+        close(y[:, -last:], xd @ w.T, rounded(xd @ w.T, xd.abs() @ w.abs().T, k, dtype, 2))
+        dy, dx = torch.zeros_like(y), torch.empty_like(x)
+        dy[:, -last:] = normal(t + 1, t, last, dtype=dtype)
+        q.product_t(dy, dx)
+        dd = dy[:, -last:].double()
+        close(dx, dd @ w, rounded(dd @ w, dd.abs() @ w.abs(), n, dtype, 2))
+        ds, dv = torch.empty_like(scales), torch.empty_like(val)
+        q.grad(x, dy, ds, dv)
+        steps, _ = steps64(end)
+        g, size = dd.T @ xd, dd.abs().T @ xd.abs()
+        sums = lambda a: a.view(last, -1, 128).sum(2)  # noqa: E731
+        close(ds[-last:], sums(g * steps), rounded(sums(g * steps), sums(size * steps.abs()), t + 128, dtype, 0))
+        row, at, _ = entries(end)
+        close(dv[-2 * last:], g[row, at], rounded(g[row, at], size[row, at], t, dtype, 0))
+    del x, y, dy, dx, ds, dv
+    dense = torch.empty(n, k, dtype=dtype, device="cuda")
+    q.expand(dense)
+    close(dense[-last:], w, w.abs() * U[dtype] * 1.01 + TINY[dtype])
+    codes.zero_()
+    val.zero_()
+    q.quantize(dense, threshold=1e30)
+    assert int(ptr[-1]) == 0
+    # a group reaches over 15 of its old steps at most, so the new step is no larger; half a step is the code's rounding,
+    # half the zero point's, and the step's own rounding makes 15 x 2^-8 of one
+    close(dense[-last:], dense64(dict(end, residual=None)), 1.07 * scales[-last:].double().repeat_interleave(128, 1))
+
+
 def test_captured_and_replayed():
     m = make(200, 384, 128, torch.float16, True, 0.02, 21)
     q = matrix(m)
