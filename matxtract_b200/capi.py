@@ -647,56 +647,64 @@ class Q4Matrix:
                             a(scales), a(zeros), a(res_row_ptr), a(res_col_ind), a(res_val))
         self._r = C.byref(self._m)
 
+    # What is wrong is put into words only when something is: these run in front of every call.
     def _tensor(self, a, name, dtype, shape):
-        _need(str(a.dtype) == str(dtype), f"{name} has type {a.dtype}, not {dtype}")
-        _need(a.device == self.device and a.is_cuda, f"{name} is on {a.device}, the scales on {self.device}")
-        if shape is not None:
-            _need(tuple(a.shape) == shape and a.is_contiguous(), f"{name}: a contiguous {shape} tensor is wanted")
+        if a.dtype is not dtype and str(a.dtype) != str(dtype):
+            _need(False, f"{name} has type {a.dtype}, not {dtype}")
+        if a.device != self.device or not a.is_cuda:
+            _need(False, f"{name} is on {a.device}, the scales on {self.device}")
+        if shape is not None and (a.shape != shape or not a.is_contiguous()):
+            _need(False, f"{name}: a contiguous {tuple(shape)} tensor is wanted")
 
     def _rows(self, a, name, cols, dtype=None):
-        """Leading dimension of a row-major [n, cols] tensor of the matrix's type."""
-        _need(a.dim() == 2 and a.shape[1] == cols, f"{name}: [n, {cols}] is wanted, not {tuple(a.shape)}")
-        _need(a.dtype == (dtype or self.vdt) and a.device == self.device, f"{name}: another type or GPU than the matrix")
-        ld = a.stride(0) if a.shape[0] > 1 else max(cols, 1)
-        _need((cols <= 1 or a.stride(1) == 1) and ld >= cols, f"{name}: the entries of a row are adjacent, rows apart")
-        return ld
+        """Rows and leading dimension of a row-major [n, cols] tensor of the matrix's type."""
+        shape = a.shape
+        if len(shape) != 2 or shape[1] != cols:
+            _need(False, f"{name}: [n, {cols}] is wanted, not {tuple(shape)}")
+        if a.dtype is not (dtype or self.vdt) or a.device != self.device:
+            _need(False, f"{name}: another type or GPU than the matrix")
+        rows, (apart, step) = shape[0], a.stride()
+        ld = apart if rows > 1 else max(cols, 1)
+        if (cols > 1 and step != 1) or ld < cols:
+            _need(False, f"{name}: the entries of a row are adjacent, rows apart")
+        return rows, ld
 
     def quantize(self, w, threshold=None, stream=0):
         """Fills codes, scales, zeros and residual from the dense w [n_rows, n_cols] (float16, bfloat16 or float32);
         with a residual, entries above ``threshold`` in magnitude go there."""
         _need(self.res_row_ptr is None or threshold is not None, "a matrix with a residual wants a threshold")
         _need(str(w.dtype) in self._TYPES and w.shape[0] == self.n_rows, "w: [n_rows, n_cols] of a floating type")
-        ld = self._rows(w, "w", self.n_cols, w.dtype)
+        _, ld = self._rows(w, "w", self.n_cols, w.dtype)
         _raise(lib().mx_q4_quantize(self._r, self._TYPES[str(w.dtype)], w.data_ptr(), ld, threshold or 0.0, stream))
 
     def expand(self, w, stream=0):
         """w [n_rows, n_cols] = the dense matrix."""
-        ld = self._rows(w, "w", self.n_cols)
-        _need(w.shape[0] == self.n_rows, "w: [n_rows, n_cols]")
+        rows, ld = self._rows(w, "w", self.n_cols)
+        _need(rows == self.n_rows, "w: [n_rows, n_cols]")
         _raise(lib().mx_q4_expand(self._r, w.data_ptr(), ld, stream))
 
     def product(self, x, y, stream=0):
         """y [n, n_rows] = x [n, n_cols] times the transposed matrix: one product per row of x."""
-        ld_x, ld_y = self._rows(x, "x", self.n_cols), self._rows(y, "y", self.n_rows)
-        _need(x.shape[0] == y.shape[0], "x and y: as many rows")
-        _raise(lib().mx_q4_product(self._r, x.shape[0], x.data_ptr(), ld_x, y.data_ptr(), ld_y, stream))
+        (n, ld_x), (n_y, ld_y) = self._rows(x, "x", self.n_cols), self._rows(y, "y", self.n_rows)
+        _need(n == n_y, "x and y: as many rows")
+        _raise(lib().mx_q4_product(self._r, n, x.data_ptr(), ld_x, y.data_ptr(), ld_y, stream))
 
     def product_t(self, dy, dx, stream=0):
         """dx [n, n_cols] = dy [n, n_rows] times the matrix: the gradient of ``product``'s x."""
-        ld_dy, ld_dx = self._rows(dy, "dy", self.n_rows), self._rows(dx, "dx", self.n_cols)
-        _need(dx.shape[0] == dy.shape[0], "dy and dx: as many rows")
-        _raise(lib().mx_q4_product_t(self._r, dy.shape[0], dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, stream))
+        (n, ld_dy), (n_dx, ld_dx) = self._rows(dy, "dy", self.n_rows), self._rows(dx, "dx", self.n_cols)
+        _need(n == n_dx, "dy and dx: as many rows")
+        _raise(lib().mx_q4_product_t(self._r, n, dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, stream))
 
     def grad(self, x, dy, d_scales=None, d_res_val=None, stream=0):
         """Gradients of the scales and of the residual's values for ``product``'s x and the gradient dy of its y."""
-        ld_x, ld_dy = self._rows(x, "x", self.n_cols), self._rows(dy, "dy", self.n_rows)
-        _need(x.shape[0] == dy.shape[0], "x and dy: as many rows")
+        (n, ld_x), (n_dy, ld_dy) = self._rows(x, "x", self.n_cols), self._rows(dy, "dy", self.n_rows)
+        _need(n == n_dy, "x and dy: as many rows")
         if d_scales is not None:
-            self._tensor(d_scales, "d_scales", self.vdt, tuple(self.scales.shape))
+            self._tensor(d_scales, "d_scales", self.vdt, self.scales.shape)
         if d_res_val is not None:
             _need(self.res_val is not None, "d_res_val: the matrix has no residual")
-            self._tensor(d_res_val, "d_res_val", self.vdt, tuple(self.res_val.shape))
-        _raise(lib().mx_q4_grad(self._r, x.shape[0], x.data_ptr(), ld_x, dy.data_ptr(), ld_dy, _address(d_scales),
+            self._tensor(d_res_val, "d_res_val", self.vdt, self.res_val.shape)
+        _raise(lib().mx_q4_grad(self._r, n, x.data_ptr(), ld_x, dy.data_ptr(), ld_dy, _address(d_scales),
                                 _address(d_res_val), stream))
 
     def check(self, stream=0):
