@@ -109,7 +109,8 @@ __device__ __forceinline__ void turned_values(float (&x)[8 * NT], const V *at) {
 //             without having seen its last phase, which a wait for a parity cannot tell from the wanted one.
 // What bounds it is the ALU pipe, which takes the codes apart (7 operations for 8 codes and as many again for all the
 // rest): tiles fetched by the converting warps themselves, 16 rows a warp, cost 470 instructions for 2048 codes and
-// 44 us for 16384 x 8192 and one vector.
+// 44 us for 16384 x 8192 and one vector.  This form takes 25.8 us (the codes at 2.6 TB/s), 8 vectors 26.8, with a residual
+// of 0.5 % of the entries 30 and 37; the gradients for one vector 25.4, for 16 vectors 34.
 constexpr int STREAM_THREADS = 32 * 12, DEPTH = 8;
 constexpr int CODE_BYTES = 128 * 64;
 template <int NT>
@@ -497,9 +498,11 @@ __global__ void turn_kernel(const V *x, long long ld, int n_vec, int n_cols, int
     }
 }
 
-// dx = dy W for up to 8 vectors and no residual.  A block has 256 columns, its warps take 16 rows at a time; the contraction runs over
-// rows, whose scales differ, so the values are s (c - z), rounded once to the type.  The blocks of a cluster share the
-// rows.  A lane holds 32 columns of four rows; two rows' codes of a column are brought into one register.
+// dx = dy W for up to 8 vectors, no residual and matrices of up to 2^22 entries (product_t says why).  A block has 256
+// columns, its warps take 16 rows at a time; the contraction runs over rows, whose scales differ, so the values are
+// s (c - z), rounded once to the type.  The blocks of a cluster share the rows.  A lane holds 32 columns of four rows; two
+// rows' codes of a column are brought into one register.  2048 x 2048, 8 vectors: 7.0 us, most of it the time of the
+// launch, of loads that wait for one another and of adding up the warps' parts.
 constexpr int COLS = 256, VEC = 8, VEC_STRIDE = 268, WARP_PART = VEC * VEC_STRIDE;
 constexpr int T_DEPTH = 4, T_SLOT = 2048 + 256;  // steps of a warp under way; bytes of one: codes, dy
 constexpr int T_SMEM = WARPS * (T_DEPTH * T_SLOT > 4 * WARP_PART ? T_DEPTH * T_SLOT : 4 * WARP_PART);
@@ -730,7 +733,7 @@ template <typename V>
 cudaError_t product_t(const Matrix<V> &m, int n_vec, const V *dy, long long ld_dy, V *dx, long long ld_dx,
                       cudaStream_t s) {
     // The residual's entries meet in columns: where there are some, the tiles that they are put into are faster even for
-    // one vector (4096 x 4096: 19 us there, 28 us with a search and ordered additions here).  Those also take the larger
+    // one vector (4096 x 4096: 15 us there, 28 us with a search and ordered additions here).  Those also take the larger
     // matrices (8 vectors, 2048 x 2048: 7.0 us here, 8.0 there; 4096 x 4096: 13.7 and 10.4, with groups of 32 and zero
     // points 15.5 and 11.3), which few clusters of eight do not spread over the GPU.
     if (n_vec > VEC || m.res_ptr || (long long)m.n_rows * m.n_cols > 1 << 22) return product_t_many(m, n_vec, dy, ld_dy, dx, ld_dx, s);

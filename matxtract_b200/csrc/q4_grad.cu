@@ -7,6 +7,11 @@
 // rows x 256 columns of it: each brings its 128 rows' dy and half of the columns' x into its shared memory, so that a
 // step's operands cross the L2 and the shared memories half as often as with a block on its own.  The pairs go on from
 // tile to tile, and the tensor memory holds two, so that one is reduced while the next is computed.
+//
+// Measured, bfloat16: 8192 x 8192, 2048 vectors 170 to 182 us with and without a residual (1.5 to 1.6 PFLOP/s: the tensor
+// cores and the L2 that feeds them bound it); 16384 x 8192, 64 vectors 65 us (the reduction of 256 x 256 numbers a tile
+// bounds it), with a residual of 0.5 % of the entries 165: a search for the place of its entries in every row and tile.
+// Searched for in front, by a kernel of its own, that was 144, but 2 to 3 us more for everything smaller.
 #include <limits.h>
 
 #include <algorithm>
