@@ -206,29 +206,43 @@ struct Eight {
 // number when it starts (so that all in front of it have started, too), tells how many entries it has as soon as it has
 // its values, works on its codes, and then walks back over the blocks in front: it adds up what they have until it meets
 // one that knows its end.  W is read once; a counting pass in front took 31 us of 8192 x 8192 (2 bytes).
-// A block's word: entries << 2 | 1 (its own) or 2 (with all in front).
+// A block's word: entries << 2 | 1 (its own) or 2 (with all in front); it is all that is told, so that it orders nothing else.
 __device__ __forceinline__ void tell(unsigned long long *word, long long n, int kind) {
-    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(word), "l"((unsigned long long)n << 2 | kind) : "memory");
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(word), "l"((unsigned long long)n << 2 | kind) : "memory");
 }
 __device__ int wait_ran_out_quant;
-// entries in front of block `me`, for one warp; -1 when a block in front does not tell in time
+// Entries in front of block `me`, for one warp; -1 when a block in front does not tell in time.  Blocks that run together
+// come here together, hundreds of them, before any of them knows its end: 128 words are looked at at a time.
 __device__ __forceinline__ long long entries_before(const unsigned long long *words, long long me) {
+    constexpr int WORDS = 4;
     const int lane = threadIdx.x % 32;
     long long n = 0;
-    for (long long end = me; end > 0; end -= 32) {  // lanes: the 32 blocks in front of `end`, the nearest first
-        const long long b = end - 1 - lane;
-        unsigned long long w = 2;  // in front of the first block: nothing, and that is all
-        if (b >= 0) {
-            w = 0;
-            for (unsigned polls = 0; polls < 1u << 22 && w == 0; ++polls)
-                asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(w) : "l"(words + b) : "memory");
+    for (long long end = me; end > 0; end -= 32 * WORDS) {  // the blocks in front of `end`, the nearest first
+        unsigned long long w[WORDS];
+        bool all = false;
+        for (unsigned polls = 0; polls < 1u << 22 && !all; ++polls) {
+            all = true;
+#pragma unroll
+            for (int u = 0; u < WORDS; ++u) {
+                const long long b = end - 1 - lane - 32 * u;
+                w[u] = 2;  // in front of the first block: nothing, and that is all
+                if (b >= 0) asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(w[u]) : "l"(words + b) : "memory");
+                all &= w[u] != 0;
+            }
         }
-        if (__any_sync(0xffffffffu, w == 0)) return -1;
-        const unsigned whole = __ballot_sync(0xffffffffu, (w & 3) == 2);
-        long long mine = whole && lane > __ffs(whole) - 1 ? 0 : (long long)(w >> 2);
+        if (!__all_sync(0xffffffffu, all)) return -1;
+        bool found = false;
+        long long mine = 0;
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u) {
+            if (found) break;
+            const unsigned whole = __ballot_sync(0xffffffffu, (w[u] & 3) == 2);
+            mine += whole && lane > __ffs(whole) - 1 ? 0 : (long long)(w[u] >> 2);
+            found = whole != 0;
+        }
         for (int d = 16; d; d /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, d);
         n += mine;
-        if (whole) break;
+        if (found) break;
     }
     return n;
 }
