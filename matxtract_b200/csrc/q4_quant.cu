@@ -119,12 +119,6 @@ struct Eight<float> {
         __device__ __forceinline__ float high() const { return hi; }
         __device__ __forceinline__ bool is_nan() const { return nan; }
     };
-    __device__ __forceinline__ float at(int j) const {  // no indexing: the values stay in registers
-        float r = v[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) r = i == j ? v[i] : r;
-        return r;
-    }
     __device__ __forceinline__ void all(float (&f)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = v[j];
@@ -187,11 +181,6 @@ struct Eight {
             return a != a || b != b || c != c;
         }
     };
-    __device__ __forceinline__ float at(int j) const {
-        const uint32_t w = j < 4 ? j < 2 ? u[0] : u[1] : j < 6 ? u[2] : u[3];
-        const uint16_t b = (uint16_t)(w >> 16 * (j & 1));
-        return to_float(*reinterpret_cast<const W *>(&b));
-    }
     __device__ __forceinline__ void all(float (&f)[8]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -212,9 +201,9 @@ __device__ __forceinline__ void tell(unsigned long long *word, long long n, int 
 }
 __device__ int wait_ran_out_quant;
 // Entries in front of block `me`, for one warp; -1 when a block in front does not tell in time.  Blocks that run together
-// come here together, hundreds of them, before any of them knows its end: 128 words are looked at at a time.
+// come here together, hundreds of them, before any of them knows its end: 64 words are looked at at a time.
 __device__ __forceinline__ long long entries_before(const unsigned long long *words, long long me) {
-    constexpr int WORDS = 4;
+    constexpr int WORDS = 2;
     const int lane = threadIdx.x % 32;
     long long n = 0;
     for (long long end = me; end > 0; end -= 32 * WORDS) {  // the blocks in front of `end`, the nearest first
@@ -341,8 +330,8 @@ template <typename V, typename W, bool ZEROS, int SPAN>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(W) == 2 ? 4 : 2)
     quantize_kernel(const Out<V> o, const W *w, long long ld, bool wide, float threshold) {
     __shared__ Places places;
-    constexpr int KEPT = 256;  // entries of a piece that wait for their place here, column of the piece << 16 | value
-    __shared__ uint32_t kept[WARPS][KEPT];
+    constexpr int KEPT = 256;  // entries of a piece whose columns wait for their place here
+    __shared__ uint16_t kept[WARPS][KEPT];
     const bool split = o.res_ptr != nullptr;
     const int lane = threadIdx.x % 32;
     const long long pieces = (long long)o.n_rows * o.per_row;
@@ -371,9 +360,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(W) == 2 ? 4 : 2)
                                (k + 16 <= o.n_cols ? 0xffffu : (1u << max(o.n_cols - k, 0)) - 1);
             far[c / 2] |= f << 16 * (c % 2);
             in_order(f, at, [&](long long e, int j) {
-                const V x = from_float<V>(j < 8 ? v[c][0].at(j) : v[c][1].at(j - 8));
-                if (e < KEPT)
-                    kept[threadIdx.x / 32][e] = (uint32_t)(c * CHUNK + 16 * lane + j) << 16 | *reinterpret_cast<const uint16_t *>(&x);
+                if (e < KEPT) kept[threadIdx.x / 32][e] = (uint16_t)(c * CHUNK + 16 * lane + j);
             });
             v[c][0].drop(limit);
             v[c][1].drop(limit);
@@ -442,6 +429,12 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(W) == 2 ? 4 : 2)
         }
     }
     if (!split) return;
+    // their values are read once more (which takes fewer operations than picking them out of registers), the first ones
+    // while the places become known
+    __syncwarp();
+    const uint16_t *columns = kept[threadIdx.x / 32];
+    V first = from_float<V>(0.f);
+    if (lane < mine) first = from_float<V>(to_float(from[start + columns[lane]]));
     long long at = places.mine(o.words);
     if (at < 0) return;  // the whole block
     if (real && lane == 0) {
@@ -451,10 +444,9 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(W) == 2 ? 4 : 2)
     if (mine <= KEPT) {
         for (int i = lane; i < mine; i += 32)
             if (at + i < o.res_cap) {
-                const uint32_t e = kept[threadIdx.x / 32][i];
-                const uint16_t x = (uint16_t)e;
-                o.res_col[at + i] = start + (e >> 16);
-                o.res_val[at + i] = *reinterpret_cast<const V *>(&x);
+                const int k = start + columns[i];
+                o.res_col[at + i] = k;
+                o.res_val[at + i] = i < 32 ? first : from_float<V>(to_float(from[k]));
             }
     } else {  // more than were kept: their values are read again
 #pragma unroll
