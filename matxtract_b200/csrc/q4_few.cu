@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                             for (int k = 0; k < 4; ++k) total[h][q][k] = fmaf(s[2 * h + k / 2], e[h][q][k], total[h][q][k]);
                 }
             }
+            // the products have used every value from the slot: nothing that a copy could overtake is under way
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(slot));
             if (GRAD && complete) {
