@@ -157,11 +157,15 @@ inline cudaError_t pool_memory(void **p, size_t bytes, cudaStream_t s) {
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
     if (device >= 64 || !(kept.load() >> device & 1)) {
+        // a process's first call may be one that is captured: this is no part of the graph, and a strict capture would end
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return e;
         cudaMemPool_t pool;
         uint64_t all = UINT64_MAX;
-        if ((e = cudaDeviceGetDefaultMemPool(&pool, device)) != cudaSuccess ||
-            (e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all)) != cudaSuccess)
-            return e;
+        e = cudaDeviceGetDefaultMemPool(&pool, device);
+        if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &all);
+        const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess || back != cudaSuccess) return e != cudaSuccess ? e : back;
         if (device < 64) kept.fetch_or(1ull << device);
     }
     return cudaMallocAsync(p, bytes, s);

@@ -552,6 +552,96 @@ def test_captured_and_replayed():
         check_product(m, t, 0, x)
 
 
+@pytest.mark.parametrize("t", [0, 1, 12, 40, 300])
+def test_either_gradient_alone(t):
+    m = make(300, 640, 96, torch.float16, True, 0.02, 28)
+    x, dy, ds, dv = check_grad(m, t, 1) if t else (torch.empty(0, 640, dtype=torch.float16, device="cuda"),
+                                                   torch.empty(0, 300, dtype=torch.float16, device="cuda"),
+                                                   torch.zeros_like(m["scales"]), None)
+    if t == 0:
+        dv = torch.full_like(m["residual"][2], 7.0)
+        dv[: int(m["residual"][0][-1])] = 0
+    alone, other = torch.full_like(ds, math.nan), torch.full_like(dv, 7.0)
+    matrix(m).grad(x, dy, alone)
+    matrix(m).grad(x, dy, None, other)
+    assert torch.equal(alone, ds) and torch.equal(other, dv)
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = [{tests!r}, {root!r}]
+import torch
+from q4_cases import make, matrix
+m = make(200, 384, 128, torch.float16, True, 0.02, 21)
+q, op, t = matrix(m), {op!r}, {t}
+x, dy = (torch.randn(t, c, device="cuda").half() for c in (384, 200))
+w, ds, dv = torch.randn(200, 384, device="cuda"), torch.empty_like(m["scales"]), torch.empty_like(m["residual"][2])
+calls = dict(product=lambda s: q.product(x, dy, stream=s), product_t=lambda s: q.product_t(dy, x, stream=s),
+             grad=lambda s: q.grad(x, dy, ds, dv, stream=s), quantize=lambda s: q.quantize(w, 2.5, stream=s))
+outputs = dict(product=dy, product_t=x, grad=ds, quantize=m["scales"])
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls[op](torch.cuda.current_stream().cuda_stream)
+outputs[op].zero_()
+graph.replay()
+torch.cuda.synchronize()
+seen = outputs[op].clone()
+calls[op](0)
+torch.cuda.synchronize()
+assert torch.equal(seen, outputs[op]) and seen.abs().max() > 0
+"""
+
+
+@pytest.mark.parametrize("op,t", [("product", 1), ("product", 40), ("product_t", 3), ("grad", 4), ("grad", 40), ("quantize", 1)])
+def test_a_process_first_call_may_be_captured(op, t):
+    import os
+    import subprocess
+    import sys
+
+    tests = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.format(tests=tests, root=os.path.dirname(tests), op=op, t=t)],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_two_graphs_at_once():
+    """Graphs of calls that need workspaces (vectors on no 16-byte border, a residual), replayed on two streams together."""
+    n, k = 517, 1037
+    m = make(n, k, 64, torch.bfloat16, True, 0.01, 27)
+    q, graphs = matrix(m), []
+    for t in (3, 21, 300):
+        x, dy = normal(t, t, k, dtype=torch.bfloat16), normal(t + 1, t, n, dtype=torch.bfloat16)
+        out = [torch.empty(t, n, dtype=torch.bfloat16, device="cuda"), torch.empty_like(x), torch.empty_like(m["scales"]),
+               torch.zeros_like(m["residual"][2])]
+
+        def run(stream, x=x, dy=dy, out=out):
+            q.product(x, out[0], stream=stream)
+            q.product_t(dy, out[1], stream=stream)
+            q.grad(x, dy, out[2], out[3], stream=stream)
+
+        run(0)
+        torch.cuda.synchronize()
+        want = [o.clone() for o in out]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(torch.cuda.current_stream().cuda_stream)
+        graphs.append((graph, torch.cuda.Stream(), out, want, x, dy))  # which the graph reads
+    for _ in range(10):
+        for _, _, out, *_ in graphs:
+            for o in out:
+                o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream, *_ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, out, want, *_ in graphs:
+            for o, w in zip(out, want):
+                assert torch.equal(o.view(torch.int16), w.view(torch.int16))
+
+
 def test_streams_do_not_disturb_each_other():
     m = make(500, 1024, 64, torch.bfloat16, True, 0.01, 22)
     q = matrix(m)
