@@ -354,9 +354,9 @@ int mx_csr_spmv_static(int dtype, int n_rows, int n_cols, int nnz, const int *ro
  * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls keep nothing between calls, are
  * asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured into a graph
  * (mx_q4_check excepted) and leave the calling thread's current device as it was.  A workspace comes from the device's
- * stream-ordered pool and goes back to it within the call: for a product at most three quarters of the codes' bytes and
- * a copy of vectors that are not on 16-byte borders.  Calls on different streams are independent of each other as far
- * as their buffers are.  Results do not depend on anything but the inputs: no sum is taken in an order that varies.
+ * stream-ordered pool and goes back to it within the call: for a product at most three quarters of the codes' bytes
+ * (rows and columns filled up to 128s) and a copy of the vectors.  Calls on different streams are independent of each
+ * other as far as their buffers are.  Results do not depend on anything but the inputs: no sum is taken in an order that varies.
  * n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do not overlap inputs.  A result that a scale, a
  * residual value or a vector's value enters which is not finite is itself infinite or NaN, not always the one of the
  * two that the formula gives.
