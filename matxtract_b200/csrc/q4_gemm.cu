@@ -78,9 +78,26 @@ __device__ int wait_ran_out;  // set when a bounded wait ended without its barri
 
 // 64 values of a row in the operand's layout, with the residual's entries among them: `a` is the row's 128 bytes in a
 // stage, whose sixteens are in an order that goes by the row.  numbers: two scales, and two zero points in a byte each.
+// Columns behind the last become 0 before the rounding: what their bytes and scale make may be infinite, and infinity times
+// the 0 that stands in the vectors there is no 0.
 template <typename V>
-__device__ __forceinline__ void convert_row(uint8_t *a, int out_row, const uint4 (&c)[2], uint2 numbers, bool slots,
+__device__ __forceinline__ void convert_row(uint8_t *a, int out_row, uint4 (&c)[2], uint2 numbers, bool slots,
                                             const uint4 &entries, const Matrix<V> &m, int row, int col) {
+    if (col + 64 > m.n_cols) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int left = m.n_cols - col - 32 * j;  // columns of these 32 that there are
+            if (left <= 0) numbers.x &= ~(0xffffu << 16 * j);
+            const uint32_t zeros = 0x11111111u * (numbers.y >> 8 * j & 15);
+            uint32_t *w[4] = {&c[j].x, &c[j].y, &c[j].z, &c[j].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = left - 8 * q;
+                const uint32_t there = n >= 8 ? 0xffffffffu : n > 0 ? (1u << 4 * n) - 1 : 0;
+                *w[q] = (*w[q] & there) | (zeros & ~there);
+            }
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const typename Pair<V>::T s = Pair<V>::both(from_bits<V>(numbers.x >> 16 * j));
