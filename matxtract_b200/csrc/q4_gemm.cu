@@ -4,8 +4,9 @@
 //   product    D[i][t] = sum_k W[i][k] x[t][k]     A = W's rows, depth-major      B = x's rows, depth-major
 //   transposed D[k][t] = sum_i W[i][k] dy[t][i]    A = W's columns, line-major    B = dy's rows, depth-major
 // x and dy come through tiled bulk copies.  W is made on the way: its codes come through a ring of their own (128 rows x
-// 128 columns = 8 KB each) and four groups of four warps turn them into 16-bit values s * (c - z), rounded once, add the
-// residual's entries that fall into the tile, and store them in the operand's swizzled layout; in this form a tile of W
+// 128 columns = 8 KB each) and four groups of four warps turn them into 16-bit values s * (c - z), rounded once, and store
+// them in the operand's swizzled layout, then, on top, W where the tile has entries of the residual (in 32 bits until its one
+// rounding, so that every W is what mx_q4_expand gives, bit for bit); in this form a tile of W
 // has the same bytes for the product and its transpose, only the operand descriptor differs.
 // Where there are fewer tiles than SMs, up to four blocks of a cluster share a tile's contraction and add their parts
 // through distributed shared memory, in the order of their ranks; large products are computed by pairs of blocks
@@ -108,23 +109,37 @@ __device__ __forceinline__ void convert_row(uint8_t *a, int out_row, uint4 (&c)[
             *reinterpret_cast<uint4 *>(a + ((4 * j + q ^ out_row & 7) << 4)) = values<V>(w[q], s, zero);
     }
     if (!slots || entries.x == NO_ENTRY) return;
-    auto add = [&](int k, V v) {
-        V *e = reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2);
-        *e = from_float<V>(to_float(*e) + to_float(v));
+    // W at column k of the 64, exact in 32 bits before the entry
+    auto core = [&](int k) {
+        const bool second = k & 32, upper = k & 16, odd = k & 8;
+        const uint32_t x = second ? c[1].x : c[0].x, y = second ? c[1].y : c[0].y;
+        const uint32_t z = second ? c[1].z : c[0].z, w = second ? c[1].w : c[0].w;
+        const uint32_t word = odd ? (upper ? w : y) : (upper ? z : x);
+        const int code = word >> 4 * (k & 7) & 15, zero = numbers.y >> (second ? 8 : 0) & 15;
+        return to_float(from_bits<V>(numbers.x >> (second ? 16 : 0))) * (float)(code - zero);
+    };
+    auto put = [&](int k, float v) {
+        *reinterpret_cast<V *>(a + ((k / 8 ^ out_row & 7) << 4) + k % 8 * 2) = from_float<V>(v);
     };
     if (entries.w != TOO_MANY) {
         const uint32_t entry[4] = {entries.x, entries.y, entries.z, entries.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (entry[j] != NO_ENTRY) add(entry[j] >> 16, from_bits<V>(entry[j]));
+        for (int j = 0; j < 4; ++j) {
+            if (entry[j] == NO_ENTRY) break;
+            const int k = entry[j] >> 16;
+            put(k, core(k) + to_float(from_bits<V>(entry[j])));
+        }
     } else {  // this thread looks for its entries itself
         const int k1 = min(col + 64, m.n_cols);
         int b, e;
         res_range(m, row, b, e);
-        for (b = first_at_least(m.res_col, b, e, col); b < e; ++b) {
+        for (b = first_at_least(m.res_col, b, e, col); b < e;) {
             const int k = m.res_col[b];
             if (k < col || k >= k1) break;
-            add(k - col, m.res_val[b]);
+            float v = core(k - col);
+            do v += to_float(m.res_val[b]);
+            while (++b < e && m.res_col[b] == k);
+            put(k - col, v);
         }
     }
 }

@@ -60,3 +60,61 @@ def test_any_codes_behind_the_last_column(k, group, t, n, dtype):
     if m["residual"] is not None:
         m["residual"][2].mul_(s / 4)
     finite_product(m, t, (0.5 if dtype is torch.float16 else 25) / s)
+
+
+# ---- a weight that a code and a residual's entries share is rounded once ---------------------------------------------
+
+
+def products_with_unit_vectors(m, t):
+    """W by mx_q4_expand, and by products and transposed products with unit vectors, t of them a call: W's own values."""
+    n, k, dtype = m["n"], m["k"], m["dtype"]
+    w = torch.empty(n, k, dtype=dtype, device="cuda")
+    q = matrix(m)
+    q.expand(w)
+    assert w.isfinite().all()
+    rows, cols = torch.empty_like(w), torch.empty_like(w)
+    for size, call, out in ((k, q.product, cols.T), (n, q.product_t, rows)):
+        unit = torch.eye(size, dtype=dtype, device="cuda")
+        for i in range(0, size, t):
+            got = torch.empty(min(t, size - i), n + k - size, dtype=dtype, device="cuda")
+            call(unit[i:i + t], got)
+            out[i:i + t] = got
+    return w, cols, rows
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("t,n,k,group,density", [
+    (3, 60, 330, 32, 0.02), (40, 60, 330, 32, 0.02), (70, 130, 330, 96, 0.3), (300, 300, 1037, 128, 0.01),
+    (1100, 4100, 1100, 64, 0.02), (2300, 1037, 2300, 128, 0.1)])
+def test_products_take_the_expanded_weights(t, n, k, group, density, dtype):
+    """More than 8 vectors, and transposed products with a residual, multiply by what mx_q4_expand gives, bit for bit."""
+    m = make(n, k, group, dtype, True, density, t)
+    w, cols, rows = products_with_unit_vectors(m, t)
+    if t > 8:
+        assert torch.equal(cols, w)
+    assert torch.equal(rows, w)
+
+
+@pytest.mark.parametrize("repeats", [1, 2, 7])
+@pytest.mark.parametrize("t", [5, 40, 1100])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_residual_entry_that_cancels_a_code(dtype, t, repeats):
+    """Little is left of a code's value and an entry (or several of one column), and a code's value alone may be no number
+    of the type: 7 x 143 = 1001 and about -994; 7 x 10000 and about -10000 in fp16."""
+    n, k = (4100 if t > 1000 else 300), 1100
+    s, parts = (10000.0, -10000.0) if dtype is torch.float16 else (143.0, -994.0)
+    m = make(n, k, 64, dtype, False, 0.0, 7)
+    m["codes"].fill_(0x88)  # nothing
+    m["scales"].fill_(s)
+    at = torch.arange(n, device="cuda") * 37 % (k - 1)
+    m["codes"].view(n, -1)[torch.arange(n, device="cuda"), at // 2] = 0xFF  # 7 steps at `at` and beside it
+    pair = (at // 2 * 2)[:, None] + torch.tensor([0, 1], device="cuda")
+    col = pair.repeat_interleave(repeats, 1).int().reshape(-1)
+    val = torch.full((col.numel(),), parts / repeats, dtype=dtype, device="cuda")
+    ptr = torch.arange(n + 1, dtype=torch.int32, device="cuda") * 2 * repeats
+    m["residual"] = (ptr, col, val)
+    exact = dense64(m)
+    w, cols, rows = products_with_unit_vectors(m, t)
+    assert torch.equal(w, exact.to(dtype)) and w.abs().max() > 0
+    assert torch.equal(rows, w)
+    assert torch.equal(cols, w)  # up to 8 vectors: codes and entries each exact in 32 bits
