@@ -158,15 +158,16 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
     const int line = lane / 4, quarter = lane % 4;
     const int rank = blockIdx.x % g.splits, row0 = blockIdx.x / g.splits * 128;
 
-    // the block's tiles
-    const int width = SEGMENTS * m.group, per_unit = S ? 1 : (m.group + 127) / 128;  // of a gradient's unit
+    // the block's tiles; a gradient's unit ends with the columns, whatever its group would have room for
+    const int width = SEGMENTS * m.group, per_unit = S ? 1 : (min(m.group, m.n_cols) + 127) / 128;
     const int pieces = (int)(((long long)m.n_cols + 127) / 128), units = (m.n_groups + SEGMENTS - 1) / SEGMENTS;
     const int from = (int)((long long)pieces * rank / g.splits);
     const int my_units = !GRAD || !g.out ? 0 : (units - rank + g.splits - 1) / g.splits;
-    const int tiles = GRAD ? my_units * per_unit : (int)((long long)pieces * (rank + 1) / g.splits) - from;
+    const int in_last = S ? 1 : (int)(((long long)m.n_cols - (long long)(units - 1) * width + 127) / 128);
+    const int missing = my_units > 0 && (units - 1) % g.splits == rank ? per_unit - in_last : 0;
+    const int tiles = GRAD ? my_units * per_unit - missing : (int)((long long)pieces * (rank + 1) / g.splits) - from;
     auto column = [&](int n) {
-        return GRAD ? (int)min((long long)(rank + n / per_unit * g.splits) * width + n % per_unit * 128, (long long)INT_MAX - 256)
-                    : (from + n) * 128;
+        return GRAD ? (rank + n / per_unit * g.splits) * width + n % per_unit * 128 : (from + n) * 128;
     };
     const uint32_t polls = (1u << 22) + 64u * min(tiles, 1 << 24);
 
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                     }
         }
         float d[SEGMENTS][H][NT][4] = {};
-        int n = group;
+        int n = group, of_unit = 0;  // the latter: tiles of the unit so far
         if (n < tiles) numbers(n);
         bool ok = true;
         while (n < tiles) {
@@ -230,7 +231,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             uint32_t two[2 * H], four[2 * H];  // this lane's rows' scales and zero points
             const int was = n;
             n += ALL ? 1 : 2;
-            const bool complete = !ALL || n % per_unit == 0;  // the unit's last tile
+            ++of_unit;
+            const bool complete = !ALL || of_unit == per_unit || n == tiles;  // the unit's last tile
             if (n < tiles) numbers(n);
             const int slot = was % DEPTH;
             if (!(ok = warp_wait(full(slot), was / DEPTH & 1, polls))) break;
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                 }
             }
             // columns from `left` on belong to the next group (which begins on a multiple of 32)
-            const int left = ALL && complete ? m.group - (per_unit - 1) * 128 : 128;
+            const int left = ALL && complete ? m.group - (of_unit - 1) * 128 : 128;
 #pragma unroll
             for (int j = 0; j < SEGMENTS; ++j) {
                 const int n32 = j * (WIDTH / 32);
@@ -310,6 +312,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(slot));
             if (GRAD && complete) {
+                of_unit = 0;
                 const int first_group = (rank + was / per_unit * g.splits) * SEGMENTS;
 #pragma unroll
                 for (int r = 0; r < 2 * H; ++r) {

@@ -6,7 +6,7 @@ import torch
 
 from conftest import has_gpu
 from q4_cases import dense64, make, matrix, rounded
-from test_gpu_q4 import TYPES, close, fresh, normal
+from test_gpu_q4 import TYPES, check_grad, check_product, check_product_t, close, fresh, normal
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not has_gpu(), reason="needs a CUDA device")]
 
@@ -118,3 +118,42 @@ def test_a_residual_entry_that_cancels_a_code(dtype, t, repeats):
     assert torch.equal(w, exact.to(dtype)) and w.abs().max() > 0
     assert torch.equal(rows, w)
     assert torch.equal(cols, w)  # up to 8 vectors: codes and entries each exact in 32 bits
+
+
+# ---- groups that are wider than the matrix --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", [1, 8, 9, 16, 40])
+@pytest.mark.parametrize("k,group", [(300, 320), (300, 4096), (300, 1 << 20), (1100, 1024), (2500, 1 << 30), (40, 1 << 30),
+                                     (1290, 640), (1400, 288)])
+def test_groups_that_reach_behind_the_last_column(k, group, t):
+    m = make(140, k, group, torch.bfloat16, True, 0.02, k)
+    check_product(m, t, 1)
+    check_product_t(m, t, 2)
+    check_grad(m, t, 3)
+    w = normal(4, 140, k, dtype=torch.bfloat16)
+    q = [matrix(fresh(140, k, g, torch.bfloat16, True, None)) for g in (group, -(-k // 32) * 32)]
+    for one in q:
+        one.quantize(w)
+    if k <= group:
+        assert torch.equal(q[0].codes, q[1].codes) and torch.equal(q[0].scales, q[1].scales)
+
+
+@pytest.mark.parametrize("t", [1, 16])
+def test_gradients_cost_what_the_columns_do(t):
+    """A group that says "the whole row" by a large number is worked on as far as the row goes."""
+    took, seen = [], []
+    for group in (320, 1 << 20):
+        m = make(140, 300, group, torch.bfloat16, True, None, 1)
+        q, ds = matrix(m), torch.empty_like(m["scales"])
+        x, dy = normal(1, t, 300, dtype=torch.bfloat16), normal(2, t, 140, dtype=torch.bfloat16)
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            q.grad(x, dy, ds)
+            b.record()
+            b.synchronize()
+        took.append(a.elapsed_time(b))
+        seen.append(ds)
+    assert torch.equal(*seen)
+    assert took[1] < 0.5 + 5 * took[0]  # 3 tiles of 128 columns, not 8192: some 4 ms
