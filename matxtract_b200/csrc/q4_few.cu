@@ -630,13 +630,14 @@ __global__ void __launch_bounds__(THREADS, 2) product_t_few_kernel(const __grid_
 // sums over no vectors: 0 for every scale and every residual entry that there is
 template <typename V>
 __global__ void no_gradient_kernel(Matrix<V> m, V *d_scales, V *d_res) {
-    const int warp = (blockIdx.x * THREADS + threadIdx.x) / 32, lane = threadIdx.x % 32;
-    if (warp >= m.n_rows) return;
+    const long long row = (long long)blockIdx.x * WARPS + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (row >= m.n_rows) return;
     if (d_scales)
-        for (int j = lane; j < m.n_groups; j += 32) d_scales[(long long)warp * m.n_groups + j] = from_float<V>(0.f);
+        for (int j = lane; j < m.n_groups; j += 32) d_scales[row * m.n_groups + j] = from_float<V>(0.f);
     if (!d_res) return;
     int begin, end;
-    res_range(m, warp, begin, end);
+    res_range(m, (int)row, begin, end);
     for (int e = begin + lane; e < end; e += 32) d_res[e] = from_float<V>(0.f);
 }
 template <typename V>

@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+import matxtract_b200 as mx
+
 from conftest import has_gpu
 from q4_cases import dense64, make, matrix, rounded
 from test_gpu_q4 import TYPES, check_grad, check_product, check_product_t, close, fresh, normal
@@ -157,3 +159,20 @@ def test_gradients_cost_what_the_columns_do(t):
         seen.append(ds)
     assert torch.equal(*seen)
     assert took[1] < 0.5 + 5 * took[0]  # 3 tiles of 128 columns, not 8192: some 4 ms
+
+
+# ---- sizes whose products pass 32 bits ------------------------------------------------------------------------------
+
+
+def test_no_vectors_and_very_many_rows():
+    """Sums over no vectors are 0 in the last of 2^27 rows and more, too."""
+    n = (1 << 27) + 300
+    codes = torch.empty(n, 16, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(n, 1, dtype=torch.float16, device="cuda")
+    ptr = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    col, val = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.float16, device="cuda")
+    q = mx.Q4Matrix(n, 1, 32, codes, scales, res_row_ptr=ptr, res_col_ind=col, res_val=val)
+    ds, dv = torch.full_like(scales, 7.0), torch.full_like(val, 7.0)
+    none = torch.empty(0, 1, dtype=torch.float16, device="cuda")
+    q.grad(none, torch.empty(0, n, dtype=torch.float16, device="cuda"), ds, dv)
+    assert not ds.any() and not dv.any()
