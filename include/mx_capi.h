@@ -393,8 +393,9 @@ typedef struct {
  * zero = -min(w, 0) / s, code = zero + w / s.  s is taken in 32 bits and rounded to dtype first, the quotients by the
  * rounded s to the nearest whole number, ties to even; codes are clamped to 1..15 (0..15 with zeros).  A group whose s is 0 gets
  * codes = zero; one that holds a NaN gets s = NaN, one that holds an infinity s = infinity.
- * res_row_ptr always receives the true counts: where res_row_ptr[n_rows] > res_cap the residual did not fit, and the
- * entries behind res_cap are lost (quantise again with more room).  Buffer parts behind the last entry stay untouched. */
+ * res_row_ptr always receives the true counts, as far as 2^31 - 1 goes: where res_row_ptr[n_rows] > res_cap, or is
+ * 2^31 - 1, the residual did not fit, and the entries behind res_cap are lost (quantise again with more room).  Buffer
+ * parts behind the last entry stay untouched. */
 int mx_q4_quantize(const mx_q4_matrix *m, int w_dtype, const void *w, long long ld_w, float threshold, void *stream);
 /* w[i][k] = W[i][k], dense row-major in the matrix's dtype, rounded once. */
 int mx_q4_expand(const mx_q4_matrix *m, void *w, long long ld_w, void *stream);

@@ -296,8 +296,8 @@ struct Places {
         __syncthreads();
         if (threadIdx.x == 0) tell(words + 1 + block, all(), block == 0 ? 2 : 1);
     }
-    __device__ __forceinline__ int all() const {
-        int n = 0;
+    __device__ __forceinline__ long long all() const {  // eight whole rows may have 2^33
+        long long n = 0;
         for (int w = 0; w < WARPS; ++w) n += counts[w];
         return n;
     }

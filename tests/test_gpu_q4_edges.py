@@ -176,3 +176,16 @@ def test_no_vectors_and_very_many_rows():
     none = torch.empty(0, 1, dtype=torch.float16, device="cuda")
     q.grad(none, torch.empty(0, n, dtype=torch.float16, device="cuda"), ds, dv)
     assert not ds.any() and not dv.any()
+
+
+def test_quantize_counts_that_pass_32_bits():
+    """Eight rows of 2^29 outliers each: the counts behind them stand at their limit, and none begins anew."""
+    k = 1 << 29
+    w = torch.ones(9, k, dtype=torch.float16, device="cuda")
+    w[8] = 2
+    m = fresh(9, k, k, torch.float16, False, 64)
+    matrix(m).quantize(w, threshold=0.5)
+    ptr, col, val = m["residual"]
+    assert ptr.tolist() == [0] + [min(i * k, 2 ** 31 - 1) for i in range(1, 10)]
+    assert torch.equal(col, torch.arange(64, dtype=torch.int32, device="cuda")) and (val == 1).all()
+    assert not m["scales"].any() and (m["codes"] == 0x88).all()
