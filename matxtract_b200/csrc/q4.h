@@ -37,11 +37,13 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Entries [begin, end) of row i, clamped into the buffers whatever the row pointers hold.
+// Entries [begin, end) of row i, clamped into the buffers whatever the row pointers hold.  Entries' places are unsigned: a
+// loop goes on behind the last one by its step, and a residual may have 2^31 - 1.
 template <typename V>
-__device__ __forceinline__ void res_range(const Matrix<V> &m, int i, int &begin, int &end) {
-    begin = max(0, min(m.res_ptr[i], m.res_cap));
-    end = max(begin, min(m.res_ptr[i + 1], m.res_cap));
+__device__ __forceinline__ void res_range(const Matrix<V> &m, int i, unsigned &begin, unsigned &end) {
+    const int b = max(0, min(m.res_ptr[i], m.res_cap));
+    begin = b;
+    end = max(b, min(m.res_ptr[i + 1], m.res_cap));
 }
 
 template <typename V>
@@ -50,9 +52,9 @@ __device__ __forceinline__ int zero_of(const Matrix<V> &m, int i, int g) {
 }
 
 // First entry of [begin, end) whose column is at least k (columns ascend).
-__device__ __forceinline__ int first_at_least(const int *col, int begin, int end, int k) {
+__device__ __forceinline__ unsigned first_at_least(const int *col, unsigned begin, unsigned end, int k) {
     while (begin < end) {
-        const int mid = begin + (end - begin) / 2;
+        const unsigned mid = begin + (end - begin) / 2;
         if (col[mid] < k)
             begin = mid + 1;
         else

@@ -365,27 +365,28 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
             // while it works on four.
             constexpr int TOGETHER = 6;  // entries a lane asks for at once: 48 of a row
             struct Entries {
-                int begin, end, k[TOGETHER];
+                unsigned begin, end;
+                int k[TOGETHER];
                 V a[TOGETHER];
             };
             auto row_of = [&](int n) { return first + 4 * (warp - 9) + 12 * (n / 4) + n % 4; };  // a warp's n-th row
-            int my_begin = 0, my_end = 0;  // of the row that is the lane's number
+            unsigned my_begin = 0, my_end = 0;  // of the row that is the lane's number
             if (row_of(lane) < last && row0 + row_of(lane) < m.n_rows) res_range(m, row0 + row_of(lane), my_begin, my_end);
-            int their_begin = 0, their_end = 0;  // and 32 rows on
+            unsigned their_begin = 0, their_end = 0;  // and 32 rows on
             if (row_of(32 + lane) < last && row0 + row_of(32 + lane) < m.n_rows)
                 res_range(m, row0 + row_of(32 + lane), their_begin, their_end);
-            auto ask = [&](Entries &n, int from) {
+            auto ask = [&](Entries &n, unsigned from) {
 #pragma unroll
                 for (int u = 0; u < TOGETHER; ++u) {
-                    const int e = from + lane % 8 + 8 * u;
+                    const unsigned e = from + lane % 8 + 8 * u;
                     n.k[u] = e < n.end ? m.res_col[e] : -1;
                     if (!GRAD) n.a[u] = e < n.end ? m.res_val[e] : from_float<V>(0.f);
                 }
             };
             auto rows = [&](Entries &n, int round) {
                 const int at = 4 * round + lane / 8;
-                const int b0 = __shfl_sync(0xffffffffu, my_begin, at & 31), e0 = __shfl_sync(0xffffffffu, my_end, at & 31);
-                const int b1 = __shfl_sync(0xffffffffu, their_begin, at & 31), e1 = __shfl_sync(0xffffffffu, their_end, at & 31);
+                const unsigned b0 = __shfl_sync(0xffffffffu, my_begin, at & 31), e0 = __shfl_sync(0xffffffffu, my_end, at & 31);
+                const unsigned b1 = __shfl_sync(0xffffffffu, their_begin, at & 31), e1 = __shfl_sync(0xffffffffu, their_end, at & 31);
                 n.begin = at < 32 ? b0 : b1;
                 n.end = at < 32 ? e0 : e1;
                 ask(n, n.begin);
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
                     for (int t = 0; t < 8 * NT; ++t)
                         v[t] = now.begin < now.end && t < g.n_vec ? to_float(g.dy[t * g.ld_dy + i]) : 0.f;
                 }
-                for (int from = now.begin;;) {
+                for (unsigned from = now.begin;;) {
 #pragma unroll
                     for (int u = 0; u < TOGETHER; ++u) {
                         const int k = now.k[u];
@@ -636,9 +637,9 @@ __global__ void no_gradient_kernel(Matrix<V> m, V *d_scales, V *d_res) {
     if (d_scales)
         for (int j = lane; j < m.n_groups; j += 32) d_scales[row * m.n_groups + j] = from_float<V>(0.f);
     if (!d_res) return;
-    int begin, end;
+    unsigned begin, end;
     res_range(m, (int)row, begin, end);
-    for (int e = begin + lane; e < end; e += 32) d_res[e] = from_float<V>(0.f);
+    for (unsigned e = begin + lane; e < end; e += 32) d_res[e] = from_float<V>(0.f);
 }
 template <typename V>
 cudaError_t no_gradient(const Matrix<V> &m, V *d_scales, V *d_res, cudaStream_t s) {

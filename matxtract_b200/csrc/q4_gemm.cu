@@ -131,7 +131,7 @@ __device__ __forceinline__ void convert_row(uint8_t *a, int out_row, uint4 (&c)[
         }
     } else {  // this thread looks for its entries itself
         const int k1 = min(col + 64, m.n_cols);
-        int b, e;
+        unsigned b, e;
         res_range(m, row, b, e);
         for (b = first_at_least(m.res_col, b, e, col); b < e;) {
             const int k = m.res_col[b];
@@ -600,13 +600,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 }
 
 // First entry of [begin, end) whose column is at least k, for a whole warp: 32 places are looked at together.
-__device__ __forceinline__ int warp_first_at_least(const int *col, int begin, int end, int k) {
-    const int lane = threadIdx.x % 32;
+__device__ __forceinline__ unsigned warp_first_at_least(const int *col, unsigned begin, unsigned end, int k) {
+    const unsigned lane = threadIdx.x % 32;
     while (end - begin > 32) {
-        const int step = (end - begin + 31) / 32, p = min(begin + (lane + 1) * step, end) - 1;  // the last of each part
+        const unsigned step = (end - begin + 31) / 32, p = min(begin + (lane + 1) * step, end) - 1;  // the last of each part
         const unsigned below = __ballot_sync(0xffffffffu, col[p] < k);
-        const int parts = below == 0xffffffffu ? 32 : __ffs(~below) - 1;  // that lie in front of k altogether
-        const int from = min(begin + parts * step, end);
+        const unsigned parts = below == 0xffffffffu ? 32 : __ffs(~below) - 1;  // that lie in front of k altogether
+        const unsigned from = min(begin + parts * step, end);
         end = min(from + step, end);
         begin = from;
     }
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(32 * SIDE_ROWS)
     const long long tiles = ((long long)m.n_cols + 127) / 128;
     const int segments = (int)min((long long)SIDE_SEGMENTS, 2 * tiles - k0 / 64);  // of whole tiles
     const bool real = row0 + r < m.n_rows;
-    int begin = 0, end = 0;
+    unsigned begin = 0, end = 0;
     if (real && m.res_ptr) res_range(m, row0 + r, begin, end);
     if (numbers) {
         const long long from = (real ? row0 + r : 0) * (long long)m.n_groups;
@@ -657,8 +657,9 @@ __global__ void __launch_bounds__(32 * SIDE_ROWS)
         const int k1 = min((long long)m.n_cols, k0 + 64ll * SIDE_SEGMENTS);
         if (k0 > 0) begin = warp_first_at_least(m.res_col, begin, end, k0);
         int segment_before = -1, column_before = -1, run = 0;  // of the entry in front, and how many its segment has
-        for (int e0 = begin; e0 < end; e0 += 32) {
-            const int e = e0 + lane, k = e < end ? m.res_col[e] : INT_MAX;
+        for (unsigned e0 = begin; e0 < end; e0 += 32) {
+            const unsigned e = e0 + lane;
+            const int k = e < end ? m.res_col[e] : INT_MAX;
             const V v = e < end ? m.res_val[e] : from_float<V>(0.f);
             const bool mine = k >= k0 && k < k1;
             const int segment = mine ? (k - k0) / 64 : SIDE_SEGMENTS;

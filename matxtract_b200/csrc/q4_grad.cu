@@ -48,9 +48,10 @@ __device__ int wait_ran_out_grad;
 // entries of one row, columns ascending, the next two already loaded
 template <typename V>
 struct Cursor {
-    int at = 0, end = 0, col[2];
+    unsigned at = 0, end = 0;
+    int col[2];
     __device__ __forceinline__ void fetch(const Matrix<V> &m, int j) {
-        const int p = at + j;
+        const unsigned p = at + j;
         col[j] = p < end ? m.res_col[p] : 0x7fffffff;
     }
     __device__ __forceinline__ void start(const Matrix<V> &m, int i, int k) {

@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per
     const uint8_t *codes = m.codes + row * m.code_ld;
     const V *scales = m.scales + (long long)row * m.n_groups;
     V *to = w + row * ld;
-    int begin = 0, end = 0;
+    unsigned begin = 0, end = 0;
     if (m.res_ptr) res_range(m, row, begin, end);
     uint32_t c[STEPS];
     V s[STEPS];
@@ -584,12 +584,13 @@ __global__ void __launch_bounds__(32 * WARPS) expand_kernel(Matrix<V> m, int per
     if (begin >= end) return;
     __syncwarp();
     const int stop = min(m.n_cols, start + PIECE);
-    for (int i = begin + lane, n = 0; i < end; i += 32, ++n) {
+    int n = 0;
+    for (unsigned i = begin + lane; i < end; i += 32, ++n) {
         const int k = n == 0 ? early[0] : n == 1 ? early[1] : m.res_col[i];
         if (k < start || k >= stop || (i > begin && m.res_col[i - 1] == k)) continue;
         const int g = k / m.group, code = codes[k / 2] >> 4 * (k & 1) & 15;
         float v = to_float(scales[g]) * (float)(code - zero_of(m, row, g));
-        for (int j = i; j < end && m.res_col[j] == k; ++j) v += to_float(m.res_val[j]);
+        for (unsigned j = i; j < end && m.res_col[j] == k; ++j) v += to_float(m.res_val[j]);
         to[k] = from_float<V>(v);
     }
 }

@@ -189,3 +189,29 @@ def test_quantize_counts_that_pass_32_bits():
     assert ptr.tolist() == [0] + [min(i * k, 2 ** 31 - 1) for i in range(1, 10)]
     assert torch.equal(col, torch.arange(64, dtype=torch.int32, device="cuda")) and (val == 1).all()
     assert not m["scales"].any() and (m["codes"] == 0x88).all()
+
+
+def test_a_residual_at_the_far_end_of_its_buffers():
+    """Entries' places up to 2^31 - 2, the last that there are: the same results as at the buffers' front."""
+    n, k, room, dtype = 140, 8400, 2 ** 31 - 1, torch.bfloat16
+    near = make(n, k, 64, dtype, True, 0.02, 41, spare=0)
+    ptr, col, val = near["residual"]
+    nnz = col.numel()
+    far = dict(near, residual=(ptr + (room - nnz), torch.empty(room, dtype=torch.int32, device="cuda"),
+                               torch.empty(room, dtype=dtype, device="cuda")))
+    far["residual"][1][room - nnz:] = col
+    far["residual"][2][room - nnz:] = val
+    a, b = matrix(near), matrix(far)
+    d_near, d_far = torch.empty_like(val), torch.empty(room, dtype=dtype, device="cuda")
+    for t in (0, 1, 8, 12, 40, 1100):
+        x, dy = normal(t, t, k, dtype=dtype), normal(t + 1, t, n, dtype=dtype)
+        seen = []
+        for q, dv in ((a, d_near), (b, d_far)):
+            y, dx, ds = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(near["scales"])
+            dv[-nnz:] = 7.0
+            q.product(x, y), q.product_t(dy, dx), q.grad(x, dy, ds, dv)
+            w = torch.empty(n, k, dtype=dtype, device="cuda")
+            q.expand(w)
+            seen.append((y, dx, ds, dv[-nnz:], w))
+        for one, other in zip(*seen):
+            assert torch.equal(one, other)
