@@ -414,9 +414,14 @@ int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long 
 int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, const void *dy, long long ld_dy,
                void *d_scales, void *d_res_val, void *stream);
 /* Checks the residual once, on the device: res_row_ptr starts at 0, never decreases and ends inside res_cap, columns lie
- * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  MX_ERR_TIMEOUT when a bounded wait inside an
- * earlier mx_q4_* kernel on this GPU ran out (its results are then not complete).  Synchronises the stream. */
+ * in [0, n_cols) and ascend inside a row.  MX_ERR_INVALID when not.  MX_ERR_TIMEOUT, which goes before it, when a bounded
+ * wait inside an mx_q4_* kernel on this GPU ran out since the last mx_q4_check there (that call's results are not
+ * complete; the call itself, asynchronous, had returned MX_OK): each run-out is told once.  Synchronises the stream. */
 int mx_q4_check(const mx_q4_matrix *m, void *stream);
+/* What a program does on MX_ERR_TIMEOUT can be tried with this: one thread waits `polls` (up to 65536) polls for what never
+ * comes and tells it as the kernels of products with many vectors (which = 0), of few vectors (1), of mx_q4_quantize (2)
+ * or of gradients from many vectors (3) do.  The next mx_q4_check on the GPU answers MX_ERR_TIMEOUT. */
+int mx_q4_wait_in_vain(int device, int which, unsigned polls, void *stream);
 
 #ifdef __cplusplus
 }

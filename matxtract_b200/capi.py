@@ -139,6 +139,7 @@ SYMBOLS = {
     "mx_q4_product_t": (_i, [_vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp]),
     "mx_q4_grad": (_i, [_vp, _i, _vp, C.c_longlong, _vp, C.c_longlong, _vp, _vp, _vp]),
     "mx_q4_check": (_i, [_vp, _vp]),
+    "mx_q4_wait_in_vain": (_i, [_i, _i, C.c_uint, _vp]),
 }
 
 _lib = None
@@ -708,7 +709,8 @@ class Q4Matrix:
                                 _address(d_res_val), stream))
 
     def check(self, stream=0):
-        """Raises when the residual's row pointers or columns are not what the products rely on; waits for the GPU."""
+        """Raises when the residual's row pointers or columns are not what the products rely on, or (once) when a bounded
+        wait inside an earlier call on this GPU ran out; waits for the GPU."""
         _raise(lib().mx_q4_check(self._r, stream))
 
 

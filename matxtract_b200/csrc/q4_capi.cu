@@ -4,6 +4,7 @@
 #include "mx_internal.h"
 #include "q4.h"
 #include "q4_gemm.h"
+#include "q4_ptx.cuh"
 
 namespace mx {
 namespace q4 {
@@ -79,6 +80,27 @@ int done(cudaError_t e) {
     if (e == cudaSuccess) return MX_OK;
     cudaGetLastError();
     return MX_ERR_CUDA;
+}
+
+struct Flags {
+    int *flag[4];
+};
+cudaError_t late_flags(Flags &f) {
+    const cudaError_t e[4] = {late_flag(&f.flag[0]), late_flag_few(&f.flag[1]), late_flag_quant(&f.flag[2]),
+                              late_flag_grad(&f.flag[3])};
+    return *std::max_element(e, e + 4);  // cudaSuccess is the least
+}
+
+// *late: whether a flag is set; none is afterwards
+__global__ void late_kernel(Flags f, int *late) {
+    if (atomicExch(f.flag[threadIdx.x], 0)) *late = 1;
+}
+
+// one thread that waits for a barrier at which nobody arrives
+__global__ void wait_in_vain_kernel(int *flag, uint32_t polls) {
+    __shared__ uint64_t bar;
+    mbar_init(smem_addr(&bar), 1);
+    if (!mbar_wait(smem_addr(&bar), 0, polls)) *flag = 1;
 }
 
 // *bad is set when row pointers or columns are not ascending and in range
@@ -185,25 +207,39 @@ int mx_q4_check(const mx_q4_matrix *m, void *stream) {
     OnDevice on(m->device);
     if (on.status != MX_OK) return on.status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int *flag = nullptr, bad = 0, late[4] = {0, 0, 0, 0};
-    cudaError_t e = cudaMallocAsync((void **)&flag, sizeof(int), s);
+    int *found = nullptr, is[2] = {0, 0};  // the residual is bad, a wait ran out
+    Flags flags;
+    cudaError_t e = late_flags(flags);
+    if (e == cudaSuccess) e = cudaMallocAsync((void **)&found, sizeof(is), s);
     if (e != cudaSuccess) return done(e);
-    e = cudaMemsetAsync(flag, 0, sizeof(int), s);
+    e = cudaMemsetAsync(found, 0, sizeof(is), s);
     if (e == cudaSuccess && m->res_row_ptr) {
         const int blocks = (int)std::min<long long>(((long long)m->n_rows + 256) / 256, 148 * 8);
-        check_kernel<<<blocks, 256, 0, s>>>(m->n_rows, m->n_cols, m->res_cap, m->res_row_ptr, m->res_col_ind, flag);
+        check_kernel<<<blocks, 256, 0, s>>>(m->n_rows, m->n_cols, m->res_cap, m->res_row_ptr, m->res_col_ind, found);
         e = cudaGetLastError();
     }
-    if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof(int), cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = waits_ran_out(&late[0], s);
-    if (e == cudaSuccess) e = waits_ran_out_few(&late[1], s);
-    if (e == cudaSuccess) e = waits_ran_out_quant(&late[2], s);
-    if (e == cudaSuccess) e = waits_ran_out_grad(&late[3], s);
-    cudaError_t f = cudaFreeAsync(flag, s);
+    if (e == cudaSuccess) {
+        late_kernel<<<1, 4, 0, s>>>(flags, found + 1);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = cudaMemcpyAsync(is, found, sizeof(is), cudaMemcpyDeviceToHost, s);
+    cudaError_t f = cudaFreeAsync(found, s);
     if (e == cudaSuccess) e = f;
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    f = cudaStreamSynchronize(s);  // whatever happened: the copy ends in this frame
+    if (e == cudaSuccess) e = f;
     if (e != cudaSuccess) return done(e);
-    return late[0] || late[1] || late[2] || late[3] ? MX_ERR_TIMEOUT : bad ? MX_ERR_INVALID : MX_OK;
+    return is[1] ? MX_ERR_TIMEOUT : is[0] ? MX_ERR_INVALID : MX_OK;
+}
+
+int mx_q4_wait_in_vain(int device, int which, unsigned polls, void *stream) {
+    if (device < 0 || which < 0 || which > 3 || polls > 1u << 16) return MX_ERR_INVALID;
+    OnDevice on(device);
+    if (on.status != MX_OK) return on.status;
+    Flags flags;
+    cudaError_t e = late_flags(flags);
+    if (e != cudaSuccess) return done(e);
+    wait_in_vain_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(flags.flag[which], polls);
+    return done(cudaGetLastError());
 }
 
 }  // extern "C"

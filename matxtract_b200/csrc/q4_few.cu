@@ -781,11 +781,7 @@ cudaError_t grad(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, cons
     return one ? stream<V, 0, 1, true>(g, codes, map_x, s) : stream<V, 0, 2, true>(g, codes, map_x, s);
 }
 
-cudaError_t waits_ran_out_few(int *flag, cudaStream_t s) {
-    void *p = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_few);
-    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
-}
+cudaError_t late_flag_few(int **flag) { return cudaGetSymbolAddress(reinterpret_cast<void **>(flag), wait_ran_out_few); }
 
 #define INSTANTIATE(V)                                                                                                \
     template cudaError_t product<V>(const Matrix<V> &, int, const V *, long long, V *, long long, cudaStream_t);      \

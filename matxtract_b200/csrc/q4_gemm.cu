@@ -798,11 +798,7 @@ cudaError_t product_t_many(const Matrix<V> &m, int n_vec, const V *dy, long long
     return tiles_of<V, TRANSPOSED>(m, n_vec, dy, ld_dy, dx, ld_dx, s);
 }
 
-cudaError_t waits_ran_out(int *flag, cudaStream_t s) {
-    void *p = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out);
-    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
-}
+cudaError_t late_flag(int **flag) { return cudaGetSymbolAddress(reinterpret_cast<void **>(flag), wait_ran_out); }
 
 #define INSTANTIATE(V)                                                                                             \
     template cudaError_t product_many<V>(const Matrix<V> &, int, const V *, long long, V *, long long, cudaStream_t); \

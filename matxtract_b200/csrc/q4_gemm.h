@@ -13,11 +13,11 @@ cudaError_t product_t_many(const Matrix<V> &m, int n_vec, const V *dy, long long
 template <typename V>
 cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, const V *dy, long long ld_dy,
                       V *d_scales, V *d_res, cudaStream_t s);
-// *flag = whether a bounded wait of an earlier call on the current device ended without its barrier (async copy)
-cudaError_t waits_ran_out(int *flag, cudaStream_t s);
-cudaError_t waits_ran_out_few(int *flag, cudaStream_t s);
-cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s);
-cudaError_t waits_ran_out_quant(int *flag, cudaStream_t s);
+// where the kernels of each file write on the current device that a bounded wait ended without what it waited for
+cudaError_t late_flag(int **flag);
+cudaError_t late_flag_few(int **flag);
+cudaError_t late_flag_quant(int **flag);
+cudaError_t late_flag_grad(int **flag);
 
 }  // namespace q4
 }  // namespace mx

@@ -357,11 +357,7 @@ cudaError_t grad_many(const Matrix<V> &m, int n_vec, const V *x, long long ld_x,
                             : launch<V, false>(map_dy, map_x, g, tiles, s);
 }
 
-cudaError_t waits_ran_out_grad(int *flag, cudaStream_t s) {
-    void *p = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_grad);
-    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
-}
+cudaError_t late_flag_grad(int **flag) { return cudaGetSymbolAddress(reinterpret_cast<void **>(flag), wait_ran_out_grad); }
 
 #define INSTANTIATE(V)                                                                                              \
     template cudaError_t grad_many<V>(const Matrix<V> &, int, const V *, long long, const V *, long long, V *, V *, \

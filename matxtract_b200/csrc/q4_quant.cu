@@ -667,11 +667,7 @@ cudaError_t expand(const Matrix<V> &m, V *w, long long ld, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-cudaError_t waits_ran_out_quant(int *flag, cudaStream_t s) {
-    void *p = nullptr;
-    const cudaError_t e = cudaGetSymbolAddress(&p, wait_ran_out_quant);
-    return e == cudaSuccess ? cudaMemcpyAsync(flag, p, sizeof(int), cudaMemcpyDeviceToHost, s) : e;
-}
+cudaError_t late_flag_quant(int **flag) { return cudaGetSymbolAddress(reinterpret_cast<void **>(flag), wait_ran_out_quant); }
 
 #define INSTANTIATE(V)                                                                                              \
     template cudaError_t quantize<V>(const mx_q4_matrix &, int, const void *, long long, float, cudaStream_t);      \

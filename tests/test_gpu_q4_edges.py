@@ -215,3 +215,29 @@ def test_a_residual_at_the_far_end_of_its_buffers():
             seen.append((y, dx, ds, dv[-nnz:], w))
         for one, other in zip(*seen):
             assert torch.equal(one, other)
+
+
+# ---- waits that ran out -----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_a_wait_that_ran_out_is_told_once(which):
+    """By the next check on the GPU, which goes on to tell of a bad residual afterwards; results that follow are right."""
+    good = make(50, 300, 64, torch.bfloat16, True, 0.05, 11)
+    matrix(good).check()
+    ptr, col, val = good["residual"]
+    bad = matrix(dict(good, residual=(ptr, col.clone().index_fill_(0, torch.tensor([3], device="cuda"), 300), val)))
+
+    def status(q):
+        try:
+            q.check()
+        except mx.MxError as e:
+            return e.status
+        return 0
+
+    assert mx.lib().mx_q4_wait_in_vain(0, which, 100, None) == 0
+    assert [status(matrix(good)) for _ in range(2)] == [6, 0]
+    assert mx.lib().mx_q4_wait_in_vain(0, which, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert [status(bad) for _ in range(2)] == [6, 1]
+    assert status(matrix(good)) == 0
+    check_product(good, 12, 1)

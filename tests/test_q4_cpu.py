@@ -124,3 +124,9 @@ def test_gradients_of_the_definition():
     e = torch.zeros_like(x)
     e[1, 69] = h
     assert abs((loss(scales, v64, x + e) - loss(scales, v64, x - e)) / (2 * h) - (dy @ dense64(m))[1, 69]) < 1e-6
+
+
+def test_waiting_in_vain_is_bounded():
+    L = capi.lib()
+    for bad in ((-1, 0, 1), (0, -1, 1), (0, 4, 1), (0, 0, (1 << 16) + 1)):
+        assert L.mx_q4_wait_in_vain(*bad, None) == 1
