@@ -418,9 +418,10 @@ int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, 
  * wait inside an mx_q4_* kernel on this GPU ran out since the last mx_q4_check there (that call's results are not
  * complete; the call itself, asynchronous, had returned MX_OK): each run-out is told once.  Synchronises the stream. */
 int mx_q4_check(const mx_q4_matrix *m, void *stream);
-/* What a program does on MX_ERR_TIMEOUT can be tried with this: one thread waits `polls` (up to 65536) polls for what never
- * comes and tells it as the kernels of products with many vectors (which = 0), of few vectors (1), of mx_q4_quantize (2)
- * or of gradients from many vectors (3) do.  The next mx_q4_check on the GPU answers MX_ERR_TIMEOUT. */
+/* What a program does on MX_ERR_TIMEOUT can be tried with this: one thread waits `polls` polls (up to 65536; 0: as many as
+ * a wait in a short kernel has, some 2 s) for what never comes and tells it as the kernels of products with many vectors
+ * (which = 0), of few vectors (1), of mx_q4_quantize (2) or of gradients from many vectors (3) do.  The next mx_q4_check
+ * on the GPU answers MX_ERR_TIMEOUT. */
 int mx_q4_wait_in_vain(int device, int which, unsigned polls, void *stream);
 
 #ifdef __cplusplus

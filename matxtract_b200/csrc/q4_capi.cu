@@ -100,7 +100,7 @@ __global__ void late_kernel(Flags f, int *late) {
 __global__ void wait_in_vain_kernel(int *flag, uint32_t polls) {
     __shared__ uint64_t bar;
     mbar_init(smem_addr(&bar), 1);
-    if (!mbar_wait(smem_addr(&bar), 0, polls)) *flag = 1;
+    if (!mbar_wait(smem_addr(&bar), 0, polls ? polls : polls_for(0))) *flag = 1;
 }
 
 // *bad is set when row pointers or columns are not ascending and in range

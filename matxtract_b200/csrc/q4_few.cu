@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, NT == 1 ? 2 : 1)
     auto column = [&](int n) {
         return GRAD ? (rank + n / per_unit * g.splits) * width + n % per_unit * 128 : (from + n) * 128;
     };
-    const uint32_t polls = (1u << 22) + 64u * min(tiles, 1 << 24);
+    const uint32_t polls = polls_for(tiles);
 
     if (threadIdx.x == 0) {
         failed = 0;

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int blocks128 = (int)(((long long)depth + 127) / 128);
     const int block0 = (int)((long long)blocks128 * rank / g.splits);
     const int blocks = (int)((long long)blocks128 * (rank + 1) / g.splits) - block0, steps = 2 * blocks;
-    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
+    const uint32_t polls = polls_for(steps);
 
     if (threadIdx.x == 0) {
         failed = 0;
@@ -425,7 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     const int blocks = (int)(((long long)depth + 127) / 128), steps = 2 * blocks;
     auto line_of = [&](int tile) { return tile % g.tiles_m * 256 + 128 * (int)rank; };
     auto vector_of = [&](int tile) { return tile / g.tiles_m * S::COLS; };
-    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
+    const uint32_t polls = polls_for(steps);
 
     if (threadIdx.x == 0) {
         failed = 0;

@@ -135,7 +135,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
     const int steps = (g.n_vec + 63) / 64, tiles = g.tiles_m * g.units, pairs = gridDim.x / 2;
-    const uint32_t polls = (1u << 22) + 64u * min(steps, 1 << 24);
+    const uint32_t polls = polls_for(steps);
     // A tile: 256 rows, of which this block has 128, and a unit: the columns of a whole number of groups, in turns of 256.
     struct Tile {
         int band, unit;

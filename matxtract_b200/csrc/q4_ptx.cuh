@@ -28,6 +28,9 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok;
 }
+// How many polls a wait in a kernel that takes `steps` steps may have: a poll waits some 4 us itself before it says no, so
+// that this is about 2 s and 64 us a step, of which none takes 1 us.
+__device__ __forceinline__ uint32_t polls_for(int steps) { return (1u << 19) + 16u * min(steps, 1 << 24); }
 // Waits until the phase of the given parity is over; false after `polls` polls.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls) {
     if (mbar_try(bar, parity)) return true;

@@ -237,7 +237,19 @@ def test_a_wait_that_ran_out_is_told_once(which):
 
     assert mx.lib().mx_q4_wait_in_vain(0, which, 100, None) == 0
     assert [status(matrix(good)) for _ in range(2)] == [6, 0]
-    assert mx.lib().mx_q4_wait_in_vain(0, which, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert mx.lib().mx_q4_wait_in_vain(0, which, 1, torch.cuda.current_stream().cuda_stream) == 0
     assert [status(bad) for _ in range(2)] == [6, 1]
     assert status(matrix(good)) == 0
     check_product(good, 12, 1)
+
+
+def test_a_wait_ends_within_seconds():
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    assert mx.lib().mx_q4_wait_in_vain(0, 1, 0, torch.cuda.current_stream().cuda_stream) == 0
+    b.record()
+    b.synchronize()
+    m = make(50, 300, 64, torch.bfloat16, True, 0.05, 11)
+    with pytest.raises(mx.MxError) as e:
+        matrix(m).check()
+    assert e.value.status == 6 and 100 < a.elapsed_time(b) < 8000
