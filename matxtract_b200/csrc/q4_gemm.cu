@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 constexpr int PAIR_THREADS = 32 * 24, WRITE = 20;  // first of the writing warps
 struct PairShape {
     static constexpr int STAGE = 2 * A_BYTES, STAGES = 6, CODES = 2, COLS = 256;
-    static constexpr int BARS = STAGES + 3 * TURN + 4;
+    static constexpr int BARS = STAGES + 4 * TURN + 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + CODES * PAIR_TILE + BARS * 8;
     static_assert(SMEM <= 227 * 1024 && STAGES <= TURN && CODES <= TURN, "as above");
 };
@@ -407,6 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     __shared__ volatile int failed;
     uint8_t *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const uint32_t base = smem_addr(smem);
+    __shared__ uint4 word;  // block 0's: where block 1's words land
     uint8_t *codes_at = smem + S::STAGES * S::STAGE;
     const uint32_t bars = smem_addr(codes_at + S::CODES * PAIR_TILE);
     auto full = [&](int s) { return bars + 8 * s; };                                // block 0's: of both blocks' stage
@@ -415,6 +416,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     auto c_empty = [&](int n) { return bars + 8 * (S::STAGES + 2 * TURN + n % TURN); };
     auto done = [&](int b) { return bars + 8 * (S::STAGES + 3 * TURN + b); };         // each block's: D is complete
     auto drained = [&](int b) { return bars + 8 * (S::STAGES + 3 * TURN + 2 + b); };  // block 0's: both have written it
+    auto made = [&](int step) { return bars + 8 * (S::STAGES + 3 * TURN + 4 + step % TURN); };  // block 1's: its W is there
 
     const Matrix<V> &m = g.m;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -429,11 +431,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), 1 + 8);  // the copies, and a group's warps of each block
+        for (int s = 0; s < S::STAGES; ++s) mbar_init(full(s), 1 + 4);  // the copies (block 1's word is one), a group's warps
         for (int n = 0; n < TURN; ++n) {
             mbar_init(empty(n), 1);
             mbar_init(c_full(n), 1);
             mbar_init(c_empty(n), 8);
+            mbar_init(made(n), 4);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(done(b), 1);
@@ -464,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             for (int step = 0; step < steps; ++step, ++n) {
                 const int s = n % S::STAGES;
                 if (!(ok = stage_free(n))) break;
-                if (rank == 0) mbar_expect(full(s), 2 * A_BYTES);
+                if (rank == 0) mbar_expect(full(s), 2 * A_BYTES + 16);
                 tma_load_pair(base + s * S::STAGE + A_BYTES, &map_b, step * 64, vector, in_block(full(s), 0));
             }
         }
@@ -501,6 +504,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 }
             }
             if (ok) tc_commit_pair(done(b));
+        }
+        if (!ok) failed = 1;
+    } else if (rank == 1 && warp == 3 && lane == 0) {  // ---- tells block 0 what block 1's groups have made
+        // The matrix instruction in block 0 reads W in both.  What was made here reaches block 0's barrier by a copy of its
+        // first 16 bytes, whose end the barrier counts as it does those of the vectors' copies.  (An arrival that makes sure
+        // of this thread's memory in the other block takes 1000 to 2000 clocks: 245 us for 2048 vectors, 8192 x 8192, if
+        // the groups' warps make it, 273 if two threads make it for them.)
+        const uint32_t there = in_block(bars, 0), to = in_block(smem_addr(&word), 0);
+        bool ok = true;
+        for (int n = 0; n < mine * steps; ++n) {
+            const int s = n % S::STAGES;
+            if (!(ok = mbar_wait(made(n), n / TURN & 1, polls))) break;
+            bulk_send(to, base + s * S::STAGE, 16, there + 8 * s);
         }
         if (!ok) failed = 1;
     } else if (warp == 2 && lane == 0) {  // ---- codes of this block's lines
@@ -562,7 +578,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             convert_row<V>(smem + s * S::STAGE + out_at, out_row, c, numbers, slots, entries, m, row, col);
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive_own_at(in_block(full(s), 0));
+            if (lane == 0) mbar_arrive(rank == 0 ? full(s) : made(step));
         }
         if (!ok) failed = 1;
     } else if (warp >= WRITE) {  // ---- D leaves tensor memory

@@ -32,7 +32,7 @@ constexpr int REDUCE = 4, THREADS = 32 * 20;
 constexpr int HALF = 128 * 64 * 2;  // bytes of 128 lines x 64 deep: a block's part of A, and of B
 constexpr int STAGE = 2 * HALF, STAGES = 6, COLS = 256;
 constexpr int PART = 136, SUMS = 8 * PART;  // parts of the scales' gradients: [32 columns][row], a little apart
-constexpr int BARS = 2 * STAGES + 5;
+constexpr int BARS = 2 * STAGES + 7;
 constexpr int SMEM = 1024 + STAGES * STAGE + 2 * SUMS * 4 + BARS * 8;
 static_assert(SMEM <= 227 * 1024, "shared memory of one block");
 
@@ -129,7 +129,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     auto empty = [&](int s) { return bars + 8 * (STAGES + s); };   // each block's: the stage is used up
     auto done = [&](int b) { return bars + 8 * (2 * STAGES + b); };         // each block's: D is complete
     auto drained = [&](int b) { return bars + 8 * (2 * STAGES + 2 + b); };  // block 0's: both blocks have taken it
-    const uint32_t together = bars + 8 * (2 * STAGES + 4);                  // the sixteen warps that reduce
+    auto taken = [&](int b) { return bars + 8 * (2 * STAGES + 4 + b); };    // block 1's: its warps have taken it
+    const uint32_t together = bars + 8 * (2 * STAGES + 6);                  // the sixteen warps that reduce
 
     const Matrix<V> &m = g.m;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -153,7 +154,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(done(b), 1);
-            mbar_init(drained(b), 32);
+            mbar_init(drained(b), 16 + 1);  // block 0's warps, block 1's word
+            mbar_init(taken(b), 16);
         }
         mbar_init(together, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -231,6 +233,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             if (ok) tc_commit_pair(done(b));
         }
         if (!ok) failed = 1;
+    } else if (rank == 1 && warp == 3 && lane == 0) {  // ---- tells block 0 what block 1's warps have taken
+        // (each of them would wait a thousand clocks for its word to go: 64 vectors, 16384 x 8192: 81 us instead of 64)
+        const uint32_t there = in_block(drained(0), 0);
+        int all = 0;
+        bool ok = true;
+        Tile t = first;
+        for (int at = blockIdx.x / 2; at < tiles; at += pairs, go_on(t)) all += turns(t);
+        for (int u = 0; u < all; ++u) {
+            if (!(ok = mbar_wait(taken(u & 1), u / 2 & 1, polls))) break;
+            mbar_arrive_at(there + 8 * (u & 1));
+        }
+        if (!ok) failed = 1;
     } else if (warp >= REDUCE) {
         const int group = (warp - REDUCE) / 4, row = warp % 4 * 32 + lane;
         const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
@@ -297,7 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_own_at(in_block(drained(b), 0));
+                if (lane == 0) mbar_arrive(rank == 0 ? drained(b) : taken(b));
             }
             if (!ok) break;
 #pragma unroll

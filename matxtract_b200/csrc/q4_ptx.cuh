@@ -64,6 +64,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
+// the same from this block's shared memory into that of any block of the cluster, whose barrier counts it
+__device__ __forceinline__ void bulk_send(uint32_t cluster_dst, uint32_t src, uint32_t bytes, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     cluster_dst),
+                 "r"(src), "r"(bytes), "r"(cluster_bar)
+                 : "memory");
+}
 // what ordinary stores put into shared memory becomes visible to the tensor cores' reads
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -151,13 +158,9 @@ __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {  // of any block of the cluster
+// At a barrier of any block of the cluster: what this thread has done, and what it has seen done, is seen there.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// The same without a wait for what this thread has under way in global memory (1300 clocks with a scale on its way): for
-// values that this block's own tensor core reads from this block's shared memory, where a proxy fence has put them.
-__device__ __forceinline__ void mbar_arrive_own_at(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // A wait for arrivals that come from the other block, too.
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t polls) {
