@@ -611,12 +611,14 @@ class Q4Matrix:
     Calls run asynchronously on ``stream`` (a cudaStream_t as int; 0 = the default stream) of the tensors' GPU."""
 
     _TYPES = {"torch.float16": FP16, "torch.bfloat16": BF16, "torch.float32": FP32}
+    _MOST = 1 << 30  # rows, columns, vectors, a group's columns: the ABI takes them as int
 
     def __init__(self, n_rows: int, n_cols: int, group: int, codes, scales, zeros=None, res_row_ptr=None,
                  res_col_ind=None, res_val=None):
         n_rows, n_cols, group = int(n_rows), int(n_cols), int(group)
         _need(n_rows >= 0 and n_cols >= 0 and group > 0 and group % 32 == 0, "sizes are not negative, the group a "
               "positive multiple of 32")
+        _need(max(n_rows, n_cols, group) <= self._MOST, "sizes and the group are at most 2^30")
         n_groups = -(-n_cols // group)
         self.vdt, self.device = scales.dtype, scales.device
         _need(str(self.vdt) in ("torch.float16", "torch.bfloat16"), "scales are float16 or bfloat16")
@@ -634,6 +636,7 @@ class Q4Matrix:
         if res_row_ptr is not None:
             _need(res_col_ind is not None and res_val is not None, "a residual has row pointers, columns and values")
             cap = res_col_ind.numel()
+            _need(cap < 1 << 31, "a residual has room for at most 2^31 - 1 entries")
             self._tensor(res_row_ptr, "res_row_ptr", "torch.int32", (n_rows + 1,))
             self._tensor(res_col_ind, "res_col_ind", "torch.int32", (cap,))
             self._tensor(res_val, "res_val", self.vdt, (cap,))
@@ -665,6 +668,8 @@ class Q4Matrix:
         if a.dtype is not (dtype or self.vdt) or a.device != self.device:
             _need(False, f"{name}: another type or GPU than the matrix")
         rows, (apart, step) = shape[0], a.stride()
+        if rows > self._MOST:
+            _need(False, f"{name}: at most 2^30 rows")
         ld = apart if rows > 1 else max(cols, 1)
         if (cols > 1 and step != 1) or ld < cols:
             _need(False, f"{name}: the entries of a row are adjacent, rows apart")

@@ -130,3 +130,19 @@ def test_waiting_in_vain_is_bounded():
     L = capi.lib()
     for bad in ((-1, 0, 1), (0, -1, 1), (0, 4, 1), (0, 0, (1 << 16) + 1)):
         assert L.mx_q4_wait_in_vain(*bad, None) == 1
+
+
+def test_the_binding_hands_no_size_on_that_an_int_does_not_hold():
+    """2^32 + 1 vectors are not one vector."""
+    q = object.__new__(mx.Q4Matrix)
+    q.vdt, q.device = torch.float16, torch.device("meta")
+    assert q._rows(torch.empty(1 << 30, 1, dtype=torch.float16, device="meta"), "x", 1) == (1 << 30, 1)
+    for rows in ((1 << 30) + 1, (1 << 32) + 1):
+        with pytest.raises(mx.MxError) as e:
+            q._rows(torch.empty(rows, 1, dtype=torch.float16, device="meta"), "x", 1)
+        assert e.value.status == 1 and "2^30" in str(e.value)
+    for n, k, g in (((1 << 32) + 4, 64, 32), (4, (1 << 32) + 64, 32), (4, 64, (1 << 32) + 32)):
+        with pytest.raises(mx.MxError) as e:
+            mx.Q4Matrix(n, k, g, torch.empty(n, max(16, k // 2), dtype=torch.uint8, device="meta"),
+                        torch.empty(n, -(-k // g), dtype=torch.float16, device="meta"))
+        assert e.value.status == 1 and "2^30" in str(e.value)
