@@ -7,7 +7,7 @@ import torch
 import matxtract_b200 as mx
 
 from conftest import has_gpu
-from q4_cases import dense64, make, matrix, rounded
+from q4_cases import dense64, entries, make, matrix, rounded
 from test_gpu_q4 import TYPES, check_grad, check_product, check_product_t, close, fresh, normal
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not has_gpu(), reason="needs a CUDA device")]
@@ -253,3 +253,63 @@ def test_a_wait_ends_within_seconds():
     with pytest.raises(mx.MxError) as e:
         matrix(m).check()
     assert e.value.status == 6 and 100 < a.elapsed_time(b) < 8000
+
+
+# ---- values that are not finite -----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("group", [32, 64, 96, 128, 4096])
+@pytest.mark.parametrize("t,n", [(2, 150), (7, 150), (9, 150), (16, 150), (40, 300), (1100, 4100)])
+def test_values_that_are_not_finite_stay_where_they_belong(t, n, group):
+    """A NaN or an infinity in one vector, one row's numbers or one entry shows in what it enters and changes nothing else."""
+    k, i, j, v = 710, 77, 333, t - 1  # a row, a column, a vector
+    m = make(n, k, group, torch.bfloat16, True, 0.02, 3)
+    q = matrix(m)
+    x, dy = normal(1, t, k, dtype=torch.bfloat16), normal(2, t, n, dtype=torch.bfloat16)
+    row, col, val = entries(m)
+
+    def run(x=x, dy=dy):
+        y, dx = torch.empty_like(dy), torch.empty_like(x)
+        ds, dv = torch.empty_like(m["scales"]), torch.empty_like(m["residual"][2])
+        q.product(x, y), q.product_t(dy, dx), q.grad(x, dy, ds, dv)
+        return y, dx, ds, dv[: val.numel()]
+
+    def only(got, want, hit):
+        hit = hit.expand_as(want)
+        assert not got[hit].isfinite().any() and torch.equal(got[~hit], want[~hit])
+
+    def mask(size, at):
+        return torch.arange(size, device="cuda") == at
+
+    clean = run()
+    groups = torch.arange(m["scales"].shape[1], device="cuda")
+    for bad in (math.nan, math.inf, -math.inf):
+        x2, dy2 = x.clone(), dy.clone()
+        x2[v, j] = bad
+        y, _, ds, dv = run(x=x2)
+        only(y, clean[0], mask(t, v)[:, None])
+        # G's column j: all rows' sums of that group but where every code in it is its zero point, which NaN turns up in too
+        only(ds, clean[2], (groups == j // group)[None])
+        only(dv, clean[3], col == j)
+        dy2[v, i] = bad
+        _, dx, ds, dv = run(dy=dy2)
+        only(dx, clean[1], mask(t, v)[:, None])
+        only(ds, clean[2], mask(n, i)[:, None])
+        only(dv, clean[3], row == i)
+        # the row's scale of that group
+        was = m["scales"][i, j // group].clone()
+        m["scales"][i, j // group] = bad
+        y, dx, ds, dv = run()
+        m["scales"][i, j // group] = was
+        only(y, clean[0], mask(n, i)[None])
+        only(dx, clean[1], (torch.arange(k, device="cuda") // group == j // group)[None])
+        assert torch.equal(ds, clean[2]) and torch.equal(dv, clean[3])
+        # an entry
+        e = val.numel() // 2
+        was = m["residual"][2][e].clone()
+        m["residual"][2][e] = bad
+        y, dx, ds, dv = run()
+        m["residual"][2][e] = was
+        only(y, clean[0], mask(n, row[e])[None])
+        only(dx, clean[1], mask(k, col[e])[None])
+        assert torch.equal(ds, clean[2]) and torch.equal(dv, clean[3])
