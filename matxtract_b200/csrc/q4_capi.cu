@@ -1,4 +1,6 @@
 // Entry points of the 4-bit matrix operators (mx_q4_*, include/mx_capi.h): argument checks, device, dispatch on type.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "mx_internal.h"
@@ -54,6 +56,22 @@ Matrix<V> view(const mx_q4_matrix &m) {
             m.res_row_ptr ? m.res_cap : 0};
 }
 
+// Whether the calling thread has a context.  The runtime gives it one at its first launch or allocation, which is too late
+// for the tensor maps: those ask the driver.
+bool has_context() {
+    using Current = CUresult (*)(CUcontext *);
+    static const Current current = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuCtxGetCurrent", &p, 4000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<Current>(p);
+    }();
+    CUcontext c = nullptr;
+    return current && current(&c) == CUDA_SUCCESS && c;
+}
+
 // The matrix's GPU for the length of a call; the thread's own device comes back afterwards.
 struct OnDevice {
     int before = -1, status = MX_OK;
@@ -65,10 +83,9 @@ struct OnDevice {
             status = MX_ERR_INVALID;
         else if (cudaGetDevice(&before) != cudaSuccess)
             status = MX_ERR_CUDA;
-        else if (before == device)
-            before = -1;
-        else if (cudaSetDevice(device) != cudaSuccess)
+        else if ((before != device || !has_context()) && cudaSetDevice(device) != cudaSuccess)
             status = MX_ERR_CUDA;
+        if (before == device) before = -1;
         if (status != MX_OK) cudaGetLastError();
     }
     ~OnDevice() {

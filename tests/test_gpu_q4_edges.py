@@ -1,5 +1,6 @@
 """4-bit matrices on the GPU: numbers at the ends of their types, and what lies behind a matrix's last column."""
 import math
+import threading
 
 import pytest
 import torch
@@ -313,3 +314,76 @@ def test_values_that_are_not_finite_stay_where_they_belong(t, n, group):
         only(y, clean[0], mask(n, row[e])[None])
         only(dx, clean[1], mask(k, col[e])[None])
         assert torch.equal(ds, clean[2]) and torch.equal(dv, clean[3])
+
+
+# ---- calls from several threads ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", [1, 5, 12, 40, 1100])
+@pytest.mark.parametrize("name", ["product", "product_t", "grad", "expand", "quantize", "check"])
+def test_a_thread_s_first_call(name, t):
+    n, k = 512, 1024  # rows on 16-byte borders: no workspace is taken before the call's own work
+    m = make(n, k, 64, torch.bfloat16, True, 0.01 if t == 5 else None, 27)
+    q, f = matrix(m), matrix(fresh(n, k, 64, torch.bfloat16, True, None))
+    x, dy = normal(t, t, k, dtype=torch.bfloat16), normal(t, t, n, dtype=torch.bfloat16)
+    w, ds = normal(1, n, k, dtype=torch.bfloat16), torch.empty_like(m["scales"])
+    call = {"product": lambda: q.product(x, dy), "product_t": lambda: q.product_t(dy, x), "grad": lambda: q.grad(x, dy, ds),
+            "expand": lambda: q.expand(w), "quantize": lambda: f.quantize(w), "check": lambda: q.check()}[name]
+    told = []
+
+    def work():
+        try:
+            call()
+        except Exception as e:  # noqa: BLE001
+            told.append(e)
+
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not told
+
+
+def test_threads_that_call_at_once():
+    """Each with a stream and vectors of its own, on one matrix: what each gets alone."""
+    n, k, jobs = 517, 1037, []  # rows on no 16-byte border: every call takes workspaces
+    m = make(n, k, 64, torch.bfloat16, True, 0.01, 27)
+    q = matrix(m)
+
+    def run(job, stream):
+        x, dy, (y, dx, ds, dv, w) = job
+        q.product(x, y, stream=stream)
+        q.product_t(dy, dx, stream=stream)
+        q.grad(x, dy, ds, dv, stream=stream)
+        q.expand(w, stream=stream)
+
+    for t in (1, 5, 12, 40, 300, 1100):
+        x, dy = normal(t, t, k, dtype=torch.bfloat16), normal(t + 1, t, n, dtype=torch.bfloat16)
+        out = (torch.empty_like(dy), torch.empty_like(x), torch.empty_like(m["scales"]), torch.zeros_like(m["residual"][2]),
+               torch.empty(n, k, dtype=torch.bfloat16, device="cuda"))
+        run((x, dy, out), 0)
+        torch.cuda.synchronize()
+        jobs.append((x, dy, out, [o.clone() for o in out], torch.cuda.Stream()))
+        for o in out:
+            o.zero_()
+    torch.cuda.synchronize()
+    told = []
+
+    def work(job):
+        try:
+            for _ in range(30):
+                run(job[:3], job[4].cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            told.append(e)
+
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for one in threads:
+        one.start()
+    for one in threads:
+        one.join()
+    torch.cuda.synchronize()
+    assert not told
+    for _, _, out, want, _ in jobs:
+        for o, w in zip(out, want):
+            assert torch.equal(o.view(torch.int16), w.view(torch.int16))
