@@ -354,9 +354,17 @@ int mx_csr_spmv_static(int dtype, int n_rows, int n_cols, int nnz, const int *ro
  * All buffers are DEVICE memory of GPU `device` and belong to the caller; the calls keep nothing between calls, are
  * asynchronous on `stream` (a cudaStream_t, NULL = the device's default stream), may be captured into a graph
  * (mx_q4_check excepted) and leave the calling thread's current device as it was.  A workspace comes from the device's
- * stream-ordered pool and goes back to it within the call: for a product at most three quarters of the codes' bytes
- * (rows and columns filled up to 128s) and a copy of the vectors.  Calls on different streams are independent of each
- * other as far as their buffers are.  Results do not depend on anything but the inputs: no sum is taken in an order that varies.
+ * stream-ordered pool and goes back to it within the call:
+ *   vectors that do not lie on 16-byte borders (base, and ld where there are several): a copy, rows filled up to 8 values;
+ *   products with up to 8 and gradients from up to 16 vectors, from 3 on and where the residual takes part: 8 values a
+ *     column (gradients from 9 on: 16);
+ *   products with more than 8 vectors and transposed products: half of the codes' bytes (rows and columns filled up to
+ *     128s) with a residual, and a quarter of them for large ones;
+ *   mx_q4_quantize with a residual: a byte for every 2048 columns, begun or whole, of a row.
+ * Calls on different streams, from any threads, are independent of each other as far as their buffers are.  Results do
+ * not depend on anything but the inputs: no sum is taken in an order that varies.  (The number of vectors is one of them:
+ * it decides how W is rounded, see below, and how a sum is split, so that a vector's result may differ in its last bits
+ * with how many others are in the call.)
  * n_rows, n_cols and n_vec may be 0 and are at most 2^30; results do not overlap inputs.  A result that a scale, a
  * residual value or a vector's value enters which is not finite is itself infinite or NaN, not always the one of the
  * two that the formula gives.
@@ -401,16 +409,16 @@ int mx_q4_quantize(const mx_q4_matrix *m, int w_dtype, const void *w, long long 
 int mx_q4_expand(const mx_q4_matrix *m, void *w, long long ld_w, void *stream);
 /* y[t][i] = sum_k W[i][k] x[t][k] for n_vec vectors (rows of x and y, ld_x and ld_y elements apart): what mx_spmv is
  * for a sparse matrix.  Sums in 32 bits, rounded once at the end; for more than 8 vectors W[i][k] is rounded to dtype
- * before it is multiplied (and is infinite where it leaves dtype's range, as in mx_q4_expand). */
+ * before it is multiplied: it is what mx_q4_expand gives, and infinite where that is. */
 int mx_q4_product(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, void *y, long long ld_y, void *stream);
 /* dx[t][k] = sum_i W[i][k] dy[t][i]: the product with the transposed matrix, which is also the gradient of x.  W[i][k]
- * is rounded to dtype before it is multiplied, for any number of vectors. */
+ * is what mx_q4_expand gives, for any number of vectors. */
 int mx_q4_product_t(const mx_q4_matrix *m, int n_vec, const void *dy, long long ld_dy, void *dx, long long ld_dx,
                     void *stream);
 /* Gradients of the matrix's own numbers, G[i][k] = sum_t dy[t][i] x[t][k] (never stored):
  *     d_scales[i][g] = sum of (codes - zeros)[i][k] G[i][k] over the group's columns,   [n_rows][n_groups]
  *     d_res_val[e]   = G[row of e][column of e] for every residual entry e < res_row_ptr[n_rows],   [res_cap]
- * both in the matrix's dtype; either may be NULL.  The matrix's scales and res_val are not read. */
+ * both in the matrix's dtype; either may be NULL.  What the matrix's scales and res_val hold does not count. */
 int mx_q4_grad(const mx_q4_matrix *m, int n_vec, const void *x, long long ld_x, const void *dy, long long ld_dy,
                void *d_scales, void *d_res_val, void *stream);
 /* Checks the residual once, on the device: res_row_ptr starts at 0, never decreases and ends inside res_cap, columns lie

@@ -608,7 +608,9 @@ class Q4Matrix:
     ``codes`` uint8 [n_rows, >= ceil(n_cols / 2)] (rows a multiple of 16 bytes apart), ``scales`` float16 or bfloat16
     [n_rows, ceil(n_cols / group)], ``zeros`` uint8 of the same shape or None (= 8 everywhere); the residual is
     ``res_row_ptr`` int32 [n_rows + 1], ``res_col_ind`` int32 and ``res_val`` in the scales' type, or None.
-    Calls run asynchronously on ``stream`` (a cudaStream_t as int; 0 = the default stream) of the tensors' GPU."""
+    Calls run asynchronously on ``stream`` (a cudaStream_t as int) of the tensors' GPU.  0 is the default stream, with which
+    torch's side streams are not in order: tensors that are used inside ``torch.cuda.stream(...)`` want
+    ``stream=torch.cuda.current_stream().cuda_stream``."""
 
     _TYPES = {"torch.float16": FP16, "torch.bfloat16": BF16, "torch.float32": FP32}
     _MOST = 1 << 30  # rows, columns, vectors, a group's columns: the ABI takes them as int

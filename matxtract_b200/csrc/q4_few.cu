@@ -107,10 +107,12 @@ __device__ __forceinline__ void turned_values(float (&x)[8 * NT], const V *at) {
 //             vector are weighed with dy; the blocks of a row take units in turn.  For S = 0 every warp has 16 rows and
 //             takes every tile: with units of several tiles taken in turn, a group of warps would meet a slot's barrier
 //             without having seen its last phase, which a wait for a parity cannot tell from the wanted one.
-// What bounds it is the ALU pipe, which takes the codes apart (7 operations for 8 codes and as many again for all the
-// rest): tiles fetched by the converting warps themselves, 16 rows a warp, cost 470 instructions for 2048 codes and
-// 44 us for 16384 x 8192 and one vector.  This form takes 25.8 us (the codes at 2.6 TB/s), 8 vectors 26.8, with a residual
-// of 0.5 % of the entries 30 and 37; the gradients for one vector 25.4, for 16 vectors 34.
+// Taking the codes apart (7 operations for 8 codes and as many again for all the rest) bounded an earlier form, whose
+// converting warps fetched tiles themselves, 16 rows a warp: 470 instructions for 2048 codes, 44 us for 16384 x 8192 and one
+// vector.  This form takes 25.4 us (the codes at 2.6 TB/s), 8 vectors 26.4, with a residual of 0.5 % of the entries 30.6 and
+// 37; the gradients for one vector 25.7, for 16 vectors 34.  Nothing is full any more (one vector with residual: ALU pipe
+// 44 %, issue slots 47 %, DRAM a third): a tile is a chain of a wait, loads, the taking apart and products that follow one
+// another, with eight warps a block to hide it, and 256 blocks on 148 SMs leave 40 SMs with one of two.
 constexpr int STREAM_THREADS = 32 * 12, DEPTH = 8;
 constexpr int CODE_BYTES = 128 * 64;
 template <int NT>
@@ -717,7 +719,8 @@ cudaError_t stream_inputs(Few<V> &g, const V *x, long long ld_x, CUtensorMap &co
 
 template <typename V>
 cudaError_t product(const Matrix<V> &m, int n_vec, const V *x, long long ld_x, V *y, long long ld_y, cudaStream_t s) {
-    // 16 vectors, 4096 x 4096: 16.5 us here (one block an SM then), 10.2 us there; 8 vectors: 7 and 10
+    // 16 vectors, 4096 x 4096: 16.5 us here, 10.2 us there; 8 vectors: 7 and 10.  (The form for 16 was launched for two blocks
+    // an SM, as parts_of counts, while its registers leave room for one: two rounds.  One that fits was not measured.)
     if (n_vec > 8) return product_many(m, n_vec, x, ld_x, y, ld_y, s);
     Few<V> g = {};
     g.m = m;

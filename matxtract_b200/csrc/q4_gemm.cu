@@ -12,10 +12,14 @@
 // through distributed shared memory, in the order of their ranks; large products are computed by pairs of blocks
 // (pair_kernel).
 //
-// Measured, 8192 x 8192 in bfloat16: 16 vectors 23.5 us (the codes at 1.4 TB/s: the conversion bounds it, 800 clocks for
-// 128 x 128 of them), 128 vectors 28 us, 512 vectors 55 us, 2048 vectors 191 us (1.44 PFLOP/s, 0.87 of what a library's
-// dense product reaches), with a residual of 0.5 % of the entries 219 us: 13 us for laying it out, the rest for putting
-// it into the tiles.
+// W's rounding to 16 bits is what the tensor cores' operands ask for.  Against 64 bits the results are 1.3 times as far off
+// as those of weights in 32 bits; up to 8 vectors (q4_few.cu) no weight is rounded.
+//
+// Measured, 8192 x 8192 in bfloat16: 16 vectors 23.4 us (the codes at 1.4 TB/s), 128 vectors 28 us, 512 vectors 54 us, 2048
+// vectors 192 us (1.43 PFLOP/s; a library's product of these sizes with a dense W takes 181 us), with a residual of 0.5 % of
+// the entries 221 us: 13 us for laying it out, the rest for putting it into the tiles.  With few vectors nothing is full
+// (16 vectors: ALU pipe 50 %, issue slots 52 %, DRAM a fifth): a code tile takes 800 clocks from its arrival to its values,
+// most of them waits, and a block has only 16 of them to hide its beginning and its end behind.
 #include <limits.h>
 
 #include <algorithm>

@@ -8,10 +8,11 @@
 // step's operands cross the L2 and the shared memories half as often as with a block on its own.  The pairs go on from
 // tile to tile, and the tensor memory holds two, so that one is reduced while the next is computed.
 //
-// Measured, bfloat16: 8192 x 8192, 2048 vectors 170 to 182 us with and without a residual (1.5 to 1.6 PFLOP/s: the tensor
-// cores and the L2 that feeds them bound it); 16384 x 8192, 64 vectors 65 us (the reduction of 256 x 256 numbers a tile
-// bounds it), with a residual of 0.5 % of the entries 165: a search for the place of its entries in every row and tile.
-// Searched for in front, by a kernel of its own, that was 144, but 2 to 3 us more for everything smaller.
+// Measured, bfloat16: 8192 x 8192, 2048 vectors 169 us, with a residual 173 (1.6 PFLOP/s: the tensor cores and the L2 that
+// feeds them bound it); 16384 x 8192, 64 vectors 64 to 78 us (it goes by where the matrix lies): a tile's one step of matrix
+// work is followed by 65,536 numbers to weigh, a chain of loads from tensor memory and sums (issue slots 54 %, tensor pipe
+// 12 %); with a residual of 0.5 % of the entries 150 to 179: a search for the place of its entries in every row and tile.
+// Searched for in front, by a kernel of its own, that was 144 for 167, but 2 to 3 us more for everything smaller.
 #include <limits.h>
 
 #include <algorithm>
